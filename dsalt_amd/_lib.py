@@ -128,6 +128,46 @@ class GatherArgs(ctypes.Structure):
                 ("cu_seqlens", _vp), ("lmk_idx", _vp), ("lmk_k", _vp), ("lmk_v", _vp)]
 
 
+class Cache(ctypes.Structure):
+    _fields_ = [("n_blocks", _i32), ("n_kv_heads", _i32), ("block_tokens", _i32), ("head_dim", _i32),
+                ("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp)]
+
+
+class CacheRowsArgs(ctypes.Structure):
+    _fields_ = [("n_reqs", _i32), ("table_cols", _i32), ("block_tokens", _i32), ("n_rows", _i32), ("n_pieces", _i32),
+                ("n_free", _i64), ("seq_len", _vp), ("new_len", _vp), ("table", _vp), ("table_stride", _i64),
+                ("free_blocks", _vp), ("span", _vp), ("seq_out", _vp), ("span_out", _vp), ("granted", _vp), ("cu", _vp),
+                ("req", _vp), ("pos", _vp), ("slot", _vp), ("pieces", _vp), ("workspace", _vp),
+                ("workspace_bytes", _sz)]
+
+
+class CacheWriteArgs(ctypes.Structure):
+    _fields_ = [("c", Cache), ("n_rows", _i32), ("n_pieces", _i32), ("dtype", _i32),
+                ("k", _vp), ("k_stride_t", _i64), ("k_stride_h", _i64),
+                ("v", _vp), ("v_stride_t", _i64), ("v_stride_h", _i64), ("pieces", _vp)]
+
+
+class CacheReadArgs(ctypes.Structure):
+    _fields_ = [("c", Cache), ("n_reqs", _i32), ("table_cols", _i32), ("n_rows", _i32), ("dtype", _i32),
+                ("table", _vp), ("table_stride", _i64), ("cu_seqlens", _vp), ("start", _vp), ("k", _vp), ("v", _vp)]
+
+
+class CacheAttnArgs(ctypes.Structure):
+    _fields_ = [("c", Cache), ("n_rows", _i32), ("n_heads", _i32), ("n_reqs", _i32), ("table_cols", _i32),
+                ("k_lmk", _i32), ("dtype", _i32), ("w_max", _i32), ("table", _vp), ("table_stride", _i64),
+                ("q", _vp), ("q_stride_t", _i64), ("q_stride_h", _i64),
+                ("req", _vp), ("pos", _vp), ("w", _vp), ("lmk_idx", _vp), ("lmk_bias", _vp),
+                ("out", _vp), ("o_stride_t", _i64), ("o_stride_h", _i64), ("lse", _vp), ("scale", _f32),
+                ("workspace", _vp), ("workspace_bytes", _sz)]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [("rows", _i32), ("n_cols", _i32), ("dtype", _i32), ("u_bytes", _i32), ("logits", _vp),
+                ("logits_stride", _i64), ("u", _vp), ("temperature", _vp), ("top_p", _vp), ("min_p", _vp), ("top_k", _vp),
+                ("temperature_all", _f32), ("top_p_all", _f32), ("min_p_all", _f32), ("top_k_all", _i32),
+                ("token", _vp), ("logp", _vp)]
+
+
 # name -> (argtypes, restype); every function declared in include/dsalt_amd.h
 SIGNATURES = {
     "dsalt_abi_version": ([], ctypes.c_int),
@@ -158,6 +198,13 @@ SIGNATURES = {
     "dsalt_sort_landmarks": ([ctypes.POINTER(SortArgs), _vp], ctypes.c_int),
     "dsalt_export_probs": ([ctypes.POINTER(ProbsArgs), _vp], ctypes.c_int),
     "dsalt_cross_entropy_rows": ([ctypes.POINTER(CeArgs), _vp], ctypes.c_int),
+    "dsalt_cache_rows_workspace_bytes": ([ctypes.POINTER(CacheRowsArgs)], _sz),
+    "dsalt_cache_rows": ([ctypes.POINTER(CacheRowsArgs), _vp], ctypes.c_int),
+    "dsalt_cache_write": ([ctypes.POINTER(CacheWriteArgs), _vp], ctypes.c_int),
+    "dsalt_cache_read": ([ctypes.POINTER(CacheReadArgs), _vp], ctypes.c_int),
+    "dsalt_cache_attn_workspace_bytes": ([ctypes.POINTER(CacheAttnArgs)], _sz),
+    "dsalt_cache_attn": ([ctypes.POINTER(CacheAttnArgs), _vp], ctypes.c_int),
+    "dsalt_sample_rows": ([ctypes.POINTER(SampleArgs), _vp], ctypes.c_int),
     "dsalt_timing_enable": ([ctypes.c_int], ctypes.c_int),
     "dsalt_timing_report": ([ctypes.c_char_p, _sz], ctypes.c_int),
 }

@@ -32,6 +32,9 @@ SOURCES = {
     # one rounding per operation, as the torch expression
     "layer.hip": ["-ffp-contract=off"],
     "ce.hip": [],
+    "cache.hip": [],
+    "cache_attn.hip": [],
+    "sample.hip": [],
     "capi.hip": [],
     "timing.hip": [],
 }

@@ -8,11 +8,13 @@
 #include <string>
 
 #include "attn.h"
+#include "cache.h"
 #include "ce.h"
 #include "ffn.h"
 #include "layer.h"
 #include "probs.h"
 #include "rope.h"
+#include "sample.h"
 #include "select.h"
 #include "sets.h"
 #include "common.h"
@@ -81,6 +83,77 @@ int check_rows(const void* ptr, int64_t st, int64_t sh, int dtype, const char* n
     if (st * (int64_t)es > (int64_t)(1u << 20))
         return fail(DSALT_ERR_UNSUPPORTED, "%s token stride of %lld bytes exceeds 1 MiB", name,
                     (long long)(st * (int64_t)es));
+    return DSALT_OK;
+}
+
+// pages of the 8-bit cache
+int check_cache(const dsalt_cache& c) {
+    if (c.n_blocks < 1 || c.n_kv_heads < 1 || c.n_kv_heads > 65535)
+        return fail(DSALT_ERR_INVALID, "the cache needs n_blocks >= 1 and n_kv_heads in [1, 65535] (got %d, %d)", c.n_blocks,
+                    c.n_kv_heads);
+    if (c.block_tokens != 16 && c.block_tokens != 32 && c.block_tokens != 64 && c.block_tokens != 128)
+        return fail(DSALT_ERR_INVALID, "block_tokens must be 16, 32, 64 or 128, got %d", c.block_tokens);
+    if (c.head_dim != 64 && c.head_dim != 128)
+        return fail(DSALT_ERR_UNSUPPORTED, "head_dim %d not supported (64 or 128)", c.head_dim);
+    if (!c.k || !c.v || !c.k_scale || !c.v_scale || !aligned16(c.k) || !aligned16(c.v))
+        return fail(DSALT_ERR_INVALID, "the cache's k, v (16-byte aligned) and scales are required");
+    return DSALT_OK;
+}
+
+dsalt::CachePages cache_pages(const dsalt_cache& c) {
+    return {c.n_blocks, c.n_kv_heads, __builtin_ctz((unsigned)c.block_tokens), c.head_dim, (uint8_t*)c.k, (uint8_t*)c.v,
+            c.k_scale, c.v_scale};
+}
+
+int check_table(const void* table, int64_t stride, int n_reqs, int cols) {
+    if (n_reqs < 1 || cols < 1) return fail(DSALT_ERR_INVALID, "n_reqs >= 1 and table_cols >= 1 required (got %d, %d)", n_reqs, cols);
+    if (!table || stride < cols) return fail(DSALT_ERR_INVALID, "table needs rows of at least table_cols entries");
+    return DSALT_OK;
+}
+
+dsalt::CacheAttnParams cache_attn_params(const dsalt_cache_attn_args* a) {
+    dsalt::CacheAttnParams p = {};
+    p.c = cache_pages(a->c);
+    p.n_rows = a->n_rows;
+    p.n_heads = a->n_heads;
+    p.n_reqs = a->n_reqs;
+    p.cols = a->table_cols;
+    p.k_lmk = a->k_lmk;
+    p.dtype = a->dtype;
+    p.w_max = a->w_max;
+    p.table_st = a->table_stride;
+    p.q = a->q;
+    p.q_st = a->q_stride_t;
+    p.q_sh = a->q_stride_h;
+    p.table = a->table;
+    p.req = a->req;
+    p.pos = a->pos;
+    p.w = a->w;
+    p.lmk = a->lmk_idx;
+    p.lbias = a->lmk_bias;
+    p.out = a->out;
+    p.o_st = a->o_stride_t;
+    p.o_sh = a->o_stride_h;
+    p.lse = a->lse;
+    p.scale = a->scale;
+    p.ws = (char*)a->workspace;
+    p.ws_bytes = a->workspace_bytes;
+    return p;
+}
+
+int check_cache_attn(const dsalt_cache_attn_args* a) {
+    if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
+    int rc = check_cache(a->c);
+    if (rc) return rc;
+    if (a->n_rows < 0) return fail(DSALT_ERR_INVALID, "n_rows must be >= 0, got %d", a->n_rows);
+    if (a->n_heads < 1 || a->n_heads > 65535 || a->n_heads % a->c.n_kv_heads)
+        return fail(DSALT_ERR_INVALID, "n_heads (%d) must be a positive multiple of n_kv_heads (%d)", a->n_heads, a->c.n_kv_heads);
+    if ((rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols))) return rc;
+    if (a->k_lmk < 0 || a->k_lmk > dsalt::kMaxLandmarks)
+        return fail(DSALT_ERR_INVALID, "k_lmk %d outside [0, %d]", a->k_lmk, dsalt::kMaxLandmarks);
+    if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if (a->w_max < 0) return fail(DSALT_ERR_INVALID, "w_max must be >= 0 (0: not known), got %d", a->w_max);
+    if (!(a->scale > 0.f)) return fail(DSALT_ERR_INVALID, "scale must be positive");
     return DSALT_OK;
 }
 
@@ -735,6 +808,156 @@ int dsalt_layer_selectors(const dsalt_selectors_args* a, dsalt_stream_t stream) 
     p.w = a->w;
     p.alpha = a->alpha;
     return hip_status(dsalt::selectors_launch(p, (hipStream_t)stream), "dsalt_layer_selectors");
+}
+
+size_t dsalt_cache_rows_workspace_bytes(const dsalt_cache_rows_args* a) {
+    return a && a->n_reqs >= 1 ? dsalt::cache_rows_ws_bytes(a->n_reqs) : 0;
+}
+
+int dsalt_cache_rows(const dsalt_cache_rows_args* a, dsalt_stream_t stream) {
+    if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
+    int rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols);
+    if (rc) return rc;
+    if (a->block_tokens != 16 && a->block_tokens != 32 && a->block_tokens != 64 && a->block_tokens != 128)
+        return fail(DSALT_ERR_INVALID, "block_tokens must be 16, 32, 64 or 128, got %d", a->block_tokens);
+    if ((int64_t)a->table_cols * a->block_tokens > 0x7fffffff)
+        return fail(DSALT_ERR_INVALID, "table_cols x block_tokens must stay below 2^31 (got %d x %d)", a->table_cols, a->block_tokens);
+    if (a->n_rows < 0) return fail(DSALT_ERR_INVALID, "n_rows must be >= 0, got %d", a->n_rows);
+    const int64_t most = (int64_t)a->n_rows / a->block_tokens + 2 * (int64_t)a->n_reqs;
+    if (a->n_pieces < (most < a->n_rows ? most : a->n_rows) || a->n_pieces > a->n_rows)
+        return fail(DSALT_ERR_INVALID, "n_pieces must be in [min(n_rows, n_rows / block_tokens + 2 n_reqs), n_rows], got %d", a->n_pieces);
+    if (a->n_free < 1) return fail(DSALT_ERR_INVALID, "the ring of free pages needs an entry");
+    if (!a->seq_len || !a->new_len || !a->free_blocks || !a->span || !a->seq_out || !a->span_out || !a->granted || !a->cu)
+        return fail(DSALT_ERR_INVALID, "seq_len, new_len, free_blocks, span, seq_out, span_out, granted and cu are required");
+    if (a->n_rows > 0 && (!a->req || !a->pos || !a->slot || !a->pieces || !aligned16(a->pieces)))
+        return fail(DSALT_ERR_INVALID, "req, pos, slot and pieces (16-byte aligned) are required");
+    if (a->seq_out == a->seq_len || a->span_out == a->span || a->seq_out == a->new_len)
+        return fail(DSALT_ERR_INVALID, "outputs may not be the inputs");
+    if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < dsalt::cache_rows_ws_bytes(a->n_reqs))
+        return fail(DSALT_ERR_WORKSPACE, "workspace of %zu bytes required", dsalt::cache_rows_ws_bytes(a->n_reqs));
+    dsalt::CacheRowsParams p;
+    p.n_reqs = a->n_reqs;
+    p.cols = a->table_cols;
+    p.bt_log = __builtin_ctz((unsigned)a->block_tokens);
+    p.n_rows = a->n_rows;
+    p.n_pieces = a->n_pieces;
+    p.n_free = a->n_free;
+    p.table_st = a->table_stride;
+    p.seq_len = a->seq_len;
+    p.new_len = a->new_len;
+    p.table = a->table;
+    p.ring = a->free_blocks;
+    p.span = a->span;
+    p.seq_out = a->seq_out;
+    p.span_out = a->span_out;
+    p.granted = a->granted;
+    p.cu = a->cu;
+    p.req = a->req;
+    p.pos = a->pos;
+    p.slot = a->slot;
+    p.pieces = a->pieces;
+    p.ws = (char*)a->workspace;
+    return hip_status(dsalt::cache_rows_launch(p, (hipStream_t)stream), "dsalt_cache_rows");
+}
+
+int dsalt_cache_write(const dsalt_cache_write_args* a, dsalt_stream_t stream) {
+    if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
+    int rc = check_cache(a->c);
+    if (rc) return rc;
+    if (a->n_rows < 0 || a->n_pieces < 0)
+        return fail(DSALT_ERR_INVALID, "n_rows >= 0 and n_pieces >= 0 required (got %d, %d)", a->n_rows, a->n_pieces);
+    if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if (a->n_rows == 0 || a->n_pieces == 0) return DSALT_OK;
+    if ((rc = check_rows(a->k, a->k_stride_t, a->k_stride_h, a->dtype, "k"))) return rc;
+    if ((rc = check_rows(a->v, a->v_stride_t, a->v_stride_h, a->dtype, "v"))) return rc;
+    if (!a->pieces || !aligned16(a->pieces)) return fail(DSALT_ERR_INVALID, "pieces (16-byte aligned) are required");
+    dsalt::CacheWriteParams p;
+    p.c = cache_pages(a->c);
+    p.n_rows = a->n_rows;
+    p.n_pieces = a->n_pieces;
+    p.dtype = a->dtype;
+    p.k = a->k;
+    p.k_st = a->k_stride_t;
+    p.k_sh = a->k_stride_h;
+    p.v = a->v;
+    p.v_st = a->v_stride_t;
+    p.v_sh = a->v_stride_h;
+    p.pieces = a->pieces;
+    return hip_status(dsalt::cache_write_launch(p, (hipStream_t)stream), "dsalt_cache_write");
+}
+
+int dsalt_cache_read(const dsalt_cache_read_args* a, dsalt_stream_t stream) {
+    if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
+    int rc = check_cache(a->c);
+    if (rc) return rc;
+    if ((rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols))) return rc;
+    if (a->n_rows < 0) return fail(DSALT_ERR_INVALID, "n_rows must be >= 0, got %d", a->n_rows);
+    if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if (a->n_rows == 0) return DSALT_OK;
+    if (!a->cu_seqlens || !a->k || !a->v || !aligned16(a->k) || !aligned16(a->v))
+        return fail(DSALT_ERR_INVALID, "cu_seqlens, k and v (16-byte aligned) are required");
+    dsalt::CacheReadParams p;
+    p.c = cache_pages(a->c);
+    p.n_reqs = a->n_reqs;
+    p.cols = a->table_cols;
+    p.n_rows = a->n_rows;
+    p.dtype = a->dtype;
+    p.table_st = a->table_stride;
+    p.table = a->table;
+    p.cu = a->cu_seqlens;
+    p.start = a->start;
+    p.k = a->k;
+    p.v = a->v;
+    return hip_status(dsalt::cache_read_launch(p, (hipStream_t)stream), "dsalt_cache_read");
+}
+
+size_t dsalt_cache_attn_workspace_bytes(const dsalt_cache_attn_args* a) {
+    return check_cache_attn(a) ? 0 : dsalt::cache_attn_ws_bytes(cache_attn_params(a));
+}
+
+int dsalt_cache_attn(const dsalt_cache_attn_args* a, dsalt_stream_t stream) {
+    int rc = check_cache_attn(a);
+    if (rc || a->n_rows == 0) return rc;
+    if ((rc = check_rows(a->q, a->q_stride_t, a->q_stride_h, a->dtype, "q"))) return rc;
+    if ((rc = check_rows(a->out, a->o_stride_t, a->o_stride_h, a->dtype, "out"))) return rc;
+    if (!a->req || !a->pos || !a->w || !a->lse || (a->k_lmk > 0 && !a->lmk_idx))
+        return fail(DSALT_ERR_INVALID, "req, pos, w, lse and lmk_idx are required");
+    const dsalt::CacheAttnParams p = cache_attn_params(a);
+    const size_t need = dsalt::cache_attn_ws_bytes(p);
+    if (need && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need))
+        return fail(DSALT_ERR_WORKSPACE, "workspace of %zu bytes required", need);
+    return hip_status(dsalt::cache_attn_launch(p, (hipStream_t)stream), "dsalt_cache_attn");
+}
+
+int dsalt_sample_rows(const dsalt_sample_args* a, dsalt_stream_t stream) {
+    if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
+    if (a->rows < 0 || a->n_cols < 1 || a->n_cols > dsalt::kSampleMaxCols)
+        return fail(DSALT_ERR_INVALID, "rows >= 0 and n_cols in [1, %d] required (got %d, %d)", dsalt::kSampleMaxCols, a->rows, a->n_cols);
+    if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if (a->u_bytes != 4 && a->u_bytes != 8) return fail(DSALT_ERR_INVALID, "u_bytes must be 4 or 8, got %d", a->u_bytes);
+    if (a->rows == 0) return DSALT_OK;
+    if (!a->logits || (uintptr_t)a->logits % esize(a->dtype) || a->logits_stride < 0)
+        return fail(DSALT_ERR_INVALID, "logits need element alignment and a row stride >= 0");
+    if (!a->u || !a->token || !a->logp) return fail(DSALT_ERR_INVALID, "u, token and logp are required");
+    dsalt::SampleParams p;
+    p.rows = a->rows;
+    p.n_cols = a->n_cols;
+    p.dtype = a->dtype;
+    p.u_f64 = a->u_bytes == 8;
+    p.x = a->logits;
+    p.x_st = a->logits_stride;
+    p.u = a->u;
+    p.temperature = a->temperature;
+    p.top_p = a->top_p;
+    p.min_p = a->min_p;
+    p.top_k = a->top_k;
+    p.temperature_all = a->temperature_all;
+    p.top_p_all = a->top_p_all;
+    p.min_p_all = a->min_p_all;
+    p.top_k_all = a->top_k_all;
+    p.token = a->token;
+    p.logp = a->logp;
+    return hip_status(dsalt::sample_launch(p, (hipStream_t)stream), "dsalt_sample_rows");
 }
 
 int dsalt_gather_landmarks(const dsalt_gather_args* a, dsalt_stream_t stream) {

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from typing import NamedTuple
 
 import torch
 from torch.autograd import forward_ad
@@ -15,8 +16,8 @@ from torch.autograd import forward_ad
 from . import _lib
 from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, SELECT_BLOCK, SELECT_GLOBAL, STATS_PACKED,
                    STATS_SEQUENCE, VARIANT_DEFAULT, VARIANT_DQ_BN64, VARIANT_FWD_BN32, VARIANT_FWD_RG2,
-                   VARIANT_LMK_SHORT, BwdArgs, CeArgs, FwdArgs, GatherArgs, Problem, ProbsArgs, RopeArgs, SelectArgs,
-                   SelectorsArgs, SiluMulArgs, SortArgs,
+                   VARIANT_LMK_SHORT, BwdArgs, Cache, CacheAttnArgs, CacheReadArgs, CacheRowsArgs, CacheWriteArgs, CeArgs, FwdArgs,
+                   GatherArgs, Problem, ProbsArgs, RopeArgs, SampleArgs, SelectArgs, SelectorsArgs, SiluMulArgs, SortArgs,
                    TrainBwdArgs,
                    TrainFwdArgs)
 
@@ -730,3 +731,238 @@ def sort_landmarks(idx: torch.Tensor, bias: torch.Tensor | None = None):
     out = torch.where(srt == big, torch.full_like(srt, -1), srt).to(torch.int32)
     b = bias.gather(-1, perm) if bias is not None else None
     return out, b, perm
+
+
+# ------------------------------------------------------------------ decoding over an 8-bit cache
+BLOCK_TOKENS = (16, 32, 64, 128)  # tokens a page of the cache may hold
+MAX_VOCAB = 1 << 20               # columns of sample_rows
+
+
+class Cache8(NamedTuple):
+    """Pages of an 8-bit key/value cache: k, v [n_blocks, n_kv, block_tokens, D] float8_e4m3fn and
+    k_scale, v_scale [n_blocks, n_kv] float32 (powers of two); an element is code * scale."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+class CacheRows(NamedTuple):
+    """Row maps of one decoding step (cache_rows_): tokens held after it, the ring's counters, granted [R]
+    (1 granted or ended, 0 refused), cu [R+1] rows of each request, and of each row its request,
+    position and slot (page * block_tokens + place in it); pieces [P, 4] for cache_write_."""
+    seq_len: torch.Tensor
+    span: torch.Tensor
+    granted: torch.Tensor
+    cu: torch.Tensor
+    req: torch.Tensor
+    pos: torch.Tensor
+    slot: torch.Tensor
+    pieces: torch.Tensor
+
+
+def new_cache(n_blocks: int, n_kv_heads: int, head_dim: int, *, block_tokens: int = 64, device="cuda") -> Cache8:
+    """An empty cache of one layer (head_dim 64 or 128; other head_dims pad their heads)."""
+    if block_tokens not in BLOCK_TOKENS or head_dim not in (64, 128):
+        raise ValueError(f"block_tokens must be one of {BLOCK_TOKENS} and head_dim 64 or 128, got {block_tokens}, {head_dim}")
+    shape = (n_blocks, n_kv_heads, block_tokens, head_dim)
+    codes = [torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
+    return Cache8(*codes, *(torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _cache_args(c: Cache8) -> Cache:
+    k, v, ks, vs = c
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn \
+            or not k.is_contiguous() or not v.is_contiguous():
+        raise ValueError("the cache's k and v must be contiguous float8_e4m3fn [n_blocks, n_kv, block_tokens, D]")
+    if ks.shape != k.shape[:2] or vs.shape != k.shape[:2] or ks.dtype != torch.float32 or vs.dtype != torch.float32 \
+            or not ks.is_contiguous() or not vs.is_contiguous():
+        raise ValueError("the cache's scales must be contiguous float32 [n_blocks, n_kv]")
+    return Cache(*k.shape, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr())
+
+
+def _check_table(table: torch.Tensor):
+    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1) \
+            or (table.shape[0] > 1 and table.stride(0) < table.shape[1]):
+        raise ValueError("table must be int32 [R, pages] with unit stride along the pages and rows that do not overlap")
+
+
+def _table_stride(table: torch.Tensor) -> int:
+    return max(table.stride(0), table.shape[1])
+
+
+def _rows16(t: torch.Tensor, name: str):
+    """([T, H, D] tensor, its (address, token stride, head stride)) as the kernels' 16-byte loads need them:
+    the tensor itself, or a copy of one with other strides or alignment."""
+    t = _rows3(t, name)
+    T, H, D = t.shape
+    es = t.element_size()
+
+    def strides():
+        return t.stride(0) if T > 1 else H * D, t.stride(1) if H > 1 else D
+
+    st, sh = strides()
+    if t.data_ptr() % 16 or st <= 0 or st * es % 16 or st * es > 1 << 20 or sh * es % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st, sh = strides()
+    return t, (t.data_ptr(), st, sh)
+
+
+def _vec_i32(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must have {n} entries, got shape {tuple(t.shape)}")
+    return _i32(t)
+
+
+def _call(name: str, args, dev: torch.device):
+    """One library call on the current stream of ``dev`` (made current for it where it is not)."""
+    fn = getattr(_lib.load(), name)
+    if dev.index is not None and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            rc = fn(ctypes.byref(args), _stream(dev))
+    else:
+        rc = fn(ctypes.byref(args), _stream(dev))
+    _lib.check(name, rc)
+
+
+def cache_rows_(seq_len, new_len, table, free_blocks, span, n_rows: int, *, block_tokens: int = 64) -> CacheRows:
+    """Row maps of one step over R requests, on the device alone (no synchronisation): request r holds
+    ``seq_len[r]`` tokens and brings ``new_len[r]`` (negative: it ends).  ``table`` [R, pages] int32 receives
+    the new pages, taken from the ring ``free_blocks`` (int32) at ``span`` [2] int64 (pages ever taken from
+    it, pages ever given to it); pages of ended requests go back into the ring.  ``n_rows``: rows of the step's
+    batch (host value); rows past the requests' last are inert.  Requests are served in order, one whose pages
+    are not there, or whose tokens fit neither the table nor the rows, is refused: it keeps its length and its
+    rows are inert (position and slot -1).  ``seq_len`` and ``span`` stay as they are: the step's come back in
+    the CacheRows."""
+    dev = _gpu(seq_len, new_len, table, free_blocks, span)
+    _check_table(table)
+    R, M = table.shape
+    if free_blocks.dim() != 1 or free_blocks.dtype != torch.int32 or not free_blocks.is_contiguous():
+        raise ValueError("free_blocks must be contiguous int32 [entries]")
+    if span.shape != (2,) or span.dtype != torch.int64 or not span.is_contiguous():
+        raise ValueError("span must be int64 [2]")
+    if n_rows < 0 or block_tokens not in BLOCK_TOKENS:
+        raise ValueError(f"n_rows must be >= 0 and block_tokens one of {BLOCK_TOKENS}, got {n_rows}, {block_tokens}")
+    old, new = _vec_i32(seq_len, R, "seq_len"), _vec_i32(new_len, R, "new_len")
+    n_pieces = min(n_rows, n_rows // block_tokens + 2 * R)
+    i32, i64 = torch.int32, torch.int64
+    out = CacheRows(torch.empty(R, dtype=i32, device=dev), torch.empty(2, dtype=i64, device=dev),
+                    torch.empty(R, dtype=i32, device=dev), torch.empty(R + 1, dtype=i32, device=dev),
+                    torch.empty(n_rows, dtype=i32, device=dev), torch.empty(n_rows, dtype=i32, device=dev),
+                    torch.empty(n_rows, dtype=i64, device=dev), torch.empty((n_pieces, 4), dtype=i32, device=dev))
+    a = CacheRowsArgs(R, M, block_tokens, n_rows, n_pieces, free_blocks.shape[0], old.data_ptr(), new.data_ptr(),
+                      table.data_ptr(), _table_stride(table), free_blocks.data_ptr(), span.data_ptr(), out.seq_len.data_ptr(),
+                      out.span.data_ptr(), out.granted.data_ptr(), out.cu.data_ptr(), out.req.data_ptr(), out.pos.data_ptr(),
+                      out.slot.data_ptr(), out.pieces.data_ptr())
+    ws = _set_workspace(a, _lib.load().dsalt_cache_rows_workspace_bytes(ctypes.byref(a)), dev)  # noqa: F841 (kept alive)
+    _call("dsalt_cache_rows", a, dev)
+    return out
+
+
+def cache_write_(k, v, cache: Cache8, pieces) -> Cache8:
+    """Writes the step's keys and values k, v [T, n_kv, D] into the cache, the rows of ``pieces`` [P, 4] int32
+    (CacheRows.pieces: first row, rows, page, first token in the page; each page in one piece at most).  A page's
+    scale is the least power of two that keeps its finite elements within 448 of it; codes it held follow a
+    larger one.  Values that are not finite are held as NaN."""
+    dev = _gpu(k, v, *cache, pieces)
+    (k, k_at), (v, v_at) = _rows16(k, "k"), _rows16(v, "v")
+    c = _cache_args(cache)
+    if k.shape != v.shape or k.dtype != v.dtype or k.shape[1] != c.n_kv_heads or k.shape[2] != c.head_dim:
+        raise ValueError(f"k and v must be [T, {c.n_kv_heads}, {c.head_dim}] of one dtype, got {tuple(k.shape)}, {tuple(v.shape)}")
+    if pieces.dim() != 2 or pieces.shape[1] != 4 or pieces.dtype != torch.int32 or not pieces.is_contiguous():
+        raise ValueError("pieces must be contiguous int32 [P, 4]")
+    a = CacheWriteArgs(c, k.shape[0], pieces.shape[0], dtype_code(k.dtype), *k_at, *v_at, pieces.data_ptr())
+    _call("dsalt_cache_write", a, dev)
+    return cache
+
+
+def cache_read(cache: Cache8, table, cu_seqlens, *, start=None, n_rows: int, dtype=torch.bfloat16):
+    """(k, v) [n_rows, n_kv, D]: tokens of the cache as a packed batch.  Row t is token ``start[r]`` (default 0)
+    + t - cu_seqlens[r] of the request r whose rows hold it; zeros past the last row and where the table names
+    no page."""
+    dev = _gpu(*cache, table, cu_seqlens, start)
+    _check_table(table)
+    c = _cache_args(cache)
+    R, M = table.shape
+    cu = _vec_i32(cu_seqlens, R + 1, "cu_seqlens")
+    st = _vec_i32(start, R, "start") if start is not None else None
+    if n_rows < 0:
+        raise ValueError(f"n_rows must be >= 0, got {n_rows}")
+    k = torch.empty((n_rows, c.n_kv_heads, c.head_dim), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    a = CacheReadArgs(c, R, M, n_rows, dtype_code(dtype), table.data_ptr(), _table_stride(table), cu.data_ptr(),
+                      st.data_ptr() if st is not None else None, k.data_ptr(), v.data_ptr())
+    _call("dsalt_cache_read", a, dev)
+    return k, v
+
+
+def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None, *, scale=None, w_max=None):
+    """(out [T, H, D] in q.dtype, lse [T, H] fp32): the operator's attention of query tokens over the cache, the
+    form for single tokens of many requests.  Row t is the token at position ``pos[t]`` of request ``req[t]``
+    (CacheRows.req, .pos), its own key and value written; it attends its window [pos - w + 1, pos] and the
+    landmarks before the window of its head's set in lmk_idx [H, R, 1, K] (any order, negative slots empty, a
+    position may repeat; select_landmarks' sets).  Rows without a key (inert rows, pages that the table does not
+    name) give zeros and -inf.  ``w_max``: no window is longer (host value; splits the work, longer windows only
+    cost time).  Not differentiable."""
+    dev = _gpu(q, *cache, table, req, pos, w, lmk_idx, lmk_bias)
+    q, q_at = _rows16(q, "q")
+    _check_table(table)
+    c = _cache_args(cache)
+    T, H, D = q.shape
+    R, M = table.shape
+    if D != c.head_dim or H % c.n_kv_heads:
+        raise ValueError(f"q must be [T, H, {c.head_dim}] with H a multiple of {c.n_kv_heads}, got {tuple(q.shape)}")
+    if lmk_idx.dim() != 4 or lmk_idx.shape[:3] != (H, R, 1):
+        raise ValueError(f"lmk_idx must be [H, R, 1, K] = [{H}, {R}, 1, K], got {tuple(lmk_idx.shape)}")
+    if lmk_bias is not None and lmk_bias.shape != lmk_idx.shape:
+        raise ValueError("lmk_bias must have the shape of lmk_idx")
+    K = lmk_idx.shape[3]
+    rq, ps, wc = _vec_i32(req, T, "req"), _vec_i32(pos, T, "pos"), _vec_i32(w, T, "w")
+    li = _i32(lmk_idx)
+    lb = _f32(lmk_bias) if lmk_bias is not None else None
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((T, H), dtype=torch.float32, device=dev)
+    a = CacheAttnArgs(c, T, H, R, M, K, dtype_code(q.dtype), 0 if w_max is None else int(w_max), table.data_ptr(),
+                      _table_stride(table), *q_at, rq.data_ptr(), ps.data_ptr(), wc.data_ptr(),
+                      li.data_ptr() if K else None, lb.data_ptr() if lb is not None and K else None,
+                      out.data_ptr(), H * D, D, lse.data_ptr(), scale)
+    ws = _set_workspace(a, _lib.load().dsalt_cache_attn_workspace_bytes(ctypes.byref(a)), dev)  # noqa: F841 (kept alive)
+    _call("dsalt_cache_attn", a, dev)
+    return out, lse
+
+
+def sample_rows(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(token [R] int64, logp [R] fp32): a token a row of ``logits`` [R, V] from given random numbers ``u`` [R]
+    in [0, 1) (float32 or float64).  ``temperature`` (<= 0: the largest logit), ``top_k`` (<= 0: all), ``top_p``
+    and ``min_p`` are numbers or tensors [R].  Kept are the first top_k tokens by logit (equal ones by index, NaN
+    as -inf), of those the ones before which less than top_p of their weight lies, of those the ones that weigh
+    at least min_p of the first, and always the first; the token is the first index whose running sum of kept
+    weights passes u times their total.  Weights are whole multiples of 2^-42 of the largest.  logp: the token's
+    log probability among the kept.  Rows without a logit above -inf give -1 and -inf."""
+    per_row = [t if isinstance(t, torch.Tensor) else None for t in (temperature, top_k, top_p, min_p)]
+    dev = _gpu(logits, u, *per_row)
+    if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_VOCAB:
+        raise ValueError(f"logits must be [R, V] with V in [1, {MAX_VOCAB}], got {tuple(logits.shape)}")
+    R, V = logits.shape
+    if V > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    for t, name in zip([u] + per_row, ("u", "temperature", "top_k", "top_p", "min_p")):
+        if t is not None and (t.dim() != 1 or t.shape[0] != R):
+            raise ValueError(f"{name} must be [{R}], got shape {tuple(t.shape)}")
+    if u.dtype not in (torch.float32, torch.float64):
+        raise TypeError(f"u must be float32 or float64, got {u.dtype}")
+    u = u.contiguous()
+    t, k, p, m = per_row
+    t, p, m = (x if x is None else _f32(x) for x in (t, p, m))
+    if k is not None and k.dtype != torch.int32:
+        k = k.clamp(-1, MAX_VOCAB)
+    k = k if k is None else _i32(k)
+    token = torch.empty(R, dtype=torch.int64, device=dev)
+    logp = torch.empty(R, dtype=torch.float32, device=dev)
+    a = SampleArgs(R, V, dtype_code(logits.dtype), u.element_size(), logits.data_ptr(), logits.stride(0), u.data_ptr(),
+                   *(x.data_ptr() if x is not None else None for x in (t, p, m, k)),
+                   *(0.0 if isinstance(x, torch.Tensor) else float(x) for x in (temperature, top_p, min_p)),
+                   0 if k is not None else max(-1, min(int(top_k), MAX_VOCAB)), token.data_ptr(), logp.data_ptr())
+    _call("dsalt_sample_rows", a, dev)
+    return token, logp

@@ -351,6 +351,157 @@ typedef struct dsalt_sort_args {
 
 int    dsalt_sort_landmarks(const dsalt_sort_args* a, dsalt_stream_t stream);
 
+/*
+ * Decoding step over a paged 8-bit key/value cache.  No counterpart in the reference, which
+ * stops at the prompt's logits: these entry points continue from there, a token a request
+ * and step: row maps, the cache's write, attention over it, a token from the logits.
+ *
+ * The cache holds pages of block_tokens tokens: k and v [n_blocks, n_kv_heads, block_tokens,
+ * head_dim] in e4m3 (largest 448, no infinities), k_scale and v_scale [n_blocks, n_kv_heads]
+ * float32; an element is code * scale.  A block's scale is the least power of two in
+ * [2^-126, 2^119] that keeps every finite element written to it within 448; where a later
+ * token needs a larger one, the codes held are rounded to it (to nearest even, as every
+ * rounding here).  Larger magnitudes are held as 448 * scale, values that are not finite as
+ * NaN.  table [n_reqs, table_cols] names the page of tokens j * block_tokens ... of a request;
+ * entries outside [0, n_blocks) are never read through: what lies there counts as absent.
+ */
+typedef struct dsalt_cache {
+    int32_t n_blocks;
+    int32_t n_kv_heads;
+    int32_t block_tokens;      /* 16, 32, 64 or 128                                  */
+    int32_t head_dim;          /* 64 or 128                                          */
+    void* k; void* v;          /* e4m3 codes, 16-byte aligned                        */
+    float* k_scale; float* v_scale;
+} dsalt_cache;
+
+/* Row maps of one step.  Request r holds seq_len[r] tokens and brings new_len[r] more (>= 0;
+ * negative: it ends, its pages go back).  New pages come from the ring `free_blocks` (n_free
+ * entries, a power of two is not needed): span[0] counts the pages ever taken from it, span[1]
+ * those ever given to it, entry i mod n_free is page number i.  Requests are served in order: one
+ * is granted while the pages needed up to and with it do not pass span[1] - span[0] (one that
+ * needs no page is always granted), if its tokens fit table_cols pages and its rows end within
+ * n_rows; otherwise it keeps its length and its rows are inert (position and slot -1).  Pages given
+ * back in a call can be taken from the next one on; what the ring has no room for is dropped.
+ * The packed rows are the requests' new tokens in order: rows cu[r] .. cu[r + 1], rows past the last
+ * have request -1.  A piece is a run of a request's rows within one page: (first row, rows, page,
+ * first token in the page); pieces past the last are zero.  Inputs stay as they are but for the new
+ * entries of `table` and the pages given back in the ring; outputs may not alias inputs. */
+typedef struct dsalt_cache_rows_args {
+    int32_t n_reqs;
+    int32_t table_cols;
+    int32_t block_tokens;
+    int32_t n_rows;            /* rows of req, pos and slot (host value)              */
+    int32_t n_pieces;          /* rows of pieces, at least
+                                  min(n_rows, n_rows / block_tokens + 2 n_reqs)       */
+    int64_t n_free;            /* entries of the ring, >= the pages in circulation    */
+    const int32_t* seq_len;    /* [n_reqs]                                            */
+    const int32_t* new_len;    /* [n_reqs]                                            */
+    int32_t* table; int64_t table_stride;                     /* in and out           */
+    int32_t* free_blocks;      /* [n_free] in and out                                 */
+    const int64_t* span;       /* [2]                                                 */
+    int32_t* seq_out;          /* out [n_reqs] tokens held after the step             */
+    int64_t* span_out;         /* out [2]                                             */
+    int32_t* granted;          /* out [n_reqs] 1 granted or ended, 0 refused          */
+    int32_t* cu;               /* out [n_reqs + 1]                                    */
+    int32_t* req;              /* out [n_rows]                                        */
+    int32_t* pos;              /* out [n_rows] position in the request                */
+    int64_t* slot;             /* out [n_rows] page * block_tokens + place in the page */
+    int32_t* pieces;           /* out [n_pieces, 4], 16-byte aligned                  */
+    void* workspace; size_t workspace_bytes;
+} dsalt_cache_rows_args;
+
+size_t dsalt_cache_rows_workspace_bytes(const dsalt_cache_rows_args* a);
+int    dsalt_cache_rows(const dsalt_cache_rows_args* a, dsalt_stream_t stream);
+
+/* Writes the rows of `pieces` (each within one page) into the cache: k and v [n_rows, n_kv_heads,
+ * head_dim] in dtype.  A piece that does not lie within the rows and one page is skipped; no page
+ * may appear in two pieces.  Needs no workspace. */
+typedef struct dsalt_cache_write_args {
+    dsalt_cache c;
+    int32_t n_rows;
+    int32_t n_pieces;
+    int32_t dtype;             /* DSALT_DTYPE_*                                      */
+    const void* k; int64_t k_stride_t; int64_t k_stride_h;
+    const void* v; int64_t v_stride_t; int64_t v_stride_h;
+    const int32_t* pieces;     /* [n_pieces, 4], 16-byte aligned                     */
+} dsalt_cache_write_args;
+
+int    dsalt_cache_write(const dsalt_cache_write_args* a, dsalt_stream_t stream);
+
+/* Tokens of the cache as a packed batch, rounded once to dtype: row t of k and v [n_rows,
+ * n_kv_heads, head_dim] (contiguous) is token start[r] + t - cu_seqlens[r] of its request r; zeros
+ * for rows past cu_seqlens[n_reqs] and tokens outside the table.  Needs no workspace. */
+typedef struct dsalt_cache_read_args {
+    dsalt_cache c;
+    int32_t n_reqs;
+    int32_t table_cols;
+    int32_t n_rows;
+    int32_t dtype;
+    const int32_t* table; int64_t table_stride;
+    const int32_t* cu_seqlens; /* [n_reqs + 1]                                       */
+    const int32_t* start;      /* [n_reqs] or NULL (0)                               */
+    void* k; void* v;
+} dsalt_cache_read_args;
+
+int    dsalt_cache_read(const dsalt_cache_read_args* a, dsalt_stream_t stream);
+
+/* The operator's attention of single query tokens over the cache: row t is the token at position
+ * pos[t] of request req[t] and attends W = [pos - w + 1, pos] and the landmarks p < pos - w + 1 of
+ * its head's set (any order; negative slots are empty; a position may repeat, each copy counts).  out
+ * and lse as dsalt_fwd; rows that attend nothing (pos or req outside their ranges, all pages absent)
+ * give zeros and -inf.  Masked keys are never read into a result, whatever their pages hold. */
+typedef struct dsalt_cache_attn_args {
+    dsalt_cache c;
+    int32_t n_rows;            /* T                                                  */
+    int32_t n_heads;           /* H, a multiple of c.n_kv_heads                      */
+    int32_t n_reqs;
+    int32_t table_cols;
+    int32_t k_lmk;             /* landmark slots per set, 0..2048                    */
+    int32_t dtype;             /* of q and out                                       */
+    int32_t w_max;             /* no window is longer (0: not known); longer ones give the same
+                                  result, later: it sets how the work is split        */
+    const int32_t* table; int64_t table_stride;
+    const void* q;  int64_t q_stride_t; int64_t q_stride_h;   /* [T, H, D]           */
+    const int32_t* req;        /* [T]                                                */
+    const int32_t* pos;        /* [T]                                                */
+    const int32_t* w;          /* [T] (values < 1 act as 1)                          */
+    const int32_t* lmk_idx;    /* [H, n_reqs, 1, k_lmk]                              */
+    const float* lmk_bias;     /* like lmk_idx, added to the landmark logits, or NULL */
+    void* out; int64_t o_stride_t; int64_t o_stride_h;
+    float* lse;                /* [T, H]                                             */
+    float scale;
+    void* workspace; size_t workspace_bytes;
+} dsalt_cache_attn_args;
+
+size_t dsalt_cache_attn_workspace_bytes(const dsalt_cache_attn_args* a);
+int    dsalt_cache_attn(const dsalt_cache_attn_args* a, dsalt_stream_t stream);
+
+/* One token a row of logits from given random numbers u in [0, 1) (clamped into it).  In the order of
+ * the logits, largest first, equal ones by index, NaN as -inf, a token weighs
+ * round(2^42 exp((x - max) / temperature)); kept are the first top_k tokens (<= 0: all), of those the
+ * ones before which less than top_p of their weight lies, of those the ones that weigh at least
+ * min_p 2^42, and always the first.  token[r] is the first index whose running sum of kept weights,
+ * in the order of the vocabulary, passes u times their total; logp its log probability among the
+ * kept.  temperature <= 0: the largest logit, logp 0.  A row without a logit above -inf: -1 and -inf.
+ * Comparisons of sums are made in float64.  Needs no workspace. */
+typedef struct dsalt_sample_args {
+    int32_t rows;
+    int32_t n_cols;            /* vocabulary, 1 .. 2^20                              */
+    int32_t dtype;             /* DSALT_DTYPE_* of the logits                        */
+    int32_t u_bytes;           /* 4 (float32) or 8 (float64)                         */
+    const void* logits; int64_t logits_stride;
+    const void* u;             /* [rows]                                             */
+    /* a value a row, or NULL: the one of the same name for all */
+    const float* temperature; const float* top_p; const float* min_p;
+    const int32_t* top_k;
+    float temperature_all; float top_p_all; float min_p_all;
+    int32_t top_k_all;
+    int64_t* token;            /* out [rows]                                         */
+    float* logp;               /* out [rows]                                         */
+} dsalt_sample_args;
+
+int    dsalt_sample_rows(const dsalt_sample_args* a, dsalt_stream_t stream);
+
 /* Tile variants of the attention kernels (dsalt_fwd_args.variant, dsalt_bwd_args.variant).
  * Bits are independent; a bit a shape cannot use is ignored.  Without forward bits the
  * forward picks its tiling by the call's size (dsalt_fwd_tile tells which); the bit of a

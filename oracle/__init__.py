@@ -7,6 +7,8 @@ CPU restatements of the reference algorithm that the HIP library is checked agai
   kernels follow bit for bit;
 * ``attention.py``: float64 forward/backward of the kernel semantics, dense brute force,
   and the reference's literal CPU-fallback mask;
+* ``decode.py``: float64 row maps, 8-bit cache, attention of single tokens and sampling of a
+  decoding step, from the definitions in ``include/dsalt_amd.h``;
 * ``sdpa_cpu.py``: the reference's masked-SDPA CPU path (torch CPU), timed as the CPU
   baseline.
 
