@@ -105,8 +105,10 @@ dsalt::CachePages cache_pages(const dsalt_cache& c) {
             c.k_scale, c.v_scale};
 }
 
-int check_table(const void* table, int64_t stride, int n_reqs, int cols) {
+int check_table(const void* table, int64_t stride, int n_reqs, int cols, int block_tokens) {
     if (n_reqs < 1 || cols < 1) return fail(DSALT_ERR_INVALID, "n_reqs >= 1 and table_cols >= 1 required (got %d, %d)", n_reqs, cols);
+    if ((int64_t)cols * block_tokens > (1 << 30))
+        return fail(DSALT_ERR_INVALID, "table_cols x block_tokens must not pass 2^30 (got %d x %d)", cols, block_tokens);
     if (!table || stride < cols) return fail(DSALT_ERR_INVALID, "table needs rows of at least table_cols entries");
     return DSALT_OK;
 }
@@ -148,7 +150,9 @@ int check_cache_attn(const dsalt_cache_attn_args* a) {
     if (a->n_rows < 0) return fail(DSALT_ERR_INVALID, "n_rows must be >= 0, got %d", a->n_rows);
     if (a->n_heads < 1 || a->n_heads > 65535 || a->n_heads % a->c.n_kv_heads)
         return fail(DSALT_ERR_INVALID, "n_heads (%d) must be a positive multiple of n_kv_heads (%d)", a->n_heads, a->c.n_kv_heads);
-    if ((rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols))) return rc;
+    if ((rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols, a->c.block_tokens))) return rc;
+    if ((int64_t)a->n_rows * a->n_heads > 0x7fffffff)
+        return fail(DSALT_ERR_INVALID, "n_rows x n_heads must stay below 2^31 (got %d x %d)", a->n_rows, a->n_heads);
     if (a->k_lmk < 0 || a->k_lmk > dsalt::kMaxLandmarks)
         return fail(DSALT_ERR_INVALID, "k_lmk %d outside [0, %d]", a->k_lmk, dsalt::kMaxLandmarks);
     if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
@@ -816,12 +820,10 @@ size_t dsalt_cache_rows_workspace_bytes(const dsalt_cache_rows_args* a) {
 
 int dsalt_cache_rows(const dsalt_cache_rows_args* a, dsalt_stream_t stream) {
     if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
-    int rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols);
-    if (rc) return rc;
     if (a->block_tokens != 16 && a->block_tokens != 32 && a->block_tokens != 64 && a->block_tokens != 128)
         return fail(DSALT_ERR_INVALID, "block_tokens must be 16, 32, 64 or 128, got %d", a->block_tokens);
-    if ((int64_t)a->table_cols * a->block_tokens > 0x7fffffff)
-        return fail(DSALT_ERR_INVALID, "table_cols x block_tokens must stay below 2^31 (got %d x %d)", a->table_cols, a->block_tokens);
+    int rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols, a->block_tokens);
+    if (rc) return rc;
     if (a->n_rows < 0) return fail(DSALT_ERR_INVALID, "n_rows must be >= 0, got %d", a->n_rows);
     const int64_t most = (int64_t)a->n_rows / a->block_tokens + 2 * (int64_t)a->n_reqs;
     if (a->n_pieces < (most < a->n_rows ? most : a->n_rows) || a->n_pieces > a->n_rows)
@@ -890,7 +892,7 @@ int dsalt_cache_read(const dsalt_cache_read_args* a, dsalt_stream_t stream) {
     if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
     int rc = check_cache(a->c);
     if (rc) return rc;
-    if ((rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols))) return rc;
+    if ((rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols, a->c.block_tokens))) return rc;
     if (a->n_rows < 0) return fail(DSALT_ERR_INVALID, "n_rows must be >= 0, got %d", a->n_rows);
     if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
     if (a->n_rows == 0) return DSALT_OK;
