@@ -95,6 +95,9 @@ int check_cache(const dsalt_cache& c) {
         return fail(DSALT_ERR_INVALID, "block_tokens must be 16, 32, 64 or 128, got %d", c.block_tokens);
     if (c.head_dim != 64 && c.head_dim != 128)
         return fail(DSALT_ERR_UNSUPPORTED, "head_dim %d not supported (64 or 128)", c.head_dim);
+    if ((int64_t)c.n_blocks * c.n_kv_heads >= 0xffffffffll / c.block_tokens)
+        return fail(DSALT_ERR_INVALID, "n_blocks x n_kv_heads x block_tokens must stay below 2^32 - 1 (got %d x %d x %d)", c.n_blocks,
+                    c.n_kv_heads, c.block_tokens);
     if (!c.k || !c.v || !c.k_scale || !c.v_scale || !aligned16(c.k) || !aligned16(c.v))
         return fail(DSALT_ERR_INVALID, "the cache's k, v (16-byte aligned) and scales are required");
     return DSALT_OK;

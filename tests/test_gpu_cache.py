@@ -306,20 +306,58 @@ def test_attention_several_rows_of_a_request():
     _check_attend(q[order], cache, table, [req[i] for i in order], [pos[i] for i in order], [w[i] for i in order], lmk, w_max=60)
 
 
-def test_attention_inert_rows_and_absent_pages():
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_inert_rows_and_absent_pages(wide):
     q, cache, table, req, pos, w, lmk = _attend_case(6, 4, 2, 64, 16, 8, torch.float32, 11, 100, 50, lens=[100, 3, 50, 77, 64, 20])
     req[0], pos[1], req[2] = -1, -1, 6           # no request, no position, a request past the table
     table[3] = -1                                 # no page at all
     table[4, 1], table[4, 3] = -3, len(cache.k)   # pages below and past the cache
     pos[5] = 10 ** 6                              # past the table: only landmarks are there
     w[5] = 5
-    out, lse = _check_attend(q, cache, table, req, pos, w, lmk, w_max=50)
+    if wide:
+        table, pos[5] = _widened(table, 16, 1 << 15), 1 << 20
+    out, lse = _check_attend(q, cache, table, req, pos, w, lmk, w_max=None if wide else 50)
     assert np.isneginf(lse[:4]).all() and np.isfinite(lse[4:]).all()
 
 
+def _widened(table, bt, tokens):
+    """The table with empty columns up to `tokens` tokens a request: with the bound on the windows not given, the
+    kernels are chosen for windows that long."""
+    return np.pad(table, ((0, 0), (0, max(0, tokens // bt - table.shape[1]))), constant_values=-1)
+
+
+# what the size rules choose between, and a shape each (R, H, G, D, bt, K, lens or the longest, largest window, bound given)
+RULES = {
+    "heads, four waves": (9, 4, 4, 64, 32, 20, 300, 200, 200),
+    "heads, eight waves": (2, 4, 4, 128, 64, 40, 900, 700, 700),
+    "heads, split": (1, 2, 2, 128, 64, 70, [3001], 2900, 2900),
+    "heads of a group, split": (1, 8, 2, 64, 16, 9, [2500], 2500, 2500),
+    "groups, split, most splits empty": (3, 8, 2, 64, 16, 130, [300, 33, 1], 290, 1 << 15),
+    "groups, split, float rows full": (2, 12, 4, 128, 128, 70, [4100, 2000], 4100, 1 << 14),
+    "groups, eight waves": (128, 8, 2, 64, 64, 17, 90, 60, 300),
+    "groups, four waves": (140, 8, 2, 128, 32, 33, 90, 60, 300),
+    "groups of 17 heads": (70, 34, 2, 64, 16, 5, 70, 40, 150),
+    "groups of 16 heads of 128": (40, 32, 2, 128, 64, 6, 150, 100, 256),
+}
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rule", RULES)
+def test_attention_on_each_side_of_the_size_rules(rule, dt):
+    R, H, G, D, bt, K, lens, w, bound = RULES[rule]
+    c = list(_attend_case(R, H, G, D, bt, K, dt, R + H, lens if isinstance(lens, int) else max(lens), w, lens=None if isinstance(lens, int) else lens))
+    if isinstance(lens, list):
+        c[5] = [w, w // 2, 5][:R]
+    c[2] = _widened(c[2], bt, bound)
+    _check_attend(*c, w_max=bound)
+    bias = np.random.RandomState(3).randn(*c[-1].shape)
+    _check_attend(*c, bias=bias, w_max=bound)
+
+
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("G", [2, 8])
-def test_attention_reads_nothing_masked(dt, G):
+def test_attention_reads_nothing_masked(dt, G, wide):
     """NaN codes in every token that a row does not attend (behind the last, before the window, landmarks of
     other heads, pages of nobody, scales of pages without a key): results as without them.  A NaN that a
     row attends reaches its own heads alone."""
@@ -337,13 +375,15 @@ def test_attention_reads_nothing_masked(dt, G):
     for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
         codes.view(torch.uint8)[hide] = 0x7f
         scale[~torch.from_numpy(seen.any(-1)).to(DEV)] = float("nan")
-    a, _ = _check_attend(q, cache, table, req, pos, w, lmk, pages=clean, w_max=30)
+    bound = (1 << 15) + 31 if wide else 30  # (a key/value head's query heads as a group, or one by one)
+    table = _widened(table, bt, bound)
+    a, _ = _check_attend(q, cache, table, req, pos, w, lmk, pages=clean, w_max=bound)
     assert np.isfinite(a).all()
     # one landmark of head 3 of request 0 now holds NaN values: rows of the other heads stay
     only = int(next(p for p in lmk[3, 0, 0] if 0 <= p < pos[0] - 29))
     users = [h for h in range(H) if h // (H // G) == 3 // (H // G) and only in lmk[h, 0, 0]]
     cache.v.view(torch.uint8)[table[0, only // bt], 3 // (H // G), only % bt] = 0x7f
-    b = f64(ops.cache_attention(q.to(DEV), cache, _i32(table), _i32(req), _i32(pos), _i32(w), _i32(lmk), w_max=30)[0])
+    b = f64(ops.cache_attention(q.to(DEV), cache, _i32(table), _i32(req), _i32(pos), _i32(w), _i32(lmk), w_max=bound)[0])
     for h in range(H):
         assert np.isnan(b[0, h]).all() if h in users else np.array_equal(a[0, h], b[0, h])
     assert np.array_equal(a[1:], b[1:])
