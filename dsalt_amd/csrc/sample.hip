@@ -7,9 +7,10 @@
 // those the ones that weigh at least min_p 2^42.  The token is the first index whose running sum of kept
 // weights, in the order of the vocabulary, passes u times the total.
 //
-// A block takes a row.  The end of a prefix is found by a radix search over order-preserving keys: a
-// histogram (of counts for top_k, of weights for top_p) over twelve bits of the key at a time, the bins
-// summed from the top down to the one that holds the end.
+// A block takes a row.  With top_k up to 1024 (or a vocabulary up to kList) the few tokens that can be kept
+// are listed and sorted.  Otherwise the end of a prefix is found by a radix search over order-preserving
+// keys: a histogram (of counts for top_k, of weights for top_p) over twelve bits of the key at a time, the
+// bins summed from the top down to the one that holds the end.
 #include "common.h"
 #include "sample.h"
 #include "timing.h"
@@ -18,8 +19,8 @@ namespace dsalt {
 
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 4096;
-constexpr double kUnit = 4398046511104.0;  // 2^42: sums over 2^20 tokens stay below 2^62
+constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 4096, kList = 2048;
+constexpr unsigned long long kUnit = 1ull << 42;  // sums over 2^20 tokens stay below 2^62
 
 // keys: larger logits, larger keys; 0 where there is no element
 template <typename T> struct Key;
@@ -42,8 +43,10 @@ struct Cut {  // kept: key above, or equal with a lower index
 
 struct Shared {
     unsigned long long bin[kBins + 8];  // histogram bins, or a sum a chunk of the row
+    unsigned long long list[kList];     // tokens that can be kept: key, then the index's complement
     unsigned long long part[kWaves];
     unsigned long long found[4];
+    int count;
 };
 
 // exclusive prefix of v over the block, and the total
@@ -67,106 +70,181 @@ __device__ __forceinline__ unsigned long long block_scan(Shared& sh, unsigned lo
     return base + in - v;
 }
 
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+}
+// sum over the wave of values whose sum stays below 2^32 (every lane gets it)
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+    v = dpp_add<0x128>(dpp_add<0x124>(dpp_add<0x122>(dpp_add<0x121>(v))));  // rotations within sixteen lanes
+    auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = a[0] + a[1];
+    auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return b[0] + b[1];
+}
+// the same for weights: sums of at most 64 x 8 of 2^42, in two parts of 25 and 20 bits a lane
+__device__ __forceinline__ unsigned long long wave_sum_weights(unsigned long long v) {
+    return ((unsigned long long)wave_sum((uint32_t)(v >> 25)) << 25) + wave_sum((uint32_t)v & 0x1ffffffu);
+}
+
+// 2^f - 1 = f P(f) for f in [-1/2, 1/2], P the degree 9 polynomial through the ten Chebyshev nodes (relative
+// error of 2^f below 2^-50)
+__device__ constexpr double kPow2[10] = {0x1.62e42fefa39f7p-1,  0x1.ebfbdff82c590p-3,  0x1.c6b08d7044119p-5,  0x1.3b2ab6fba385fp-7,
+                                         0x1.5d87fe908f88ap-10, 0x1.4309130378460p-13, 0x1.ffcb76789860fp-17, 0x1.62bfe46117445p-20,
+                                         0x1.b6571de2f2351p-24, 0x1.e5e9f548e5725p-28};
+
 template <typename T>
 struct Row {
-    static constexpr int VEC = 16 / sizeof(T), CHUNK = 64 * VEC;
+    static constexpr int VEC = 16 / sizeof(T), CHUNK = 64 * VEC, U = 4;
+    typedef T vec __attribute__((ext_vector_type(VEC), aligned(16)));
     const T* x;
     int n, shift;  // elements, and those of the first 16-byte vector that lie before the row
     int chunks;
     float m;       // largest logit
-    double inv_t;  // 1 / temperature
+    double rate;   // log2(e) / temperature
 
-    // Chunk c: elements c CHUNK - shift ..., VEC a lane from `first`; absent ones get key 0.
+    // Chunk c: elements c CHUNK - shift ..., VEC a lane from `first`; absent ones are given as NaN.
     __device__ __forceinline__ int first(int c) const { return c * CHUNK + (int)(threadIdx.x & 63) * VEC - shift; }
+    __device__ __forceinline__ bool inside(int c) const { return c * CHUNK >= shift && (c + 1) * CHUNK - shift <= n; }
     __device__ __forceinline__ void load(int at, float* v) const {
-        typedef T vec __attribute__((ext_vector_type(VEC), aligned(16)));
         if (at >= 0 && at + VEC <= n) {
             const vec u = *(const vec*)(x + at);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = to_float(u[e]);
         } else {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = at + e >= 0 && at + e < n ? to_float(x[at + e]) : 0.f;
+            for (int e = 0; e < VEC; ++e) v[e] = at + e >= 0 && at + e < n ? to_float(x[at + e]) : NAN;
         }
     }
-    __device__ __forceinline__ uint32_t key(int i, float v) const { return i >= 0 && i < n ? key_of<T>(v) : 0u; }
+    // f(chunk, first element of the lane, its VEC values) for the wave's chunks, U of them requested at once
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        float v[VEC];
+        for (int c = threadIdx.x >> 6; c < chunks; c += kWaves * U) {
+            if (inside(c) && inside(c + (U - 1) * kWaves)) {
+                vec r[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) r[u] = *(const vec*)(x + first(c + u * kWaves));
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) v[e] = to_float(r[u][e]);
+                    f(c + u * kWaves, first(c + u * kWaves), v);
+                }
+            } else {
+                for (int k = c; k < min(c + kWaves * U, chunks); k += kWaves) {
+                    load(first(k), v);
+                    f(k, first(k), v);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ bool has(int i) const { return (unsigned)i < (unsigned)n; }
+    // round(2^42 2^t), t = (v - m) log2(e) / temperature.  (v - m is exact, and t below -43 rounds to 0, NaN and
+    // absent elements among it; a whole number below 2^52 is what the sum with 2^52 leaves in the mantissa.)
     __device__ __forceinline__ unsigned long long weight(float v) const {
-        if (!(v > -INFINITY)) return 0;
-        if (m == INFINITY) return v == m ? (unsigned long long)kUnit : 0;
-        return (unsigned long long)rint(exp(((double)v - (double)m) * inv_t) * kUnit);
+        if (m == INFINITY) return v == m ? kUnit : 0;
+        const double t = fmax(((double)v - (double)m) * rate, -60.0), i = rint(t), f = t - i;
+        double y = kPow2[9];
+#pragma unroll
+        for (int k = 8; k >= 0; --k) y = fma(y, f, kPow2[k]);
+        y = fma(y, f, 1.0);
+        y = __hiloint2double(__double2hiint(y) + (((int)i + 42) << 20), __double2loint(y)) + 4503599627370496.0;
+        return (unsigned long long)__double_as_longlong(y) & 0xfffffffffffffull;
+    }
+    // the logit of a key
+    __device__ __forceinline__ float value(uint32_t key) const {
+        constexpr int low = 32 - Key<T>::bits;
+        const uint32_t full = key << low;
+        return __uint_as_float(full >> 31 ? full ^ 0x80000000u : ~(full | (low ? (1u << low) - 1 : 0u)));
     }
 };
+
+// One level of a radix search: the bins of `width` bits hold amounts; from the top down, the bin b in which
+// ends(amount above, its own) holds.  False where none does.
+template <typename F>
+__device__ bool find_bin(Shared& sh, int width, unsigned long long above, F ends, unsigned long long& total, uint32_t& bin,
+                         unsigned long long& before, unsigned long long& own) {
+    const int nb = 1 << width, tid = threadIdx.x;
+    unsigned long long h[kBins / kThreads], sum = 0;
+#pragma unroll
+    for (int e = 0; e < kBins / kThreads; ++e) {
+        const int b = nb - 1 - (tid * (kBins / kThreads) + e);
+        h[e] = b >= 0 ? sh.bin[b] : 0;
+        sum += h[e];
+    }
+    if (tid == 0) sh.found[0] = ~0ull;
+    unsigned long long cum = above + block_scan(sh, sum, total);
+#pragma unroll
+    for (int e = 0; e < kBins / kThreads; ++e) {
+        if (ends(cum, h[e])) {  // one bin at most
+            sh.found[0] = (unsigned long long)(nb - 1 - (tid * (kBins / kThreads) + e));
+            sh.found[1] = cum;
+            sh.found[2] = h[e];
+        }
+        cum += h[e];
+    }
+    __syncthreads();
+    bin = (uint32_t)sh.found[0];
+    before = sh.found[1];
+    own = sh.found[2];
+    return sh.found[0] != ~0ull;
+}
+
+__device__ __forceinline__ void clear_bins(Shared& sh, int n) {
+    __syncthreads();
+    for (int b = threadIdx.x; b < n; b += kThreads) sh.bin[b] = 0;
+    __syncthreads();
+}
 
 // Narrows `cut` to the end of a prefix.  COUNT: the first k elements.  Otherwise those before which less
 // than top_p of the weight of `cut` lies (kept as it is if all are).
 template <typename T, bool COUNT>
 __device__ void narrow(Shared& sh, const Row<T>& row, Cut& cut, unsigned long long k, float top_p) {
+    constexpr int VEC = Row<T>::VEC, BITS = Key<T>::bits;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const Cut old = cut;
-    unsigned long long above = 0;  // counted or weighed above the bins searched
+    unsigned long long above = 0, own = 0, total;  // counted or weighed above the bins searched, in the one found
     double thr = 0;
     uint32_t prefix = 0;
-    int shift = Key<T>::bits, width = 0;
-    while (shift > 0) {
-        width = min(shift, 12);
-        const int upper = shift;
+    for (int shift = BITS; shift > 0;) {
+        const int width = min(shift, 12), upper = shift;
         shift -= width;
-        __syncthreads();
-        for (int b = tid; b < (1 << width); b += kThreads) sh.bin[b] = 0;
-        __syncthreads();
-        for (int c = wv; c < row.chunks; c += kWaves) {
-            float v[Row<T>::VEC];
-            const int at = row.first(c);
-            row.load(at, v);
+        clear_bins(sh, 1 << width);
+        row.each([&](int, int at, const float* v) {
 #pragma unroll
-            for (int e = 0; e < Row<T>::VEC; ++e) {
-                const uint32_t kk = row.key(at + e, v[e]);
-                if (kk != 0 && (upper == Key<T>::bits || (kk >> upper) == prefix) && old.keeps(kk, at + e)) {
+            for (int e = 0; e < VEC; ++e) {
+                const uint32_t kk = key_of<T>(v[e]);
+                if ((upper == BITS || (kk >> upper) == prefix) && row.has(at + e) && old.keeps(kk, at + e)) {
                     const unsigned long long w = COUNT ? 1ull : row.weight(v[e]);
                     if (w) atomicAdd(&sh.bin[(kk >> shift) & ((1u << width) - 1)], w);
                 }
             }
-        }
+        });
         __syncthreads();
-        // bins from the top: thread t sums those from 4 t on
-        const int nb = 1 << width;
-        unsigned long long h[4], sum = 0, total;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int b = nb - 1 - (tid * 4 + e);
-            h[e] = b >= 0 ? sh.bin[b] : 0;
-            sum += h[e];
+        const bool top = upper == BITS;
+        if (!COUNT && top) {  // the threshold is a part of the whole
+            unsigned long long s = 0;
+            for (int b = tid; b < (1 << width); b += kThreads) s += sh.bin[b];
+            block_scan(sh, s, total);
+            thr = (double)top_p * (double)total;
+            __syncthreads();
         }
-        unsigned long long cum = above + block_scan(sh, sum, total);
-        if (!COUNT && upper == Key<T>::bits) thr = (double)top_p * (double)total;
-        if (tid == 0) sh.found[0] = ~0ull;
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const bool ends = COUNT ? cum < k && k <= cum + h[e] : (double)cum < thr && !((double)(cum + h[e]) < thr);
-            if (ends) {  // one bin at most
-                sh.found[0] = (unsigned long long)(nb - 1 - (tid * 4 + e));
-                sh.found[1] = cum;
-                sh.found[2] = h[e];
-            }
-            cum += h[e];
-        }
-        __syncthreads();
-        if (sh.found[0] == ~0ull) return;  // everything is kept
-        prefix = (prefix << width) | (uint32_t)sh.found[0];
-        above = sh.found[1];
+        uint32_t bin;
+        auto ends = [&](unsigned long long a, unsigned long long h) {
+            return COUNT ? a < k && k <= a + h : (double)a < thr && !((double)(a + h) < thr);
+        };
+        if (!find_bin(sh, width, above, ends, total, bin, above, own)) return;  // everything is kept
+        prefix = (prefix << width) | bin;
     }
     // equal keys: the first `keep` of them
-    const unsigned long long in_bin = sh.found[2];
     unsigned long long keep, ties;
     if (COUNT) {
-        ties = in_bin;
+        ties = own;
         keep = k - above;
     } else {
-        const uint32_t full = prefix << (32 - Key<T>::bits);
-        const uint32_t u = full >> 31 ? full ^ 0x80000000u : ~(full | (Key<T>::bits < 32 ? (1u << (32 - Key<T>::bits)) - 1 : 0u));
-        const unsigned long long w = row.weight(__uint_as_float(u));
-        ties = in_bin / w;
+        const unsigned long long w = row.weight(row.value(prefix));
+        ties = own / w;
         unsigned long long lo = 1, hi = ties;  // the least number after which the weight is reached
         while (lo < hi) {
             const unsigned long long mid = (lo + hi) >> 1;
@@ -179,21 +257,18 @@ __device__ void narrow(Shared& sh, const Row<T>& row, Cut& cut, unsigned long lo
     cut.idx = prefix == old.key ? old.idx : 0x7fffffff;
     if (keep >= ties) return;
     // the index of the first equal key left out
+    auto tie = [&](float v, int i) { return row.has(i) && key_of<T>(v) == prefix && old.keeps(prefix, i); };
     __syncthreads();
-    for (int c = wv; c < row.chunks; c += kWaves) {
-        float v[Row<T>::VEC];
-        const int at = row.first(c);
-        row.load(at, v);
-        int n = 0;
+    row.each([&](int c, int at, const float* v) {
+        uint32_t n = 0;
 #pragma unroll
-        for (int e = 0; e < Row<T>::VEC; ++e) n += row.key(at + e, v[e]) == prefix && old.keeps(prefix, at + e);
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) n += wave_xor(n, o);
+        for (int e = 0; e < VEC; ++e) n += tie(v[e], at + e);
+        n = wave_sum(n);
         if (lane == 0) sh.bin[c] = n;
-    }
+    });
     __syncthreads();
     const int per = ceil_div(row.chunks, kThreads), c0 = min(tid * per, row.chunks), c1 = min(c0 + per, row.chunks);
-    unsigned long long sum = 0, total;
+    unsigned long long sum = 0;
     for (int c = c0; c < c1; ++c) sum += sh.bin[c];
     unsigned long long cum = block_scan(sh, sum, total);
     for (int c = c0; c < c1; ++c) {
@@ -206,11 +281,11 @@ __device__ void narrow(Shared& sh, const Row<T>& row, Cut& cut, unsigned long lo
     __syncthreads();
     if (wv == 0) {
         const int at = row.first((int)sh.found[0]);
-        float v[Row<T>::VEC];
+        float v[VEC];
         row.load(at, v);
         int n = 0;
 #pragma unroll
-        for (int e = 0; e < Row<T>::VEC; ++e) n += row.key(at + e, v[e]) == prefix && old.keeps(prefix, at + e);
+        for (int e = 0; e < VEC; ++e) n += tie(v[e], at + e);
         int in = n;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -219,8 +294,8 @@ __device__ void narrow(Shared& sh, const Row<T>& row, Cut& cut, unsigned long lo
         }
         int before = (int)sh.found[1] + in - n;
 #pragma unroll
-        for (int e = 0; e < Row<T>::VEC; ++e) {
-            if (row.key(at + e, v[e]) == prefix && old.keeps(prefix, at + e)) {
+        for (int e = 0; e < VEC; ++e) {
+            if (tie(v[e], at + e)) {
                 if ((unsigned long long)before == keep) sh.found[2] = (unsigned long long)(at + e);
                 ++before;
             }
@@ -228,6 +303,93 @@ __device__ void narrow(Shared& sh, const Row<T>& row, Cut& cut, unsigned long lo
     }
     __syncthreads();
     cut.idx = (int)sh.found[2];
+}
+
+// A key that at least k of the threads' largest keys reach, so at least k elements do: the k-th largest of them, of
+// keys over 24 bits to those.  k at most kThreads.
+template <int BITS>
+__device__ uint32_t reached_by(Shared& sh, uint32_t mine, unsigned long long k) {
+    unsigned long long above = 0, own, total;
+    uint32_t prefix = 0;
+    int shift = BITS;
+    for (int level = 0; level < 2 && shift > 0; ++level) {
+        const int width = min(shift, 12), upper = shift;
+        shift -= width;
+        clear_bins(sh, 1 << width);
+        if (upper == BITS || (mine >> upper) == prefix) atomicAdd(&sh.bin[(mine >> shift) & ((1u << width) - 1)], 1ull);
+        __syncthreads();
+        uint32_t bin;
+        find_bin(sh, width, above, [&](unsigned long long a, unsigned long long h) { return a < k && k <= a + h; }, total, bin, above,
+                 own);
+        prefix = (prefix << width) | bin;
+    }
+    return prefix << shift;
+}
+
+// The filters on a list: the elements of keys `least` and more are listed, sorted and cut.  On return sh.bin holds the
+// kept weights a chunk.  False where the list is too short for them.
+template <typename T>
+__device__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut, uint32_t least, int k, float top_p, unsigned long long least_w) {
+    constexpr int VEC = Row<T>::VEC, PER = kList / kThreads;
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    row.each([&](int, int at, const float* v) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const uint32_t kk = key_of<T>(v[e]);
+            if (kk >= least && row.has(at + e)) {
+                const int o = atomicAdd(&sh.count, 1);
+                if (o < kList) sh.list[o] = ((unsigned long long)kk << 32) | (uint32_t)~(at + e);
+            }
+        }
+    });
+    __syncthreads();
+    const int n = sh.count;
+    if (n > kList) return false;
+    int len = 64;
+    while (len < n) len <<= 1;
+    for (int i = n + tid; i < len; i += kThreads) sh.list[i] = 0;
+    // bitonic sort, largest first
+    for (int size = 2; size <= len; size <<= 1)
+        for (int d = size >> 1; d > 0; d >>= 1) {
+            __syncthreads();
+            for (int i = tid; i < len >> 1; i += kThreads) {
+                const int a = ((i & ~(d - 1)) << 1) | (i & (d - 1)), b = a | d;
+                const unsigned long long x = sh.list[a], y = sh.list[b];
+                if ((x < y) == ((a & size) == 0)) {
+                    sh.list[a] = y;
+                    sh.list[b] = x;
+                }
+            }
+        }
+    clear_bins(sh, row.chunks);
+    const int nk = min(n, k);
+    unsigned long long w[PER], sum = 0, total;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int i = tid * PER + e;
+        w[e] = i < nk ? row.weight(row.value((uint32_t)(sh.list[i] >> 32))) : 0;
+        sum += w[e];
+    }
+    unsigned long long before = block_scan(sh, sum, total);
+    const double thr = (double)top_p * (double)total;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int i = tid * PER + e;
+        // (what weighs nothing is never drawn, so that it does not matter where it lies to the cut)
+        if (i < nk && w[e] >= least_w && w[e] > 0 && (i == 0 || top_p >= 1.f || (double)before < thr)) {
+            const int idx = (int)~(uint32_t)sh.list[i];
+            atomicAdd(&sh.bin[(idx + row.shift) / Row<T>::CHUNK], w[e]);
+            atomicMax(&sh.count, n + 1 + i);
+        }
+        before += w[e];
+    }
+    __syncthreads();
+    const unsigned long long last = sh.list[sh.count - n - 1];
+    cut = {(uint32_t)(last >> 32), (int)~(uint32_t)last + 1};
+    return true;
 }
 
 template <typename T>
@@ -244,28 +406,30 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     const float top_p = p.top_p ? p.top_p[r] : p.top_p_all, min_p = p.min_p ? p.min_p[r] : p.min_p_all;
     const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
     // the largest logit and its first index
-    unsigned long long best = 0;
-    for (int c = wv; c < row.chunks; c += kWaves) {
-        float v[VEC];
-        const int at = row.first(c);
-        row.load(at, v);
+    float best = -INFINITY;
+    int best_i = 0;
+    row.each([&](int, int at, const float* v) {
+        float m = v[0];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const uint32_t k = row.key(at + e, v[e]);
-            const unsigned long long o = ((unsigned long long)k << 32) | (uint32_t)~(at + e);
-            if (k && o > best) best = o;
+        for (int e = 1; e < VEC; ++e) m = fmaxf(m, v[e]);
+        if (m > best) {
+            best = m;
+#pragma unroll
+            for (int e = VEC - 1; e >= 0; --e) best_i = v[e] == m ? at + e : best_i;
         }
-    }
+    });
+    const uint32_t own = key_of<T>(best);
+    unsigned long long first = ((unsigned long long)own << 32) | (uint32_t)~best_i;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
-        const unsigned long long b = __shfl_xor(best, o);
-        best = b > best ? b : best;
+        const unsigned long long b = __shfl_xor(first, o);
+        first = b > first ? b : first;
     }
-    if (lane == 0) sh.part[wv] = best;
+    if (lane == 0) sh.part[wv] = first;
     __syncthreads();
-    for (int k = 0; k < kWaves; ++k) best = sh.part[k] > best ? sh.part[k] : best;
-    const uint32_t top = (uint32_t)(best >> 32);
-    const int top_i = (int)~(uint32_t)best;
+    for (int k = 0; k < kWaves; ++k) first = sh.part[k] > first ? sh.part[k] : first;
+    const uint32_t top = __builtin_amdgcn_readfirstlane((uint32_t)(first >> 32));
+    const int top_i = (int)~(uint32_t)first;
     if (top == key_of<T>(-INFINITY)) {  // nothing to draw
         if (tid == 0) {
             p.token[r] = -1;
@@ -273,40 +437,47 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
         }
         return;
     }
-    if (!(temp > 0.f) || top_k == 1) {
+    // the first token alone: greedy, or filters that leave no more (min_p above 1 and NaN among them)
+    if (!(temp > 0.f) || top_k == 1 || !(top_p > 0.f) || !(min_p <= 1.f)) {
         if (tid == 0) {
             p.token[r] = top_i;
             p.logp[r] = 0.f;
         }
         return;
     }
-    row.m = to_float(row.x[top_i]);
-    row.inv_t = 1.0 / (double)temp;
+    row.m = row.value(top);
+    row.rate = 1.4426950408889634 / (double)temp;
+    const unsigned long long least_w = min_p > 0.f ? (unsigned long long)ceil((double)min_p * (double)kUnit) : 0;
     Cut cut = {0u, 0};
-    if (top_k > 0 && top_k < row.n) narrow<T, true>(sh, row, cut, (unsigned long long)top_k, 1.f);
-    if (!(top_p > 0.f)) cut = {top, top_i + 1};
-    else if (top_p < 1.f) narrow<T, false>(sh, row, cut, 0, top_p);
+    const bool filters = (top_k > 0 && top_k < row.n) || top_p < 1.f;
+    bool summed = false;
+    if (row.n <= kList) {
+        if (filters) summed = cut_list(sh, row, cut, 1, top_k > 0 ? top_k : row.n, top_p, least_w);
+    } else if (top_k > 0 && top_k <= kThreads) {
+        const uint32_t least = reached_by<Key<T>::bits>(sh, own, (unsigned long long)top_k);
+        summed = cut_list(sh, row, cut, least, top_k, top_p, least_w);
+    }
+    if (!summed) {
+        if (top_k > 0 && top_k < row.n) narrow<T, true>(sh, row, cut, (unsigned long long)top_k, 1.f);
+        if (top_p < 1.f) narrow<T, false>(sh, row, cut, 0, top_p);
+    }
     // kept weights a chunk, then the chunk, lane and element in which the running sum passes u times the total
-    const double least = (double)min_p * kUnit;
     auto kept = [&](float v, int i) -> unsigned long long {
-        const uint32_t k = row.key(i, v);
-        if (k == 0 || !cut.keeps(k, i)) return 0;
+        if (cut.key && !cut.keeps(key_of<T>(v), i)) return 0;
         const unsigned long long w = row.weight(v);
-        return (double)w >= least || i == top_i ? w : 0;
+        return w >= least_w ? w : 0;
     };
     __syncthreads();
-    for (int c = wv; c < row.chunks; c += kWaves) {
-        float v[VEC];
-        const int at = row.first(c);
-        row.load(at, v);
-        unsigned long long s = 0;
+    if (!summed) {
+        row.each([&](int c, int at, const float* v) {
+            unsigned long long s = 0;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) s += kept(v[e], at + e);
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
-        if (lane == 0) sh.bin[c] = s;
+            for (int e = 0; e < VEC; ++e) s += kept(v[e], at + e);
+            s = wave_sum_weights(s);
+            if (lane == 0) sh.bin[c] = s;
+        });
+        __syncthreads();
     }
-    __syncthreads();
     const int per = ceil_div(row.chunks, kThreads), c0 = min(tid * per, row.chunks), c1 = min(c0 + per, row.chunks);
     unsigned long long sum = 0, total;
     for (int c = c0; c < c1; ++c) sum += sh.bin[c];
@@ -331,7 +502,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
         row.load(at, v);
         unsigned long long w[VEC], s = 0;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) s += w[e] = kept(v[e], at + e);
+        for (int e = 0; e < VEC; ++e) s += w[e] = row.has(at + e) ? kept(v[e], at + e) : 0;
         unsigned long long in = s;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
