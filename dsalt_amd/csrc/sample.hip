@@ -87,20 +87,27 @@ __device__ __forceinline__ unsigned long long wave_sum_weights(unsigned long lon
     return ((unsigned long long)wave_sum((uint32_t)(v >> 25)) << 25) + wave_sum((uint32_t)v & 0x1ffffffu);
 }
 
-// 2^f - 1 = f P(f) for f in [-1/2, 1/2], P the degree 9 polynomial through the ten Chebyshev nodes (relative
+// 2^42 (2^f - 1) = f P(f) for f in [-1/2, 1/2], P the degree 9 polynomial through the ten Chebyshev nodes (relative
 // error of 2^f below 2^-50)
-__device__ constexpr double kPow2[10] = {0x1.62e42fefa39f7p-1,  0x1.ebfbdff82c590p-3,  0x1.c6b08d7044119p-5,  0x1.3b2ab6fba385fp-7,
-                                         0x1.5d87fe908f88ap-10, 0x1.4309130378460p-13, 0x1.ffcb76789860fp-17, 0x1.62bfe46117445p-20,
-                                         0x1.b6571de2f2351p-24, 0x1.e5e9f548e5725p-28};
+__device__ constexpr double kPow2[10] = {0x1.62e42fefa39f7p41, 0x1.ebfbdff82c590p39, 0x1.c6b08d7044119p37, 0x1.3b2ab6fba385fp35,
+                                         0x1.5d87fe908f88ap32, 0x1.4309130378460p29, 0x1.ffcb76789860fp25, 0x1.62bfe46117445p22,
+                                         0x1.b6571de2f2351p18, 0x1.e5e9f548e5725p14};
+
+// x f + c with c in scalar registers (from vector registers it would be copied before each sum)
+__device__ __forceinline__ double fma_s(double x, double f, double c) {
+    double y;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(y) : "v"(x), "v"(f), "s"(c));
+    return y;
+}
 
 template <typename T>
 struct Row {
-    static constexpr int VEC = 16 / sizeof(T), CHUNK = 64 * VEC, U = 4;
+    static constexpr int VEC = 16 / sizeof(T), CHUNK = 64 * VEC;
     typedef T vec __attribute__((ext_vector_type(VEC), aligned(16)));
     const T* x;
     int n, shift;  // elements, and those of the first 16-byte vector that lie before the row
     int chunks;
-    float m;       // largest logit
+    double m;      // largest logit (beside infinity 1e39, above every other)
     double rate;   // log2(e) / temperature
 
     // Chunk c: elements c CHUNK - shift ..., VEC a lane from `first`; absent ones are given as NaN.
@@ -116,40 +123,68 @@ struct Row {
             for (int e = 0; e < VEC; ++e) v[e] = at + e >= 0 && at + e < n ? to_float(x[at + e]) : NAN;
         }
     }
-    // f(chunk, first element of the lane, its VEC values) for the wave's chunks, U of them requested at once
+    // f(chunk, first element of the lane, its VEC values) for the wave's chunks, three of them requested ahead
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
-        float v[VEC];
-        for (int c = threadIdx.x >> 6; c < chunks; c += kWaves * U) {
-            if (inside(c) && inside(c + (U - 1) * kWaves)) {
-                vec r[U];
+        auto fetch = [&](int c) {
+            vec u = {};
+            if (inside(c)) u = *(const vec*)(x + first(c));
+            return u;
+        };
+        int c = threadIdx.x >> 6;
+        vec r0 = fetch(c), r1 = fetch(c + kWaves), r2 = fetch(c + 2 * kWaves);
+        for (; c < chunks; c += kWaves) {
+            float v[VEC];
 #pragma unroll
-                for (int u = 0; u < U; ++u) r[u] = *(const vec*)(x + first(c + u * kWaves));
+            for (int e = 0; e < VEC; ++e) v[e] = to_float(r0[e]);
+            if (!inside(c)) load(first(c), v);
+            r0 = r1;
+            r1 = r2;
+            r2 = fetch(c + 3 * kWaves);
+            f(c, first(c), v);
+        }
+    }
+    // the same for passes of few instructions, which wait for memory: eight chunks requested ahead
+    template <typename F>
+    __device__ __forceinline__ void skim(F f) const {
+        constexpr int N = 4;
+        auto fetch = [&](int c, vec* r) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
+            for (int k = 0; k < N; ++k) {
+                r[k] = vec{};
+                if (inside(c + k * kWaves)) r[k] = *(const vec*)(x + first(c + k * kWaves));
+            }
+        };
+        int c = threadIdx.x >> 6;
+        vec r[N], next[N];
+        fetch(c, r);
+        for (; c < chunks; c += N * kWaves) {
+            fetch(c + N * kWaves, next);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) v[e] = to_float(r[u][e]);
-                    f(c + u * kWaves, first(c + u * kWaves), v);
+            for (int k = 0; k < N; ++k) {
+                const int ck = c + k * kWaves;
+                if (ck < chunks) {
+                    float v[VEC];
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) v[e] = to_float(r[k][e]);
+                    if (!inside(ck)) load(first(ck), v);
+                    f(ck, first(ck), v);
                 }
-            } else {
-                for (int k = c; k < min(c + kWaves * U, chunks); k += kWaves) {
-                    load(first(k), v);
-                    f(k, first(k), v);
-                }
+                r[k] = next[k];
             }
         }
     }
     __device__ __forceinline__ bool has(int i) const { return (unsigned)i < (unsigned)n; }
     // round(2^42 2^t), t = (v - m) log2(e) / temperature.  (v - m is exact, and t below -43 rounds to 0, NaN and
-    // absent elements among it; a whole number below 2^52 is what the sum with 2^52 leaves in the mantissa.)
+    // absent elements among it.  Sums with 1.5 2^52 and 2^52 round to a whole number and leave it in the mantissa.)
     __device__ __forceinline__ unsigned long long weight(float v) const {
-        if (m == INFINITY) return v == m ? kUnit : 0;
-        const double t = fmax(((double)v - (double)m) * rate, -60.0), i = rint(t), f = t - i;
+        const double t = fmin(fmax(((double)v - m) * rate, -60.0), 0.0), s = t + 6755399441055744.0;
+        const double f = t - (s - 6755399441055744.0);
         double y = kPow2[9];
 #pragma unroll
-        for (int k = 8; k >= 0; --k) y = fma(y, f, kPow2[k]);
-        y = fma(y, f, 1.0);
-        y = __hiloint2double(__double2hiint(y) + (((int)i + 42) << 20), __double2loint(y)) + 4503599627370496.0;
+        for (int k = 8; k >= 0; --k) y = fma_s(y, f, kPow2[k]);
+        y = fma_s(y, f, 0x1p42);
+        y = __hiloint2double(__double2hiint(y) + (__double2loint(s) << 20), __double2loint(y)) + 4503599627370496.0;
         return (unsigned long long)__double_as_longlong(y) & 0xfffffffffffffull;
     }
     // the logit of a key
@@ -335,35 +370,48 @@ __device__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut, uint32_t least
     __syncthreads();
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    row.each([&](int, int at, const float* v) {
+    const float low = row.value(least);
+    row.skim([&](int, int at, const float* v) {
+        float m = v[0];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const uint32_t kk = key_of<T>(v[e]);
-            if (kk >= least && row.has(at + e)) {
-                const int o = atomicAdd(&sh.count, 1);
-                if (o < kList) sh.list[o] = ((unsigned long long)kk << 32) | (uint32_t)~(at + e);
-            }
+        for (int e = 1; e < VEC; ++e) m = fmaxf(m, v[e]);
+        if (m >= low) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (v[e] >= low) {  // (NaN and absent elements are not)
+                    const int o = atomicAdd(&sh.count, 1);
+                    if (o < kList) sh.list[o] = ((unsigned long long)key_of<T>(v[e]) << 32) | (uint32_t)~(at + e);
+                }
         }
     });
     __syncthreads();
     const int n = sh.count;
     if (n > kList) return false;
-    int len = 64;
-    while (len < n) len <<= 1;
-    for (int i = n + tid; i < len; i += kThreads) sh.list[i] = 0;
-    // bitonic sort, largest first
-    for (int size = 2; size <= len; size <<= 1)
-        for (int d = size >> 1; d > 0; d >>= 1) {
-            __syncthreads();
-            for (int i = tid; i < len >> 1; i += kThreads) {
-                const int a = ((i & ~(d - 1)) << 1) | (i & (d - 1)), b = a | d;
-                const unsigned long long x = sh.list[a], y = sh.list[b];
-                if ((x < y) == ((a & size) == 0)) {
-                    sh.list[a] = y;
-                    sh.list[b] = x;
+    // sorted, largest first: few by counting those above each, more by a bitonic sort
+    if (n <= kThreads / 2) {
+        const unsigned long long mine = tid < n ? sh.list[tid] : 0;
+        int above = 0;
+        if (tid < n)
+            for (int i = 0; i < n; ++i) above += sh.list[i] > mine;
+        __syncthreads();
+        if (tid < n) sh.list[above] = mine;
+    } else {
+        int len = kThreads;
+        while (len < n) len <<= 1;
+        for (int i = n + tid; i < len; i += kThreads) sh.list[i] = 0;
+        for (int size = 2; size <= len; size <<= 1)
+            for (int d = size >> 1; d > 0; d >>= 1) {
+                __syncthreads();
+                for (int i = tid; i < len >> 1; i += kThreads) {
+                    const int a = ((i & ~(d - 1)) << 1) | (i & (d - 1)), b = a | d;
+                    const unsigned long long x = sh.list[a], y = sh.list[b];
+                    if ((x < y) == ((a & size) == 0)) {
+                        sh.list[a] = y;
+                        sh.list[b] = x;
+                    }
                 }
             }
-        }
+    }
     clear_bins(sh, row.chunks);
     const int nk = min(n, k);
     unsigned long long w[PER], sum = 0, total;
@@ -408,7 +456,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     // the largest logit and its first index
     float best = -INFINITY;
     int best_i = 0;
-    row.each([&](int, int at, const float* v) {
+    row.skim([&](int, int at, const float* v) {
         float m = v[0];
 #pragma unroll
         for (int e = 1; e < VEC; ++e) m = fmaxf(m, v[e]);
@@ -445,17 +493,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
         }
         return;
     }
-    row.m = row.value(top);
-    row.rate = 1.4426950408889634 / (double)temp;
+    const bool inf = row.value(top) == INFINITY;
+    row.m = inf ? 1e39 : (double)row.value(top);
+    row.rate = inf ? 1.0 : 1.4426950408889634 / (double)temp;
     const unsigned long long least_w = min_p > 0.f ? (unsigned long long)ceil((double)min_p * (double)kUnit) : 0;
     Cut cut = {0u, 0};
     const bool filters = (top_k > 0 && top_k < row.n) || top_p < 1.f;
     bool summed = false;
-    if (row.n <= kList) {
-        if (filters) summed = cut_list(sh, row, cut, 1, top_k > 0 ? top_k : row.n, top_p, least_w);
-    } else if (top_k > 0 && top_k <= kThreads) {
-        const uint32_t least = reached_by<Key<T>::bits>(sh, own, (unsigned long long)top_k);
-        summed = cut_list(sh, row, cut, least, top_k, top_p, least_w);
+    if (filters && (row.n <= kList || (top_k > 0 && top_k <= kThreads))) {
+        uint32_t least = key_of<T>(-INFINITY);
+        if (top_k > 0 && top_k <= kThreads) least = max(least, reached_by<Key<T>::bits>(sh, own, (unsigned long long)top_k));
+        summed = cut_list(sh, row, cut, least, top_k > 0 ? top_k : row.n, top_p, least_w);
     }
     if (!summed) {
         if (top_k > 0 && top_k < row.n) narrow<T, true>(sh, row, cut, (unsigned long long)top_k, 1.f);
@@ -469,13 +517,20 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     };
     __syncthreads();
     if (!summed) {
-        row.each([&](int c, int at, const float* v) {
-            unsigned long long s = 0;
+        auto sums = [&](auto of) {
+            row.each([&](int c, int at, const float* v) {
+                unsigned long long s = 0;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s += kept(v[e], at + e);
-            s = wave_sum_weights(s);
-            if (lane == 0) sh.bin[c] = s;
+                for (int e = 0; e < VEC; ++e) s += of(v[e], at + e);
+                s = wave_sum_weights(s);
+                if (lane == 0) sh.bin[c] = s;
+            });
+        };
+        if (cut.key == 0) sums([&](float v, int) {
+            const unsigned long long w = row.weight(v);
+            return w >= least_w ? w : 0;
         });
+        else sums(kept);
         __syncthreads();
     }
     const int per = ceil_div(row.chunks, kThreads), c0 = min(tid * per, row.chunks), c1 = min(c0 + per, row.chunks);
@@ -509,14 +564,19 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
             const unsigned long long o = __shfl_up(in, d);
             if (lane >= d) in += o;
         }
-        unsigned long long before = sh.found[1] + in - s;
+        unsigned long long before = sh.found[1] + in - s, weighs = 0;
+        int drawn = -1;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             if (!((double)before > goal) && (double)(before + w[e]) > goal) {
-                p.token[r] = at + e;
-                p.logp[r] = (float)log((double)w[e] / (double)total);
+                drawn = at + e;
+                weighs = w[e];
             }
             before += w[e];
+        }
+        if (drawn >= 0) {  // one lane
+            p.token[r] = drawn;
+            p.logp[r] = (float)log((double)weighs / (double)total);
         }
     }
 }
