@@ -198,7 +198,7 @@ struct Row {
 // One level of a radix search: the bins of `width` bits hold amounts; from the top down, the bin b in which
 // ends(amount above, its own) holds.  False where none does.
 template <typename F>
-__device__ bool find_bin(Shared& sh, int width, unsigned long long above, F ends, unsigned long long& total, uint32_t& bin,
+__device__ __forceinline__ bool find_bin(Shared& sh, int width, unsigned long long above, F ends, unsigned long long& total, uint32_t& bin,
                          unsigned long long& before, unsigned long long& own) {
     const int nb = 1 << width, tid = threadIdx.x;
     unsigned long long h[kBins / kThreads], sum = 0;
@@ -232,69 +232,30 @@ __device__ __forceinline__ void clear_bins(Shared& sh, int n) {
     __syncthreads();
 }
 
-// Narrows `cut` to the end of a prefix.  COUNT: the first k elements.  Otherwise those before which less
-// than top_p of the weight of `cut` lies (kept as it is if all are).
-template <typename T, bool COUNT>
-__device__ void narrow(Shared& sh, const Row<T>& row, Cut& cut, unsigned long long k, float top_p) {
-    constexpr int VEC = Row<T>::VEC, BITS = Key<T>::bits;
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+// the least number, of at most n, of weights w after which a weight of thr is reached
+__device__ __forceinline__ unsigned long long reach(unsigned long long above, unsigned long long w, unsigned long long n, double thr) {
+    unsigned long long lo = 1, hi = n;
+    while (lo < hi) {
+        const unsigned long long mid = (lo + hi) >> 1;
+        if ((double)(above + mid * w) < thr) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// `cut` moved up to the first `keep` of its `ties` elements of key `prefix`
+template <typename T>
+__device__ __forceinline__ void keep_equal(Shared& sh, const Row<T>& row, Cut& cut, uint32_t prefix, unsigned long long keep, unsigned long long ties) {
+    constexpr int VEC = Row<T>::VEC;
     const Cut old = cut;
-    unsigned long long above = 0, own = 0, total;  // counted or weighed above the bins searched, in the one found
-    double thr = 0;
-    uint32_t prefix = 0;
-    for (int shift = BITS; shift > 0;) {
-        const int width = min(shift, 12), upper = shift;
-        shift -= width;
-        clear_bins(sh, 1 << width);
-        row.each([&](int, int at, const float* v) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const uint32_t kk = key_of<T>(v[e]);
-                if ((upper == BITS || (kk >> upper) == prefix) && row.has(at + e) && old.keeps(kk, at + e)) {
-                    const unsigned long long w = COUNT ? 1ull : row.weight(v[e]);
-                    if (w) atomicAdd(&sh.bin[(kk >> shift) & ((1u << width) - 1)], w);
-                }
-            }
-        });
-        __syncthreads();
-        const bool top = upper == BITS;
-        if (!COUNT && top) {  // the threshold is a part of the whole
-            unsigned long long s = 0;
-            for (int b = tid; b < (1 << width); b += kThreads) s += sh.bin[b];
-            block_scan(sh, s, total);
-            thr = (double)top_p * (double)total;
-            __syncthreads();
-        }
-        uint32_t bin;
-        auto ends = [&](unsigned long long a, unsigned long long h) {
-            return COUNT ? a < k && k <= a + h : (double)a < thr && !((double)(a + h) < thr);
-        };
-        if (!find_bin(sh, width, above, ends, total, bin, above, own)) return;  // everything is kept
-        prefix = (prefix << width) | bin;
-    }
-    // equal keys: the first `keep` of them
-    unsigned long long keep, ties;
-    if (COUNT) {
-        ties = own;
-        keep = k - above;
-    } else {
-        const unsigned long long w = row.weight(row.value(prefix));
-        ties = own / w;
-        unsigned long long lo = 1, hi = ties;  // the least number after which the weight is reached
-        while (lo < hi) {
-            const unsigned long long mid = (lo + hi) >> 1;
-            if ((double)(above + mid * w) < thr) lo = mid + 1;
-            else hi = mid;
-        }
-        keep = lo;
-    }
     cut.key = prefix;
     cut.idx = prefix == old.key ? old.idx : 0x7fffffff;
     if (keep >= ties) return;
-    // the index of the first equal key left out
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    // the index of the first one left out
     auto tie = [&](float v, int i) { return row.has(i) && key_of<T>(v) == prefix && old.keeps(prefix, i); };
     __syncthreads();
-    row.each([&](int c, int at, const float* v) {
+    row.skim([&](int c, int at, const float* v) {
         uint32_t n = 0;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) n += tie(v[e], at + e);
@@ -303,7 +264,7 @@ __device__ void narrow(Shared& sh, const Row<T>& row, Cut& cut, unsigned long lo
     });
     __syncthreads();
     const int per = ceil_div(row.chunks, kThreads), c0 = min(tid * per, row.chunks), c1 = min(c0 + per, row.chunks);
-    unsigned long long sum = 0;
+    unsigned long long sum = 0, total;
     for (int c = c0; c < c1; ++c) sum += sh.bin[c];
     unsigned long long cum = block_scan(sh, sum, total);
     for (int c = c0; c < c1; ++c) {
@@ -340,10 +301,63 @@ __device__ void narrow(Shared& sh, const Row<T>& row, Cut& cut, unsigned long lo
     cut.idx = (int)sh.found[2];
 }
 
+// Narrows `cut` to the end of a prefix.  `counts`: the first k elements.  Otherwise those before which less
+// than top_p of the weight of `cut` lies (kept as it is if all are).
+template <typename T>
+__device__ __forceinline__ void narrow(Shared& sh, const Row<T>& row, Cut& cut, bool counts, unsigned long long k, float top_p) {
+    constexpr int VEC = Row<T>::VEC, BITS = Key<T>::bits;
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const Cut old = cut;
+    unsigned long long above = 0, own = 0, total;  // counted or weighed above the bins searched, in the one found
+    double thr = 0;
+    uint32_t prefix = 0;
+    for (int shift = BITS; shift > 0;) {
+        const int width = min(shift, 12), upper = shift;
+        shift -= width;
+        clear_bins(sh, 1 << width);
+        row.each([&](int, int at, const float* v) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const uint32_t kk = key_of<T>(v[e]);
+                if ((upper == BITS || (kk >> upper) == prefix) && row.has(at + e) && old.keeps(kk, at + e)) {
+                    const unsigned long long w = counts ? 1ull : row.weight(v[e]);
+                    if (w) atomicAdd(&sh.bin[(kk >> shift) & ((1u << width) - 1)], w);
+                }
+            }
+        });
+        __syncthreads();
+        const bool top = upper == BITS;
+        if (!counts && top) {  // the threshold is a part of the whole
+            unsigned long long s = 0;
+            for (int b = tid; b < (1 << width); b += kThreads) s += sh.bin[b];
+            block_scan(sh, s, total);
+            thr = (double)top_p * (double)total;
+            __syncthreads();
+        }
+        uint32_t bin;
+        auto ends = [&](unsigned long long a, unsigned long long h) {
+            return counts ? a < k && k <= a + h : (double)a < thr && !((double)(a + h) < thr);
+        };
+        if (!find_bin(sh, width, above, ends, total, bin, above, own)) return;  // everything is kept
+        prefix = (prefix << width) | bin;
+    }
+    // equal keys: the first `keep` of them
+    unsigned long long keep, ties;
+    if (counts) {
+        ties = own;
+        keep = k - above;
+    } else {
+        const unsigned long long w = row.weight(row.value(prefix));
+        ties = own / w;
+        keep = reach(above, w, ties, thr);
+    }
+    keep_equal(sh, row, cut, prefix, keep, ties);
+}
+
 // A key that at least k of the threads' largest keys reach, so at least k elements do: the k-th largest of them, of
 // keys over 24 bits to those.  k at most kThreads.
 template <int BITS>
-__device__ uint32_t reached_by(Shared& sh, uint32_t mine, unsigned long long k) {
+__device__ __forceinline__ uint32_t reached_by(Shared& sh, uint32_t mine, unsigned long long k) {
     unsigned long long above = 0, own, total;
     uint32_t prefix = 0;
     int shift = BITS;
@@ -364,7 +378,7 @@ __device__ uint32_t reached_by(Shared& sh, uint32_t mine, unsigned long long k) 
 // The filters on a list: the elements of keys `least` and more are listed, sorted and cut.  On return sh.bin holds the
 // kept weights a chunk.  False where the list is too short for them.
 template <typename T>
-__device__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut, uint32_t least, int k, float top_p, unsigned long long least_w) {
+__device__ __forceinline__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut, uint32_t least, int k, float top_p, unsigned long long least_w) {
     constexpr int VEC = Row<T>::VEC, PER = kList / kThreads;
     const int tid = threadIdx.x;
     __syncthreads();
@@ -387,14 +401,22 @@ __device__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut, uint32_t least
     __syncthreads();
     const int n = sh.count;
     if (n > kList) return false;
-    // sorted, largest first: few by counting those above each, more by a bitonic sort
+    // sorted, largest first: few by counting those above each (threads side by side over parts of the list), more by a
+    // bitonic sort
     if (n <= kThreads / 2) {
-        const unsigned long long mine = tid < n ? sh.list[tid] : 0;
-        int above = 0;
-        if (tid < n)
-            for (int i = 0; i < n; ++i) above += sh.list[i] > mine;
+        int* rank = (int*)sh.bin;
+        int len = 64;
+        while (len < n) len <<= 1;
+        const int i = tid & (len - 1), parts = kThreads / len, per = ceil_div(n, parts), j0 = tid / len * per;
+        if (tid < len) rank[tid] = 0;
+        const unsigned long long mine = i < n ? sh.list[i] : 0;
         __syncthreads();
-        if (tid < n) sh.list[above] = mine;
+        int above = 0;
+        for (int j = j0; j < min(j0 + per, n); ++j) above += sh.list[j] > mine;
+        if (above) atomicAdd(&rank[i], above);
+        __syncthreads();
+        const int at = i < n && tid < len ? rank[i] : -1;
+        if (at >= 0) sh.list[at] = mine;
     } else {
         int len = kThreads;
         while (len < n) len <<= 1;
@@ -440,9 +462,141 @@ __device__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut, uint32_t least
     return true;
 }
 
+// Weights of bfloat16 logits by value: few values lie between the largest logit and where weights round to 0, so each is
+// formed once (an element then costs a look-up, about a third of its polynomial).  Entries are the keys kmin ..
+// zlo - 1, then zhi + 1 .. kmax; the keys between, magnitudes too small for kEntries to hold (zeros always), are
+// weighed directly.
+constexpr int kEntries = 4094, kTableCols = 8192;
+
+struct Table {
+    unsigned long long* w;  // entries, then a 0
+    uint32_t kmin, zlo, zhi, high;  // entry of key k: k - kmin below the zone, k - high above it
+    int n, below;                   // entries, those below the zone
+
+    // the table of a row whose largest key is kmax; weights are 0 below the logit `low`
+    __device__ __forceinline__ Table(unsigned long long* lds, const Row<bf16>& row, uint32_t kmax, float low) : w(lds) {
+        kmin = low > -3e38f ? max(plain_key(low) - 1, 0x80u) : 0x80u;
+        const int am = (int)kmax - 0x8000, al = 0x7fff - (int)kmin;  // largest magnitudes (below 0: none)
+        const int m = max(am, -1), l = max(al, -1);
+        int a0 = (m + l + 3 - kEntries) >> 1;
+        if (a0 > min(m, l) + 1) a0 = max(m, l) + 1 - kEntries;
+        a0 = max(a0, 1);
+        zlo = 0x8000u - a0;
+        zhi = 0x8000u + a0 - 1;
+        below = max((int)min(zlo, kmax + 1) - (int)kmin, 0);
+        const uint32_t p0 = max(zhi + 1, kmin);
+        high = p0 - below;
+        n = below + max((int)kmax - (int)p0 + 1, 0);
+        __syncthreads();
+        for (int i = threadIdx.x; i <= n; i += kThreads) w[i] = i < n ? row.weight(row.value(key(i))) : 0;
+        __syncthreads();
+    }
+    __device__ __forceinline__ static uint32_t plain_key(float v) {  // as key_of but for zeros and NaN
+        const uint32_t u = __float_as_uint(v);
+        return (u ^ ((uint32_t)((int)u >> 31) | 0x80000000u)) >> 16;
+    }
+    __device__ __forceinline__ uint32_t key(int i) const { return (uint32_t)i + (i < below ? kmin : high); }
+    __device__ __forceinline__ bool in_zone(uint32_t k) const { return k - zlo <= zhi - zlo; }
+    // the entry of a key outside the zone, n where there is none (and NaN)
+    __device__ __forceinline__ int entry(uint32_t k) const { return (int)min(k - (k > zhi ? high : kmin), (uint32_t)n); }
+};
+
+// The filters from counts of each entry (no list, or more than it holds).  False where a prefix ends among
+// the keys that have none.
+__device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, const Table& tab, Cut& cut, int top_k, float top_p) {
+    constexpr int PER = (kEntries + 2) / kThreads;
+    uint32_t* count = (uint32_t*)sh.list;
+    unsigned long long* zone = sh.bin;  // elements and weight of the zone
+    const int tid = threadIdx.x;
+    __syncthreads();
+    for (int i = tid; i < kEntries + 2; i += kThreads) count[i] = 0;
+    if (tid < 2) zone[tid] = 0;
+    __syncthreads();
+    row.skim([&](int, int at, const float* v) {
+#pragma unroll
+        for (int e = 0; e < Row<bf16>::VEC; ++e) {
+            const uint32_t k = Table::plain_key(v[e]);
+            if (tab.in_zone(k)) {
+                const unsigned long long w = row.weight(v[e]);
+                atomicAdd(&zone[0], 1ull);
+                atomicAdd(&zone[1], w);
+            } else {
+                const int i = tab.entry(k);
+                if (i < tab.n) atomicAdd(&count[i], 1u);
+            }
+        }
+    });
+    __syncthreads();
+    const unsigned long long zn = zone[0], zw = zone[1];
+    // a thread's entries from the largest key down, what lies above them, and of how many
+    unsigned long long c[PER], w[PER], ca, wa, cn = 0, wn = 0, call, wall;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+        const int i = tab.n - 1 - (tid * PER + e);
+        c[e] = i >= 0 ? count[i] : 0;
+        w[e] = i >= 0 ? tab.w[i] : 0;
+        cn += c[e];
+        wn += c[e] * w[e];
+    }
+    ca = block_scan(sh, cn, call);
+    wa = block_scan(sh, wn, wall);
+    call += zn;
+    wall += zw;
+    auto search = [&](auto ends) {  // the entry in which ends(counted above, weighed above, its count, its weight) holds
+        if (tid == 0) sh.found[0] = ~0ull;
+        __syncthreads();
+        unsigned long long cc = ca, ww = wa;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+            const int i = tab.n - 1 - (tid * PER + e);
+            const unsigned long long c0 = cc + (i < tab.below ? zn : 0), w0 = ww + (i < tab.below ? zw : 0);
+            if (i >= 0 && ends(c0, w0, c[e], w[e])) {
+                sh.found[0] = (unsigned long long)i;
+                sh.found[1] = c0;
+                sh.found[2] = w0;
+                sh.found[3] = c[e];
+            }
+            cc += c[e];
+            ww += c[e] * w[e];
+        }
+        __syncthreads();
+        return sh.found[0] != ~0ull;
+    };
+    int end = -1;  // the entry that is cut, how many of it are kept, of how many
+    unsigned long long keep = 0, ties = 0, whole = wall;
+    if (top_k > 0 && (unsigned long long)top_k < call) {
+        const unsigned long long k = (unsigned long long)top_k;
+        if (!search([&](unsigned long long c0, unsigned long long, unsigned long long n, unsigned long long) { return c0 < k && k <= c0 + n; }))
+            return false;
+        end = (int)sh.found[0];
+        keep = k - sh.found[1];
+        ties = sh.found[3];
+        whole = sh.found[2] + keep * tab.w[end];
+        __syncthreads();
+    }
+    if (top_p < 1.f) {
+        const double thr = (double)top_p * (double)whole;
+        if (search([&](unsigned long long, unsigned long long w0, unsigned long long n, unsigned long long w) {
+                return (double)w0 < thr && !((double)(w0 + n * w) < thr);
+            })) {
+            const int i = (int)sh.found[0];
+            const unsigned long long r = reach(sh.found[2], tab.w[i], sh.found[3], thr);
+            keep = i == end && keep < r ? keep : r;
+            end = i;
+            ties = sh.found[3];
+        } else if (!((double)wall < thr)) {
+            return false;
+        }
+        __syncthreads();
+    }
+    if (end >= 0) keep_equal(sh, row, cut, tab.key(end), keep, ties);
+    return true;
+}
+
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     __shared__ Shared sh;
+    extern __shared__ unsigned long long dyn[];  // bfloat16: the table
     constexpr int VEC = Row<T>::VEC;
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     Row<T> row;
@@ -505,18 +659,40 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
         if (top_k > 0 && top_k <= kThreads) least = max(least, reached_by<Key<T>::bits>(sh, own, (unsigned long long)top_k));
         summed = cut_list(sh, row, cut, least, top_k > 0 ? top_k : row.n, top_p, least_w);
     }
-    if (!summed) {
-        if (top_k > 0 && top_k < row.n) narrow<T, true>(sh, row, cut, (unsigned long long)top_k, 1.f);
-        if (top_p < 1.f) narrow<T, false>(sh, row, cut, 0, top_p);
-    }
     // kept weights a chunk, then the chunk, lane and element in which the running sum passes u times the total
     auto kept = [&](float v, int i) -> unsigned long long {
         if (cut.key && !cut.keeps(key_of<T>(v), i)) return 0;
         const unsigned long long w = row.weight(v);
         return w >= least_w ? w : 0;
     };
-    __syncthreads();
+    if constexpr (Key<T>::bits == 16) {
+        if (!summed && row.n >= kTableCols && !inf) {
+            const Table tab(dyn, row, top, row.value(top) - 30.f * temp);
+            summed = !filters || cut_table(sh, row, tab, cut, top_k, top_p);
+            __syncthreads();
+            if (summed)
+                row.skim([&](int c, int at, const float* v) {
+                    unsigned long long s = 0;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const uint32_t k = Table::plain_key(v[e]);
+                        const bool zone = tab.in_zone(k);
+                        unsigned long long w = tab.w[zone ? tab.n : tab.entry(k)];
+                        if (cut.key && !cut.keeps(k, at + e)) w = 0;
+                        if (zone) w = kept(v[e], at + e);
+                        s += w >= least_w ? w : 0;
+                    }
+                    s = wave_sum_weights(s);
+                    if (lane == 0) sh.bin[c] = s;
+                });
+        }
+    }
     if (!summed) {
+#pragma unroll 1
+        for (int by_weight = 0; by_weight < 2; ++by_weight)
+            if (by_weight ? top_p < 1.f : top_k > 0 && top_k < row.n)
+                narrow(sh, row, cut, !by_weight, (unsigned long long)top_k, top_p);
+        __syncthreads();
         auto sums = [&](auto of) {
             row.each([&](int c, int at, const float* v) {
                 unsigned long long s = 0;
@@ -531,8 +707,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
             return w >= least_w ? w : 0;
         });
         else sums(kept);
-        __syncthreads();
     }
+    __syncthreads();
     const int per = ceil_div(row.chunks, kThreads), c0 = min(tid * per, row.chunks), c1 = min(c0 + per, row.chunks);
     unsigned long long sum = 0, total;
     for (int c = c0; c < c1; ++c) sum += sh.bin[c];
@@ -588,7 +764,14 @@ hipError_t sample_launch(const SampleParams& p, hipStream_t stream) {
     const dim3 grid((unsigned)p.rows);
     switch (p.dtype) {
         case 0: DSALT_LAUNCH("sample", sample_kernel<float>, grid, dim3(kThreads), 0, stream, p); break;
-        case 1: DSALT_LAUNCH("sample", sample_kernel<bf16>, grid, dim3(kThreads), 0, stream, p); break;
+        case 1: {
+            const unsigned lds = p.n_cols >= kTableCols ? (kEntries + 2) * sizeof(unsigned long long) : 0;
+            if (lds)
+                if (hipError_t e = hipFuncSetAttribute((const void*)sample_kernel<bf16>, hipFuncAttributeMaxDynamicSharedMemorySize, lds))
+                    return e;
+            DSALT_LAUNCH("sample", sample_kernel<bf16>, grid, dim3(kThreads), lds, stream, p);
+            break;
+        }
         default: DSALT_LAUNCH("sample", sample_kernel<f16>, grid, dim3(kThreads), 0, stream, p); break;
     }
     return hipGetLastError();
