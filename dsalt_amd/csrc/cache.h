@@ -62,7 +62,7 @@ struct CacheAttnParams {
     size_t ws_bytes;
 };
 
-size_t cache_rows_ws_bytes(int n_reqs);
+size_t cache_rows_ws_bytes(int n_reqs, int cols);
 hipError_t cache_rows_launch(const CacheRowsParams& p, hipStream_t stream);
 hipError_t cache_write_launch(const CacheWriteParams& p, hipStream_t stream);
 hipError_t cache_read_launch(const CacheReadParams& p, hipStream_t stream);

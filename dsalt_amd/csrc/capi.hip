@@ -818,7 +818,7 @@ int dsalt_layer_selectors(const dsalt_selectors_args* a, dsalt_stream_t stream) 
 }
 
 size_t dsalt_cache_rows_workspace_bytes(const dsalt_cache_rows_args* a) {
-    return a && a->n_reqs >= 1 ? dsalt::cache_rows_ws_bytes(a->n_reqs) : 0;
+    return a && a->n_reqs >= 1 ? dsalt::cache_rows_ws_bytes(a->n_reqs, a->table_cols) : 0;
 }
 
 int dsalt_cache_rows(const dsalt_cache_rows_args* a, dsalt_stream_t stream) {
@@ -838,8 +838,9 @@ int dsalt_cache_rows(const dsalt_cache_rows_args* a, dsalt_stream_t stream) {
         return fail(DSALT_ERR_INVALID, "req, pos, slot and pieces (16-byte aligned) are required");
     if (a->seq_out == a->seq_len || a->span_out == a->span || a->seq_out == a->new_len)
         return fail(DSALT_ERR_INVALID, "outputs may not be the inputs");
-    if (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < dsalt::cache_rows_ws_bytes(a->n_reqs))
-        return fail(DSALT_ERR_WORKSPACE, "workspace of %zu bytes required", dsalt::cache_rows_ws_bytes(a->n_reqs));
+    const size_t need = dsalt::cache_rows_ws_bytes(a->n_reqs, a->table_cols);
+    if (need && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need))
+        return fail(DSALT_ERR_WORKSPACE, "workspace of %zu bytes required", need);
     dsalt::CacheRowsParams p;
     p.n_reqs = a->n_reqs;
     p.cols = a->table_cols;

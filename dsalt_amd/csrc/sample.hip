@@ -43,7 +43,7 @@ struct Cut {  // kept: key above, or equal with a lower index
 
 struct Shared {
     unsigned long long bin[kBins + 8];  // histogram bins, or a sum a chunk of the row
-    unsigned long long list[kList];     // tokens that can be kept: key, then the index's complement
+    unsigned long long list[kList];     // (2 kThreads) tokens that can be kept: key, then the index's complement
     unsigned long long part[kWaves];
     unsigned long long found[4];
     int count;
@@ -247,13 +247,14 @@ __device__ __forceinline__ unsigned long long reach(unsigned long long above, un
 template <typename T>
 __device__ __forceinline__ void keep_equal(Shared& sh, const Row<T>& row, Cut& cut, uint32_t prefix, unsigned long long keep, unsigned long long ties) {
     constexpr int VEC = Row<T>::VEC;
-    const Cut old = cut;
+    cut.idx = prefix == cut.key ? cut.idx : 0x7fffffff;
     cut.key = prefix;
-    cut.idx = prefix == old.key ? old.idx : 0x7fffffff;
-    if (keep >= ties) return;
+    // (which of those at minus infinity, NaN among them, does not matter: they weigh nothing)
+    if (keep >= ties || prefix == key_of<T>(-INFINITY)) return;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     // the index of the first one left out
-    auto tie = [&](float v, int i) { return row.has(i) && key_of<T>(v) == prefix && old.keeps(prefix, i); };
+    const float value = row.value(prefix);
+    auto tie = [&](float v, int i) { return v == value && i < cut.idx; };
     __syncthreads();
     row.skim([&](int c, int at, const float* v) {
         uint32_t n = 0;
@@ -401,36 +402,52 @@ __device__ __forceinline__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut
     __syncthreads();
     const int n = sh.count;
     if (n > kList) return false;
-    // sorted, largest first: few by counting those above each (threads side by side over parts of the list), more by a
-    // bitonic sort
-    if (n <= kThreads / 2) {
+    // sorted, largest first: up to 256 by counting those above each, threads side by side over parts of the list; more by
+    // a bitonic sort, an element a thread, whose exchanges within a wave need no barrier (four rows of 997 with top_p 0.9:
+    // 22 us, 48 by counting, 26 with every exchange through LDS)
+    if (n <= 256) {
         int* rank = (int*)sh.bin;
         int len = 64;
         while (len < n) len <<= 1;
-        const int i = tid & (len - 1), parts = kThreads / len, per = ceil_div(n, parts), j0 = tid / len * per;
+        const int i = tid & (len - 1), parts = kThreads / len, per = ceil_div(n, parts), j0 = tid / len * per, j1 = min(j0 + per, n);
         if (tid < len) rank[tid] = 0;
         const unsigned long long mine = i < n ? sh.list[i] : 0;
         __syncthreads();
         int above = 0;
-        for (int j = j0; j < min(j0 + per, n); ++j) above += sh.list[j] > mine;
+#pragma unroll 4
+        for (int j = j0; j < j1; ++j) above += sh.list[j] > mine;
         if (above) atomicAdd(&rank[i], above);
         __syncthreads();
         const int at = i < n && tid < len ? rank[i] : -1;
         if (at >= 0) sh.list[at] = mine;
+    } else if (n <= kThreads) {
+        unsigned long long x = tid < n ? sh.list[tid] : 0;
+        for (int size = 2; size <= kThreads; size <<= 1)
+            for (int d = size >> 1; d > 0; d >>= 1) {
+                unsigned long long y;
+                if (d >= 64) {
+                    __syncthreads();
+                    sh.list[tid] = x;
+                    __syncthreads();
+                    y = sh.list[tid ^ d];
+                } else {
+                    y = __shfl_xor(x, d);
+                }
+                const bool larger = ((tid & d) == 0) == ((tid & size) == 0);
+                if ((y > x) == larger) x = y;
+            }
+        __syncthreads();
+        sh.list[tid] = x;
     } else {
-        int len = kThreads;
-        while (len < n) len <<= 1;
-        for (int i = n + tid; i < len; i += kThreads) sh.list[i] = 0;
-        for (int size = 2; size <= len; size <<= 1)
+        for (int i = n + tid; i < kList; i += kThreads) sh.list[i] = 0;
+        for (int size = 2; size <= kList; size <<= 1)
             for (int d = size >> 1; d > 0; d >>= 1) {
                 __syncthreads();
-                for (int i = tid; i < len >> 1; i += kThreads) {
-                    const int a = ((i & ~(d - 1)) << 1) | (i & (d - 1)), b = a | d;
-                    const unsigned long long x = sh.list[a], y = sh.list[b];
-                    if ((x < y) == ((a & size) == 0)) {
-                        sh.list[a] = y;
-                        sh.list[b] = x;
-                    }
+                const int a = ((tid & ~(d - 1)) << 1) | (tid & (d - 1)), b = a | d;
+                const unsigned long long x = sh.list[a], y = sh.list[b];
+                if ((x < y) == ((a & size) == 0)) {
+                    sh.list[a] = y;
+                    sh.list[b] = x;
                 }
             }
     }
@@ -463,78 +480,86 @@ __device__ __forceinline__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut
 }
 
 // Weights of bfloat16 logits by value: few values lie between the largest logit and where weights round to 0, so each is
-// formed once (an element then costs a look-up, about a third of its polynomial).  Entries are the keys kmin ..
-// zlo - 1, then zhi + 1 .. kmax; the keys between, magnitudes too small for kEntries to hold (zeros always), are
-// weighed directly.
-constexpr int kEntries = 4094, kTableCols = 8192;
+// formed once and an element costs a look-up.  An entry a sign and magnitude (the upper bits of the float32) from a0,
+// the last of each sign for all beyond, of weight 0.  Magnitudes below a0 (2^-16 of the largest that weighs, and always
+// zeros) are weighed directly.
+constexpr int kSide = 2048, kTableCols = 8192;
 
 struct Table {
-    unsigned long long* w;  // entries, then a 0
-    uint32_t kmin, zlo, zhi, high;  // entry of key k: k - kmin below the zone, k - high above it
-    int n, below;                   // entries, those below the zone
+    unsigned long long* w;  // [2 kSide]
+    uint32_t a0;
 
-    // the table of a row whose largest key is kmax; weights are 0 below the logit `low`
-    __device__ __forceinline__ Table(unsigned long long* lds, const Row<bf16>& row, uint32_t kmax, float low) : w(lds) {
-        kmin = low > -3e38f ? max(plain_key(low) - 1, 0x80u) : 0x80u;
-        const int am = (int)kmax - 0x8000, al = 0x7fff - (int)kmin;  // largest magnitudes (below 0: none)
-        const int m = max(am, -1), l = max(al, -1);
-        int a0 = (m + l + 3 - kEntries) >> 1;
-        if (a0 > min(m, l) + 1) a0 = max(m, l) + 1 - kEntries;
-        a0 = max(a0, 1);
-        zlo = 0x8000u - a0;
-        zhi = 0x8000u + a0 - 1;
-        below = max((int)min(zlo, kmax + 1) - (int)kmin, 0);
-        const uint32_t p0 = max(zhi + 1, kmin);
-        high = p0 - below;
-        n = below + max((int)kmax - (int)p0 + 1, 0);
+    // the table of a row; weights are 0 below the logit `low`
+    __device__ __forceinline__ Table(unsigned long long* lds, const Row<bf16>& row, float low) : w(lds) {
+        const float m = (float)row.m;
+        const uint32_t up = m > 0.f ? __float_as_uint(m) >> 16 : 0;
+        const uint32_t down = low < 0.f ? min((__float_as_uint(-low) >> 16) + 1, 0x7f7fu) : 0;
+        const uint32_t most = max(up, down);
+        a0 = most > kSide - 1 ? most - (kSide - 2) : 1;
         __syncthreads();
-        for (int i = threadIdx.x; i <= n; i += kThreads) w[i] = i < n ? row.weight(row.value(key(i))) : 0;
+        for (int i = threadIdx.x; i < 2 * kSide; i += kThreads) {
+            const float v = value(i);
+            w[i] = (i & (kSide - 1)) < kSide - 1 && v <= m ? row.weight(v) : 0;
+        }
         __syncthreads();
     }
-    __device__ __forceinline__ static uint32_t plain_key(float v) {  // as key_of but for zeros and NaN
+    __device__ __forceinline__ float value(int i) const {
+        return __uint_as_float((uint32_t)(i / kSide) << 31 | ((uint32_t)(i & (kSide - 1)) + a0) << 16);
+    }
+    __device__ __forceinline__ int entry(float v) const {
         const uint32_t u = __float_as_uint(v);
-        return (u ^ ((uint32_t)((int)u >> 31) | 0x80000000u)) >> 16;
+        return (int)(((u >> 31) * kSide) + min(((u >> 16) & 0x7fffu) - a0, (uint32_t)(kSide - 1)));
     }
-    __device__ __forceinline__ uint32_t key(int i) const { return (uint32_t)i + (i < below ? kmin : high); }
-    __device__ __forceinline__ bool in_zone(uint32_t k) const { return k - zlo <= zhi - zlo; }
-    // the entry of a key outside the zone, n where there is none (and NaN)
-    __device__ __forceinline__ int entry(uint32_t k) const { return (int)min(k - (k > zhi ? high : kmin), (uint32_t)n); }
+    __device__ __forceinline__ bool in_zone(float v) const { return fabsf(v) < __uint_as_float(a0 << 16); }
+    // whether any of eight values is
+    __device__ __forceinline__ bool any_in_zone(const float* v) const {
+        float m = fabsf(v[0]);
+#pragma unroll
+        for (int e = 1; e < 8; ++e) m = fminf(m, fabsf(v[e]));
+        return in_zone(m);
+    }
 };
 
 // The filters from counts of each entry (no list, or more than it holds).  False where a prefix ends among
 // the keys that have none.
 __device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, const Table& tab, Cut& cut, int top_k, float top_p) {
-    constexpr int PER = (kEntries + 2) / kThreads;
+    constexpr int PER = 2 * kSide / kThreads;
     uint32_t* count = (uint32_t*)sh.list;
+    static_assert(2 * kSide * sizeof(uint32_t) <= sizeof(sh.list), "a count an entry");
     unsigned long long* zone = sh.bin;  // elements and weight of the zone
     const int tid = threadIdx.x;
     __syncthreads();
-    for (int i = tid; i < kEntries + 2; i += kThreads) count[i] = 0;
+    for (int i = tid; i < 2 * kSide; i += kThreads) count[i] = 0;
     if (tid < 2) zone[tid] = 0;
     __syncthreads();
     row.skim([&](int, int at, const float* v) {
+        if (tab.any_in_zone(v)) {
+#pragma unroll
+            for (int e = 0; e < Row<bf16>::VEC; ++e)
+                if (tab.in_zone(v[e])) {
+                    atomicAdd(&zone[0], 1ull);
+                    atomicAdd(&zone[1], row.weight(v[e]));
+                }
+        }
 #pragma unroll
         for (int e = 0; e < Row<bf16>::VEC; ++e) {
-            const uint32_t k = Table::plain_key(v[e]);
-            if (tab.in_zone(k)) {
-                const unsigned long long w = row.weight(v[e]);
-                atomicAdd(&zone[0], 1ull);
-                atomicAdd(&zone[1], w);
-            } else {
-                const int i = tab.entry(k);
-                if (i < tab.n) atomicAdd(&count[i], 1u);
-            }
+            const int i = tab.entry(v[e]);
+            if ((i & (kSide - 1)) != kSide - 1) atomicAdd(&count[i], 1u);
         }
     });
     __syncthreads();
     const unsigned long long zn = zone[0], zw = zone[1];
-    // a thread's entries from the largest key down, what lies above them, and of how many
+    // a thread's entries from the largest value down, what lies above them, and of how many: positive ones first, then
+    // the zone, then negative ones
+    auto at = [&](int e) {
+        const int r = tid * PER + e;
+        return r < kSide ? kSide - 1 - r : r;
+    };
     unsigned long long c[PER], w[PER], ca, wa, cn = 0, wn = 0, call, wall;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-        const int i = tab.n - 1 - (tid * PER + e);
-        c[e] = i >= 0 ? count[i] : 0;
-        w[e] = i >= 0 ? tab.w[i] : 0;
+        c[e] = count[at(e)];
+        w[e] = tab.w[at(e)];
         cn += c[e];
         wn += c[e] * w[e];
     }
@@ -548,10 +573,10 @@ __device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, cons
         unsigned long long cc = ca, ww = wa;
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            const int i = tab.n - 1 - (tid * PER + e);
-            const unsigned long long c0 = cc + (i < tab.below ? zn : 0), w0 = ww + (i < tab.below ? zw : 0);
-            if (i >= 0 && ends(c0, w0, c[e], w[e])) {
-                sh.found[0] = (unsigned long long)i;
+            const bool below = at(e) >= kSide;
+            const unsigned long long c0 = cc + (below ? zn : 0), w0 = ww + (below ? zw : 0);
+            if (ends(c0, w0, c[e], w[e])) {
+                sh.found[0] = (unsigned long long)at(e);
                 sh.found[1] = c0;
                 sh.found[2] = w0;
                 sh.found[3] = c[e];
@@ -589,7 +614,7 @@ __device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, cons
         }
         __syncthreads();
     }
-    if (end >= 0) keep_equal(sh, row, cut, tab.key(end), keep, ties);
+    if (end >= 0) keep_equal(sh, row, cut, key_of<bf16>(tab.value(end)), keep, ties);
     return true;
 }
 
@@ -667,20 +692,23 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     };
     if constexpr (Key<T>::bits == 16) {
         if (!summed && row.n >= kTableCols && !inf) {
-            const Table tab(dyn, row, top, row.value(top) - 30.f * temp);
+            const Table tab(dyn, row, row.value(top) - 30.f * temp);
             summed = !filters || cut_table(sh, row, tab, cut, top_k, top_p);
+            const float edge = row.value(cut.key);
             __syncthreads();
             if (summed)
                 row.skim([&](int c, int at, const float* v) {
                     unsigned long long s = 0;
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
-                        const uint32_t k = Table::plain_key(v[e]);
-                        const bool zone = tab.in_zone(k);
-                        unsigned long long w = tab.w[zone ? tab.n : tab.entry(k)];
-                        if (cut.key && !cut.keeps(k, at + e)) w = 0;
-                        if (zone) w = kept(v[e], at + e);
+                        unsigned long long w = tab.w[tab.entry(v[e])];
+                        if (cut.key && !(v[e] > edge || (v[e] == edge && at + e < cut.idx))) w = 0;
                         s += w >= least_w ? w : 0;
+                    }
+                    if (tab.any_in_zone(v)) {
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e)
+                            if (tab.in_zone(v[e])) s += kept(v[e], at + e);
                     }
                     s = wave_sum_weights(s);
                     if (lane == 0) sh.bin[c] = s;
@@ -765,7 +793,7 @@ hipError_t sample_launch(const SampleParams& p, hipStream_t stream) {
     switch (p.dtype) {
         case 0: DSALT_LAUNCH("sample", sample_kernel<float>, grid, dim3(kThreads), 0, stream, p); break;
         case 1: {
-            const unsigned lds = p.n_cols >= kTableCols ? (kEntries + 2) * sizeof(unsigned long long) : 0;
+            const unsigned lds = p.n_cols >= kTableCols ? 2 * kSide * sizeof(unsigned long long) : 0;
             if (lds)
                 if (hipError_t e = hipFuncSetAttribute((const void*)sample_kernel<bf16>, hipFuncAttributeMaxDynamicSharedMemorySize, lds))
                     return e;

@@ -770,42 +770,57 @@ def new_cache(n_blocks: int, n_kv_heads: int, head_dim: int, *, block_tokens: in
     return Cache8(*codes, *(torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)))
 
 
+_E4M3 = torch.float8_e4m3fn
+_device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _on(*ts) -> int:
+    """The index of the device all tensors are on (None among them is passed over)."""
+    at = ts[0].get_device()
+    for t in ts:
+        if t is not None and (at < 0 or t.get_device() != at):
+            _gpu(*ts)
+            raise ValueError("all tensors must be on the same device")
+    return at
+
+
 def _cache_args(c: Cache8) -> Cache:
     k, v, ks, vs = c
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != torch.float8_e4m3fn or v.dtype != torch.float8_e4m3fn \
-            or not k.is_contiguous() or not v.is_contiguous():
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or k.dtype != _E4M3 or v.dtype != _E4M3 or not k.is_contiguous() \
+            or not v.is_contiguous():
         raise ValueError("the cache's k and v must be contiguous float8_e4m3fn [n_blocks, n_kv, block_tokens, D]")
-    if ks.shape != k.shape[:2] or vs.shape != k.shape[:2] or ks.dtype != torch.float32 or vs.dtype != torch.float32 \
+    if ks.shape != shape[:2] or vs.shape != shape[:2] or ks.dtype != torch.float32 or vs.dtype != torch.float32 \
             or not ks.is_contiguous() or not vs.is_contiguous():
         raise ValueError("the cache's scales must be contiguous float32 [n_blocks, n_kv]")
-    return Cache(*k.shape, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr())
+    return Cache(*shape, k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr())
 
 
-def _check_table(table: torch.Tensor):
-    if table.dim() != 2 or table.dtype != torch.int32 or (table.shape[1] > 1 and table.stride(1) != 1) \
-            or (table.shape[0] > 1 and table.stride(0) < table.shape[1]):
-        raise ValueError("table must be int32 [R, pages] with unit stride along the pages and rows that do not overlap")
-
-
-def _table_stride(table: torch.Tensor) -> int:
-    return max(table.stride(0), table.shape[1])
+def _table_args(table: torch.Tensor):
+    """(R, pages, row stride) of a block table."""
+    shape = table.shape
+    if len(shape) != 2 or table.dtype != torch.int32:
+        raise ValueError("table must be int32 [R, pages]")
+    R, M = shape
+    st = table.stride(0) if R > 1 else M
+    if (M > 1 and table.stride(1) != 1) or st < M:
+        raise ValueError("table must have unit stride along the pages and rows that do not overlap")
+    return R, M, st
 
 
 def _rows16(t: torch.Tensor, name: str):
     """([T, H, D] tensor, its (address, token stride, head stride)) as the kernels' 16-byte loads need them:
     the tensor itself, or a copy of one with other strides or alignment."""
-    t = _rows3(t, name)
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [T, H, D], got shape {tuple(t.shape)}")
     T, H, D = t.shape
-    es = t.element_size()
-
-    def strides():
-        return t.stride(0) if T > 1 else H * D, t.stride(1) if H > 1 else D
-
-    st, sh = strides()
-    if t.data_ptr() % 16 or st <= 0 or st * es % 16 or st * es > 1 << 20 or sh * es % 16:
+    st, sh, sd = t.stride()
+    st, sh = st if T > 1 else H * D, sh if H > 1 else D
+    es, at = t.element_size(), t.data_ptr()
+    if sd != 1 or at % 16 or st <= 0 or st * es % 16 or st * es > 1 << 20 or sh * es % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-        st, sh = strides()
-    return t, (t.data_ptr(), st, sh)
+        st, sh, at = H * D, D, t.data_ptr()
+    return t, (at, st, sh)
 
 
 def _vec_i32(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
@@ -814,15 +829,16 @@ def _vec_i32(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     return _i32(t)
 
 
-def _call(name: str, args, dev: torch.device):
-    """One library call on the current stream of ``dev`` (made current for it where it is not)."""
+def _call(name: str, args, at: int):
+    """One library call on the current stream of device ``at`` (made current for it where it is not)."""
     fn = getattr(_lib.load(), name)
-    if dev.index is not None and dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            rc = fn(ctypes.byref(args), _stream(dev))
+    if _device_now() != at:
+        with torch.cuda.device(at):
+            rc = fn(ctypes.byref(args), _stream(torch.device("cuda", at)))
     else:
-        rc = fn(ctypes.byref(args), _stream(dev))
-    _lib.check(name, rc)
+        rc = fn(ctypes.byref(args), _raw_stream(at) if _raw_stream is not None else _stream(torch.device("cuda", at)))
+    if rc:
+        _lib.check(name, rc)
 
 
 def cache_rows_(seq_len, new_len, table, free_blocks, span, n_rows: int, *, block_tokens: int = 64) -> CacheRows:
@@ -834,9 +850,8 @@ def cache_rows_(seq_len, new_len, table, free_blocks, span, n_rows: int, *, bloc
     are not there, or whose tokens fit neither the table nor the rows, is refused: it keeps its length and its
     rows are inert (position and slot -1).  ``seq_len`` and ``span`` stay as they are: the step's come back in
     the CacheRows."""
-    dev = _gpu(seq_len, new_len, table, free_blocks, span)
-    _check_table(table)
-    R, M = table.shape
+    at = _on(table, seq_len, new_len, free_blocks, span)
+    R, M, st = _table_args(table)
     if free_blocks.dim() != 1 or free_blocks.dtype != torch.int32 or not free_blocks.is_contiguous():
         raise ValueError("free_blocks must be contiguous int32 [entries]")
     if span.shape != (2,) or span.dtype != torch.int64 or not span.is_contiguous():
@@ -845,18 +860,16 @@ def cache_rows_(seq_len, new_len, table, free_blocks, span, n_rows: int, *, bloc
         raise ValueError(f"n_rows must be >= 0 and block_tokens one of {BLOCK_TOKENS}, got {n_rows}, {block_tokens}")
     old, new = _vec_i32(seq_len, R, "seq_len"), _vec_i32(new_len, R, "new_len")
     n_pieces = min(n_rows, n_rows // block_tokens + 2 * R)
-    i32, i64 = torch.int32, torch.int64
-    out = CacheRows(torch.empty(R, dtype=i32, device=dev), torch.empty(2, dtype=i64, device=dev),
-                    torch.empty(R, dtype=i32, device=dev), torch.empty(R + 1, dtype=i32, device=dev),
-                    torch.empty(n_rows, dtype=i32, device=dev), torch.empty(n_rows, dtype=i32, device=dev),
-                    torch.empty(n_rows, dtype=i64, device=dev), torch.empty((n_pieces, 4), dtype=i32, device=dev))
+    # the outputs lie side by side in two buffers
+    pieces, seq, granted, cu, req, pos = torch.empty(4 * n_pieces + 3 * R + 1 + 2 * n_rows, dtype=torch.int32, device=at).split(
+        [4 * n_pieces, R, R, R + 1, n_rows, n_rows])
+    span_out, slot = torch.empty(2 + n_rows, dtype=torch.int64, device=at).split([2, n_rows])
     a = CacheRowsArgs(R, M, block_tokens, n_rows, n_pieces, free_blocks.shape[0], old.data_ptr(), new.data_ptr(),
-                      table.data_ptr(), _table_stride(table), free_blocks.data_ptr(), span.data_ptr(), out.seq_len.data_ptr(),
-                      out.span.data_ptr(), out.granted.data_ptr(), out.cu.data_ptr(), out.req.data_ptr(), out.pos.data_ptr(),
-                      out.slot.data_ptr(), out.pieces.data_ptr())
-    ws = _set_workspace(a, _lib.load().dsalt_cache_rows_workspace_bytes(ctypes.byref(a)), dev)  # noqa: F841 (kept alive)
-    _call("dsalt_cache_rows", a, dev)
-    return out
+                      table.data_ptr(), st, free_blocks.data_ptr(), span.data_ptr(), seq.data_ptr(), span_out.data_ptr(),
+                      granted.data_ptr(), cu.data_ptr(), req.data_ptr(), pos.data_ptr(), slot.data_ptr(), pieces.data_ptr())
+    ws = _set_workspace(a, _lib.load().dsalt_cache_rows_workspace_bytes(ctypes.byref(a)), at)  # noqa: F841 (kept alive)
+    _call("dsalt_cache_rows", a, at)
+    return CacheRows(seq, span_out, granted, cu, req, pos, slot, pieces.view(n_pieces, 4))
 
 
 def cache_write_(k, v, cache: Cache8, pieces) -> Cache8:
@@ -864,7 +877,7 @@ def cache_write_(k, v, cache: Cache8, pieces) -> Cache8:
     (CacheRows.pieces: first row, rows, page, first token in the page; each page in one piece at most).  A page's
     scale is the least power of two that keeps its finite elements within 448 of it; codes it held follow a
     larger one.  Values that are not finite are held as NaN."""
-    dev = _gpu(k, v, *cache, pieces)
+    at = _on(k, v, *cache, pieces)
     (k, k_at), (v, v_at) = _rows16(k, "k"), _rows16(v, "v")
     c = _cache_args(cache)
     if k.shape != v.shape or k.dtype != v.dtype or k.shape[1] != c.n_kv_heads or k.shape[2] != c.head_dim:
@@ -872,7 +885,7 @@ def cache_write_(k, v, cache: Cache8, pieces) -> Cache8:
     if pieces.dim() != 2 or pieces.shape[1] != 4 or pieces.dtype != torch.int32 or not pieces.is_contiguous():
         raise ValueError("pieces must be contiguous int32 [P, 4]")
     a = CacheWriteArgs(c, k.shape[0], pieces.shape[0], dtype_code(k.dtype), *k_at, *v_at, pieces.data_ptr())
-    _call("dsalt_cache_write", a, dev)
+    _call("dsalt_cache_write", a, at)
     return cache
 
 
@@ -880,19 +893,18 @@ def cache_read(cache: Cache8, table, cu_seqlens, *, start=None, n_rows: int, dty
     """(k, v) [n_rows, n_kv, D]: tokens of the cache as a packed batch.  Row t is token ``start[r]`` (default 0)
     + t - cu_seqlens[r] of the request r whose rows hold it; zeros past the last row and where the table names
     no page."""
-    dev = _gpu(*cache, table, cu_seqlens, start)
-    _check_table(table)
+    at = _on(table, *cache, cu_seqlens, start)
     c = _cache_args(cache)
-    R, M = table.shape
+    R, M, ts = _table_args(table)
     cu = _vec_i32(cu_seqlens, R + 1, "cu_seqlens")
     st = _vec_i32(start, R, "start") if start is not None else None
     if n_rows < 0:
         raise ValueError(f"n_rows must be >= 0, got {n_rows}")
-    k = torch.empty((n_rows, c.n_kv_heads, c.head_dim), dtype=dtype, device=dev)
+    k = torch.empty((n_rows, c.n_kv_heads, c.head_dim), dtype=dtype, device=at)
     v = torch.empty_like(k)
-    a = CacheReadArgs(c, R, M, n_rows, dtype_code(dtype), table.data_ptr(), _table_stride(table), cu.data_ptr(),
+    a = CacheReadArgs(c, R, M, n_rows, dtype_code(dtype), table.data_ptr(), ts, cu.data_ptr(),
                       st.data_ptr() if st is not None else None, k.data_ptr(), v.data_ptr())
-    _call("dsalt_cache_read", a, dev)
+    _call("dsalt_cache_read", a, at)
     return k, v
 
 
@@ -904,12 +916,11 @@ def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None
     position may repeat; select_landmarks' sets).  Rows without a key (inert rows, pages that the table does not
     name) give zeros and -inf.  ``w_max``: no window is longer (host value; splits the work, longer windows only
     cost time).  Not differentiable."""
-    dev = _gpu(q, *cache, table, req, pos, w, lmk_idx, lmk_bias)
+    at = _on(q, *cache, table, req, pos, w, lmk_idx, lmk_bias)
     q, q_at = _rows16(q, "q")
-    _check_table(table)
     c = _cache_args(cache)
     T, H, D = q.shape
-    R, M = table.shape
+    R, M, ts = _table_args(table)
     if D != c.head_dim or H % c.n_kv_heads:
         raise ValueError(f"q must be [T, H, {c.head_dim}] with H a multiple of {c.n_kv_heads}, got {tuple(q.shape)}")
     if lmk_idx.dim() != 4 or lmk_idx.shape[:3] != (H, R, 1):
@@ -921,14 +932,14 @@ def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None
     li = _i32(lmk_idx)
     lb = _f32(lmk_bias) if lmk_bias is not None else None
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
-    lse = torch.empty((T, H), dtype=torch.float32, device=dev)
+    out = torch.empty((T, H, D), dtype=q.dtype, device=at)
+    lse = torch.empty((T, H), dtype=torch.float32, device=at)
     a = CacheAttnArgs(c, T, H, R, M, K, dtype_code(q.dtype), 0 if w_max is None else int(w_max), table.data_ptr(),
-                      _table_stride(table), *q_at, rq.data_ptr(), ps.data_ptr(), wc.data_ptr(),
+                      ts, *q_at, rq.data_ptr(), ps.data_ptr(), wc.data_ptr(),
                       li.data_ptr() if K else None, lb.data_ptr() if lb is not None and K else None,
                       out.data_ptr(), H * D, D, lse.data_ptr(), scale)
-    ws = _set_workspace(a, _lib.load().dsalt_cache_attn_workspace_bytes(ctypes.byref(a)), dev)  # noqa: F841 (kept alive)
-    _call("dsalt_cache_attn", a, dev)
+    ws = _set_workspace(a, _lib.load().dsalt_cache_attn_workspace_bytes(ctypes.byref(a)), at)  # noqa: F841 (kept alive)
+    _call("dsalt_cache_attn", a, at)
     return out, lse
 
 
@@ -941,7 +952,7 @@ def sample_rows(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     weights passes u times their total.  Weights are whole multiples of 2^-42 of the largest.  logp: the token's
     log probability among the kept.  Rows without a logit above -inf give -1 and -inf."""
     per_row = [t if isinstance(t, torch.Tensor) else None for t in (temperature, top_k, top_p, min_p)]
-    dev = _gpu(logits, u, *per_row)
+    at = _on(logits, u, *per_row)
     if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_VOCAB:
         raise ValueError(f"logits must be [R, V] with V in [1, {MAX_VOCAB}], got {tuple(logits.shape)}")
     R, V = logits.shape
@@ -958,11 +969,11 @@ def sample_rows(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if k is not None and k.dtype != torch.int32:
         k = k.clamp(-1, MAX_VOCAB)
     k = k if k is None else _i32(k)
-    token = torch.empty(R, dtype=torch.int64, device=dev)
-    logp = torch.empty(R, dtype=torch.float32, device=dev)
+    token = torch.empty(R, dtype=torch.int64, device=at)
+    logp = torch.empty(R, dtype=torch.float32, device=at)
     a = SampleArgs(R, V, dtype_code(logits.dtype), u.element_size(), logits.data_ptr(), logits.stride(0), u.data_ptr(),
                    *(x.data_ptr() if x is not None else None for x in (t, p, m, k)),
                    *(0.0 if isinstance(x, torch.Tensor) else float(x) for x in (temperature, top_p, min_p)),
                    0 if k is not None else max(-1, min(int(top_k), MAX_VOCAB)), token.data_ptr(), logp.data_ptr())
-    _call("dsalt_sample_rows", a, dev)
+    _call("dsalt_sample_rows", a, at)
     return token, logp

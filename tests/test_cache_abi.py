@@ -68,6 +68,9 @@ def _rows_args():
     ("workspace_bytes", 300, 3)])
 def test_rows_refusals(field, value, code):
     a = _rows_args()
+    if code == 3:  # only many requests need a workspace
+        a.n_reqs, a.n_pieces = 5000, 256
+        assert _lib.load().dsalt_cache_rows_workspace_bytes(ctypes.byref(a)) > 300
     setattr(a, field, value)
     _refused("dsalt_cache_rows", a, code)
 

@@ -72,10 +72,11 @@ def test_rows_of_a_decoding_step(bt):
     _check_rows(seq, [1] * len(seq), 4, bt, len(seq) + 40)  # rows past the last request
 
 
-@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("seed", range(8))
 def test_rows_of_mixed_steps(seed):
+    """Request counts on both sides of a thread each, and of one launch (4096)."""
     r = np.random.RandomState(seed)
-    R, bt, M = [1, 5, 70, 1024, 1025, 3001][seed], [16, 64, 32, 128, 64, 16][seed], 9
+    R, bt, M = [1, 5, 70, 1024, 1025, 3001, 4096, 4097][seed], [16, 64, 32, 128, 64, 16, 16, 32][seed], 9 if seed < 6 else 3
     seq = r.randint(0, bt * M + 1, R).tolist()
     new = [int(x) for x in np.where(r.rand(R) < 0.2, -r.randint(1, 4, R), np.where(r.rand(R) < 0.4, 1, r.randint(0, bt * 4, R)))]
     total = sum(max(n, 0) for n in new)
