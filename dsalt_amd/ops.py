@@ -900,7 +900,7 @@ def cache_read(cache: Cache8, table, cu_seqlens, *, start=None, n_rows: int, dty
     st = _vec_i32(start, R, "start") if start is not None else None
     if n_rows < 0:
         raise ValueError(f"n_rows must be >= 0, got {n_rows}")
-    k = torch.empty((n_rows, c.n_kv_heads, c.head_dim), dtype=dtype, device=at)
+    k = torch.empty(n_rows, c.n_kv_heads, c.head_dim, dtype=dtype, device=at)
     v = torch.empty_like(k)
     a = CacheReadArgs(c, R, M, n_rows, dtype_code(dtype), table.data_ptr(), ts, cu.data_ptr(),
                       st.data_ptr() if st is not None else None, k.data_ptr(), v.data_ptr())
@@ -932,8 +932,8 @@ def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None
     li = _i32(lmk_idx)
     lb = _f32(lmk_bias) if lmk_bias is not None else None
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    out = torch.empty((T, H, D), dtype=q.dtype, device=at)
-    lse = torch.empty((T, H), dtype=torch.float32, device=at)
+    out = torch.empty(T, H, D, dtype=q.dtype, device=at)
+    lse = torch.empty(T, H, dtype=torch.float32, device=at)
     a = CacheAttnArgs(c, T, H, R, M, K, dtype_code(q.dtype), 0 if w_max is None else int(w_max), table.data_ptr(),
                       ts, *q_at, rq.data_ptr(), ps.data_ptr(), wc.data_ptr(),
                       li.data_ptr() if K else None, lb.data_ptr() if lb is not None and K else None,
