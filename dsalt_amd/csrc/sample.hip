@@ -46,8 +46,13 @@ struct Shared {
     unsigned long long list[kList];     // (2 kThreads) tokens that can be kept: key, then the index's complement
     unsigned long long part[kWaves];
     unsigned long long found[4];
-    int count;
+    int count, unused;
 };
+
+// All of a block's LDS: Shared, then the table of bfloat16 rows.  Dynamic, so that a function that is called rather than
+// inlined reaches it by name (through a pointer it would with flat instructions).
+extern __shared__ unsigned long long sample_lds[];
+__device__ __forceinline__ Shared& shared() { return *(Shared*)sample_lds; }
 
 // exclusive prefix of v over the block, and the total
 __device__ __forceinline__ unsigned long long block_scan(Shared& sh, unsigned long long v, unsigned long long& total) {
@@ -104,7 +109,9 @@ template <typename T>
 struct Row {
     static constexpr int VEC = 16 / sizeof(T), CHUNK = 64 * VEC;
     typedef T vec __attribute__((ext_vector_type(VEC), aligned(16)));
-    const T* x;
+    typedef const T __attribute__((address_space(1))) global;  // (known to be global memory in called functions too)
+    typedef const vec __attribute__((address_space(1))) global_vec;
+    global* x;
     int n, shift;  // elements, and those of the first 16-byte vector that lie before the row
     int chunks;
     double m;      // largest logit (beside infinity 1e39, above every other)
@@ -115,7 +122,7 @@ struct Row {
     __device__ __forceinline__ bool inside(int c) const { return c * CHUNK >= shift && (c + 1) * CHUNK - shift <= n; }
     __device__ __forceinline__ void load(int at, float* v) const {
         if (at >= 0 && at + VEC <= n) {
-            const vec u = *(const vec*)(x + at);
+            const vec u = *(global_vec*)(x + at);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[e] = to_float(u[e]);
         } else {
@@ -128,7 +135,7 @@ struct Row {
     __device__ __forceinline__ void each(F f) const {
         auto fetch = [&](int c) {
             vec u = {};
-            if (inside(c)) u = *(const vec*)(x + first(c));
+            if (inside(c)) u = *(global_vec*)(x + first(c));
             return u;
         };
         int c = threadIdx.x >> 6;
@@ -152,7 +159,7 @@ struct Row {
 #pragma unroll
             for (int k = 0; k < N; ++k) {
                 r[k] = vec{};
-                if (inside(c + k * kWaves)) r[k] = *(const vec*)(x + first(c + k * kWaves));
+                if (inside(c + k * kWaves)) r[k] = *(global_vec*)(x + first(c + k * kWaves));
             }
         };
         int c = threadIdx.x >> 6;
@@ -302,84 +309,12 @@ __device__ __forceinline__ void keep_equal(Shared& sh, const Row<T>& row, Cut& c
     cut.idx = (int)sh.found[2];
 }
 
-// Narrows `cut` to the end of a prefix.  `counts`: the first k elements.  Otherwise those before which less
-// than top_p of the weight of `cut` lies (kept as it is if all are).
+// The filters on a list: the elements of keys `least` and more are listed, sorted and cut to the first k and to top_p of
+// `whole` (0: of those k).  On return sh.bin holds the kept weights a chunk.  False where the list is too short for them,
+// or top_p of `whole` not in it.
 template <typename T>
-__device__ __forceinline__ void narrow(Shared& sh, const Row<T>& row, Cut& cut, bool counts, unsigned long long k, float top_p) {
-    constexpr int VEC = Row<T>::VEC, BITS = Key<T>::bits;
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const Cut old = cut;
-    unsigned long long above = 0, own = 0, total;  // counted or weighed above the bins searched, in the one found
-    double thr = 0;
-    uint32_t prefix = 0;
-    for (int shift = BITS; shift > 0;) {
-        const int width = min(shift, 12), upper = shift;
-        shift -= width;
-        clear_bins(sh, 1 << width);
-        row.each([&](int, int at, const float* v) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const uint32_t kk = key_of<T>(v[e]);
-                if ((upper == BITS || (kk >> upper) == prefix) && row.has(at + e) && old.keeps(kk, at + e)) {
-                    const unsigned long long w = counts ? 1ull : row.weight(v[e]);
-                    if (w) atomicAdd(&sh.bin[(kk >> shift) & ((1u << width) - 1)], w);
-                }
-            }
-        });
-        __syncthreads();
-        const bool top = upper == BITS;
-        if (!counts && top) {  // the threshold is a part of the whole
-            unsigned long long s = 0;
-            for (int b = tid; b < (1 << width); b += kThreads) s += sh.bin[b];
-            block_scan(sh, s, total);
-            thr = (double)top_p * (double)total;
-            __syncthreads();
-        }
-        uint32_t bin;
-        auto ends = [&](unsigned long long a, unsigned long long h) {
-            return counts ? a < k && k <= a + h : (double)a < thr && !((double)(a + h) < thr);
-        };
-        if (!find_bin(sh, width, above, ends, total, bin, above, own)) return;  // everything is kept
-        prefix = (prefix << width) | bin;
-    }
-    // equal keys: the first `keep` of them
-    unsigned long long keep, ties;
-    if (counts) {
-        ties = own;
-        keep = k - above;
-    } else {
-        const unsigned long long w = row.weight(row.value(prefix));
-        ties = own / w;
-        keep = reach(above, w, ties, thr);
-    }
-    keep_equal(sh, row, cut, prefix, keep, ties);
-}
-
-// A key that at least k of the threads' largest keys reach, so at least k elements do: the k-th largest of them, of
-// keys over 24 bits to those.  k at most kThreads.
-template <int BITS>
-__device__ __forceinline__ uint32_t reached_by(Shared& sh, uint32_t mine, unsigned long long k) {
-    unsigned long long above = 0, own, total;
-    uint32_t prefix = 0;
-    int shift = BITS;
-    for (int level = 0; level < 2 && shift > 0; ++level) {
-        const int width = min(shift, 12), upper = shift;
-        shift -= width;
-        clear_bins(sh, 1 << width);
-        if (upper == BITS || (mine >> upper) == prefix) atomicAdd(&sh.bin[(mine >> shift) & ((1u << width) - 1)], 1ull);
-        __syncthreads();
-        uint32_t bin;
-        find_bin(sh, width, above, [&](unsigned long long a, unsigned long long h) { return a < k && k <= a + h; }, total, bin, above,
-                 own);
-        prefix = (prefix << width) | bin;
-    }
-    return prefix << shift;
-}
-
-// The filters on a list: the elements of keys `least` and more are listed, sorted and cut.  On return sh.bin holds the
-// kept weights a chunk.  False where the list is too short for them.
-template <typename T>
-__device__ __forceinline__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut, uint32_t least, int k, float top_p, unsigned long long least_w) {
+__device__ __forceinline__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut, uint32_t least, int k, float top_p, unsigned long long least_w,
+                                         unsigned long long whole) {
     constexpr int VEC = Row<T>::VEC, PER = kList / kThreads;
     const int tid = threadIdx.x;
     __syncthreads();
@@ -461,7 +396,8 @@ __device__ __forceinline__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut
         sum += w[e];
     }
     unsigned long long before = block_scan(sh, sum, total);
-    const double thr = (double)top_p * (double)total;
+    const double thr = (double)top_p * (double)(whole ? whole : total);
+    if (whole && (double)total < thr) return false;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         const int i = tid * PER + e;
@@ -477,6 +413,93 @@ __device__ __forceinline__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut
     const unsigned long long last = sh.list[sh.count - n - 1];
     cut = {(uint32_t)(last >> 32), (int)~(uint32_t)last + 1};
     return true;
+}
+
+// Narrows `cut` to the end of a prefix.  `counts`: the first k elements.  Otherwise those before which less
+// than top_p of the weight of `cut` lies (kept as it is if all are); where few elements reach the bin in which that
+// part ends, they are listed instead of searched further.  True where that has cut the row (see cut_list).
+// A call of its own: inlined, the registers it needs cost every row that does without it (float32 rows, temperature
+// alone, 75 -> 83 us).
+struct Narrowed {
+    Cut cut;
+    bool summed;
+};
+
+template <typename T>
+__device__ __attribute__((noinline)) Narrowed narrow(const Row<T> row, Cut cut, bool counts, unsigned long long k, float top_p,
+                                                     unsigned long long least_w) {
+    Shared& sh = shared();
+    constexpr int VEC = Row<T>::VEC, BITS = Key<T>::bits;
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const Cut old = cut;
+    unsigned long long above = 0, own = 0, total;  // counted or weighed above the bins searched, in the one found
+    double thr = 0;
+    uint32_t prefix = 0;
+    for (int shift = BITS; shift > 0;) {
+        const int width = min(shift, 12), upper = shift;
+        shift -= width;
+        clear_bins(sh, 1 << width);
+        row.each([&](int, int at, const float* v) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const uint32_t kk = key_of<T>(v[e]);
+                if ((upper == BITS || (kk >> upper) == prefix) && row.has(at + e) && old.keeps(kk, at + e)) {
+                    const unsigned long long w = counts ? 1ull : row.weight(v[e]);
+                    if (w) atomicAdd(&sh.bin[(kk >> shift) & ((1u << width) - 1)], w);
+                }
+            }
+        });
+        __syncthreads();
+        const bool top = upper == BITS;
+        if (!counts && top) {  // the threshold is a part of the whole
+            unsigned long long s = 0;
+            for (int b = tid; b < (1 << width); b += kThreads) s += sh.bin[b];
+            block_scan(sh, s, total);
+            thr = (double)top_p * (double)total;
+            __syncthreads();
+        }
+        uint32_t bin;
+        auto ends = [&](unsigned long long a, unsigned long long h) {
+            return counts ? a < k && k <= a + h : (double)a < thr && !((double)(a + h) < thr);
+        };
+        const unsigned long long whole = total;
+        if (!find_bin(sh, width, above, ends, total, bin, above, own)) return {cut, false};  // everything is kept
+        prefix = (prefix << width) | bin;
+        if (!counts && top && old.key == 0 && cut_list(sh, row, cut, prefix << shift, row.n, top_p, least_w, whole)) return {cut, true};
+    }
+    // equal keys: the first `keep` of them
+    unsigned long long keep, ties;
+    if (counts) {
+        ties = own;
+        keep = k - above;
+    } else {
+        const unsigned long long w = row.weight(row.value(prefix));
+        ties = own / w;
+        keep = reach(above, w, ties, thr);
+    }
+    keep_equal(sh, row, cut, prefix, keep, ties);
+    return {cut, false};
+}
+
+// A key that at least k of the threads' largest keys reach, so at least k elements do: the k-th largest of them, of
+// keys over 24 bits to those.  k at most kThreads.
+template <int BITS>
+__device__ __forceinline__ uint32_t reached_by(Shared& sh, uint32_t mine, unsigned long long k) {
+    unsigned long long above = 0, own, total;
+    uint32_t prefix = 0;
+    int shift = BITS;
+    for (int level = 0; level < 2 && shift > 0; ++level) {
+        const int width = min(shift, 12), upper = shift;
+        shift -= width;
+        clear_bins(sh, 1 << width);
+        if (upper == BITS || (mine >> upper) == prefix) atomicAdd(&sh.bin[(mine >> shift) & ((1u << width) - 1)], 1ull);
+        __syncthreads();
+        uint32_t bin;
+        find_bin(sh, width, above, [&](unsigned long long a, unsigned long long h) { return a < k && k <= a + h; }, total, bin, above,
+                 own);
+        prefix = (prefix << width) | bin;
+    }
+    return prefix << shift;
 }
 
 // Weights of bfloat16 logits by value: few values lie between the largest logit and where weights round to 0, so each is
@@ -620,12 +643,11 @@ __device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, cons
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
-    __shared__ Shared sh;
-    extern __shared__ unsigned long long dyn[];  // bfloat16: the table
+    Shared& sh = shared();
     constexpr int VEC = Row<T>::VEC;
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     Row<T> row;
-    row.x = (const T*)p.x + (int64_t)r * p.x_st;
+    row.x = (typename Row<T>::global*)p.x + (int64_t)r * p.x_st;
     row.n = p.n_cols;
     row.shift = (int)(((uintptr_t)row.x & 15) / sizeof(T));
     row.chunks = ceil_div(row.n + row.shift, Row<T>::CHUNK);
@@ -682,7 +704,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     if (filters && (row.n <= kList || (top_k > 0 && top_k <= kThreads))) {
         uint32_t least = key_of<T>(-INFINITY);
         if (top_k > 0 && top_k <= kThreads) least = max(least, reached_by<Key<T>::bits>(sh, own, (unsigned long long)top_k));
-        summed = cut_list(sh, row, cut, least, top_k > 0 ? top_k : row.n, top_p, least_w);
+        summed = cut_list(sh, row, cut, least, top_k > 0 ? top_k : row.n, top_p, least_w, 0);
     }
     // kept weights a chunk, then the chunk, lane and element in which the running sum passes u times the total
     auto kept = [&](float v, int i) -> unsigned long long {
@@ -692,44 +714,71 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     };
     if constexpr (Key<T>::bits == 16) {
         if (!summed && row.n >= kTableCols && !inf) {
-            const Table tab(dyn, row, row.value(top) - 30.f * temp);
+            const Table tab(sample_lds + sizeof(Shared) / sizeof(unsigned long long), row, row.value(top) - 30.f * temp);
             summed = !filters || cut_table(sh, row, tab, cut, top_k, top_p);
             const float edge = row.value(cut.key);
             __syncthreads();
-            if (summed)
+            auto zones = [&](int at, const float* v) {
+                unsigned long long s = 0;
+                if (tab.any_in_zone(v)) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (tab.in_zone(v[e])) s += kept(v[e], at + e);
+                }
+                return s;
+            };
+            if (summed && cut.key == 0) {
                 row.skim([&](int c, int at, const float* v) {
-                    unsigned long long s = 0;
+                    unsigned long long s = zones(at, v);
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
-                        unsigned long long w = tab.w[tab.entry(v[e])];
-                        if (cut.key && !(v[e] > edge || (v[e] == edge && at + e < cut.idx))) w = 0;
+                        const unsigned long long w = tab.w[tab.entry(v[e])];
                         s += w >= least_w ? w : 0;
-                    }
-                    if (tab.any_in_zone(v)) {
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e)
-                            if (tab.in_zone(v[e])) s += kept(v[e], at + e);
                     }
                     s = wave_sum_weights(s);
                     if (lane == 0) sh.bin[c] = s;
                 });
+            } else if (summed) {  // mostly few are kept: what no lane keeps costs its comparison
+                row.skim([&](int c, int at, const float* v) {
+                    unsigned long long s = zones(at, v);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (v[e] >= edge && (v[e] > edge || at + e < cut.idx)) {
+                            const unsigned long long w = tab.w[tab.entry(v[e])];
+                            s += w >= least_w ? w : 0;
+                        }
+                    if (__any(s != 0)) s = wave_sum_weights(s);
+                    if (lane == 0) sh.bin[c] = s;
+                });
+            }
         }
     }
-    if (!summed) {
-#pragma unroll 1
-        for (int by_weight = 0; by_weight < 2; ++by_weight)
-            if (by_weight ? top_p < 1.f : top_k > 0 && top_k < row.n)
-                narrow(sh, row, cut, !by_weight, (unsigned long long)top_k, top_p);
+    const int per = ceil_div(row.chunks, kThreads), c0 = min(tid * per, row.chunks), c1 = min(c0 + per, row.chunks);
+    unsigned long long total;
+    auto chunk_scan = [&] {  // what lies before the thread's chunks, and the total
+        unsigned long long s = 0;
+        for (int c = c0; c < c1; ++c) s += sh.bin[c];
+        return block_scan(sh, s, total);
+    };
+    auto sums = [&](auto of) {  // a sum a chunk
         __syncthreads();
-        auto sums = [&](auto of) {
-            row.each([&](int c, int at, const float* v) {
-                unsigned long long s = 0;
+        row.each([&](int c, int at, const float* v) {
+            unsigned long long s = 0;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) s += of(v[e], at + e);
-                s = wave_sum_weights(s);
-                if (lane == 0) sh.bin[c] = s;
-            });
-        };
+            for (int e = 0; e < VEC; ++e) s += of(v[e], at + e);
+            s = wave_sum_weights(s);
+            if (lane == 0) sh.bin[c] = s;
+        });
+        __syncthreads();
+    };
+#pragma unroll 1
+    for (int by_weight = 0; by_weight < 2 && !summed; ++by_weight)
+        if (by_weight ? top_p < 1.f : top_k > 0 && top_k < row.n) {
+            const Narrowed o = narrow<T>(row, cut, !by_weight, (unsigned long long)top_k, top_p, least_w);
+            cut = o.cut;
+            summed = o.summed;
+        }
+    if (!summed) {
         if (cut.key == 0) sums([&](float v, int) {
             const unsigned long long w = row.weight(v);
             return w >= least_w ? w : 0;
@@ -737,10 +786,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
         else sums(kept);
     }
     __syncthreads();
-    const int per = ceil_div(row.chunks, kThreads), c0 = min(tid * per, row.chunks), c1 = min(c0 + per, row.chunks);
-    unsigned long long sum = 0, total;
-    for (int c = c0; c < c1; ++c) sum += sh.bin[c];
-    unsigned long long cum = block_scan(sh, sum, total);
+    unsigned long long cum = chunk_scan();
     double u = p.u_f64 ? ((const double*)p.u)[r] : (double)((const float*)p.u)[r];
     if (!(u >= 0.0)) u = 0.0;
     double goal = u * (double)total;
@@ -791,16 +837,17 @@ hipError_t sample_launch(const SampleParams& p, hipStream_t stream) {
     if (p.rows == 0) return hipSuccess;
     const dim3 grid((unsigned)p.rows);
     switch (p.dtype) {
-        case 0: DSALT_LAUNCH("sample", sample_kernel<float>, grid, dim3(kThreads), 0, stream, p); break;
+        case 0: DSALT_LAUNCH("sample", sample_kernel<float>, grid, dim3(kThreads), sizeof(Shared), stream, p); break;
         case 1: {
-            const unsigned lds = p.n_cols >= kTableCols ? 2 * kSide * sizeof(unsigned long long) : 0;
-            if (lds)
-                if (hipError_t e = hipFuncSetAttribute((const void*)sample_kernel<bf16>, hipFuncAttributeMaxDynamicSharedMemorySize, lds))
+            const unsigned table = p.n_cols >= kTableCols ? 2 * kSide * sizeof(unsigned long long) : 0;
+            if (table)
+                if (hipError_t e = hipFuncSetAttribute((const void*)sample_kernel<bf16>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                       (int)(sizeof(Shared) + table)))
                     return e;
-            DSALT_LAUNCH("sample", sample_kernel<bf16>, grid, dim3(kThreads), lds, stream, p);
+            DSALT_LAUNCH("sample", sample_kernel<bf16>, grid, dim3(kThreads), sizeof(Shared) + table, stream, p);
             break;
         }
-        default: DSALT_LAUNCH("sample", sample_kernel<f16>, grid, dim3(kThreads), 0, stream, p); break;
+        default: DSALT_LAUNCH("sample", sample_kernel<f16>, grid, dim3(kThreads), sizeof(Shared), stream, p); break;
     }
     return hipGetLastError();
 }
