@@ -345,61 +345,84 @@ __global__ __launch_bounds__(kPlanThreads) void rows_one_kernel(CacheRowsParams 
 // A block takes one piece (rows of one request within one page), one head, keys or values: the largest
 // finite magnitude of the rows gives the scale, codes held before the rows follow it where it grew, and
 // the rows are rounded to e4m3.  A scale is a power of two, so that dividing by it is exact and codes
-// that follow a larger one lose nothing above the subnormals.
-template <typename T>
-__global__ __launch_bounds__(256) void write_kernel(CacheWriteParams p) {
-    constexpr int VEC = 16 / sizeof(T);
+// that follow a larger one lose nothing above the subnormals.  Bound by memory: up to kKept vectors a thread
+// stay in registers between the two passes, more are read again (16001 float32 rows of 8 heads of 64: 18 us, 4.6 TB/s;
+// 21 with every row read twice).
+constexpr int kKept = 4;
+
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void write_kernel(CacheWriteParams p) {
+    constexpr int VEC = 16 / sizeof(T), WAVES = THREADS / 64;
     typedef T vec __attribute__((ext_vector_type(VEC), aligned(16)));
-    __shared__ float red[4];
+    __shared__ float red[WAVES], held_s;
     const int4 piece = ((const int4*)p.pieces)[blockIdx.x];
     const int row0 = piece.x, rows = piece.y, page = piece.z, off = piece.w;
     const int bt = 1 << p.c.bt_log, D = p.c.head_dim, g = blockIdx.y;
     // pieces past the last (no rows), and any that does not lie within the rows and one page
     if (rows <= 0 || row0 < 0 || rows > p.n_rows - row0 || page < 0 || page >= p.c.n_blocks || off < 0 || rows > bt - off) return;
+    const int tid = threadIdx.x;
     const bool val = blockIdx.z != 0;
     const T* x = (const T*)(val ? p.v : p.k) + (int64_t)row0 * (val ? p.v_st : p.k_st) + (int64_t)g * (val ? p.v_sh : p.k_sh);
     const int64_t st = val ? p.v_st : p.k_st;
     const int64_t tile = (int64_t)page * p.c.n_kv + g;
     uint8_t* codes = (val ? p.c.v : p.c.k) + tile * bt * D;
     float* scale = (val ? p.c.vs : p.c.ks) + tile;
-    const int per = D / VEC, n = rows * per, tid = threadIdx.x;
+    float held = 0.f;  // (one thread reads the scale, and it alone writes it)
+    if (tid == 0 && off > 0) held = *scale;
+    const int per = D / VEC, shift = __builtin_ctz(per), n = rows * per;
+    auto at = [&](int i) { return *(const vec*)(x + (i >> shift) * st + (i & (per - 1)) * VEC); };
+    vec kept[kKept];
     float amax = 0.f;
-    for (int i = tid; i < n; i += 256) {
-        const int r = i / per, c = (i - r * per) * VEC;
-        const vec v = *(const vec*)(x + r * st + c);
+    auto most = [&](const vec& v) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const float f = fabsf(to_float(v[e]));
             if (finite(f)) amax = fmaxf(amax, f);
         }
+    };
+#pragma unroll
+    for (int k = 0; k < kKept; ++k) {
+        kept[k] = vec{};
+        if (tid + k * THREADS < n) kept[k] = at(tid + k * THREADS);
     }
 #pragma unroll
+    for (int k = 0; k < kKept; ++k) most(kept[k]);
+    for (int i = tid + kKept * THREADS; i < n; i += THREADS) most(at(i));
+#pragma unroll
     for (int o = 32; o >= 1; o >>= 1) amax = fmaxf(amax, wave_xor(amax, o));
-    if ((tid & 63) == 0) red[tid >> 6] = amax;
-    __syncthreads();
-    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float held = off > 0 ? *scale : 0.f;
+    if constexpr (WAVES > 1) {
+        if ((tid & 63) == 0) red[tid >> 6] = amax;
+        if (tid == 0) held_s = held;
+        __syncthreads();
+        for (int k = 0; k < WAVES; ++k) amax = fmaxf(amax, red[k]);
+        held = held_s;
+    } else {
+        held = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(held)));
+    }
     const float s = fmaxf(scale_of(amax), held), inv = 1.f / s;
     if (s != held) {
         const float ratio = held * inv;
         uint32_t* u = (uint32_t*)codes;
-        for (int i = tid; i < off * D / 4; i += 256) {
+        for (int i = tid; i < off * D / 4; i += THREADS) {
             float f[4];
             e4m3_x4(u[i], f);
             u[i] = to_e4m3_x4(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
         }
+        if (tid == 0) *scale = s;
     }
-    for (int i = tid; i < n; i += 256) {
-        const int r = i / per, c = (i - r * per) * VEC;
-        const vec v = *(const vec*)(x + r * st + c);
-        uint32_t* o = (uint32_t*)(codes + (off + r) * D + c);
+    auto put = [&](int i, const vec& v) {
+        typedef uint32_t words __attribute__((ext_vector_type(VEC / 4)));
+        words o;
 #pragma unroll
         for (int e = 0; e < VEC; e += 4)
             o[e / 4] = to_e4m3_x4(to_float(v[e]) * inv, to_float(v[e + 1]) * inv, to_float(v[e + 2]) * inv,
                                   to_float(v[e + 3]) * inv);
-    }
-    __syncthreads();  // every thread has read the held scale
-    if (tid == 0) *scale = s;
+        *(words*)(codes + off * D + i * VEC) = o;
+    };
+#pragma unroll
+    for (int k = 0; k < kKept; ++k)
+        if (tid + k * THREADS < n) put(tid + k * THREADS, kept[k]);
+    for (int i = tid + kKept * THREADS; i < n; i += THREADS) put(i, at(i));
 }
 
 // ---------------------------------------------------------------------- read
@@ -445,8 +468,8 @@ __global__ __launch_bounds__(256) void read_kernel(CacheReadParams p) {
 
 }  // namespace
 
-// One launch while a block's sums are its own small share (and page counts fit 31 bits): 64 requests 10.2 -> 6 us, 1500
-// requests with 32768 rows 16.4 -> 9.
+// One launch while every block can form the sums for itself (and page counts fit 31 bits): 64 requests 7.7 us, 10.2 in two
+// launches, 1500 requests with 32768 rows 11.8 and 16.4.
 static bool rows_in_one(int n_reqs, int cols) { return n_reqs <= kOneReqs && (int64_t)n_reqs * cols < 0x7fffffff; }
 
 size_t cache_rows_ws_bytes(int n_reqs, int cols) { return rows_in_one(n_reqs, cols) ? 0 : 256 + (size_t)n_reqs * sizeof(ReqPlan); }
@@ -463,13 +486,22 @@ hipError_t cache_rows_launch(const CacheRowsParams& p, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <typename T>
+static void write_pieces(const CacheWriteParams& p, hipStream_t stream) {
+    const dim3 grid((unsigned)p.n_pieces, (unsigned)p.c.n_kv, 2);
+    // a wave where there are as many pieces as rows (200 rows, 16 heads of 128: 9.1 us with four waves, 6.8 with one), or a
+    // whole page is what it keeps (16384 bfloat16 rows of 8 heads of 128 in pages of 16: 37 and 24)
+    const int vecs = (p.c.head_dim * (int)sizeof(T) / 16) << p.c.bt_log;
+    if (p.n_pieces == p.n_rows || vecs <= 64 * kKept) DSALT_LAUNCH("cache_write", (write_kernel<T, 64>), grid, dim3(64), 0, stream, p);
+    else DSALT_LAUNCH("cache_write", (write_kernel<T, 256>), grid, dim3(256), 0, stream, p);
+}
+
 hipError_t cache_write_launch(const CacheWriteParams& p, hipStream_t stream) {
     if (p.n_pieces == 0 || p.n_rows == 0) return hipSuccess;
-    const dim3 grid((unsigned)p.n_pieces, (unsigned)p.c.n_kv, 2);
     switch (p.dtype) {
-        case 0: DSALT_LAUNCH("cache_write", write_kernel<float>, grid, dim3(256), 0, stream, p); break;
-        case 1: DSALT_LAUNCH("cache_write", write_kernel<bf16>, grid, dim3(256), 0, stream, p); break;
-        default: DSALT_LAUNCH("cache_write", write_kernel<f16>, grid, dim3(256), 0, stream, p); break;
+        case 0: write_pieces<float>(p, stream); break;
+        case 1: write_pieces<bf16>(p, stream); break;
+        default: write_pieces<f16>(p, stream); break;
     }
     return hipGetLastError();
 }

@@ -145,6 +145,8 @@ struct List {
             acc[e] = 0.f;
         }
     }
+    // a bias in base 2 (the type's lowest values stay finite, as masks of them are apart from minus infinity)
+    __device__ __forceinline__ static float base2(float b) { return b > -INFINITY ? fmaxf(b * kLog2e, -3e38f) : b; }
     // the page of position j where it is attended, else -1
     __device__ __forceinline__ int page(int j, bool attended) const {
         const int b = j >> p.c.bt_log;
@@ -179,7 +181,7 @@ struct List {
             x[i] = -INFINITY;
             if (i >= used) continue;
             const bool on = __shfl(s.key, i * KPW + sub) != kNone;
-            const float ks = __shfl(s.ks, i * KPW + sub), bias = p.lbias ? __shfl(s.bias, i * KPW + sub) * kLog2e : 0.f;
+            const float ks = __shfl(s.ks, i * KPW + sub), bias = p.lbias ? base2(__shfl(s.bias, i * KPW + sub)) : 0.f;
             float d = 0.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) e4m3_x4(ku[i][e], f + 4 * e);
@@ -277,7 +279,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void cache_attn_list_kernel(CacheAt
     auto look = [&](int i) {
         const bool lm = i >= nwin && i < b1;
         const int64_t at = lm ? set + i - nwin : -1;
-        int j = r.low + i;
+        int j = (int)((unsigned)r.low + (unsigned)i);
         if (lm) j = p.lmk[at];
         return list.place(j, list.page(j, lm ? j < r.low : i < b1), at);
     };

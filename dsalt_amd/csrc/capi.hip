@@ -899,6 +899,8 @@ int dsalt_cache_read(const dsalt_cache_read_args* a, dsalt_stream_t stream) {
     if ((rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols, a->c.block_tokens))) return rc;
     if (a->n_rows < 0) return fail(DSALT_ERR_INVALID, "n_rows must be >= 0, got %d", a->n_rows);
     if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if ((int64_t)a->n_rows * a->c.n_kv_heads > 0x7fffffff)
+        return fail(DSALT_ERR_INVALID, "n_rows x n_kv_heads must stay below 2^31 (got %d x %d)", a->n_rows, a->c.n_kv_heads);
     if (a->n_rows == 0) return DSALT_OK;
     if (!a->cu_seqlens || !a->k || !a->v || !aligned16(a->k) || !aligned16(a->v))
         return fail(DSALT_ERR_INVALID, "cu_seqlens, k and v (16-byte aligned) are required");

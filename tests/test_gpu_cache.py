@@ -400,6 +400,31 @@ def test_attention_empty_by_bias():
     assert np.isneginf(lse[0]).all() and np.isfinite(lse[1]).all()
 
 
+@pytest.mark.parametrize("lowest", [-1e4, -3.4e38])
+def test_attention_masks_of_the_lowest_value(lowest):
+    """Landmarks masked by a large negative bias weigh nothing beside others, and share the weight where they are all
+    that a row attends."""
+    q, cache, table, req, pos, w, lmk = _attend_case(2, 2, 1, 64, 16, 8, torch.float32, 2, 60, 4, lens=[60, 60])
+    w, table[0, 3] = [4, 4], -1
+    lmk[:] = np.arange(8) * 4
+    bias = np.zeros(lmk.shape)
+    bias[:, 0] = lowest
+    bias[:, 1, :, ::2] = lowest
+    out, _ = ops.cache_attention(q.to(DEV), cache, _i32(table), _i32(req), _i32(pos), _i32(w), _i32(lmk),
+                                 torch.from_numpy(bias).float().to(DEV))
+    pages = _host_pages(cache)
+    same = np.zeros(lmk.shape)  # a bias common to all that is attended changes no weight
+    if lowest == -1e4:
+        ref, *_ = OD.attention(f64(q), pages, table, req, pos, w, lmk, same, 0.125)
+        assert np.allclose(f64(out)[0], ref[0], rtol=0, atol=2e-3 * np.abs(ref[0]).max())  # logits beside 1e4 keep 2^-10 of a unit
+    else:  # beside 3.4e38 logits do not count: the mean of the values
+        v = np.stack([pages.token(table[0], int(p))[1][0] for p in lmk[0, 0, 0]])
+        assert np.allclose(f64(out)[0], v.mean(0), rtol=0, atol=1e-5 * np.abs(v).max())
+    keep = np.where(bias[:, 1:2] < 0, -1, lmk[:, 1:2])
+    ref, *_ = OD.attention(f64(q)[1:], pages, table[1:], [0], pos[1:], w[1:], keep, None, 0.125)
+    assert np.allclose(f64(out)[1], ref[0], rtol=0, atol=1e-5 * np.abs(ref).max())
+
+
 def test_attention_strides_and_layouts():
     c = _attend_case(5, 4, 2, 64, 32, 6, torch.bfloat16, 8, 120, 30)
     x = torch.randn(5, 3, 4, 64).to(torch.bfloat16)
@@ -569,6 +594,40 @@ def test_step_captured_and_replayed():
         for a, b in zip(live["cache"], eager["cache"]):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
     assert live["span"][0] > 9 and live["span"][1] > 80  # pages were taken and given back
+
+
+def test_large_calls_captured_and_replayed():
+    """A call whose window is split and joined, one with more than 64 KB of LDS, and a row whose weights are by value: each
+    replay equals the eager call on the inputs of the moment."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    a = _attend_case(1, 32, 2, 128, 64, 20, torch.bfloat16, 3, 12000, 9000, lens=[12000])
+    b = _attend_case(140, 32, 2, 128, 64, 20, torch.bfloat16, 4, 200, 120)
+    cases = [(q.to(DEV), cache, *(_i32(x) for x in rest[:4]), _i32(rest[4])) for q, cache, *rest in (a, b)]
+    x, u = torch.zeros(5, 9001, device=DEV, dtype=torch.bfloat16), torch.zeros(5, device=DEV)
+
+    def step():
+        return [*ops.cache_attention(*cases[0], w_max=9000), *ops.cache_attention(*cases[1], w_max=200), *ops.sample_rows(x, u, top_p=0.9),
+                *ops.sample_rows(x, u, top_k=20)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for rep in range(4):
+        x.copy_(torch.randn(x.shape, generator=g, device=DEV) * 3)
+        u.copy_(torch.rand(5, generator=g, device=DEV))
+        for c in cases:
+            c[0].copy_(torch.randn(c[0].shape, generator=g, device=DEV))
+        ref = step()
+        torch.cuda.synchronize()
+        for t in outs:
+            t.fill_(-3)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(outs, ref)), rep
 
 
 def test_two_streams_at_once():

@@ -110,16 +110,19 @@ def test_random_numbers_at_the_ends():
 
 
 @pytest.mark.parametrize("dt", TYPES)
-def test_layouts(dt):
+@pytest.mark.parametrize("V", [2005, 9001])
+def test_layouts(dt, V):
     """Rows off 16-byte boundaries, columns of a wider buffer, a transposed buffer, rows that repeat."""
-    x, u = _logits(6, 2005, dt, 9)
+    x, u = _logits(6, V, dt, 9)
     ref = _check(x, u, top_p=0.9)
-    wide = torch.zeros(6, 2077, dtype=dt, device=DEV)
+    wide = torch.zeros(6, V + 72, dtype=dt, device=DEV)
     for off in range(1, 9):
-        y = wide[:, off:off + 2005]
+        y = wide[:, off:off + V]
         y.copy_(x)
-        wide[:, :off], wide[:, off + 2005:] = 1e4, 1e4  # what lies beside a row is not its own
+        wide[:, :off], wide[:, off + V:] = 1e4, 1e4  # what lies beside a row is not its own
         assert torch.equal(_check(y, u, top_p=0.9), ref)
+        _check(y, u)
+        _check(y, u, top_k=30, min_p=0.01)
     assert torch.equal(_check(x.t().contiguous().t(), u, top_p=0.9), ref)
     _check(x[:1].expand(6, -1), u, top_k=50)
 
@@ -129,6 +132,37 @@ def test_large_vocabularies(dt, V):
     x, u = _logits(3, V, dt, 1)
     x[2] = 1.0  # sums as large as they get
     for kw in (dict(), dict(top_k=50, top_p=0.95), dict(top_p=0.95), dict(top_k=V // 2), dict(min_p=1e-4), dict(temperature=30.0, top_p=0.9)):
+        _check(x, u, **kw)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("V", [2047, 2048, 2049, 8191, 8193, 20011])
+def test_each_side_of_the_size_rules(dt, V):
+    """Rows that are listed whole, searched, and (bfloat16 from 8192 on) weighed by value; lists of up to 256, 1024 and
+    2048 tokens, and more than they hold; flat and peaked rows."""
+    for spread in (0.02, 2.5, 12.0):
+        x, u = _logits(4, V, dt, V, spread)
+        for kw in (dict(), dict(top_p=0.9), dict(top_p=0.5, min_p=0.001), dict(top_k=200), dict(top_k=700, top_p=0.999), dict(top_k=1024),
+                   dict(top_k=1025, top_p=0.7), dict(temperature=0.1, top_p=0.95), dict(temperature=20.0, top_p=0.3)):
+            _check(x, u, **kw)
+
+
+def test_bfloat16_values_on_both_sides_of_zero():
+    """What the weights by value treat apart: zeros of both signs, subnormals and small magnitudes (most of the
+    row, and where a prefix ends), all logits negative, all positive, magnitudes up to the largest."""
+    V = 10007
+    g = torch.Generator().manual_seed(0)
+    tiny = torch.randn(V, generator=g) * 1e-30
+    rows = [torch.zeros(V), tiny, torch.where(torch.rand(V, generator=g) < 0.7, torch.zeros(V), torch.randn(V, generator=g)),
+            -torch.rand(V, generator=g) * 20 - 3, torch.rand(V, generator=g) * 5 + 40, torch.randn(V, generator=g) * 1e-3,
+            torch.randn(V, generator=g) * 1e37, torch.full((V,), -0.0), torch.randn(V, generator=g).abs() * 1e-6 - 25]
+    x = torch.stack(rows).to(torch.bfloat16)
+    x[:, ::997] = torch.finfo(torch.bfloat16).min
+    x[5, 13], x[8, 77], x[2, 5] = 0.0, 3e-7, float("nan")
+    x = x.to(DEV)
+    u = torch.rand(len(rows), generator=g).to(DEV)
+    for kw in (dict(), dict(top_p=0.6), dict(top_p=0.97), dict(top_k=3000), dict(top_k=5000, top_p=0.5), dict(top_k=9999), dict(min_p=0.5),
+               dict(temperature=1e-4, top_p=0.9), dict(temperature=1e30, top_p=0.9), dict(temperature=1e-38), dict(top_k=64, top_p=0.9)):
         _check(x, u, **kw)
 
 
