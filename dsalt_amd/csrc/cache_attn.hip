@@ -154,10 +154,12 @@ struct List {
         const int pg = r.table[in ? b : 0];
         return in && pg >= 0 && pg < p.c.n_blocks ? pg : -1;
     }
+    // (a bias of minus infinity masks its key, so that what the cache holds there is not read)
     __device__ __forceinline__ Slot place(int j, int pg, int64_t bias_at) const {
         const uint32_t tile = (uint32_t)max(pg, 0) * (uint32_t)p.c.n_kv + (uint32_t)g;
         const uint32_t key = (tile << p.c.bt_log) + (uint32_t)(j & ((1 << p.c.bt_log) - 1));
-        return Slot{pg < 0 ? kNone : key, p.c.ks[tile], p.c.vs[tile], p.lbias && bias_at >= 0 ? p.lbias[bias_at] : 0.f};
+        const float bias = p.lbias && bias_at >= 0 ? p.lbias[bias_at] : 0.f;
+        return Slot{pg < 0 || bias == -INFINITY ? kNone : key, p.c.ks[tile], p.c.vs[tile], bias};
     }
     // the wave's NB slots (`n` of them used); `next` is called once the batch's keys and values are requested
     template <typename F>

@@ -913,7 +913,7 @@ def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None
     form for single tokens of many requests.  Row t is the token at position ``pos[t]`` of request ``req[t]``
     (CacheRows.req, .pos), its own key and value written; it attends its window [pos - w + 1, pos] and the
     landmarks before the window of its head's set in lmk_idx [H, R, 1, K] (any order, negative slots empty, a
-    position may repeat; select_landmarks' sets).  Rows without a key (inert rows, pages that the table does not
+    position may repeat; select_landmarks' sets; a bias of -inf masks its landmark).  Rows without a key (inert rows, pages that the table does not
     name) give zeros and -inf.  ``w_max``: no window is longer (host value; splits the work, longer windows only
     cost time).  Not differentiable."""
     at = _on(q, *cache, table, req, pos, w, lmk_idx, lmk_bias)

@@ -449,7 +449,8 @@ int    dsalt_cache_read(const dsalt_cache_read_args* a, dsalt_stream_t stream);
  * pos[t] of request req[t] and attends W = [pos - w + 1, pos] and the landmarks p < pos - w + 1 of
  * its head's set (any order; negative slots are empty; a position may repeat, each copy counts).  out
  * and lse as dsalt_fwd; rows that attend nothing (pos or req outside their ranges, all pages absent)
- * give zeros and -inf.  Masked keys are never read into a result, whatever their pages hold. */
+ * give zeros and -inf.  Masked keys, a landmark of bias -inf among them, are never read into a result,
+ * whatever their pages hold. */
 typedef struct dsalt_cache_attn_args {
     dsalt_cache c;
     int32_t n_rows;            /* T                                                  */

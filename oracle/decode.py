@@ -146,8 +146,9 @@ def attention(q, pages, table, req, pos, w, lmk, bias, scale):
             mine = list(window)
             for s in range(lmk.shape[3]):
                 p = int(lmk[h, r, 0, s])
-                if 0 <= p < low and token(p) is not None:
-                    mine.append((p, float(bias[h, r, 0, s]) if bias is not None else 0.0))
+                b = float(bias[h, r, 0, s]) if bias is not None else 0.0
+                if 0 <= p < low and b > -np.inf and token(p) is not None:
+                    mine.append((p, b))
             if not mine:
                 continue
             K = np.stack([token(p)[0][g] for p, _ in mine])

@@ -400,6 +400,26 @@ def test_attention_empty_by_bias():
     assert np.isneginf(lse[0]).all() and np.isfinite(lse[1]).all()
 
 
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_attention_reads_nothing_behind_a_bias_of_minus_infinity(dt, wide):
+    """Landmarks masked by their bias hold NaN (keys, values or scales): results as without them."""
+    H, G, bt = 8, 2, 16
+    q, cache, table, req, pos, w, lmk = _attend_case(3, H, G, 64, bt, 6, dt, 5, 200, 9, lens=[200, 150, 90])
+    w = [9, 9, 9]
+    lmk[:] = np.array([0, 17, 33, 40, 49, 64])
+    bias = np.random.RandomState(0).randn(*lmk.shape)
+    bias[..., [1, 2, 4]] = -np.inf
+    clean = _host_pages(cache)
+    for r in range(3):
+        cache.k.view(torch.uint8)[table[r, 1], :, 1] = 0x7f
+        cache.v.view(torch.uint8)[table[r, 2], :, 1] = 0xff
+        cache.k_scale[table[r, 3]] = cache.v_scale[table[r, 3]] = float("nan")
+    bound = (1 << 15) + 31 if wide else 30
+    out, lse = _check_attend(q, cache, _widened(table, bt, bound), req, pos, w, lmk, bias=bias, pages=clean, w_max=bound)
+    assert np.isfinite(out).all() and np.isfinite(lse).all()
+
+
 @pytest.mark.parametrize("lowest", [-1e4, -3.4e38])
 def test_attention_masks_of_the_lowest_value(lowest):
     """Landmarks masked by a large negative bias weigh nothing beside others, and share the weight where they are all
