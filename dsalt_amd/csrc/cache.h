@@ -7,6 +7,8 @@
 
 namespace dsalt {
 
+constexpr int64_t kLaunchThreads = 0xffffffffll;  // a launch's threads along its first dimension
+
 // k and v [n_blocks, n_kv, 1 << bt_log, head_dim] e4m3, scales [n_blocks, n_kv]
 struct CachePages {
     int n_blocks, n_kv, bt_log, head_dim;

@@ -432,38 +432,39 @@ template <typename T>
 __global__ __launch_bounds__(256) void read_kernel(CacheReadParams p) {
     typedef T vec __attribute__((ext_vector_type(8), aligned(16)));
     const int D = p.c.head_dim, per = p.c.n_kv * (D / 8);
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)p.n_rows * per) return;
-    const int t = (int)(i / per), x = (int)(i - (int64_t)t * per), g = x / (D / 8), c = (x - g * (D / 8)) * 8;
-    int lo = 0, hi = p.n_reqs;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (p.cu[mid + 1] > t) hi = mid;
-        else lo = mid + 1;
-    }
-    vec k = {}, v = {};
-    if (lo < p.n_reqs && t >= p.cu[lo]) {
-        const int64_t pos = (int64_t)(p.start ? p.start[lo] : 0) + t - p.cu[lo];
-        const int64_t b = pos >> p.c.bt_log;
-        const int page = pos >= 0 && b < p.cols ? p.table[lo * p.table_st + b] : -1;
-        if (page >= 0 && page < p.c.n_blocks) {
-            const int64_t tile = (int64_t)page * p.c.n_kv + g;
-            const int64_t at = ((tile << p.c.bt_log) + (pos & ((1 << p.c.bt_log) - 1))) * D + c;
-            const u32x2 ku = *(const u32x2*)(p.c.k + at), vu = *(const u32x2*)(p.c.v + at);
-            const float ks = p.c.ks[tile], vs = p.c.vs[tile];
-            float f[8];
-            e4m3_x4(ku[0], f);
-            e4m3_x4(ku[1], f + 4);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) k[e] = from_float<T>(f[e] * ks);
-            e4m3_x4(vu[0], f);
-            e4m3_x4(vu[1], f + 4);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = from_float<T>(f[e] * vs);
+    const int64_t n = (int64_t)p.n_rows * per;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int t = (int)(i / per), x = (int)(i - (int64_t)t * per), g = x / (D / 8), c = (x - g * (D / 8)) * 8;
+        int lo = 0, hi = p.n_reqs;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (p.cu[mid + 1] > t) hi = mid;
+            else lo = mid + 1;
         }
+        vec k = {}, v = {};
+        if (lo < p.n_reqs && t >= p.cu[lo]) {
+            const int64_t pos = (int64_t)(p.start ? p.start[lo] : 0) + t - p.cu[lo];
+            const int64_t b = pos >> p.c.bt_log;
+            const int page = pos >= 0 && b < p.cols ? p.table[lo * p.table_st + b] : -1;
+            if (page >= 0 && page < p.c.n_blocks) {
+                const int64_t tile = (int64_t)page * p.c.n_kv + g;
+                const int64_t at = ((tile << p.c.bt_log) + (pos & ((1 << p.c.bt_log) - 1))) * D + c;
+                const u32x2 ku = *(const u32x2*)(p.c.k + at), vu = *(const u32x2*)(p.c.v + at);
+                const float ks = p.c.ks[tile], vs = p.c.vs[tile];
+                float f[8];
+                e4m3_x4(ku[0], f);
+                e4m3_x4(ku[1], f + 4);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) k[e] = from_float<T>(f[e] * ks);
+                e4m3_x4(vu[0], f);
+                e4m3_x4(vu[1], f + 4);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = from_float<T>(f[e] * vs);
+            }
+        }
+        *(vec*)((T*)p.k + (int64_t)t * p.c.n_kv * D + g * D + c) = k;
+        *(vec*)((T*)p.v + (int64_t)t * p.c.n_kv * D + g * D + c) = v;
     }
-    *(vec*)((T*)p.k + (int64_t)t * p.c.n_kv * D + g * D + c) = k;
-    *(vec*)((T*)p.v + (int64_t)t * p.c.n_kv * D + g * D + c) = v;
 }
 
 }  // namespace
@@ -488,12 +489,18 @@ hipError_t cache_rows_launch(const CacheRowsParams& p, hipStream_t stream) {
 
 template <typename T>
 static void write_pieces(const CacheWriteParams& p, hipStream_t stream) {
-    const dim3 grid((unsigned)p.n_pieces, (unsigned)p.c.n_kv, 2);
     // a wave where there are as many pieces as rows (200 rows, 16 heads of 128: 9.1 us with four waves, 6.8 with one), or a
     // whole page is what it keeps (16384 bfloat16 rows of 8 heads of 128 in pages of 16: 37 and 24)
     const int vecs = (p.c.head_dim * (int)sizeof(T) / 16) << p.c.bt_log;
-    if (p.n_pieces == p.n_rows || vecs <= 64 * kKept) DSALT_LAUNCH("cache_write", (write_kernel<T, 64>), grid, dim3(64), 0, stream, p);
-    else DSALT_LAUNCH("cache_write", (write_kernel<T, 256>), grid, dim3(256), 0, stream, p);
+    const bool wave = p.n_pieces == p.n_rows || vecs <= 64 * kKept;
+    CacheWriteParams s = p;
+    for (int64_t k = 0; k < p.n_pieces; k += s.n_pieces) {
+        s.n_pieces = (int)std::min(p.n_pieces - k, kLaunchThreads / 256);
+        s.pieces = p.pieces + 4 * k;
+        const dim3 grid((unsigned)s.n_pieces, (unsigned)p.c.n_kv, 2);
+        if (wave) DSALT_LAUNCH("cache_write", (write_kernel<T, 64>), grid, dim3(64), 0, stream, s);
+        else DSALT_LAUNCH("cache_write", (write_kernel<T, 256>), grid, dim3(256), 0, stream, s);
+    }
 }
 
 hipError_t cache_write_launch(const CacheWriteParams& p, hipStream_t stream) {
@@ -509,7 +516,7 @@ hipError_t cache_write_launch(const CacheWriteParams& p, hipStream_t stream) {
 hipError_t cache_read_launch(const CacheReadParams& p, hipStream_t stream) {
     if (p.n_rows == 0) return hipSuccess;
     const int64_t n = (int64_t)p.n_rows * p.c.n_kv * (p.c.head_dim / 8);
-    const dim3 grid((unsigned)((n + 255) / 256));
+    const dim3 grid((unsigned)std::min((n + 255) / 256, (int64_t)1 << 20));
     switch (p.dtype) {
         case 0: DSALT_LAUNCH("cache_read", read_kernel<float>, grid, dim3(256), 0, stream, p); break;
         case 1: DSALT_LAUNCH("cache_read", read_kernel<bf16>, grid, dim3(256), 0, stream, p); break;

@@ -595,8 +595,7 @@ AttnPlan attn_plan(const CacheAttnParams& p) {
 }
 
 template <typename T, int D>
-hipError_t run(const CacheAttnParams& p, hipStream_t stream) {
-    const AttnPlan a = attn_plan(p);
+hipError_t run_rows(const CacheAttnParams& p, const AttnPlan& a, hipStream_t stream) {
     const dim3 grid((unsigned)((int64_t)p.n_rows * p.c.n_kv * a.tiles), (unsigned)a.ns);
     if (a.list) {
         auto kernel = a.waves == 8 ? cache_attn_list_kernel<T, D, 8> : cache_attn_list_kernel<T, D, 4>;
@@ -613,6 +612,24 @@ hipError_t run(const CacheAttnParams& p, hipStream_t stream) {
         DSALT_LAUNCH("cache_attn_join", (cache_attn_join_kernel<T, D>), join, dim3(64 * kJoinWaves), 0, stream, p, a.ns);
     }
     return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t run(const CacheAttnParams& p, hipStream_t stream) {
+    const AttnPlan a = attn_plan(p);
+    const int most = (int)(kLaunchThreads / 256 / (p.c.n_kv * a.tiles));  // rows of a launch (more than one launch: blocks of four waves, no splits)
+    CacheAttnParams s = p;
+    for (int t = 0; t < p.n_rows; t += s.n_rows) {
+        s.n_rows = std::min(most, p.n_rows - t);
+        s.q = (const T*)p.q + (int64_t)t * p.q_st;
+        s.out = (T*)p.out + (int64_t)t * p.o_st;
+        s.lse = p.lse + (int64_t)t * p.n_heads;
+        s.req = p.req + t;
+        s.pos = p.pos + t;
+        s.w = p.w + t;
+        if (hipError_t e = run_rows<T, D>(s, a, stream)) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace

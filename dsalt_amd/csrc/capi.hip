@@ -827,7 +827,8 @@ int dsalt_cache_rows(const dsalt_cache_rows_args* a, dsalt_stream_t stream) {
         return fail(DSALT_ERR_INVALID, "block_tokens must be 16, 32, 64 or 128, got %d", a->block_tokens);
     int rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols, a->block_tokens);
     if (rc) return rc;
-    if (a->n_rows < 0) return fail(DSALT_ERR_INVALID, "n_rows must be >= 0, got %d", a->n_rows);
+    if (a->n_rows < 0 || a->n_rows > (1 << 30) || a->n_reqs > (1 << 24))
+        return fail(DSALT_ERR_INVALID, "n_rows must be in [0, 2^30] and n_reqs at most 2^24, got %d, %d", a->n_rows, a->n_reqs);
     const int64_t most = (int64_t)a->n_rows / a->block_tokens + 2 * (int64_t)a->n_reqs;
     if (a->n_pieces < (most < a->n_rows ? most : a->n_rows) || a->n_pieces > a->n_rows)
         return fail(DSALT_ERR_INVALID, "n_pieces must be in [min(n_rows, n_rows / block_tokens + 2 n_reqs), n_rows], got %d", a->n_pieces);

@@ -19,6 +19,8 @@
 // us on the device, 256 bfloat16 rows of 151936 (77.8 MB, 15.6 at the copy rate): largest logit 18, top_k 50 42,
 // temperature alone 47, top_p 0.9 at temperature 0.5 67, at temperature 2, where most is kept, 94.  One row: 12, 31,
 // 38, 46, 79.
+#include <algorithm>
+
 #include "common.h"
 #include "sample.h"
 #include "timing.h"
@@ -839,10 +841,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     }
 }
 
-}  // namespace
-
-hipError_t sample_launch(const SampleParams& p, hipStream_t stream) {
-    if (p.rows == 0) return hipSuccess;
+hipError_t sample_some(const SampleParams& p, hipStream_t stream) {
     const dim3 grid((unsigned)p.rows);
     switch (p.dtype) {
         case 0: DSALT_LAUNCH("sample", sample_kernel<float>, grid, dim3(kThreads), sizeof(Shared), stream, p); break;
@@ -858,6 +857,28 @@ hipError_t sample_launch(const SampleParams& p, hipStream_t stream) {
         default: DSALT_LAUNCH("sample", sample_kernel<f16>, grid, dim3(kThreads), sizeof(Shared), stream, p); break;
     }
     return hipGetLastError();
+}
+
+}  // namespace
+
+// (rows of a launch: its threads stay below 2^32)
+hipError_t sample_launch(const SampleParams& p, hipStream_t stream) {
+    constexpr int most = (1 << 22) - 1;
+    const size_t esize = p.dtype == 0 ? 4 : 2;
+    SampleParams s = p;
+    for (int64_t r = 0; r < p.rows; r += s.rows) {
+        s.rows = (int)std::min((int64_t)most, p.rows - r);
+        s.x = (const char*)p.x + r * p.x_st * (int64_t)esize;
+        s.u = (const char*)p.u + r * (p.u_f64 ? 8 : 4);
+        s.temperature = p.temperature ? p.temperature + r : nullptr;
+        s.top_p = p.top_p ? p.top_p + r : nullptr;
+        s.min_p = p.min_p ? p.min_p + r : nullptr;
+        s.top_k = p.top_k ? p.top_k + r : nullptr;
+        s.token = p.token + r;
+        s.logp = p.logp + r;
+        if (hipError_t e = sample_some(s, stream)) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace dsalt

@@ -856,8 +856,8 @@ def cache_rows_(seq_len, new_len, table, free_blocks, span, n_rows: int, *, bloc
         raise ValueError("free_blocks must be contiguous int32 [entries]")
     if span.shape != (2,) or span.dtype != torch.int64 or not span.is_contiguous():
         raise ValueError("span must be int64 [2]")
-    if n_rows < 0 or block_tokens not in BLOCK_TOKENS:
-        raise ValueError(f"n_rows must be >= 0 and block_tokens one of {BLOCK_TOKENS}, got {n_rows}, {block_tokens}")
+    if not 0 <= n_rows <= 1 << 30 or block_tokens not in BLOCK_TOKENS:
+        raise ValueError(f"n_rows must be in [0, 2^30] and block_tokens one of {BLOCK_TOKENS}, got {n_rows}, {block_tokens}")
     old, new = _vec_i32(seq_len, R, "seq_len"), _vec_i32(new_len, R, "new_len")
     n_pieces = min(n_rows, n_rows // block_tokens + 2 * R)
     # the outputs lie side by side in two buffers
@@ -898,8 +898,8 @@ def cache_read(cache: Cache8, table, cu_seqlens, *, start=None, n_rows: int, dty
     R, M, ts = _table_args(table)
     cu = _vec_i32(cu_seqlens, R + 1, "cu_seqlens")
     st = _vec_i32(start, R, "start") if start is not None else None
-    if n_rows < 0:
-        raise ValueError(f"n_rows must be >= 0, got {n_rows}")
+    if not 0 <= n_rows < 1 << 31:
+        raise ValueError(f"n_rows must be in [0, 2^31), got {n_rows}")
     k = torch.empty(n_rows, c.n_kv_heads, c.head_dim, dtype=dtype, device=at)
     v = torch.empty_like(k)
     a = CacheReadArgs(c, R, M, n_rows, dtype_code(dtype), table.data_ptr(), ts, cu.data_ptr(),
@@ -934,7 +934,7 @@ def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     out = torch.empty(T, H, D, dtype=q.dtype, device=at)
     lse = torch.empty(T, H, dtype=torch.float32, device=at)
-    a = CacheAttnArgs(c, T, H, R, M, K, dtype_code(q.dtype), 0 if w_max is None else int(w_max), table.data_ptr(),
+    a = CacheAttnArgs(c, T, H, R, M, K, dtype_code(q.dtype), 0 if w_max is None else max(-1, min(int(w_max), 1 << 30)), table.data_ptr(),
                       ts, *q_at, rq.data_ptr(), ps.data_ptr(), wc.data_ptr(),
                       li.data_ptr() if K else None, lb.data_ptr() if lb is not None and K else None,
                       out.data_ptr(), H * D, D, lse.data_ptr(), scale)
@@ -953,8 +953,8 @@ def sample_rows(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     log probability among the kept.  Rows without a logit above -inf give -1 and -inf."""
     per_row = [t if isinstance(t, torch.Tensor) else None for t in (temperature, top_k, top_p, min_p)]
     at = _on(logits, u, *per_row)
-    if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_VOCAB:
-        raise ValueError(f"logits must be [R, V] with V in [1, {MAX_VOCAB}], got {tuple(logits.shape)}")
+    if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_VOCAB or logits.shape[0] >= 1 << 31:
+        raise ValueError(f"logits must be [R, V] with R < 2^31 and V in [1, {MAX_VOCAB}], got {tuple(logits.shape)}")
     R, V = logits.shape
     if V > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()

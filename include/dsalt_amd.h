@@ -390,7 +390,7 @@ typedef struct dsalt_cache_rows_args {
     int32_t n_reqs;
     int32_t table_cols;
     int32_t block_tokens;
-    int32_t n_rows;            /* rows of req, pos and slot (host value)              */
+    int32_t n_rows;            /* rows of req, pos and slot (host value), at most 2^30 */
     int32_t n_pieces;          /* rows of pieces, at least
                                   min(n_rows, n_rows / block_tokens + 2 n_reqs)       */
     int64_t n_free;            /* entries of the ring, >= the pages in circulation    */

@@ -75,6 +75,14 @@ def test_rows_refusals(field, value, code):
     _refused("dsalt_cache_rows", a, code)
 
 
+@pytest.mark.parametrize("field,value", [("n_rows", (1 << 30) + 1), ("n_rows", 0x7fffffff), ("n_reqs", (1 << 24) + 1)])
+def test_rows_past_the_largest_sizes(field, value):
+    a = _rows_args()
+    a.n_pieces = 1 << 27
+    setattr(a, field, value)
+    _refused("dsalt_cache_rows", a, 1, b"at most 2^24")
+
+
 def _write_args(c=None):
     return _lib.CacheWriteArgs(c or _cache(), 32, 4, 1, FAKE, 128, 64, FAKE, 128, 64, FAKE)
 

@@ -676,6 +676,63 @@ def test_two_streams_at_once():
         assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+# ------------------------------------------------------------------------ more than one launch holds
+def _repeats(x, ref):
+    """x [T, ...] is ref [n, ...] over and over."""
+    n, whole = len(ref), len(x) // len(ref) * len(ref)
+    return torch.equal(x[whole:], ref[:len(x) - whole]) and bool((x[:whole].view(-1, *ref.shape) == ref).all())
+
+
+def test_attention_of_more_rows_than_a_launch_holds():
+    q, cache, table, req, pos, w, lmk = _attend_case(64, 16, 16, 64, 16, 2, torch.bfloat16, 1, 40, 5)
+    args = [_i32(x) for x in (req, pos, w)]
+    out, lse = ops.cache_attention(q.to(DEV), cache, _i32(table), *args, _i32(lmk), w_max=5)
+    T = (1 << 20) + 77
+    turn = torch.arange(T, device=DEV) % 64
+    big, bl = ops.cache_attention(q.to(DEV)[turn], cache, _i32(table), *(x[turn] for x in args), _i32(lmk), w_max=5)
+    assert _repeats(big, out) and _repeats(bl, lse)
+
+
+def test_read_of_more_rows_than_a_launch_holds():
+    cache = _random_cache(5, 4, 16, 64, 2)
+    R = (1 << 17) + 3  # requests of 64 tokens in the same four pages, the last one cut short
+    table = _i32([[3, 0, 4, 1]]).expand(R, 4).contiguous()
+    n = 64 * R - 5
+    k, v = ops.cache_read(cache, table, torch.arange(R + 1, dtype=torch.int32, device=DEV) * 64, n_rows=n)
+    rk, rv = ops.cache_read(cache, table[:1], _i32([0, 64]), n_rows=64)
+    assert rk.any() and _repeats(k, rk) and _repeats(v, rv)
+
+
+def test_write_of_more_pieces_than_a_launch_holds():
+    """Most pieces hold no rows; those that do lie on both sides of where a launch ends."""
+    P, x = (1 << 24) + 9, torch.randn(40, 2, 64).to(torch.bfloat16).to(DEV)
+    few = _i32([[4 * i, 4, i, i] for i in range(10)])
+    at = torch.tensor([0, 1, 77, (1 << 24) - 3, (1 << 24) - 2, (1 << 24) - 1, 1 << 24, (1 << 24) + 1, P - 2, P - 1], device=DEV)
+    pieces = torch.zeros((P, 4), dtype=torch.int32, device=DEV)
+    pieces[at] = few
+    a, b = (ops.cache_write_(x, x + 1, ops.new_cache(10, 2, 64, block_tokens=16), p) for p in (few, pieces))
+    assert a.k_scale.all() and all(torch.equal(s.view(torch.uint8), t.view(torch.uint8)) for s, t in zip(a, b))
+
+
+def test_sizes_past_32_bits_are_refused():
+    c = ops.new_cache(4, 2, 64, block_tokens=16)
+    t, i = _i32([[0, 1]]), _i32([0])
+    span, ring = torch.tensor([0, 4], device=DEV), _i32([0, 1, 2, 3])
+    for n in ((1 << 30) + 1, (1 << 32) + 1):
+        with pytest.raises(ValueError, match="n_rows"):
+            ops.cache_rows_(i, i, t, ring, span, n)
+    for n in (1 << 31, (1 << 32) + 1):
+        with pytest.raises(ValueError, match="n_rows"):
+            ops.cache_read(c, t, _i32([0, 4]), n_rows=n)
+    with pytest.raises(ValueError, match="logits"):
+        ops.sample_rows(torch.zeros(1, 4, device=DEV).expand((1 << 32) + 1, 4), torch.zeros(1, device=DEV))
+    lmk = _i32(np.zeros((2, 1, 1, 2)))
+    q = torch.zeros(1, 2, 64, device=DEV)
+    a = ops.cache_attention(q, c, t, i, i, i, lmk)
+    b = ops.cache_attention(q, c, t, i, i, i, lmk, w_max=1 << 40)  # (no window is longer than the table either)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_argument_checks():
     c = ops.new_cache(4, 2, 64, block_tokens=16)
     x = torch.zeros(3, 2, 64, device=DEV)

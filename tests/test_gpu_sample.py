@@ -177,6 +177,20 @@ def test_draws_follow_the_probabilities():
     assert torch.allclose(lp.double(), torch.log(p)[tok], atol=1e-6)
 
 
+def test_more_rows_than_a_launch_holds():
+    """Rows that repeat, each with settings of its own."""
+    n, R = 64, (1 << 22) + 70
+    x, u = _logits(n, 5, torch.float32, 6)
+    r = np.random.RandomState(1)
+    s = [torch.tensor(v, dtype=dt, device=DEV) for v, dt in ((r.rand(n) * 2, torch.float32), (r.randint(0, 6, n), torch.int32),
+                                                             (r.rand(n) * 1.2, torch.float32), (r.rand(n) * 0.4, torch.float32))]
+    turn = torch.arange(R, device=DEV) % n
+    for un in (u, u.double()):
+        ref = ops.sample_rows(x, un, temperature=s[0], top_k=s[1], top_p=s[2], min_p=s[3])
+        got = ops.sample_rows(x[turn], un[turn], **dict(zip(("temperature", "top_k", "top_p", "min_p"), (v[turn] for v in s))))
+        assert all(torch.equal(a, b[turn]) for a, b in zip(got, ref))
+
+
 def test_argument_checks():
     x, u = torch.zeros(3, 5, device=DEV), torch.zeros(3, device=DEV)
     for a in ((x[0], u), (x, u[:2]), (x[:, :0], u)):
