@@ -16,9 +16,9 @@
 // A pass over the row reads it from memory once and from the caches after that; what bounds it is the
 // arithmetic of one compute unit a row, in float64 where weights are formed (a float32 weight is off by 2^-24
 // of itself, which over 150000 tokens moves a border of the running sums past u once in some thousand draws).
-// us on the device, 256 bfloat16 rows of 151936 (77.8 MB, 15.6 at the copy rate): largest logit 18, top_k 50 42,
-// temperature alone 47, top_p 0.9 at temperature 0.5 67, at temperature 2, where most is kept, 94.  One row: 12, 31,
-// 38, 46, 79.
+// us on the device, 256 bfloat16 rows of 151936 (77.8 MB, 15.6 at the copy rate): largest logit 18, top_k 50 43,
+// temperature alone 46, top_p 0.9 at temperature 0.5 58, at temperature 2, where most is kept, 75 (94 where the equal
+// elements at the prefix's end are counted by a pass of their own).  One row: 12, 31, 37, 43, 63.
 #include <algorithm>
 
 #include "common.h"
@@ -553,9 +553,9 @@ struct Table {
     }
 };
 
-// The filters from counts of each entry (no list, or more than it holds).  False where a prefix ends among
-// the keys that have none.
-__device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, const Table& tab, Cut& cut, int top_k, float top_p) {
+// The filters from counts of each entry (no list, or more than it holds): `cut` is the last value kept, `keep` how many of it
+// (-1: all).  False where a prefix ends among the keys that have no entry.
+__device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, const Table& tab, Cut& cut, int& keep_out, int top_k, float top_p) {
     constexpr int PER = 2 * kSide / kThreads;
     uint32_t* count = (uint32_t*)sh.list;
     static_assert(2 * kSide * sizeof(uint32_t) <= sizeof(sh.list), "a count an entry");
@@ -647,7 +647,10 @@ __device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, cons
         }
         __syncthreads();
     }
-    if (end >= 0) keep_equal(sh, row, cut, key_of<bf16>(tab.value(end)), keep, ties);
+    if (end >= 0) {
+        cut = {key_of<bf16>(tab.value(end)), 0x7fffffff};
+        if (keep < ties) keep_out = (int)keep;
+    }
     return true;
 }
 
@@ -717,54 +720,71 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
         summed = cut_list(sh, row, cut, least, top_k > 0 ? top_k : row.n, top_p, least_w, 0);
     }
     // kept weights a chunk, then the chunk, lane and element in which the running sum passes u times the total
-    auto kept = [&](float v, int i) -> unsigned long long {
-        if (cut.key && !cut.keeps(key_of<T>(v), i)) return 0;
-        const unsigned long long w = row.weight(v);
-        return w >= least_w ? w : 0;
-    };
+    const int per = ceil_div(row.chunks, kThreads), c0 = min(tid * per, row.chunks), c1 = min(c0 + per, row.chunks);
+    unsigned long long total;
+    uint32_t* ties = (uint32_t*)sh.list;  // equal elements at the end of a prefix, a chunk: there, then kept
+    bool tied = false;
     if constexpr (Key<T>::bits == 16) {
         if (!summed && row.n >= kTableCols && !inf) {
             const Table tab(sample_lds + sizeof(Shared) / sizeof(unsigned long long), row, row.value(top) - 30.f * temp);
-            summed = !filters || cut_table(sh, row, tab, cut, top_k, top_p);
-            const float edge = row.value(cut.key);
-            __syncthreads();
-            auto zones = [&](int at, const float* v) {
-                unsigned long long s = 0;
-                if (tab.any_in_zone(v)) {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        if (tab.in_zone(v[e])) s += kept(v[e], at + e);
-                }
-                return s;
-            };
-            if (summed && cut.key == 0) {
-                row.skim([&](int c, int at, const float* v) {
-                    unsigned long long s = zones(at, v);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const unsigned long long w = tab.w[tab.entry(v[e])];
-                        s += w >= least_w ? w : 0;
+            int keep = -1;
+            summed = !filters || cut_table(sh, row, tab, cut, keep, top_k, top_p);
+            if (summed) {
+                // what is not kept weighs nothing from here on, nor does what ends the prefix where it is kept in part: a
+                // chunk's number of those is counted, and which of them are kept follows once all are
+                const float edge = cut.key ? row.value(cut.key) : -INFINITY;
+                tied = keep >= 0;
+                const unsigned long long tie_w = tied ? tab.w[tab.entry(edge)] : 0;
+                __syncthreads();
+                if (cut.key || least_w)
+                    for (int i = tid; i < 2 * kSide; i += kThreads) {
+                        const float v = tab.value(i);
+                        if (v < edge || (tied && v == edge) || tab.w[i] < least_w) tab.w[i] = 0;
                     }
-                    s = wave_sum_weights(s);
-                    if (lane == 0) sh.bin[c] = s;
-                });
-            } else if (summed) {  // mostly few are kept: what no lane keeps costs its comparison
+                __syncthreads();
                 row.skim([&](int c, int at, const float* v) {
-                    unsigned long long s = zones(at, v);
+                    unsigned long long s = 0;
+                    float m = v[0];
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        if (v[e] >= edge && (v[e] > edge || at + e < cut.idx)) {
-                            const unsigned long long w = tab.w[tab.entry(v[e])];
-                            s += w >= least_w ? w : 0;
+                    for (int e = 1; e < VEC; ++e) m = fmaxf(m, v[e]);
+                    if (m >= edge) {
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) s += tab.w[tab.entry(v[e])];
+                        if (tab.any_in_zone(v)) {
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e)
+                                if (tab.in_zone(v[e]) && v[e] > edge) {
+                                    const unsigned long long w = row.weight(v[e]);
+                                    s += w >= least_w ? w : 0;
+                                }
                         }
+                    }
                     if (__any(s != 0)) s = wave_sum_weights(s);
                     if (lane == 0) sh.bin[c] = s;
+                    if (tied) {
+                        uint32_t n = 0;
+                        if (__any(m >= edge)) {
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) n += (uint32_t)__popcll(__ballot(v[e] == edge));
+                        }
+                        if (lane == 0) ties[c] = n;
+                    }
                 });
+                __syncthreads();
+                if (tied) {
+                    unsigned long long n = 0;
+                    for (int c = c0; c < c1; ++c) n += ties[c];
+                    int64_t left = keep - (int64_t)block_scan(sh, n, total);
+                    for (int c = c0; c < c1; ++c) {
+                        const int there = (int)ties[c], stay = (int)min(max(left, (int64_t)0), (int64_t)there);
+                        left -= there;
+                        ties[c] = (uint32_t)stay;
+                        if (tie_w >= least_w) sh.bin[c] += (unsigned long long)stay * tie_w;
+                    }
+                }
             }
         }
     }
-    const int per = ceil_div(row.chunks, kThreads), c0 = min(tid * per, row.chunks), c1 = min(c0 + per, row.chunks);
-    unsigned long long total;
     auto chunk_scan = [&] {  // what lies before the thread's chunks, and the total
         unsigned long long s = 0;
         for (int c = c0; c < c1; ++c) s += sh.bin[c];
@@ -788,6 +808,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
             cut = o.cut;
             summed = o.summed;
         }
+    const float edge = row.value(cut.key);
+    auto kept = [&](float v, int i) -> unsigned long long {
+        if (cut.key && !(v > edge || (v == edge && i < cut.idx))) return 0;
+        const unsigned long long w = row.weight(v);
+        return w >= least_w ? w : 0;
+    };
     if (!summed) {
         if (cut.key == 0) sums([&](float v, int) {
             const unsigned long long w = row.weight(v);
@@ -815,6 +841,28 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
         const int at = row.first((int)sh.found[0]);
         float v[VEC];
         row.load(at, v);
+        if (tied) {  // the chunk's first equal element that is not kept
+            int n = 0, out = 0x7fffffff;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) n += v[e] == edge;
+            int in = n;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int o = __shfl_up(in, d);
+                if (lane >= d) in += o;
+            }
+            int before = in - n;
+            const int stay = (int)ties[(int)sh.found[0]];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (v[e] == edge) {
+                    if (before == stay) out = at + e;
+                    ++before;
+                }
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) out = min(out, __shfl_xor(out, o));
+            cut.idx = out;
+        }
         unsigned long long w[VEC], s = 0;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) s += w[e] = row.has(at + e) ? kept(v[e], at + e) : 0;
