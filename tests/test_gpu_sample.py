@@ -166,6 +166,21 @@ def test_bfloat16_values_on_both_sides_of_zero():
         _check(x, u, **kw)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+def test_prefixes_that_end_near_zero(dt):
+    """Logits even over [-1000, 1000] at temperature 1000: prefixes end at logits about 0, where those are closest to each
+    other beside the largest."""
+    V = 30011
+    g = torch.Generator().manual_seed(2)
+    x = (torch.rand(24, V, generator=g) * 2000 - 1000).to(dt).to(DEV)
+    x[::2, ::3] *= 1e-5
+    u = torch.rand(24, generator=g).to(DEV)
+    for p in (np.linspace(0.725, 0.737, 24), np.linspace(0.62, 0.83, 24)):
+        _check(x, u, temperature=1000.0, top_p=list(p))
+    _check(x, u, temperature=1000.0, top_k=[int(k) for k in np.linspace(9000, 21000, 24)])
+    _check(x, u, temperature=1000.0, top_k=[int(k) for k in np.linspace(1025, 2100, 24)], top_p=0.95, min_p=0.3)
+
+
 def test_draws_follow_the_probabilities():
     """65536 rows of one distribution, u an even grid: counts are the probabilities to one part of the grid a token."""
     n = 1 << 16
