@@ -15,9 +15,11 @@
 // A pass over the row reads it from memory once and from the caches after that; what bounds it is the
 // arithmetic of one compute unit a row, in float64 where weights are formed (a float32 weight is off by 2^-24
 // of itself, which over 150000 tokens moves a border of the running sums past u once in some thousand draws).
-// us on the device, 256 bfloat16 rows of 151936 (77.8 MB, 15.6 at the copy rate): largest logit 18, top_k 50 43,
-// temperature alone 46, top_p 0.9 at temperature 0.5 58, at temperature 2, where most is kept, 75 (94 where the equal
-// elements at the prefix's end are counted by a pass of their own).  One row: 12, 31, 37, 43, 63.
+// The first pass notes each chunk's largest logit, so that passes over what a filter may keep read few chunks where
+// it keeps little (256 rows, top_k 50: 34 us, 43 with every chunk read again).
+// us on the device, 256 bfloat16 rows of 151936 (77.8 MB, 15.6 at the copy rate): largest logit 18, top_k 50 34,
+// temperature alone 44, top_p 0.9 at temperature 0.5 48, at temperature 2, where most is kept, 73 (92 where the equal
+// elements at the prefix's end are counted by a pass of their own).  One row: 11, 29, 35, 39, 62.
 #include <algorithm>
 
 #include "common.h"
@@ -57,6 +59,7 @@ struct Shared {
     unsigned long long part[kWaves];
     unsigned long long found[4];
     int count;
+    uint16_t top[kBins + 8];            // upper bits of the key of a chunk's largest logit
 };
 
 // All of a block's LDS: Shared, then the table of bfloat16 rows.  Dynamic, so that a function that is called rather than
@@ -97,6 +100,19 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
     auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     return b[0] + b[1];
 }
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)));
+}
+// maxima over the wave of four values: lanes 0 to 15 get the first one's, then the third's, the second's and the fourth's
+__device__ __forceinline__ float wave_max4(const float* v) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[0]), __float_as_uint(v[1]), false, false);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[2]), __float_as_uint(v[3]), false, false);
+    const float x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])), y = fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+    auto c = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return dpp_max<0x128>(dpp_max<0x124>(dpp_max<0x122>(dpp_max<0x121>(fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]))))));
+}
+__device__ __forceinline__ uint16_t upper_key(float v) { return (uint16_t)(key_of<bf16>(v)); }
 // the same for weights: sums of at most 64 x 8 of 2^42, in two parts of 25 and 20 bits a lane
 __device__ __forceinline__ unsigned long long wave_sum_weights(unsigned long long v) {
     return ((unsigned long long)wave_sum((uint32_t)(v >> 25)) << 25) + wave_sum((uint32_t)v & 0x1ffffffu);
@@ -140,6 +156,7 @@ struct Row {
             for (int e = 0; e < VEC; ++e) v[e] = at + e >= 0 && at + e < n ? to_float(x[at + e]) : NAN;
         }
     }
+    __device__ __forceinline__ static int wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
     // f(chunk, first element of the lane, its VEC values) for the wave's chunks, three of them requested ahead
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
@@ -148,7 +165,7 @@ struct Row {
             if (inside(c)) u = *(global_vec*)(x + first(c));
             return u;
         };
-        int c = threadIdx.x >> 6;
+        int c = wave();
         vec r0 = fetch(c), r1 = fetch(c + kWaves), r2 = fetch(c + 2 * kWaves);
         for (; c < chunks; c += kWaves) {
             float v[VEC];
@@ -161,9 +178,14 @@ struct Row {
             f(c, first(c), v);
         }
     }
-    // the same for passes of few instructions, which wait for memory: eight chunks requested ahead
+    // the same for passes of few instructions, which wait for memory: eight chunks requested ahead (and `four` after each
+    // four, with the first of them)
     template <typename F>
     __device__ __forceinline__ void skim(F f) const {
+        skim(f, [](int) {});
+    }
+    template <typename F, typename G>
+    __device__ __forceinline__ void skim(F f, G four) const {
         constexpr int N = 4;
         auto fetch = [&](int c, vec* r) {
 #pragma unroll
@@ -172,7 +194,7 @@ struct Row {
                 if (inside(c + k * kWaves)) r[k] = *(global_vec*)(x + first(c + k * kWaves));
             }
         };
-        int c = threadIdx.x >> 6;
+        int c = wave();
         vec r[N], next[N];
         fetch(c, r);
         for (; c < chunks; c += N * kWaves) {
@@ -189,7 +211,59 @@ struct Row {
                 }
                 r[k] = next[k];
             }
+            four(c);
         }
+    }
+    // the same for the chunks whose largest logit may be `low` or more; the others are not read
+    template <typename F>
+    __device__ __forceinline__ void pick(const uint16_t* top, float low, F f) const {
+        constexpr int N = 4;
+        const uint32_t least = upper_key(low);
+        const int lane = threadIdx.x & 63;
+        for (int b = wave(); b < chunks; b += 64 * kWaves) {
+            const int mine = b + lane * kWaves;
+            unsigned long long left = __ballot(mine < chunks && top[min(mine, chunks - 1)] >= least);
+            auto fetch = [&](int* c, vec* r) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    c[k] = left ? b + __builtin_ctzll(left) * kWaves : -1;
+                    left &= left - 1;
+                    r[k] = vec{};
+                    if (c[k] >= 0 && inside(c[k])) r[k] = *(global_vec*)(x + first(c[k]));
+                }
+            };
+            int c[N], next_c[N];
+            vec r[N], next[N];
+            fetch(c, r);
+            while (c[0] >= 0) {
+                fetch(next_c, next);
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    if (c[k] >= 0) {
+                        float v[VEC];
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) v[e] = to_float(r[k][e]);
+                        if (!inside(c[k])) load(first(c[k]), v);
+                        f(c[k], first(c[k]), v);
+                    }
+                    c[k] = next_c[k];
+                    r[k] = next[k];
+                }
+            }
+        }
+    }
+    // the one or the other, by the number of such chunks (one row of 151936, top_p 0.9 at temperature 2: 64 us with those
+    // picked though most are, 60 with all read)
+    template <typename F>
+    __device__ __forceinline__ void seek(const uint16_t* top, float low, F f) const {
+        const uint32_t least = upper_key(low);
+        int n = 0;
+        for (int b = wave(); b < chunks; b += 64 * kWaves) {
+            const int c = b + (int)(threadIdx.x & 63) * kWaves;
+            n += __popcll(__ballot(c < chunks && top[min(c, chunks - 1)] >= least));
+        }
+        if (2 * kWaves * n < chunks) pick(top, low, f);
+        else skim(f);
     }
     __device__ __forceinline__ bool has(int i) const { return (unsigned)i < (unsigned)n; }
     // round(2^42 2^t), t = (v - m) log2(e) / temperature.  (v - m is exact, and t below -43 rounds to 0, NaN and
@@ -397,7 +471,7 @@ __device__ __forceinline__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut
     if (tid == 0) sh.count = 0;
     __syncthreads();
     const float low = row.value(least);
-    row.skim([&](int, int at, const float* v) {
+    row.seek(sh.top, low, [&](int, int at, const float* v) {
         float m = v[0];
 #pragma unroll
         for (int e = 1; e < VEC; ++e) m = fmaxf(m, v[e]);
@@ -448,7 +522,7 @@ __device__ __forceinline__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut
 // exponents, over which logits spread as they do over their range, finds the one in which the prefix ends; its elements
 // are listed and sorted, or all from there up, where those are few (True: that has cut the row, see cut_list).  Where one
 // part holds more than a list does, a radix search goes on over keys.
-// (200 float32 rows of 151936, top_p 0.9: 172 us, 270 with a radix search alone, whose first bins few of the logits fill.)
+// (200 float32 rows of 151936, top_p 0.9: 168 us, 270 with a radix search alone, whose first bins few of the logits fill.)
 // A call of its own: inlined, the registers it needs cost every row that does without it (float32 rows, temperature
 // alone, 75 -> 83 us).
 struct Narrowed {
@@ -504,7 +578,7 @@ __device__ __attribute__((noinline)) Narrowed narrow(const Row<T> row, Cut cut, 
         __syncthreads();
         if (tid == 0) sh.count = 0;
         __syncthreads();
-        row.skim([&](int, int at, const float* v) {
+        row.seek(sh.top, lo, [&](int, int at, const float* v) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
                 if (v[e] >= lo && v[e] <= hi && row.bin_of(row.exponent(v[e])) == (int)bin && inside(v[e], at + e)) {
@@ -750,19 +824,30 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     const float temp = p.temperature ? p.temperature[r] : p.temperature_all;
     const float top_p = p.top_p ? p.top_p[r] : p.top_p_all, min_p = p.min_p ? p.min_p[r] : p.min_p_all;
     const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
-    // the largest logit and its first index
+    const bool filters = (top_k > 0 && top_k < row.n) || top_p < 1.f;
+    // the largest logit and its first index, and each chunk's largest where chunks may be passed over later
     float best = -INFINITY;
     int best_i = 0;
-    row.skim([&](int, int at, const float* v) {
-        float m = v[0];
+    float four[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    row.skim(
+        [&](int, int at, const float* v) {
+            float m = v[0];
 #pragma unroll
-        for (int e = 1; e < VEC; ++e) m = fmaxf(m, v[e]);
-        if (m > best) {
-            best = m;
+            for (int e = 1; e < VEC; ++e) m = fmaxf(m, v[e]);
+            if (m > best) {
+                best = m;
 #pragma unroll
-            for (int e = VEC - 1; e >= 0; --e) best_i = v[e] == m ? at + e : best_i;
-        }
-    });
+                for (int e = VEC - 1; e >= 0; --e) best_i = v[e] == m ? at + e : best_i;
+            }
+            four[0] = four[1], four[1] = four[2], four[2] = four[3], four[3] = m;
+        },
+        [&](int c) {
+            if (!filters) return;
+            // (after fewer than four, at the row's end, the first of them is not four[0])
+            const int n = min((row.chunks - 1 - c) / kWaves + 1, 4), k = ((lane >> 5) | (lane >> 3 & 2)) - (4 - n);
+            const uint16_t key = upper_key(wave_max4(four));
+            if ((lane & 15) == 0 && k >= 0) sh.top[c + k * kWaves] = key;
+        });
     const uint32_t own = key_of<T>(best);
     unsigned long long first = ((unsigned long long)own << 32) | (uint32_t)~best_i;
 #pragma unroll
@@ -795,7 +880,6 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     row.rate = inf ? 1.0 : 1.4426950408889634 / (double)temp;
     const unsigned long long least_w = min_p > 0.f ? (unsigned long long)ceil((double)min_p * (double)kUnit) : 0;
     Cut cut = {0u, 0};
-    const bool filters = (top_k > 0 && top_k < row.n) || top_p < 1.f;
     bool summed = false;
     if (filters && (row.n <= kList || (top_k > 0 && top_k <= kThreads))) {
         uint32_t least = key_of<T>(-INFINITY);
@@ -824,8 +908,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
                         const float v = tab.value(i);
                         if (v < edge || (tied && v == edge) || tab.w[i] < least_w) tab.w[i] = 0;
                     }
+                for (int c = tid; c < row.chunks; c += kThreads) sh.bin[c] = ties[c] = 0;
                 __syncthreads();
-                row.skim([&](int c, int at, const float* v) {
+                auto draw = [&](int c, int at, const float* v) {
                     unsigned long long s = 0;
                     float m = v[0];
 #pragma unroll
@@ -852,7 +937,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
                         }
                         if (lane == 0) ties[c] = n;
                     }
-                });
+                };
+                if (cut.key) row.seek(sh.top, edge, draw);
+                else row.skim(draw);
                 __syncthreads();
                 if (tied) {
                     unsigned long long n = 0;
