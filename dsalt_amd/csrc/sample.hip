@@ -18,9 +18,10 @@
 // The first pass notes each chunk's largest logit, so that passes over what a filter may keep read few chunks where
 // it keeps little (256 rows, top_k 50: 34 us, 43 with every chunk read again).
 // us on the device, 256 bfloat16 rows of 151936 (77.8 MB, 15.6 at the copy rate): largest logit 18, top_k 50 34,
-// temperature alone 44, top_p 0.9 at temperature 0.5 48, at temperature 2, where most is kept, 73 (92 where the equal
-// elements at the prefix's end are counted by a pass of their own).  One row: 11, 29, 35, 39, 62.
+// temperature alone 41, top_p 0.9 at temperature 0.5 46, at temperature 2, where most is kept, 68 (73 with an element's
+// entry found by itself, 92 with a pass more for the equal elements at the prefix's end).  One row: 11, 29, 31, 36, 55.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "sample.h"
@@ -157,7 +158,30 @@ struct Row {
         }
     }
     __device__ __forceinline__ static int wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
-    // f(chunk, first element of the lane, its VEC values) for the wave's chunks, three of them requested ahead
+    // f(chunk, first element of the lane, its VEC values: as floats, or as they are stored where it takes those); r is what
+    // was requested of the chunk
+    template <typename F>
+    __device__ __forceinline__ void give(F f, int c, const vec& r) const {
+        if constexpr (std::is_invocable_v<F, int, int, u32x4>) {
+            u32x4 u = __builtin_bit_cast(u32x4, r);
+            if (!inside(c)) {
+                float v[VEC];
+                load(first(c), v);
+                vec y;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) y[e] = (T)v[e];
+                u = __builtin_bit_cast(u32x4, y);
+            }
+            f(c, first(c), u);
+        } else {
+            float v[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = to_float(r[e]);
+            if (!inside(c)) load(first(c), v);
+            f(c, first(c), v);
+        }
+    }
+    // f (see give) for the wave's chunks, three of them requested ahead
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
         auto fetch = [&](int c) {
@@ -168,14 +192,11 @@ struct Row {
         int c = wave();
         vec r0 = fetch(c), r1 = fetch(c + kWaves), r2 = fetch(c + 2 * kWaves);
         for (; c < chunks; c += kWaves) {
-            float v[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = to_float(r0[e]);
-            if (!inside(c)) load(first(c), v);
+            const vec r = r0;
             r0 = r1;
             r1 = r2;
             r2 = fetch(c + 3 * kWaves);
-            f(c, first(c), v);
+            give(f, c, r);
         }
     }
     // the same for passes of few instructions, which wait for memory: eight chunks requested ahead (and `four` after each
@@ -202,13 +223,7 @@ struct Row {
 #pragma unroll
             for (int k = 0; k < N; ++k) {
                 const int ck = c + k * kWaves;
-                if (ck < chunks) {
-                    float v[VEC];
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) v[e] = to_float(r[k][e]);
-                    if (!inside(ck)) load(first(ck), v);
-                    f(ck, first(ck), v);
-                }
+                if (ck < chunks) give(f, ck, r[k]);
                 r[k] = next[k];
             }
             four(c);
@@ -239,13 +254,7 @@ struct Row {
                 fetch(next_c, next);
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
-                    if (c[k] >= 0) {
-                        float v[VEC];
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e) v[e] = to_float(r[k][e]);
-                        if (!inside(c[k])) load(first(c[k]), v);
-                        f(c[k], first(c[k]), v);
-                    }
+                    if (c[k] >= 0) give(f, c[k], r[k]);
                     c[k] = next_c[k];
                     r[k] = next[k];
                 }
@@ -670,45 +679,70 @@ __device__ __forceinline__ uint32_t reached_by(Shared& sh, uint32_t mine, unsign
 }
 
 // Weights of bfloat16 logits by value: few values lie between the largest logit and where weights round to 0, so each is
-// formed once and an element costs a look-up.  An entry a sign and magnitude (the upper bits of the float32) from a0,
-// the last of each sign for all beyond, of weight 0.  Magnitudes below a0 (2^-16 of the largest that weighs, and always
-// zeros) are weighed directly.
-constexpr int kSide = 2048, kTableCols = 8192;
+// formed once and an element costs a look-up.  An entry a sign and magnitude (the upper bits of the float32) from a0, the
+// second of each sign; the last of each sign stands for all beyond, of weight 0.  Magnitudes below a0 (2^-15 of the largest
+// that weighs, and always zeros) have each sign's first entry, of weight 0: they are weighed directly.
+// What bounds the passes is the arithmetic of an element, so that entries are found two elements at a time in halves of
+// 32 bits, and an entry holds its weight in two parts of 21 bits whose sums over a wave stay below 2^32.
+constexpr int kSide = 2048, kTableCols = 16384;
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2_ __attribute__((ext_vector_type(2)));
+
+// the entries of a vector of eight logits: within a side, then of the table
+struct Entries {
+    u16x2 side[4];
+    uint32_t two[4];
+    __device__ __forceinline__ int operator[](int e) const { return (int)(two[e / 2] >> (e & 1) * 16 & 0xffffu); }
+};
 
 struct Table {
-    unsigned long long* w;  // [2 kSide]
+    u32x2_* w;  // [2 kSide] lower 21 bits, upper bits
     uint32_t a0;
 
     // the table of a row; weights are 0 below the logit `low`
-    __device__ __forceinline__ Table(unsigned long long* lds, const Row<bf16>& row, float low) : w(lds) {
+    __device__ __forceinline__ Table(unsigned long long* lds, const Row<bf16>& row, float low) : w((u32x2_*)lds) {
         const float m = (float)row.m;
         const uint32_t up = m > 0.f ? __float_as_uint(m) >> 16 : 0;
         const uint32_t down = low < 0.f ? min((__float_as_uint(-low) >> 16) + 1, 0x7f7fu) : 0;
         const uint32_t most = max(up, down);
-        a0 = most > kSide - 1 ? most - (kSide - 2) : 1;
+        a0 = most > kSide - 3 ? most - (kSide - 3) : 1;
         __syncthreads();
         for (int i = threadIdx.x; i < 2 * kSide; i += kThreads) {
             const float v = value(i);
-            w[i] = (i & (kSide - 1)) < kSide - 1 && v <= m ? row.weight(v) : 0;
+            const unsigned long long x = holds(i) && v <= m ? row.weight(v) : 0;
+            w[i] = u32x2_{(uint32_t)x & 0x1fffffu, (uint32_t)(x >> 21)};
         }
         __syncthreads();
     }
+    __device__ __forceinline__ static bool holds(int i) { return (uint32_t)((i & (kSide - 1)) - 1) < (uint32_t)(kSide - 2); }
+    __device__ __forceinline__ unsigned long long weight(int i) const { return ((unsigned long long)w[i][1] << 21) + w[i][0]; }
     __device__ __forceinline__ float value(int i) const {
-        return __uint_as_float((uint32_t)(i / kSide) << 31 | ((uint32_t)(i & (kSide - 1)) + a0) << 16);
+        return __uint_as_float((uint32_t)(i / kSide) << 31 | ((uint32_t)(i & (kSide - 1)) + a0 - 1) << 16);
+    }
+    __device__ __forceinline__ Entries entries(u32x4 u) const {
+        Entries n;
+        const u16x2 less = {(uint16_t)(a0 - 1), (uint16_t)(a0 - 1)}, most = {kSide - 1, kSide - 1};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const u16x2 mag = __builtin_bit_cast(u16x2, u[k] & 0x7fff7fffu);
+            n.side[k] = __builtin_elementwise_min(__builtin_elementwise_sub_sat(mag, less), most);
+            n.two[k] = (u[k] >> 4 & 0x08000800u) | __builtin_bit_cast(uint32_t, n.side[k]);
+        }
+        return n;
     }
     __device__ __forceinline__ int entry(float v) const {
-        const uint32_t u = __float_as_uint(v);
-        return (int)(((u >> 31) * kSide) + min(((u >> 16) & 0x7fffu) - a0, (uint32_t)(kSide - 1)));
+        return entries(u32x4{__float_as_uint(v) >> 16, 0, 0, 0})[0];
     }
     __device__ __forceinline__ bool in_zone(float v) const { return fabsf(v) < __uint_as_float(a0 << 16); }
     // whether any of eight values is
-    __device__ __forceinline__ bool any_in_zone(const float* v) const {
-        float m = fabsf(v[0]);
-#pragma unroll
-        for (int e = 1; e < 8; ++e) m = fminf(m, fabsf(v[e]));
-        return in_zone(m);
+    __device__ __forceinline__ static bool any_in_zone(const Entries& n) {
+        const u16x2 m = __builtin_elementwise_min(__builtin_elementwise_min(n.side[0], n.side[1]),
+                                                  __builtin_elementwise_min(n.side[2], n.side[3]));
+        return m[0] == 0 || m[1] == 0;
     }
 };
+__device__ __forceinline__ float element(u32x4 u, int e) { return __uint_as_float(e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16); }
 
 // The filters from counts of each entry (no list, or more than it holds): `cut` is the last value kept, `keep` how many of it
 // (-1: all).  False where a prefix ends among the keys that have no entry.
@@ -722,20 +756,19 @@ __device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, cons
     for (int i = tid; i < 2 * kSide; i += kThreads) count[i] = 0;
     if (tid < 2) zone[tid] = 0;
     __syncthreads();
-    row.skim([&](int, int at, const float* v) {
-        if (tab.any_in_zone(v)) {
+    row.skim([&](int, int, u32x4 u) {
+        const Entries n = tab.entries(u);
+        if (tab.any_in_zone(n)) {
 #pragma unroll
             for (int e = 0; e < Row<bf16>::VEC; ++e)
-                if (tab.in_zone(v[e])) {
+                if (tab.in_zone(element(u, e))) {
                     atomicAdd(&zone[0], 1ull);
-                    atomicAdd(&zone[1], row.weight(v[e]));
+                    atomicAdd(&zone[1], row.weight(element(u, e)));
                 }
         }
 #pragma unroll
-        for (int e = 0; e < Row<bf16>::VEC; ++e) {
-            const int i = tab.entry(v[e]);
-            if ((i & (kSide - 1)) != kSide - 1) atomicAdd(&count[i], 1u);
-        }
+        for (int e = 0; e < Row<bf16>::VEC; ++e)
+            if (n.side[e / 2][e & 1] != kSide - 1) atomicAdd(&count[n[e]], 1u);
     });
     __syncthreads();
     const unsigned long long zn = zone[0], zw = zone[1];
@@ -748,8 +781,8 @@ __device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, cons
     unsigned long long c[PER], w[PER], ca, wa, cn = 0, wn = 0, call, wall;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-        c[e] = count[at(e)];
-        w[e] = tab.w[at(e)];
+        c[e] = tab.holds(at(e)) ? count[at(e)] : 0;
+        w[e] = tab.weight(at(e));
         cn += c[e];
         wn += c[e] * w[e];
     }
@@ -786,7 +819,7 @@ __device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, cons
         end = (int)sh.found[0];
         keep = k - sh.found[1];
         ties = sh.found[3];
-        whole = sh.found[2] + keep * tab.w[end];
+        whole = sh.found[2] + keep * tab.weight(end);
         __syncthreads();
     }
     if (top_p < 1.f) {
@@ -795,7 +828,7 @@ __device__ __forceinline__ bool cut_table(Shared& sh, const Row<bf16>& row, cons
                 return (double)w0 < thr && !((double)(w0 + n * w) < thr);
             })) {
             const int i = (int)sh.found[0];
-            const unsigned long long r = reach(sh.found[2], tab.w[i], sh.found[3], thr);
+            const unsigned long long r = reach(sh.found[2], tab.weight(i), sh.found[3], thr);
             keep = i == end && keep < r ? keep : r;
             end = i;
             ties = sh.found[3];
@@ -892,7 +925,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     uint32_t* ties = (uint32_t*)sh.list;  // equal elements at the end of a prefix, a chunk: there, then kept
     bool tied = false;
     if constexpr (Key<T>::bits == 16) {
-        if (!summed && row.n >= kTableCols && !inf) {
+        // (one row, temperature alone: 8192 12.0 us, 13.1 with a table, 16384 14.0 and 13.5, 32000 18.7 and 15.7; filtered rows
+        // past a list's length: 2500 with top_p 0.9 36 and 21)
+        if (!summed && (filters || row.n >= kTableCols) && !inf) {
             const Table tab(sample_lds + sizeof(Shared) / sizeof(unsigned long long), row, row.value(top) - 30.f * temp);
             int keep = -1;
             summed = !filters || cut_table(sh, row, tab, cut, keep, top_k, top_p);
@@ -901,41 +936,46 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
                 // chunk's number of those is counted, and which of them are kept follows once all are
                 const float edge = cut.key ? row.value(cut.key) : -INFINITY;
                 tied = keep >= 0;
-                const unsigned long long tie_w = tied ? tab.w[tab.entry(edge)] : 0;
+                const unsigned long long tie_w = tied ? tab.weight(tab.entry(edge)) : 0;
                 __syncthreads();
                 if (cut.key || least_w)
                     for (int i = tid; i < 2 * kSide; i += kThreads) {
                         const float v = tab.value(i);
-                        if (v < edge || (tied && v == edge) || tab.w[i] < least_w) tab.w[i] = 0;
+                        if (v < edge || (tied && v == edge) || tab.weight(i) < least_w) tab.w[i] = u32x2_{0, 0};
                     }
                 for (int c = tid; c < row.chunks; c += kThreads) sh.bin[c] = ties[c] = 0;
                 __syncthreads();
-                auto draw = [&](int c, int at, const float* v) {
-                    unsigned long long s = 0;
-                    float m = v[0];
+                const uint32_t edge_bits = __float_as_uint(edge) >> 16;
+                auto draw = [&](int c, int, u32x4 u) {
+                    const Entries n = tab.entries(u);
+                    uint32_t lower = 0, upper = 0;
 #pragma unroll
-                    for (int e = 1; e < VEC; ++e) m = fmaxf(m, v[e]);
-                    if (m >= edge) {
+                    for (int e = 0; e < VEC; ++e) {
+                        const u32x2_ w = tab.w[n[e]];
+                        lower += w[0];
+                        upper += w[1];
+                    }
+                    if (tab.any_in_zone(n)) {
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) s += tab.w[tab.entry(v[e])];
-                        if (tab.any_in_zone(v)) {
-#pragma unroll
-                            for (int e = 0; e < VEC; ++e)
-                                if (tab.in_zone(v[e]) && v[e] > edge) {
-                                    const unsigned long long w = row.weight(v[e]);
-                                    s += w >= least_w ? w : 0;
-                                }
+                        for (int e = 0; e < VEC; ++e) {
+                            const float v = element(u, e);
+                            const unsigned long long w = tab.in_zone(v) && v > edge ? row.weight(v) : 0;
+                            if (w >= least_w) {
+                                lower += (uint32_t)w & 0x1fffffu;
+                                upper += (uint32_t)(w >> 21);
+                            }
                         }
                     }
-                    if (__any(s != 0)) s = wave_sum_weights(s);
-                    if (lane == 0) sh.bin[c] = s;
+                    if (__any((lower | upper) != 0)) {
+                        const unsigned long long s = ((unsigned long long)wave_sum(upper) << 21) + wave_sum(lower);
+                        if (lane == 0) sh.bin[c] = s;
+                    }
                     if (tied) {
-                        uint32_t n = 0;
-                        if (__any(m >= edge)) {
+                        uint32_t same = 0;
 #pragma unroll
-                            for (int e = 0; e < VEC; ++e) n += (uint32_t)__popcll(__ballot(v[e] == edge));
-                        }
-                        if (lane == 0) ties[c] = n;
+                        for (int e = 0; e < VEC; ++e)
+                            same += (uint32_t)__popcll(__ballot((e & 1 ? u[e / 2] >> 16 : u[e / 2] & 0xffffu) == edge_bits));
+                        if (lane == 0) ties[c] = same;
                     }
                 };
                 if (cut.key) row.seek(sh.top, edge, draw);
@@ -1064,7 +1104,7 @@ hipError_t sample_some(const SampleParams& p, hipStream_t stream) {
     switch (p.dtype) {
         case 0: DSALT_LAUNCH("sample", sample_kernel<float>, grid, dim3(kThreads), sizeof(Shared), stream, p); break;
         case 1: {
-            const unsigned table = p.n_cols >= kTableCols ? 2 * kSide * sizeof(unsigned long long) : 0;
+            const unsigned table = p.n_cols > kList ? 2 * kSide * sizeof(unsigned long long) : 0;
             if (table)
                 if (hipError_t e = hipFuncSetAttribute((const void*)sample_kernel<bf16>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                        (int)(sizeof(Shared) + table)))

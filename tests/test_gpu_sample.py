@@ -101,6 +101,22 @@ def test_masks_infinities_and_nan(dt):
         assert tok[0] == -1 and tok[1] == -1 and tok[6] in (40, 50) and tok[7] == 0
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("V", [2500, 16383, 16384])
+def test_masked_rows_of_longer_vocabularies(dt, V):
+    """Most of a row masked, by -inf, NaN or the type's lowest value, or beside infinite logits; rows past a list's length and
+    on both sides of the weights by value."""
+    x, u = _logits(6, V, dt, V)
+    x[0, 5:] = float("-inf")
+    x[1, ::2] = torch.finfo(dt).min
+    x[2, 7:] = float("nan")
+    x[3, ::3] = float("inf")
+    x[4] = torch.finfo(dt).min
+    for kw in (dict(), dict(top_p=0.8), dict(top_k=1500), dict(top_k=1500, top_p=0.6), dict(min_p=0.1), dict(top_k=30, top_p=0.9),
+               dict(temperature=3.0, top_p=0.95), dict(temperature=float("inf"), top_p=0.3)):
+        _check(x, u, **kw)
+
+
 def test_random_numbers_at_the_ends():
     x, _ = _logits(9, 3001, torch.float32, 3)
     for dt in (torch.float32, torch.float64):
