@@ -415,9 +415,9 @@ __device__ __forceinline__ void keep_equal(Shared& sh, const Row<T>& row, Cut& c
     cut.idx = (int)sh.found[2];
 }
 
-// The first n of the list sorted, largest first: up to 256 by counting those above each, threads side by side over parts of the list; more by
-// a bitonic sort, an element a thread, whose exchanges within a wave need no barrier (four rows of 997 with top_p 0.9:
-// 22 us, 48 by counting, 26 with every exchange through LDS)
+// The first n of the list sorted, largest first: up to 256 by counting those above each, threads side by side over parts of
+// the list; more by a bitonic sort, an element a thread, whose exchanges within a wave need no barrier (four rows of 997
+// with top_p 0.9: 22 us, 48 by counting, 26 with every exchange through LDS)
 __device__ __forceinline__ void sort_list(Shared& sh, int n) {
     const int tid = threadIdx.x;
     if (n <= 256) {
@@ -687,7 +687,6 @@ __device__ __forceinline__ uint32_t reached_by(Shared& sh, uint32_t mine, unsign
 constexpr int kSide = 2048, kTableCols = 16384;
 
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x2_ __attribute__((ext_vector_type(2)));
 
 // the entries of a vector of eight logits: within a side, then of the table
 struct Entries {
@@ -697,11 +696,11 @@ struct Entries {
 };
 
 struct Table {
-    u32x2_* w;  // [2 kSide] lower 21 bits, upper bits
+    u32x2* w;  // [2 kSide] lower 21 bits, upper bits
     uint32_t a0;
 
     // the table of a row; weights are 0 below the logit `low`
-    __device__ __forceinline__ Table(unsigned long long* lds, const Row<bf16>& row, float low) : w((u32x2_*)lds) {
+    __device__ __forceinline__ Table(unsigned long long* lds, const Row<bf16>& row, float low) : w((u32x2*)lds) {
         const float m = (float)row.m;
         const uint32_t up = m > 0.f ? __float_as_uint(m) >> 16 : 0;
         const uint32_t down = low < 0.f ? min((__float_as_uint(-low) >> 16) + 1, 0x7f7fu) : 0;
@@ -711,7 +710,7 @@ struct Table {
         for (int i = threadIdx.x; i < 2 * kSide; i += kThreads) {
             const float v = value(i);
             const unsigned long long x = holds(i) && v <= m ? row.weight(v) : 0;
-            w[i] = u32x2_{(uint32_t)x & 0x1fffffu, (uint32_t)(x >> 21)};
+            w[i] = u32x2{(uint32_t)x & 0x1fffffu, (uint32_t)(x >> 21)};
         }
         __syncthreads();
     }
@@ -941,7 +940,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
                 if (cut.key || least_w)
                     for (int i = tid; i < 2 * kSide; i += kThreads) {
                         const float v = tab.value(i);
-                        if (v < edge || (tied && v == edge) || tab.weight(i) < least_w) tab.w[i] = u32x2_{0, 0};
+                        if (v < edge || (tied && v == edge) || tab.weight(i) < least_w) tab.w[i] = u32x2{0, 0};
                     }
                 for (int c = tid; c < row.chunks; c += kThreads) sh.bin[c] = ties[c] = 0;
                 __syncthreads();
@@ -951,7 +950,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
                     uint32_t lower = 0, upper = 0;
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
-                        const u32x2_ w = tab.w[n[e]];
+                        const u32x2 w = tab.w[n[e]];
                         lower += w[0];
                         upper += w[1];
                     }
