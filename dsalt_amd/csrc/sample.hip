@@ -16,10 +16,11 @@
 // arithmetic of one compute unit a row, in float64 where weights are formed (a float32 weight is off by 2^-24
 // of itself, which over 150000 tokens moves a border of the running sums past u once in some thousand draws).
 // The first pass notes each chunk's largest logit, so that passes over what a filter may keep read few chunks where
-// it keeps little (256 rows, top_k 50: 34 us, 43 with every chunk read again).
-// us on the device, 256 bfloat16 rows of 151936 (77.8 MB, 15.6 at the copy rate): largest logit 18, top_k 50 34,
-// temperature alone 41, top_p 0.9 at temperature 0.5 46, at temperature 2, where most is kept, 68 (73 with an element's
-// entry found by itself, 92 with a pass more for the equal elements at the prefix's end).  One row: 11, 29, 31, 36, 55.
+// it keeps little (256 rows, top_k 50: 33 us, 43 with every chunk read again).
+// us on the device, 256 bfloat16 rows of 151936 (77.8 MB, 15.6 at the copy rate): largest logit 17, top_k 50 33,
+// temperature alone 40, top_p 0.9 at temperature 0.5 45, at temperature 2, where most is kept, 67 (73 with an element's
+// entry found by itself, 92 with a pass more for the equal elements at the prefix's end).  One row: 9, 27, 28, 33, 52.
+// Vector instructions take two thirds of a compute unit's cycles there, look-ups in LDS a third.
 #include <algorithm>
 #include <type_traits>
 
@@ -114,9 +115,18 @@ __device__ __forceinline__ float wave_max4(const float* v) {
     return dpp_max<0x128>(dpp_max<0x124>(dpp_max<0x122>(dpp_max<0x121>(fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]))))));
 }
 __device__ __forceinline__ uint16_t upper_key(float v) { return (uint16_t)(key_of<bf16>(v)); }
-// the same for weights: sums of at most 64 x 8 of 2^42, in two parts of 25 and 20 bits a lane
+// The same for two values at once, one in each half of the wave after the first step: low + high 2^BITS
+template <int BITS>
+__device__ __forceinline__ unsigned long long wave_sum2(uint32_t low, uint32_t high) {
+    auto a = __builtin_amdgcn_permlane32_swap(low, high, false, false);
+    const uint32_t v = dpp_add<0x128>(dpp_add<0x124>(dpp_add<0x122>(dpp_add<0x121>(a[0] + a[1]))));
+    auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const int both = (int)(b[0] + b[1]);
+    return ((unsigned long long)(uint32_t)__builtin_amdgcn_readlane(both, 32) << BITS) + (uint32_t)__builtin_amdgcn_readlane(both, 0);
+}
+// and for weights: sums of at most 64 x 8 of 2^42, in two parts of 25 and 20 bits a lane
 __device__ __forceinline__ unsigned long long wave_sum_weights(unsigned long long v) {
-    return ((unsigned long long)wave_sum((uint32_t)(v >> 25)) << 25) + wave_sum((uint32_t)v & 0x1ffffffu);
+    return wave_sum2<25>((uint32_t)v & 0x1ffffffu, (uint32_t)(v >> 25));
 }
 
 // 2^42 (2^f - 1) = f P(f) for f in [-1/2, 1/2], P the degree 9 polynomial through the ten Chebyshev nodes (relative
@@ -531,7 +541,7 @@ __device__ __forceinline__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut
 // exponents, over which logits spread as they do over their range, finds the one in which the prefix ends; its elements
 // are listed and sorted, or all from there up, where those are few (True: that has cut the row, see cut_list).  Where one
 // part holds more than a list does, a radix search goes on over keys.
-// (200 float32 rows of 151936, top_p 0.9: 168 us, 270 with a radix search alone, whose first bins few of the logits fill.)
+// (200 float32 rows of 151936, top_p 0.9: 166 us, 270 with a radix search alone, whose first bins few of the logits fill.)
 // A call of its own: inlined, the registers it needs cost every row that does without it (float32 rows, temperature
 // alone, 75 -> 83 us).
 struct Narrowed {
@@ -857,20 +867,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     const float top_p = p.top_p ? p.top_p[r] : p.top_p_all, min_p = p.min_p ? p.min_p[r] : p.min_p_all;
     const int top_k = p.top_k ? p.top_k[r] : p.top_k_all;
     const bool filters = (top_k > 0 && top_k < row.n) || top_p < 1.f;
-    // the largest logit and its first index, and each chunk's largest where chunks may be passed over later
+    // the largest logit and the first vector that holds it, and each chunk's largest where chunks may be passed over later
     float best = -INFINITY;
-    int best_i = 0;
+    int best_at = 0;
     float four[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     row.skim(
         [&](int, int at, const float* v) {
             float m = v[0];
 #pragma unroll
             for (int e = 1; e < VEC; ++e) m = fmaxf(m, v[e]);
-            if (m > best) {
-                best = m;
-#pragma unroll
-                for (int e = VEC - 1; e >= 0; --e) best_i = v[e] == m ? at + e : best_i;
-            }
+            best_at = m > best ? at + VEC : best_at;  // (more than 0: a row's first vector may begin before it)
+            best = fmaxf(best, m);
             four[0] = four[1], four[1] = four[2], four[2] = four[3], four[3] = m;
         },
         [&](int c) {
@@ -881,7 +888,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
             if ((lane & 15) == 0 && k >= 0) sh.top[c + k * kWaves] = key;
         });
     const uint32_t own = key_of<T>(best);
-    unsigned long long first = ((unsigned long long)own << 32) | (uint32_t)~best_i;
+    unsigned long long first = ((unsigned long long)own << 32) | (uint32_t)~best_at;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
         const unsigned long long b = __shfl_xor(first, o);
@@ -891,7 +898,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     __syncthreads();
     for (int k = 0; k < kWaves; ++k) first = sh.part[k] > first ? sh.part[k] : first;
     const uint32_t top = __builtin_amdgcn_readfirstlane((uint32_t)(first >> 32));
-    const int top_i = (int)~(uint32_t)first;
+    const int top_at = (int)~(uint32_t)first - VEC;  // where the vector of the first such logit begins
     if (top == key_of<T>(-INFINITY)) {  // nothing to draw
         if (tid == 0) {
             p.token[r] = -1;
@@ -902,6 +909,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
     // the first token alone: greedy, or filters that leave no more (min_p above 1 and NaN among them)
     if (!(temp > 0.f) || top_k == 1 || !(top_p > 0.f) || !(min_p <= 1.f)) {
         if (tid == 0) {
+            float v[VEC];
+            row.load(top_at, v);
+            int top_i = top_at;
+#pragma unroll
+            for (int e = VEC - 1; e >= 0; --e) top_i = v[e] == row.value(top) ? top_at + e : top_i;
             p.token[r] = top_i;
             p.logp[r] = 0.f;
         }
@@ -966,7 +978,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleParams p) {
                         }
                     }
                     if (__any((lower | upper) != 0)) {
-                        const unsigned long long s = ((unsigned long long)wave_sum(upper) << 21) + wave_sum(lower);
+                        const unsigned long long s = wave_sum2<21>(lower, upper);
                         if (lane == 0) sh.bin[c] = s;
                     }
                     if (tied) {
