@@ -143,6 +143,24 @@ def test_layouts(dt, V):
     _check(x[:1].expand(6, -1), u, top_k=50)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+def test_largest_logit_off_16_byte_boundaries(dt):
+    """The largest logit first, last, in the first few places and several times, rows from every offset."""
+    for V in (1, 3, 9, 700, 5003):
+        for off in range(1, 9):
+            buf = torch.full((7, V + 16), 9.0, dtype=dt, device=DEV)
+            x = buf[:, off:off + V]
+            x.copy_(torch.randn(7, V).to(dt))
+            x[1, 0] = x[2, V - 1] = x[3, min(2, V - 1)] = 8.0
+            x[4, V // 2], x[4, V - 1] = 7.0, 7.0
+            x[5] = -0.0
+            x[5, V // 3:] = 0.0
+            u = torch.full((7,), 0.5, device=DEV)
+            _check(x, u, temperature=0.0)
+            _check(x, u, top_k=1)
+            _check(x, u, top_k=2, top_p=0.5)
+
+
 @pytest.mark.parametrize("dt,V", [(torch.float32, 1 << 20), (torch.bfloat16, 1 << 20), (torch.bfloat16, 151936), (torch.float16, 262144)])
 def test_large_vocabularies(dt, V):
     x, u = _logits(3, V, dt, 1)
