@@ -573,10 +573,11 @@ AttnPlan attn_plan(const CacheAttnParams& p) {
     const int group = p.n_heads / p.c.n_kv, D = p.c.head_dim;
     const int64_t cap = (int64_t)p.cols << p.c.bt_log;
     const int64_t w = p.w_max > 0 && p.w_max < cap ? p.w_max : cap;
+    const int64_t rows = std::max(p.n_rows, 1);  // (the workspace of a call without rows is asked for too)
     int64_t ns = 1;
-    a.list = group == 1 || (int64_t)p.n_rows * p.n_heads * w <= 1 << 18;
+    a.list = group == 1 || rows * p.n_heads * w <= 1 << 18;
     if (a.list) {
-        const int64_t blocks = (int64_t)p.n_rows * p.n_heads, bytes = (w + p.k_lmk) * D;
+        const int64_t blocks = rows * p.n_heads, bytes = (w + p.k_lmk) * D;
         a.tiles = group;
         a.nh = 1;
         a.waves = bytes >= 1 << 16 && bytes <= 1 << 17 && blocks <= 512 ? 8 : 4;
@@ -584,7 +585,7 @@ AttnPlan attn_plan(const CacheAttnParams& p) {
     } else {
         a.tiles = ceil_div(group, 16);
         a.nh = std::min(group, 16);
-        const int64_t blocks = (int64_t)p.n_rows * p.c.n_kv * a.tiles;
+        const int64_t blocks = rows * p.c.n_kv * a.tiles;
         a.waves = blocks <= 256 ? 8 : 4;
         ns = std::min(256 / blocks, w / 512);
     }

@@ -141,6 +141,21 @@ def test_null_structs_and_empty_calls():
     assert lib.dsalt_sample_rows(ctypes.byref(a), None) == 0
 
 
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("n_heads", [2, 8])
+def test_calls_without_rows_need_no_workspace(head_dim, n_heads):
+    """A step without query tokens, whatever its tables and windows would hold: the query that precedes each call gives
+    zero, and the call does nothing."""
+    lib = _lib.load()
+    for cols in (1, 16, 64, 1 << 20 >> 6, 1 << 30 >> 6):
+        for w_max in (0, 1, 512, 1 << 20, 0x7fffffff):
+            for k_lmk in (0, 8, 2048):
+                a = _attn_args(_cache(head_dim=head_dim))
+                a.n_rows, a.n_heads, a.table_cols, a.table_stride, a.w_max, a.k_lmk = 0, n_heads, cols, cols, w_max, k_lmk
+                assert lib.dsalt_cache_attn_workspace_bytes(ctypes.byref(a)) == 0
+                assert lib.dsalt_cache_attn(ctypes.byref(a), None) == 0
+
+
 def test_python_refuses_cpu_tensors():
     c = ops.new_cache(2, 1, 64, device="cpu")
     i = torch.zeros(1, dtype=torch.int32)

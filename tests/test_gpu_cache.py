@@ -766,3 +766,25 @@ def test_argument_checks():
         ops.cache_read(c, t, i, n_rows=2)
     with pytest.raises(TypeError):
         ops.cache_read(c, t, _i32([0, 1, 2, 3]), n_rows=2, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,G", [(2, 2), (8, 2)])
+def test_calls_without_rows(D, H, G):
+    """No query tokens, none written, none read, whatever the table and the windows hold: outputs without rows, pages as
+    they were."""
+    bt = 64
+    cache = _random_cache(4, G, bt, D, 3)
+    before = _host_pages(cache)
+    none, x = _i32([]), torch.zeros(0, H, D, dtype=torch.bfloat16, device=DEV)
+    for M in (2, 40, 4096):
+        table, lmk = torch.zeros(3, M, dtype=torch.int32, device=DEV), torch.zeros(H, 3, 1, 8, dtype=torch.int32, device=DEV)
+        for w_max in (None, 1, 512, M * bt, 1 << 40):
+            for sets in (lmk, lmk[..., :0]):
+                out, lse = ops.cache_attention(x, cache, table, none, none, none, sets, w_max=w_max)
+                assert out.shape == (0, H, D) and out.dtype == x.dtype and lse.shape == (0, H)
+        k, v = ops.cache_read(cache, table, _i32([0, 0, 0, 0]), n_rows=0)
+        assert k.shape == v.shape == (0, G, D)
+    ops.cache_write_(x[:, :G], x[:, :G], cache, torch.zeros(0, 4, dtype=torch.int32, device=DEV))
+    ops.cache_write_(x[:, :G], x[:, :G], cache, _i32([[0, 1, 1, 0]]))
+    _same_pages(cache, before)
