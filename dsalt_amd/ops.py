@@ -943,6 +943,15 @@ def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None
     return out, lse
 
 
+def _counts(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as contiguous int32, numbers past a vocabulary's size as that size."""
+    if t.is_floating_point():
+        t = (t if t.element_size() >= 4 else t.float()).clamp(-1, MAX_VOCAB)  # (float16 ends at 65504)
+    elif t.element_size() == 8:
+        t = t.to(torch.int64).clamp(-1, MAX_VOCAB)
+    return _i32(t)  # (narrower integers fit, unsigned ones of 32 bits from 2^31 on turn negative: all, as they mean)
+
+
 def sample_rows(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """(token [R] int64, logp [R] fp32): a token a row of ``logits`` [R, V] from given random numbers ``u`` [R]
     in [0, 1) (float32 or float64).  ``temperature`` (<= 0: the largest logit), ``top_k`` (<= 0: all), ``top_p``
@@ -966,9 +975,7 @@ def sample_rows(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     u = u.contiguous()
     t, k, p, m = per_row
     t, p, m = (x if x is None else _f32(x) for x in (t, p, m))
-    if k is not None and k.dtype != torch.int32:
-        k = k.clamp(-1, MAX_VOCAB)
-    k = k if k is None else _i32(k)
+    k = k if k is None else _counts(k)
     token = torch.empty(R, dtype=torch.int64, device=at)
     logp = torch.empty(R, dtype=torch.float32, device=at)
     a = SampleArgs(R, V, dtype_code(logits.dtype), u.element_size(), logits.data_ptr(), logits.stride(0), u.data_ptr(),

@@ -173,6 +173,28 @@ def test_python_refuses_cpu_tensors():
             ops.new_cache(**{**dict(n_blocks=1, n_kv_heads=1, head_dim=64, device="cpu"), **kw})
 
 
+@pytest.mark.parametrize("dt", [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.int32, torch.uint32, torch.int64, torch.uint64,
+                                torch.float16, torch.bfloat16, torch.float32, torch.float64, torch.bool])
+def test_counts_of_every_type(dt):
+    """A row's top_k from tensors of any type: small counts as they are, negative ones negative, what passes the largest
+    vocabulary as all of it (as that size, or negative)."""
+    signed = not (dt == torch.bool or dt.is_floating_point is False and torch.iinfo(dt).min == 0)
+    top = 1 if dt == torch.bool else (min(torch.finfo(dt).max, 2.0 ** 40) if dt.is_floating_point else torch.iinfo(dt).max)
+    values = [0, 1] + ([7, 100] if dt != torch.bool else []) + ([-1, -5] if signed else []) + [top]
+    t = torch.tensor([int(v) for v in values], dtype=torch.int64 if dt != torch.uint64 else dt).to(dt)
+    if dt != torch.uint64:
+        t = torch.stack([t, t], 1)[:, 0]  # strided
+    got = ops._counts(t)
+    assert got.dtype == torch.int32 and got.is_contiguous() and got.shape == t.shape
+    for v, k in zip(values, got.tolist()):
+        if v < 0:
+            assert k < 0, (v, k)
+        elif v > ops.MAX_VOCAB:
+            assert k < 0 or k >= ops.MAX_VOCAB, (v, k)
+        else:
+            assert k == int(v), (v, k)
+
+
 # ------------------------------------------------------------------------ the oracle itself
 def test_oracle_rounds_as_torch_does():
     """Every finite bf16 within 448: the oracle's e4m3 is torch's conversion."""

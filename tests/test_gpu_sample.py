@@ -255,3 +255,13 @@ def test_argument_checks():
     assert tok.shape == lp.shape == (0,)
     big = torch.tensor([1 << 40] * 3, device=DEV)
     assert torch.equal(ops.sample_rows(x, u, top_k=big)[0], ops.sample_rows(x, u, top_k=1 << 40)[0])
+
+
+@pytest.mark.parametrize("dt", [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.int64, torch.float16, torch.float32, torch.bool])
+def test_counts_of_every_type(dt):
+    """top_k as a tensor of another type than int32 draws what the same numbers draw in it."""
+    x, u = _logits(6, 3001, torch.bfloat16, 12)
+    k = torch.tensor([1, 0, 1, 1, 0, 1] if dt == torch.bool else [1, 0, 3, 50, 100, 127], dtype=torch.int32, device=DEV)
+    ref = ops.sample_rows(x, u, top_k=k)
+    got = ops.sample_rows(x, u, top_k=k.to(dt))
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
