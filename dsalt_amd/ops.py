@@ -829,6 +829,11 @@ def _vec_i32(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
     return _i32(t)
 
 
+def _windows(w: torch.Tensor) -> torch.Tensor:
+    """``w`` with 64-bit windows held to what int32 names (in which 2^40, all there is, would turn into none)."""
+    return w.clamp(-1, 0x7fffffff) if w.dtype == torch.int64 else w
+
+
 def _call(name: str, args, at: int):
     """One library call on the current stream of device ``at`` (made current for it where it is not)."""
     fn = getattr(_lib.load(), name)
@@ -928,7 +933,7 @@ def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None
     if lmk_bias is not None and lmk_bias.shape != lmk_idx.shape:
         raise ValueError("lmk_bias must have the shape of lmk_idx")
     K = lmk_idx.shape[3]
-    rq, ps, wc = _vec_i32(req, T, "req"), _vec_i32(pos, T, "pos"), _vec_i32(w, T, "w")
+    rq, ps, wc = _vec_i32(req, T, "req"), _vec_i32(pos, T, "pos"), _vec_i32(_windows(w), T, "w")
     li = _i32(lmk_idx)
     lb = _f32(lmk_bias) if lmk_bias is not None else None
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)

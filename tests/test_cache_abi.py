@@ -195,6 +195,15 @@ def test_counts_of_every_type(dt):
             assert k == int(v), (v, k)
 
 
+def test_windows_past_32_bits():
+    """A window longer than int32 names stays longer than any cache."""
+    w = [1, 0, -3, 512, (1 << 31) - 1, 1 << 31, (1 << 32) + 5, 1 << 40, (1 << 63) - 1, -(1 << 40) + 9]
+    got = ops._i32(ops._windows(torch.tensor(w))).tolist()
+    assert [max(x, 1) for x in got] == [max(min(x, (1 << 31) - 1), 1) for x in w]
+    narrow = torch.tensor([1, 5], dtype=torch.int32)
+    assert ops._windows(narrow) is narrow
+
+
 # ------------------------------------------------------------------------ the oracle itself
 def test_oracle_rounds_as_torch_does():
     """Every finite bf16 within 448: the oracle's e4m3 is torch's conversion."""

@@ -788,3 +788,11 @@ def test_calls_without_rows(D, H, G):
     ops.cache_write_(x[:, :G], x[:, :G], cache, torch.zeros(0, 4, dtype=torch.int32, device=DEV))
     ops.cache_write_(x[:, :G], x[:, :G], cache, _i32([[0, 1, 1, 0]]))
     _same_pages(cache, before)
+
+
+def test_windows_past_32_bits_attend_all():
+    q, cache, table, req, pos, _, lmk = _attend_case(3, 4, 2, 64, 16, 5, torch.bfloat16, 4, 90, 1)
+    args = [_i32(x) for x in (table, req, pos)]
+    ref = ops.cache_attention(q.to(DEV), cache, *args, _i32([1 << 20] * 3), _i32(lmk))
+    got = ops.cache_attention(q.to(DEV), cache, *args, torch.tensor([1 << 31, (1 << 32) + 1, 1 << 40], device=DEV), _i32(lmk))
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
