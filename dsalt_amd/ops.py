@@ -926,7 +926,7 @@ def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None
     c = _cache_args(cache)
     T, H, D = q.shape
     R, M, ts = _table_args(table)
-    if D != c.head_dim or H % c.n_kv_heads:
+    if D != c.head_dim or c.n_kv_heads < 1 or H % c.n_kv_heads:
         raise ValueError(f"q must be [T, H, {c.head_dim}] with H a multiple of {c.n_kv_heads}, got {tuple(q.shape)}")
     if lmk_idx.dim() != 4 or lmk_idx.shape[:3] != (H, R, 1):
         raise ValueError(f"lmk_idx must be [H, R, 1, K] = [{H}, {R}, 1, K], got {tuple(lmk_idx.shape)}")

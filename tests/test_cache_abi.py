@@ -204,6 +204,18 @@ def test_windows_past_32_bits():
     assert ops._windows(narrow) is narrow
 
 
+@pytest.mark.parametrize("heads", [(0, 2), (0, 0), (3, 2)])
+def test_attention_refuses_head_counts(monkeypatch, heads):
+    """A cache without heads, or query heads that do not share its heads evenly, is an argument error like any other."""
+    monkeypatch.setattr(ops, "_on", lambda *ts: 0)  # (the checks come before anything runs)
+    n_kv, n = heads
+    i = torch.zeros(1, dtype=torch.int32)
+    c = ops.new_cache(2, n_kv, 64, device="cpu")
+    with pytest.raises(ValueError, match="H a multiple"):
+        ops.cache_attention(torch.zeros(1, n, 64), c, torch.zeros((1, 2), dtype=torch.int32), i, i, i,
+                            torch.zeros((n, 1, 1, 0), dtype=torch.int32))
+
+
 # ------------------------------------------------------------------------ the oracle itself
 def test_oracle_rounds_as_torch_does():
     """Every finite bf16 within 448: the oracle's e4m3 is torch's conversion."""
