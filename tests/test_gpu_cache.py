@@ -796,3 +796,65 @@ def test_windows_past_32_bits_attend_all():
     ref = ops.cache_attention(q.to(DEV), cache, *args, _i32([1 << 20] * 3), _i32(lmk))
     got = ops.cache_attention(q.to(DEV), cache, *args, torch.tensor([1 << 31, (1 << 32) + 1, 1 << 40], device=DEV), _i32(lmk))
     assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
+def test_split_windows_on_two_streams_at_once(monkeypatch):
+    """Windows split over blocks and joined from a workspace (key/value heads with their query heads, and heads one by one),
+    with inputs of their own on each of two streams in turn: equal to the same calls one after the other."""
+    need = []
+    place = ops._set_workspace
+    monkeypatch.setattr(ops, "_set_workspace", lambda a, n, dev: need.append(n) or place(a, n, dev))
+
+    def case(seed, H, G, n, w):
+        c = _attend_case(1, H, G, 128, 64, 20, torch.bfloat16, seed, 0, 1, lens=[n])
+        return c[0].to(DEV), c[1], *(_i32(x) for x in c[2:5]), _i32([w]), _i32(c[6])
+    cases = [[case(10 * i, 32, 2, 12000 + i, 9000), case(10 * i + 1, 2, 2, 3001 + i, 2900)] for i in range(2)]
+
+    def work(i):
+        return [t for c, w in zip(cases[i], (9000, 2900)) for t in ops.cache_attention(*c, w_max=w)]
+    ref = [work(i) for i in range(2)]
+    assert all(n > 0 for n in need) and len(need) == 4
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    res = [[], []]
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                res[i].append(work(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for got in res[i]:
+            assert all(torch.equal(x, y) for x, y in zip(got, ref[i]))
+
+
+def test_two_graphs_of_split_windows_replayed_in_turn():
+    """Two captured calls whose windows are split, replayed in turn on two streams with inputs of the moment: each equals its
+    eager call every time."""
+    g = torch.Generator(device=DEV).manual_seed(8)
+    cases = []
+    for i in range(2):
+        c = _attend_case(1, 32, 2, 128, 64, 20, torch.bfloat16, 20 + i, 0, 1, lens=[12000])
+        cases.append((c[0].to(DEV), c[1], *(_i32(x) for x in c[2:5]), _i32([9000 - i]), _i32(c[6])))
+    ops.cache_attention(*cases[0], w_max=9000)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for c, gr in zip(cases, graphs):
+        torch.cuda.synchronize()
+        with torch.cuda.graph(gr):
+            outs.append(ops.cache_attention(*c, w_max=9000))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rep in range(4):
+        for c in cases:
+            c[0].copy_(torch.randn(c[0].shape, generator=g, device=DEV))
+        ref = [ops.cache_attention(*c, w_max=9000) for c in cases]
+        for o in outs:
+            for t in o:
+                t.fill_(-3)
+        torch.cuda.synchronize()
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, ref):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]), rep

@@ -265,3 +265,15 @@ def test_counts_of_every_type(dt):
     ref = ops.sample_rows(x, u, top_k=k)
     got = ops.sample_rows(x, u, top_k=k.to(dt))
     assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("V", [2049, 2500, 16383, 16384, 16385])
+def test_weights_by_value_on_each_side_of_their_rule(dt, V):
+    """bfloat16 rows are weighed by value from 16384 columns on, and with filters from where a row is longer than a list
+    (2048): flat and peaked rows of lengths beside both, with settings that reach the one and the other."""
+    for spread in (0.02, 2.5, 12.0):
+        x, u = _logits(4, V, dt, V, spread)
+        for kw in (dict(), dict(temperature=0.3), dict(min_p=0.01), dict(top_p=0.9), dict(top_k=1025), dict(top_k=2000, top_p=0.7),
+                   dict(temperature=20.0, top_p=0.3, min_p=0.2)):
+            _check(x, u, **kw)
