@@ -470,7 +470,8 @@ __global__ __launch_bounds__(256) void read_kernel(CacheReadParams p) {
 }  // namespace
 
 // One launch while every block can form the sums for itself (and page counts fit 31 bits): 64 requests 7.7 us, 10.2 in two
-// launches, 1500 requests with 32768 rows 11.8 and 16.4.
+// launches, 1500 requests with 32768 rows 11.8 and 16.4.  Past that one block forms the sums of all requests, whose time grows
+// with them (a row each: 4096 requests in one launch 19 us, 4097 in two 27, 16384 126, 65536 528, 2^20 8.6 ms).
 static bool rows_in_one(int n_reqs, int cols) { return n_reqs <= kOneReqs && (int64_t)n_reqs * cols < 0x7fffffff; }
 
 size_t cache_rows_ws_bytes(int n_reqs, int cols) { return rows_in_one(n_reqs, cols) ? 0 : 256 + (size_t)n_reqs * sizeof(ReqPlan); }

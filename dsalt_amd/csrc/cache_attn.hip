@@ -22,8 +22,9 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-// number of bfloat16 parts of a query element (exact: 8, 11 and 24 bits) and of a weight (16 bits of it for
-// 16-bit outputs, 24 for float32)
+// number of bfloat16 parts of a query element (exact: 8, 11 and 24 bits) and of a weight: 16 bits of it for
+// 16-bit outputs, whose own rounding, half a step of 2^-8 or 2^-11 of a value, is far coarser, 24 for float32 (lists keep
+// weights in float32)
 template <typename T> struct Parts;
 template <> struct Parts<bf16> { static constexpr int q = 1, p = 2; };
 template <> struct Parts<f16> { static constexpr int q = 2, p = 2; };
@@ -561,7 +562,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void cache_attn_join_kernel(CacheA
 //  * A block a head reads a window once for each query head, a block a group once: the former is latency bound and
 //    smaller, so it wins up to about 2^18 pairs of a query head and a window key (w_max 512: one request 9 / 19, 8:
 //    9 / 21, 32: 17 / 21, 256: 67 / 36; w_max 1024: 8 requests 16 / 23, 24: 27 / 24; w_max 4096, 8 requests: 32 / 23),
-//    and where no two query heads share a window.
+//    and where no two query heads share a window.  With each row's whole window of 512: 16 requests 14 / 21, 32: 22 / 22,
+//    33: 23 / 22, 48: 27 / 23, 64: 31 / 23, 128: 55 / 28, 256: 102 / 44; float16 and float32 within 2 us of these.
 //  * Lists: eight waves for 64 KB of keys or more while there are at most two blocks a CU (one request 9 / 10; 60 requests
 //    of 16/16 heads 27 / 23 with four), and four waves with splits of at least 256 keys past 128 KB (one request,
 //    w_max 1024: 11 / 14, 4096: 11 / 16).

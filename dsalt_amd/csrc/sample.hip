@@ -209,8 +209,8 @@ struct Row {
             give(f, c, r);
         }
     }
-    // the same for passes of few instructions, which wait for memory: eight chunks requested ahead (and `four` after each
-    // four, with the first of them)
+    // the same for passes of few instructions, which wait for memory: four chunks at a time, the next four requested
+    // before they are looked at (and `four` after each four, with the first of them)
     template <typename F>
     __device__ __forceinline__ void skim(F f) const {
         skim(f, [](int) {});
@@ -285,8 +285,8 @@ struct Row {
         else skim(f);
     }
     __device__ __forceinline__ bool has(int i) const { return (unsigned)i < (unsigned)n; }
-    // round(2^42 2^t), t = (v - m) log2(e) / temperature.  (v - m is exact, and t below -43 rounds to 0, NaN and
-    // absent elements among it.  Sums with 1.5 2^52 and 2^52 round to a whole number and leave it in the mantissa.)
+    // round(2^42 2^t), t = (v - m) log2(e) / temperature.  (v - m is exact, or rounded to 2^-53 of itself where the two lie
+    // far apart; t below -43 rounds to 0, NaN and absent elements among it.  Sums with 1.5 2^52 and 2^52 round to a whole number and leave it in the mantissa.)
     __device__ __forceinline__ unsigned long long weight(float v) const { return weight_of(exponent(v)); }
     __device__ __forceinline__ double exponent(float v) const { return fmin(fmax(((double)v - m) * rate, -60.0), 0.0); }
     __device__ __forceinline__ static unsigned long long weight_of(double t) {
@@ -543,7 +543,8 @@ __device__ __forceinline__ bool cut_list(Shared& sh, const Row<T>& row, Cut& cut
 // part holds more than a list does, a radix search goes on over keys.
 // (200 float32 rows of 151936, top_p 0.9: 166 us, 270 with a radix search alone, whose first bins few of the logits fill.)
 // A call of its own: inlined, the registers it needs cost every row that does without it (float32 rows, temperature
-// alone, 75 -> 83 us).
+// alone, 75 -> 83 us).  As compiled, a kernel holds 120 vector registers and none of them in scratch, 100 bytes of scratch
+// a lane with the call's frame, and 38 (bfloat16: 51) scalar registers spilled.
 struct Narrowed {
     Cut cut;
     bool summed;

@@ -762,7 +762,8 @@ class CacheRows(NamedTuple):
 
 
 def new_cache(n_blocks: int, n_kv_heads: int, head_dim: int, *, block_tokens: int = 64, device="cuda") -> Cache8:
-    """An empty cache of one layer (head_dim 64 or 128; other head_dims pad their heads)."""
+    """An empty cache of one layer (head_dim 64 or 128; other head_dims pad their heads with zeros, and give
+    cache_attention the ``scale`` of their own size)."""
     if block_tokens not in BLOCK_TOKENS or head_dim not in (64, 128):
         raise ValueError(f"block_tokens must be one of {BLOCK_TOKENS} and head_dim 64 or 128, got {block_tokens}, {head_dim}")
     shape = (n_blocks, n_kv_heads, block_tokens, head_dim)
@@ -919,8 +920,8 @@ def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None
     (CacheRows.req, .pos), its own key and value written; it attends its window [pos - w + 1, pos] and the
     landmarks before the window of its head's set in lmk_idx [H, R, 1, K] (any order, negative slots empty, a
     position may repeat; select_landmarks' sets; a bias of -inf masks its landmark).  Rows without a key (inert rows, pages that the table does not
-    name) give zeros and -inf.  ``w_max``: no window is longer (host value; splits the work, longer windows only
-    cost time).  Not differentiable."""
+    name) give zeros and -inf.  ``scale``: by default 1 / sqrt(D).  ``w_max``: no window is longer (host value;
+    splits the work, longer windows only cost time).  Not differentiable."""
     at = _on(q, *cache, table, req, pos, w, lmk_idx, lmk_bias)
     q, q_at = _rows16(q, "q")
     c = _cache_args(cache)
@@ -960,7 +961,7 @@ def _counts(t: torch.Tensor) -> torch.Tensor:
 def sample_rows(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """(token [R] int64, logp [R] fp32): a token a row of ``logits`` [R, V] from given random numbers ``u`` [R]
     in [0, 1) (float32 or float64).  ``temperature`` (<= 0: the largest logit), ``top_k`` (<= 0: all), ``top_p``
-    and ``min_p`` are numbers or tensors [R].  Kept are the first top_k tokens by logit (equal ones by index, NaN
+    and ``min_p`` are numbers or tensors [R] of any number type.  Kept are the first top_k tokens by logit (equal ones by index, NaN
     as -inf), of those the ones before which less than top_p of their weight lies, of those the ones that weigh
     at least min_p of the first, and always the first; the token is the first index whose running sum of kept
     weights passes u times their total.  Weights are whole multiples of 2^-42 of the largest.  logp: the token's
