@@ -161,6 +161,45 @@ class CacheAttnArgs(ctypes.Structure):
                 ("workspace", _vp), ("workspace_bytes", _sz)]
 
 
+class Cache4(ctypes.Structure):
+    _fields_ = [("n_blocks", _i32), ("n_kv_heads", _i32), ("block_tokens", _i32), ("head_dim", _i32), ("kv", _vp), ("scale", _vp)]
+
+
+class Cache4WriteArgs(ctypes.Structure):
+    _fields_ = [("c", Cache4)] + CacheWriteArgs._fields_[1:]
+
+
+class Cache4ReadArgs(ctypes.Structure):
+    _fields_ = [("c", Cache4)] + CacheReadArgs._fields_[1:]
+
+
+class Cache4AttnArgs(ctypes.Structure):
+    _fields_ = [("c", Cache4)] + CacheAttnArgs._fields_[1:8] + [("rows_per_req", _i32)] + CacheAttnArgs._fields_[8:]
+
+
+class VerifyArgs(ctypes.Structure):
+    _fields_ = [("n_reqs", _i32), ("n_rows", _i32), ("n_cols", _i32), ("dtype", _i32), ("u_bytes", _i32),
+                ("logits", _vp), ("logits_stride", _i64), ("draft_logits", _vp), ("draft_stride", _i64),
+                ("tokens", _vp), ("cu", _vp), ("u", _vp), ("v", _vp), ("temperature", _vp), ("draft_temperature", _vp),
+                ("temperature_all", _f32), ("draft_temperature_all", _f32), ("accepted", _vp), ("out", _vp),
+                ("workspace", _vp), ("workspace_bytes", _sz)]
+
+
+class QkNormRopeArgs(ctypes.Structure):
+    _fields_ = [("total_len", _i32), ("num_seqs", _i32), ("n_q_heads", _i32), ("n_k_heads", _i32), ("head_dim", _i32),
+                ("dtype", _i32), ("weight_dtype", _i32), ("max_pos", _i32), ("eps", _f32),
+                ("q", _vp), ("q_stride_t", _i64), ("q_stride_h", _i64), ("k", _vp), ("k_stride_t", _i64), ("k_stride_h", _i64),
+                ("q_out", _vp), ("qo_stride_t", _i64), ("qo_stride_h", _i64),
+                ("k_out", _vp), ("ko_stride_t", _i64), ("ko_stride_h", _i64),
+                ("q_weight", _vp), ("k_weight", _vp), ("cu_seqlens", _vp), ("pos", _vp), ("cos", _vp), ("sin", _vp)]
+
+
+class QkNormRopeBwdArgs(ctypes.Structure):
+    _fields_ = [("base", QkNormRopeArgs), ("dq", _vp), ("dq_stride_t", _i64), ("dq_stride_h", _i64),
+                ("dk", _vp), ("dk_stride_t", _i64), ("dk_stride_h", _i64), ("dq_weight", _vp), ("dk_weight", _vp),
+                ("workspace", _vp), ("workspace_bytes", _sz)]
+
+
 class SampleArgs(ctypes.Structure):
     _fields_ = [("rows", _i32), ("n_cols", _i32), ("dtype", _i32), ("u_bytes", _i32), ("logits", _vp),
                 ("logits_stride", _i64), ("u", _vp), ("temperature", _vp), ("top_p", _vp), ("min_p", _vp), ("top_k", _vp),
@@ -193,6 +232,9 @@ SIGNATURES = {
     "dsalt_train_bwd_workspace_bytes": ([ctypes.POINTER(TrainBwdArgs)], _sz),
     "dsalt_train_bwd": ([ctypes.POINTER(TrainBwdArgs), _vp], ctypes.c_int),
     "dsalt_rope_qk": ([ctypes.POINTER(RopeArgs), _vp], ctypes.c_int),
+    "dsalt_qk_norm_rope": ([ctypes.POINTER(QkNormRopeArgs), _vp], ctypes.c_int),
+    "dsalt_qk_norm_rope_bwd_workspace_bytes": ([ctypes.POINTER(QkNormRopeBwdArgs)], _sz),
+    "dsalt_qk_norm_rope_bwd": ([ctypes.POINTER(QkNormRopeBwdArgs), _vp], ctypes.c_int),
     "dsalt_silu_mul": ([ctypes.POINTER(SiluMulArgs), _vp], ctypes.c_int),
     "dsalt_layer_selectors": ([ctypes.POINTER(SelectorsArgs), _vp], ctypes.c_int),
     "dsalt_sort_landmarks": ([ctypes.POINTER(SortArgs), _vp], ctypes.c_int),
@@ -200,10 +242,17 @@ SIGNATURES = {
     "dsalt_cross_entropy_rows": ([ctypes.POINTER(CeArgs), _vp], ctypes.c_int),
     "dsalt_cache_rows_workspace_bytes": ([ctypes.POINTER(CacheRowsArgs)], _sz),
     "dsalt_cache_rows": ([ctypes.POINTER(CacheRowsArgs), _vp], ctypes.c_int),
+    "dsalt_cache_rows_held": ([ctypes.POINTER(CacheRowsArgs), _vp, _vp], ctypes.c_int),
     "dsalt_cache_write": ([ctypes.POINTER(CacheWriteArgs), _vp], ctypes.c_int),
     "dsalt_cache_read": ([ctypes.POINTER(CacheReadArgs), _vp], ctypes.c_int),
     "dsalt_cache_attn_workspace_bytes": ([ctypes.POINTER(CacheAttnArgs)], _sz),
     "dsalt_cache_attn": ([ctypes.POINTER(CacheAttnArgs), _vp], ctypes.c_int),
+    "dsalt_cache4_write": ([ctypes.POINTER(Cache4WriteArgs), _vp], ctypes.c_int),
+    "dsalt_cache4_read": ([ctypes.POINTER(Cache4ReadArgs), _vp], ctypes.c_int),
+    "dsalt_cache4_attn_workspace_bytes": ([ctypes.POINTER(Cache4AttnArgs)], _sz),
+    "dsalt_cache4_attn": ([ctypes.POINTER(Cache4AttnArgs), _vp], ctypes.c_int),
+    "dsalt_verify_workspace_bytes": ([ctypes.POINTER(VerifyArgs)], _sz),
+    "dsalt_verify_rows": ([ctypes.POINTER(VerifyArgs), _vp], ctypes.c_int),
     "dsalt_sample_rows": ([ctypes.POINTER(SampleArgs), _vp], ctypes.c_int),
     "dsalt_timing_enable": ([ctypes.c_int], ctypes.c_int),
     "dsalt_timing_report": ([ctypes.c_char_p, _sz], ctypes.c_int),

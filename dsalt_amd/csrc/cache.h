@@ -19,7 +19,7 @@ struct CachePages {
 struct CacheRowsParams {
     int n_reqs, cols, bt_log, n_rows, n_pieces;
     int64_t n_free, table_st;
-    const int32_t *seq_len, *new_len;
+    const int32_t *seq_len, *new_len, *held;  // (held: null, or tokens whose pages are kept)
     int32_t *table, *ring;
     const int64_t* span;
     int32_t* seq_out;

@@ -12,7 +12,7 @@ namespace {
 
 // ------------------------------------------------------------------ row maps
 // Request r holds L tokens in H = ceil(L / b) pages (b tokens a page) and brings n: it needs
-// ceil((L + n) / b) - H more.  Prefix sums over the requests, in their order, place its rows, its new
+// ceil((L + n) / b) - H more (H is larger where pages of tokens that were taken back are kept).  Prefix sums over the requests, in their order, place its rows, its new
 // pages in the ring of free ones, its pieces (runs of rows within one page) and the pages it gives
 // back.  One block forms the sums; then a thread a row writes the maps and a wave a request the ring.
 struct ReqPlan {
@@ -39,6 +39,11 @@ constexpr int kPlanThreads = 1024;
 // what request r adds, given the rows before it (they decide whether its own fit)
 __device__ __forceinline__ int held_pages(const CacheRowsParams& p, int64_t len) {
     return (int)min(max((len + (1 << p.bt_log) - 1) >> p.bt_log, (int64_t)0), (int64_t)p.cols);
+}
+
+// pages that request r holds: those of its tokens, or of more where the caller tells
+__device__ __forceinline__ int pages_of(const CacheRowsParams& p, int r, int64_t len) {
+    return held_pages(p, p.held && len >= 0 ? max(len, (int64_t)p.held[r]) : len);
 }
 
 __global__ __launch_bounds__(kPlanThreads) void rows_plan_kernel(CacheRowsParams p) {
@@ -80,7 +85,7 @@ __global__ __launch_bounds__(kPlanThreads) void rows_plan_kernel(CacheRowsParams
         fits = n >= 0 && len >= 0 && len + n <= ((int64_t)p.cols << p.bt_log) && end <= p.n_rows;
         rel = n < 0 && len >= 0;
         Sums s = {0, 0, 0, 0};
-        const int held = held_pages(p, len);
+        const int held = pages_of(p, r, len);
         if (fits) s.need = max(held_pages(p, len + n) - held, 0);
         if (rel) s.give = held;
         return s;
@@ -146,7 +151,7 @@ __global__ __launch_bounds__(256) void rows_map_kernel(CacheRowsParams p, int ro
     if ((int)blockIdx.x >= row_blocks) {  // pages given back: a wave a request
         const int r = ((int)blockIdx.x - row_blocks) * 4 + (threadIdx.x >> 6);
         if (r >= p.n_reqs || plan[r].state != 2) return;
-        const int held = held_pages(p, p.seq_len[r]);
+        const int held = pages_of(p, r, p.seq_len[r]);
         const int64_t at = tail + plan[r].give;
         for (int j = threadIdx.x & 63; j < held; j += 64)
             if (at + j - head < p.n_free) p.ring[(uint64_t)(at + j) % (uint64_t)p.n_free] = p.table[r * p.table_st + j];
@@ -170,7 +175,7 @@ __global__ __launch_bounds__(256) void rows_map_kernel(CacheRowsParams p, int ro
     if (r < p.n_reqs && plan[r].state == 1) {
         const int bt = 1 << p.bt_log, row0 = p.cu[r], len = p.seq_len[r];
         pos = len + t - row0;
-        const int b = pos >> p.bt_log, off = pos & (bt - 1), held = held_pages(p, len);
+        const int b = pos >> p.bt_log, off = pos & (bt - 1), held = pages_of(p, r, len);
         int page;
         if (b < held) {
             page = p.table[r * p.table_st + b];
@@ -247,7 +252,7 @@ __global__ __launch_bounds__(kPlanThreads) void rows_one_kernel(CacheRowsParams 
 #pragma unroll
     for (int i = 0; i < kOnePer; ++i) {
         end += max(n[i], (int64_t)0);
-        held[i] = held_pages(p, len[i]);
+        held[i] = pages_of(p, min(tid * per + i, R - 1), len[i]);
         fits[i] = n[i] >= 0 && len[i] >= 0 && len[i] + n[i] <= ((int64_t)p.cols << p.bt_log) && end <= p.n_rows;
         need[i] = fits[i] ? max(held_pages(p, len[i] + n[i]) - held[i], 0) : 0;
         mine += ((unsigned long long)need[i] << 32) + (n[i] < 0 && len[i] >= 0 ? held[i] : 0);
@@ -302,7 +307,7 @@ __global__ __launch_bounds__(kPlanThreads) void rows_one_kernel(CacheRowsParams 
     // pages given back: a wave a request
     for (int r = blockIdx.x * (kPlanThreads / 64) + (tid >> 6); r < R; r += gridDim.x * (kPlanThreads / 64)) {
         if (sh.piece[r] != -2) continue;
-        const int pages = held_pages(p, p.seq_len[r]);
+        const int pages = pages_of(p, r, p.seq_len[r]);
         const int64_t to = tail + sh.take[r];
         for (int j = tid & 63; j < pages; j += 64)
             if (to + j - head < p.n_free) p.ring[(uint64_t)(to + j) % (uint64_t)p.n_free] = p.table[r * p.table_st + j];
@@ -322,7 +327,7 @@ __global__ __launch_bounds__(kPlanThreads) void rows_one_kernel(CacheRowsParams 
     if (r < R && sh.piece[r] >= 0) {
         const int first = sh.cu[r], old = p.seq_len[r];
         pos = old + t - first;
-        const int b = pos >> p.bt_log, off = pos & (bt - 1), had = held_pages(p, old);
+        const int b = pos >> p.bt_log, off = pos & (bt - 1), had = pages_of(p, r, old);
         int page;
         if (b < had) {
             page = p.table[r * p.table_st + b];

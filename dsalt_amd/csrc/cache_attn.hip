@@ -10,6 +10,7 @@
 
 #include "cache.h"
 #include "common.h"
+#include "decode_attn.h"
 #include "fp8.h"
 #include "timing.h"
 
@@ -18,17 +19,6 @@ namespace dsalt {
 namespace {
 
 constexpr int kStep = 32;  // window keys a wave takes at a time
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
-
-// number of bfloat16 parts of a query element (exact: 8, 11 and 24 bits) and of a weight: 16 bits of it for
-// 16-bit outputs, whose own rounding, half a step of 2^-8 or 2^-11 of a value, is far coarser, 24 for float32 (lists keep
-// weights in float32)
-template <typename T> struct Parts;
-template <> struct Parts<bf16> { static constexpr int q = 1, p = 2; };
-template <> struct Parts<f16> { static constexpr int q = 2, p = 2; };
-template <> struct Parts<float> { static constexpr int q = 3, p = 3; };
 
 // waves a SIMD that the registers are held to (168, 128 and 256 of them)
 template <typename T, int D> struct MinWaves { static constexpr int value = D == 64 ? 4 : 3; };
@@ -44,12 +34,6 @@ struct AttnPlan {
     int waves;   // of a block
     int chunks;  // parts of a head's landmark slots within a block (groups)
 };
-
-__device__ __forceinline__ uint32_t half_pair(uint32_t a, uint32_t b, bool hi) {  // halves of a and b side by side
-    return __builtin_amdgcn_perm(b, a, hi ? 0x07060302u : 0x05040100u);
-}
-
-__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }  // v_exp_f32: to 1 ulp, 0 below 2^-126
 
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
@@ -72,30 +56,6 @@ template <int N>
 __device__ __forceinline__ float max_over(float v) {
     if (N == 4) v = fmaxf(v, dpp<0x124>(v));
     return max_g4(fmaxf(v, dpp<0x128>(v)));
-}
-
-// eight elements of a 16-byte aligned row as floats
-template <typename T>
-__device__ __forceinline__ void load8(const T* x, float* f) {
-    typedef T vec __attribute__((ext_vector_type(8), aligned(16)));
-    const vec v = *(const vec*)x;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = to_float(v[e]);
-}
-
-// eight floats into PARTS bfloat16 operands that sum to them
-template <int PARTS>
-__device__ __forceinline__ void split8(const float* x, bf16x8* o) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        float r = x[e];
-#pragma unroll
-        for (int k = 0; k < PARTS; ++k) {
-            const bf16 h = (bf16)r;
-            o[k][e] = h;
-            r -= (float)h;
-        }
-    }
 }
 
 // One query row: its request's table, the first position of its window and the last that the table can name.
@@ -515,49 +475,6 @@ __global__ __launch_bounds__(64 * kWaves, (MinWaves<T, D>::value)) void cache_at
     join_parts<T, D, 64 * kWaves>(p, ml, accs, parts, a.nh, nh, t, h0, split, a.ns);
 }
 
-// The splits of a row and head joined: a block each, its waves over the splits, a lane D / 64 elements.
-constexpr int kJoinWaves = 8;
-
-template <typename T, int D>
-__global__ __launch_bounds__(64 * kJoinWaves) void cache_attn_join_kernel(CacheAttnParams p, int ns) {
-    constexpr int E = D / 64;
-    typedef float vec __attribute__((ext_vector_type(E)));
-    __shared__ vec outs[kJoinWaves][64];
-    __shared__ float sums[kJoinWaves];
-    const int64_t th = blockIdx.x;
-    const int t = (int)(th / p.n_heads), h = (int)(th - (int64_t)t * p.n_heads), lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    const float2* ml = (const float2*)p.ws + th * ns;
-    const float* acc = (const float*)p.ws + 2 * (int64_t)p.n_rows * p.n_heads * ns + th * ns * D + lane * E;
-    float M = -INFINITY, L = 0.f;
-    for (int k = lane; k < ns; k += 64) M = fmaxf(M, ml[k].x);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, wave_xor(M, o));
-    const float mb = M == -INFINITY ? 0.f : M;
-    vec o = {};
-#pragma unroll 4
-    for (int k = wv; k < ns; k += kJoinWaves) {
-        const float2 v = ml[k];
-        const vec x = *(const vec*)(acc + (int64_t)k * D);
-        const float f = v.x == -INFINITY ? 1.f : exp2_(v.x - mb);
-        L += v.y == 0.f ? 0.f : v.y * f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += v.y == 0.f ? 0.f : x[e] * f;  // (a split with sum 0 wrote no values)
-    }
-    outs[wv][lane] = o;
-    if (lane == 0) sums[wv] = L;
-    __syncthreads();
-    if (wv == 0) {
-        for (int k = 1; k < kJoinWaves; ++k) {
-            o += outs[k][lane];
-            L += sums[k];
-        }
-        T* y = (T*)p.out + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; ++e) y[e] = from_float<T>(L == 0.f ? 0.f : o[e] / L);
-        if (lane == 0) p.lse[th] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
-    }
-}
-
 // Which kernel, with how many waves and splits.  us on the device, 16/2 heads of 128, 128 landmarks:
 //  * A block a head reads a window once for each query head, a block a group once: the former is latency bound and
 //    smaller, so it wins up to about 2^18 pairs of a query head and a window key (w_max 512: one request 9 / 19, 8:
@@ -612,7 +529,7 @@ hipError_t run_rows(const CacheAttnParams& p, const AttnPlan& a, hipStream_t str
     }
     if (a.ns > 1) {
         const dim3 join((unsigned)((int64_t)p.n_rows * p.n_heads));
-        DSALT_LAUNCH("cache_attn_join", (cache_attn_join_kernel<T, D>), join, dim3(64 * kJoinWaves), 0, stream, p, a.ns);
+        DSALT_LAUNCH("cache_attn_join", (cache_attn_join_kernel<T, D, CacheAttnParams>), join, dim3(64 * kJoinWaves), 0, stream, p, a.ns);
     }
     return hipGetLastError();
 }

@@ -9,14 +9,17 @@
 
 #include "attn.h"
 #include "cache.h"
+#include "cache4.h"
 #include "ce.h"
 #include "ffn.h"
 #include "layer.h"
 #include "probs.h"
+#include "qknorm.h"
 #include "rope.h"
 #include "sample.h"
 #include "select.h"
 #include "sets.h"
+#include "verify.h"
 #include "common.h"
 
 namespace {
@@ -86,8 +89,9 @@ int check_rows(const void* ptr, int64_t st, int64_t sh, int dtype, const char* n
     return DSALT_OK;
 }
 
-// pages of the 8-bit cache
-int check_cache(const dsalt_cache& c) {
+// pages of a cache
+template <typename C>
+int check_pages(const C& c) {
     if (c.n_blocks < 1 || c.n_kv_heads < 1 || c.n_kv_heads > 65535)
         return fail(DSALT_ERR_INVALID, "the cache needs n_blocks >= 1 and n_kv_heads in [1, 65535] (got %d, %d)", c.n_blocks,
                     c.n_kv_heads);
@@ -98,6 +102,11 @@ int check_cache(const dsalt_cache& c) {
     if ((int64_t)c.n_blocks * c.n_kv_heads >= 0xffffffffll / c.block_tokens)
         return fail(DSALT_ERR_INVALID, "n_blocks x n_kv_heads x block_tokens must stay below 2^32 - 1 (got %d x %d x %d)", c.n_blocks,
                     c.n_kv_heads, c.block_tokens);
+    return DSALT_OK;
+}
+
+int check_cache(const dsalt_cache& c) {
+    if (int rc = check_pages(c)) return rc;
     if (!c.k || !c.v || !c.k_scale || !c.v_scale || !aligned16(c.k) || !aligned16(c.v))
         return fail(DSALT_ERR_INVALID, "the cache's k, v (16-byte aligned) and scales are required");
     return DSALT_OK;
@@ -108,6 +117,17 @@ dsalt::CachePages cache_pages(const dsalt_cache& c) {
             c.k_scale, c.v_scale};
 }
 
+int check_cache(const dsalt_cache4& c) {
+    if (int rc = check_pages(c)) return rc;
+    if (!c.kv || !c.scale || !aligned16(c.kv) || !aligned16(c.scale))
+        return fail(DSALT_ERR_INVALID, "the cache's kv and scale (16-byte aligned) are required");
+    return DSALT_OK;
+}
+
+dsalt::Cache4Pages cache_pages(const dsalt_cache4& c) {
+    return {c.n_blocks, c.n_kv_heads, __builtin_ctz((unsigned)c.block_tokens), c.head_dim, (uint8_t*)c.kv, (uint8_t*)c.scale};
+}
+
 int check_table(const void* table, int64_t stride, int n_reqs, int cols, int block_tokens) {
     if (n_reqs < 1 || cols < 1) return fail(DSALT_ERR_INVALID, "n_reqs >= 1 and table_cols >= 1 required (got %d, %d)", n_reqs, cols);
     if ((int64_t)cols * block_tokens > (1 << 30))
@@ -116,8 +136,9 @@ int check_table(const void* table, int64_t stride, int n_reqs, int cols, int blo
     return DSALT_OK;
 }
 
-dsalt::CacheAttnParams cache_attn_params(const dsalt_cache_attn_args* a) {
-    dsalt::CacheAttnParams p = {};
+template <typename Params, typename Args>
+Params attn_params_of(const Args* a) {
+    Params p = {};
     p.c = cache_pages(a->c);
     p.n_rows = a->n_rows;
     p.n_heads = a->n_heads;
@@ -142,11 +163,23 @@ dsalt::CacheAttnParams cache_attn_params(const dsalt_cache_attn_args* a) {
     p.lse = a->lse;
     p.scale = a->scale;
     p.ws = (char*)a->workspace;
+    return p;
+}
+
+dsalt::CacheAttnParams cache_attn_params(const dsalt_cache_attn_args* a) {
+    dsalt::CacheAttnParams p = attn_params_of<dsalt::CacheAttnParams>(a);
     p.ws_bytes = a->workspace_bytes;
     return p;
 }
 
-int check_cache_attn(const dsalt_cache_attn_args* a) {
+dsalt::Cache4AttnParams cache_attn_params(const dsalt_cache4_attn_args* a) {
+    dsalt::Cache4AttnParams p = attn_params_of<dsalt::Cache4AttnParams>(a);
+    p.per = a->rows_per_req < a->n_rows ? a->rows_per_req : a->n_rows > 1 ? a->n_rows : 1;
+    return p;
+}
+
+template <typename Args>
+int check_cache_attn(const Args* a) {
     if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
     int rc = check_cache(a->c);
     if (rc) return rc;
@@ -203,6 +236,174 @@ dsalt::SelectParams select_params(const dsalt_select_args* a) {
         p.plan_bounds = ap.plan_bounds;
         p.tile_wmax = ap.tile_wmax;
     }
+    return p;
+}
+
+int check_attn_call(const dsalt_cache4_attn_args* a) {
+    if (int rc = check_cache_attn(a)) return rc;
+    if (a->rows_per_req < 1) return fail(DSALT_ERR_INVALID, "rows_per_req must be positive, got %d", a->rows_per_req);
+    return DSALT_OK;
+}
+
+template <typename Params, typename Args>
+Params write_params(const Args* a) {
+    Params p;
+    p.c = cache_pages(a->c);
+    p.n_rows = a->n_rows;
+    p.n_pieces = a->n_pieces;
+    p.dtype = a->dtype;
+    p.k = a->k;
+    p.k_st = a->k_stride_t;
+    p.k_sh = a->k_stride_h;
+    p.v = a->v;
+    p.v_st = a->v_stride_t;
+    p.v_sh = a->v_stride_h;
+    p.pieces = a->pieces;
+    return p;
+}
+
+template <typename Args>
+int check_write(const Args* a) {
+    if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
+    int rc = check_cache(a->c);
+    if (rc) return rc;
+    if (a->n_rows < 0 || a->n_pieces < 0)
+        return fail(DSALT_ERR_INVALID, "n_rows >= 0 and n_pieces >= 0 required (got %d, %d)", a->n_rows, a->n_pieces);
+    if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if (a->n_rows == 0 || a->n_pieces == 0) return DSALT_OK;
+    if ((rc = check_rows(a->k, a->k_stride_t, a->k_stride_h, a->dtype, "k"))) return rc;
+    if ((rc = check_rows(a->v, a->v_stride_t, a->v_stride_h, a->dtype, "v"))) return rc;
+    if (!a->pieces || !aligned16(a->pieces)) return fail(DSALT_ERR_INVALID, "pieces (16-byte aligned) are required");
+    return DSALT_OK;
+}
+
+template <typename Params, typename Args>
+Params read_params(const Args* a) {
+    Params p;
+    p.c = cache_pages(a->c);
+    p.n_reqs = a->n_reqs;
+    p.cols = a->table_cols;
+    p.n_rows = a->n_rows;
+    p.dtype = a->dtype;
+    p.table_st = a->table_stride;
+    p.table = a->table;
+    p.cu = a->cu_seqlens;
+    p.start = a->start;
+    p.k = a->k;
+    p.v = a->v;
+    return p;
+}
+
+template <typename Args>
+int check_read(const Args* a) {
+    if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
+    int rc = check_cache(a->c);
+    if (rc) return rc;
+    if ((rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols, a->c.block_tokens))) return rc;
+    if (a->n_rows < 0) return fail(DSALT_ERR_INVALID, "n_rows must be >= 0, got %d", a->n_rows);
+    if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if ((int64_t)a->n_rows * a->c.n_kv_heads > 0x7fffffff)
+        return fail(DSALT_ERR_INVALID, "n_rows x n_kv_heads must stay below 2^31 (got %d x %d)", a->n_rows, a->c.n_kv_heads);
+    if (a->n_rows == 0) return DSALT_OK;
+    if (!a->cu_seqlens || !a->k || !a->v || !aligned16(a->k) || !aligned16(a->v))
+        return fail(DSALT_ERR_INVALID, "cu_seqlens, k and v (16-byte aligned) are required");
+    return DSALT_OK;
+}
+
+// buffers of an attention over a cache whose shape has been checked
+template <typename Args>
+int check_attn_buffers(const Args* a, size_t need) {
+    int rc;
+    if ((rc = check_rows(a->q, a->q_stride_t, a->q_stride_h, a->dtype, "q"))) return rc;
+    if ((rc = check_rows(a->out, a->o_stride_t, a->o_stride_h, a->dtype, "out"))) return rc;
+    if (!a->req || !a->pos || !a->w || !a->lse || (a->k_lmk > 0 && !a->lmk_idx))
+        return fail(DSALT_ERR_INVALID, "req, pos, w, lse and lmk_idx are required");
+    if (need && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need))
+        return fail(DSALT_ERR_WORKSPACE, "workspace of %zu bytes required", need);
+    return DSALT_OK;
+}
+
+int check_qk(const dsalt_qk_norm_rope_args* a) {
+    if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
+    if (a->total_len < 0 || a->n_q_heads < 0 || a->n_k_heads < 0 || a->n_q_heads > 65535 || a->n_k_heads > 65535)
+        return fail(DSALT_ERR_INVALID, "total_len >= 0 and heads in [0, 65535] required (got %d, %d, %d)", a->total_len, a->n_q_heads,
+                    a->n_k_heads);
+    if (a->head_dim < 16 || a->head_dim > 256 || a->head_dim % 16)
+        return fail(DSALT_ERR_INVALID, "head_dim must be a multiple of 16 in [16, 256], got %d", a->head_dim);
+    if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if (a->weight_dtype < 0 || a->weight_dtype > 2) return fail(DSALT_ERR_INVALID, "unknown weight_dtype %d", a->weight_dtype);
+    if (!(a->eps >= 0.f)) return fail(DSALT_ERR_INVALID, "eps must not be negative");
+    if (!a->cu_seqlens == !a->pos) return fail(DSALT_ERR_INVALID, "either cu_seqlens or pos is required");
+    if (a->cu_seqlens && a->num_seqs < 1) return fail(DSALT_ERR_INVALID, "num_seqs must be positive, got %d", a->num_seqs);
+    if (a->max_pos < 1 || !a->cos || !a->sin || !aligned16(a->cos) || !aligned16(a->sin))
+        return fail(DSALT_ERR_INVALID, "cos and sin (16-byte aligned) of at least one position are required");
+    if ((a->n_q_heads && (!a->q_weight || !aligned16(a->q_weight))) || (a->n_k_heads && (!a->k_weight || !aligned16(a->k_weight))))
+        return fail(DSALT_ERR_INVALID, "q_weight and k_weight (16-byte aligned) are required");
+    return DSALT_OK;
+}
+
+int check_qk_rows(const dsalt_qk_norm_rope_args* a) {
+    int rc;
+    if (a->n_q_heads && ((rc = check_rows(a->q, a->q_stride_t, a->q_stride_h, a->dtype, "q")) ||
+                         (rc = check_rows(a->q_out, a->qo_stride_t, a->qo_stride_h, a->dtype, "q_out"))))
+        return rc;
+    if (a->n_k_heads && ((rc = check_rows(a->k, a->k_stride_t, a->k_stride_h, a->dtype, "k")) ||
+                         (rc = check_rows(a->k_out, a->ko_stride_t, a->ko_stride_h, a->dtype, "k_out"))))
+        return rc;
+    return DSALT_OK;
+}
+
+dsalt::QkNormParams qk_params(const dsalt_qk_norm_rope_args* a) {
+    dsalt::QkNormParams p = {};
+    p.total_len = a->total_len;
+    p.num_seqs = a->num_seqs;
+    p.head_dim = a->head_dim;
+    p.dtype = a->dtype;
+    p.w_dtype = a->weight_dtype;
+    p.max_pos = a->max_pos;
+    p.q = {a->n_q_heads, a->q, a->q_stride_t, a->q_stride_h, a->q_out, a->qo_stride_t, a->qo_stride_h, a->q_weight};
+    p.k = {a->n_k_heads, a->k, a->k_stride_t, a->k_stride_h, a->k_out, a->ko_stride_t, a->ko_stride_h, a->k_weight};
+    p.cu = a->cu_seqlens;
+    p.pos = a->pos;
+    p.cos = a->cos;
+    p.sin = a->sin;
+    p.eps = a->eps;
+    return p;
+}
+
+int check_verify(const dsalt_verify_args* a) {
+    if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
+    if (a->n_reqs < 0 || a->n_rows < 0 || a->n_reqs > (1 << 22) || a->n_rows > (1 << 22))
+        return fail(DSALT_ERR_INVALID, "n_reqs and n_rows must be in [0, 2^22], got %d, %d", a->n_reqs, a->n_rows);
+    if (a->n_cols < 1 || a->n_cols > dsalt::kSampleMaxCols)
+        return fail(DSALT_ERR_INVALID, "n_cols must be in [1, %d], got %d", dsalt::kSampleMaxCols, a->n_cols);
+    if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
+    if (a->u_bytes != 4 && a->u_bytes != 8) return fail(DSALT_ERR_INVALID, "u_bytes must be 4 or 8, got %d", a->u_bytes);
+    return DSALT_OK;
+}
+
+dsalt::VerifyParams verify_params(const dsalt_verify_args* a) {
+    dsalt::VerifyParams p;
+    p.n_reqs = a->n_reqs;
+    p.n_rows = a->n_rows;
+    p.n_cols = a->n_cols;
+    p.dtype = a->dtype;
+    p.u_f64 = a->u_bytes == 8;
+    p.x = a->logits;
+    p.x_st = a->logits_stride;
+    p.y = a->draft_logits;
+    p.y_st = a->draft_stride;
+    p.tokens = a->tokens;
+    p.cu = a->cu;
+    p.u = a->u;
+    p.v = a->v;
+    p.temperature = a->temperature;
+    p.draft_temperature = a->draft_temperature;
+    p.temperature_all = a->temperature_all;
+    p.draft_temperature_all = a->draft_temperature_all;
+    p.accepted = a->accepted;
+    p.out = a->out;
+    p.ws = (char*)a->workspace;
     return p;
 }
 
@@ -671,6 +872,51 @@ int dsalt_rope_qk(const dsalt_rope_args* a, dsalt_stream_t stream) {
     return hip_status(dsalt::rope_launch(p, (hipStream_t)stream), "dsalt_rope_qk");
 }
 
+int dsalt_qk_norm_rope(const dsalt_qk_norm_rope_args* a, dsalt_stream_t stream) {
+    int rc = check_qk(a);
+    if (rc || a->total_len == 0) return rc;
+    if ((rc = check_qk_rows(a))) return rc;
+    dsalt::QkNormParams p = qk_params(a);
+    auto same = [](const dsalt::QkSide& s) { return s.heads == 0 || (s.x == s.y && s.st == s.y_st && s.sh == s.y_sh); };
+    if ((p.q.heads && p.q.x == p.q.y && !same(p.q)) || (p.k.heads && p.k.x == p.k.y && !same(p.k)) ||
+        (p.q.heads && p.k.heads && same(p.q) != same(p.k)))
+        return fail(DSALT_ERR_INVALID, "the outputs are both the inputs, with their strides, or neither is");
+    p.inplace = same(p.q) && same(p.k);
+    return hip_status(dsalt::qk_norm_rope_launch(p, (hipStream_t)stream), "dsalt_qk_norm_rope");
+}
+
+size_t dsalt_qk_norm_rope_bwd_workspace_bytes(const dsalt_qk_norm_rope_bwd_args* a) {
+    return check_qk(a ? &a->base : nullptr)
+               ? 0 : dsalt::qk_norm_rope_bwd_ws_bytes(a->base.total_len, a->base.n_q_heads + a->base.n_k_heads, a->base.head_dim);
+}
+
+int dsalt_qk_norm_rope_bwd(const dsalt_qk_norm_rope_bwd_args* a, dsalt_stream_t stream) {
+    int rc = check_qk(a ? &a->base : nullptr);
+    if (rc) return rc;
+    const dsalt_qk_norm_rope_args* b = &a->base;
+    if (b->total_len > 0) {
+        if ((rc = check_qk_rows(b))) return rc;
+        if (b->n_q_heads && (rc = check_rows(a->dq, a->dq_stride_t, a->dq_stride_h, b->dtype, "dq"))) return rc;
+        if (b->n_k_heads && (rc = check_rows(a->dk, a->dk_stride_t, a->dk_stride_h, b->dtype, "dk"))) return rc;
+    }
+    if ((b->n_q_heads && !a->dq_weight) || (b->n_k_heads && !a->dk_weight))
+        return fail(DSALT_ERR_INVALID, "dq_weight and dk_weight are required");
+    const size_t need = dsalt::qk_norm_rope_bwd_ws_bytes(b->total_len, b->n_q_heads + b->n_k_heads, b->head_dim);
+    if (need && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need))
+        return fail(DSALT_ERR_WORKSPACE, "workspace of %zu bytes required", need);
+    dsalt::QkNormParams p = qk_params(b);
+    p.q.d = a->dq;
+    p.q.d_st = a->dq_stride_t;
+    p.q.d_sh = a->dq_stride_h;
+    p.q.dw = b->n_q_heads ? a->dq_weight : nullptr;
+    p.k.d = a->dk;
+    p.k.d_st = a->dk_stride_t;
+    p.k.d_sh = a->dk_stride_h;
+    p.k.dw = b->n_k_heads ? a->dk_weight : nullptr;
+    p.ws = (float*)a->workspace;
+    return hip_status(dsalt::qk_norm_rope_bwd_launch(p, (hipStream_t)stream), "dsalt_qk_norm_rope_bwd");
+}
+
 int dsalt_export_probs(const dsalt_probs_args* a, dsalt_stream_t stream) {
     if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
     int rc = check_problem(a->p, true);
@@ -821,7 +1067,9 @@ size_t dsalt_cache_rows_workspace_bytes(const dsalt_cache_rows_args* a) {
     return a && a->n_reqs >= 1 ? dsalt::cache_rows_ws_bytes(a->n_reqs, a->table_cols) : 0;
 }
 
-int dsalt_cache_rows(const dsalt_cache_rows_args* a, dsalt_stream_t stream) {
+int dsalt_cache_rows(const dsalt_cache_rows_args* a, dsalt_stream_t stream) { return dsalt_cache_rows_held(a, nullptr, stream); }
+
+int dsalt_cache_rows_held(const dsalt_cache_rows_args* a, const int32_t* held, dsalt_stream_t stream) {
     if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
     if (a->block_tokens != 16 && a->block_tokens != 32 && a->block_tokens != 64 && a->block_tokens != 128)
         return fail(DSALT_ERR_INVALID, "block_tokens must be 16, 32, 64 or 128, got %d", a->block_tokens);
@@ -852,6 +1100,7 @@ int dsalt_cache_rows(const dsalt_cache_rows_args* a, dsalt_stream_t stream) {
     p.table_st = a->table_stride;
     p.seq_len = a->seq_len;
     p.new_len = a->new_len;
+    p.held = held;
     p.table = a->table;
     p.ring = a->free_blocks;
     p.span = a->span;
@@ -868,56 +1117,15 @@ int dsalt_cache_rows(const dsalt_cache_rows_args* a, dsalt_stream_t stream) {
 }
 
 int dsalt_cache_write(const dsalt_cache_write_args* a, dsalt_stream_t stream) {
-    if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
-    int rc = check_cache(a->c);
-    if (rc) return rc;
-    if (a->n_rows < 0 || a->n_pieces < 0)
-        return fail(DSALT_ERR_INVALID, "n_rows >= 0 and n_pieces >= 0 required (got %d, %d)", a->n_rows, a->n_pieces);
-    if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
-    if (a->n_rows == 0 || a->n_pieces == 0) return DSALT_OK;
-    if ((rc = check_rows(a->k, a->k_stride_t, a->k_stride_h, a->dtype, "k"))) return rc;
-    if ((rc = check_rows(a->v, a->v_stride_t, a->v_stride_h, a->dtype, "v"))) return rc;
-    if (!a->pieces || !aligned16(a->pieces)) return fail(DSALT_ERR_INVALID, "pieces (16-byte aligned) are required");
-    dsalt::CacheWriteParams p;
-    p.c = cache_pages(a->c);
-    p.n_rows = a->n_rows;
-    p.n_pieces = a->n_pieces;
-    p.dtype = a->dtype;
-    p.k = a->k;
-    p.k_st = a->k_stride_t;
-    p.k_sh = a->k_stride_h;
-    p.v = a->v;
-    p.v_st = a->v_stride_t;
-    p.v_sh = a->v_stride_h;
-    p.pieces = a->pieces;
-    return hip_status(dsalt::cache_write_launch(p, (hipStream_t)stream), "dsalt_cache_write");
+    int rc = check_write(a);
+    if (rc || a->n_rows == 0 || a->n_pieces == 0) return rc;
+    return hip_status(dsalt::cache_write_launch(write_params<dsalt::CacheWriteParams>(a), (hipStream_t)stream), "dsalt_cache_write");
 }
 
 int dsalt_cache_read(const dsalt_cache_read_args* a, dsalt_stream_t stream) {
-    if (!a) return fail(DSALT_ERR_INVALID, "null argument struct");
-    int rc = check_cache(a->c);
-    if (rc) return rc;
-    if ((rc = check_table(a->table, a->table_stride, a->n_reqs, a->table_cols, a->c.block_tokens))) return rc;
-    if (a->n_rows < 0) return fail(DSALT_ERR_INVALID, "n_rows must be >= 0, got %d", a->n_rows);
-    if (a->dtype < 0 || a->dtype > 2) return fail(DSALT_ERR_INVALID, "unknown dtype %d", a->dtype);
-    if ((int64_t)a->n_rows * a->c.n_kv_heads > 0x7fffffff)
-        return fail(DSALT_ERR_INVALID, "n_rows x n_kv_heads must stay below 2^31 (got %d x %d)", a->n_rows, a->c.n_kv_heads);
-    if (a->n_rows == 0) return DSALT_OK;
-    if (!a->cu_seqlens || !a->k || !a->v || !aligned16(a->k) || !aligned16(a->v))
-        return fail(DSALT_ERR_INVALID, "cu_seqlens, k and v (16-byte aligned) are required");
-    dsalt::CacheReadParams p;
-    p.c = cache_pages(a->c);
-    p.n_reqs = a->n_reqs;
-    p.cols = a->table_cols;
-    p.n_rows = a->n_rows;
-    p.dtype = a->dtype;
-    p.table_st = a->table_stride;
-    p.table = a->table;
-    p.cu = a->cu_seqlens;
-    p.start = a->start;
-    p.k = a->k;
-    p.v = a->v;
-    return hip_status(dsalt::cache_read_launch(p, (hipStream_t)stream), "dsalt_cache_read");
+    int rc = check_read(a);
+    if (rc || a->n_rows == 0) return rc;
+    return hip_status(dsalt::cache_read_launch(read_params<dsalt::CacheReadParams>(a), (hipStream_t)stream), "dsalt_cache_read");
 }
 
 size_t dsalt_cache_attn_workspace_bytes(const dsalt_cache_attn_args* a) {
@@ -927,15 +1135,56 @@ size_t dsalt_cache_attn_workspace_bytes(const dsalt_cache_attn_args* a) {
 int dsalt_cache_attn(const dsalt_cache_attn_args* a, dsalt_stream_t stream) {
     int rc = check_cache_attn(a);
     if (rc || a->n_rows == 0) return rc;
-    if ((rc = check_rows(a->q, a->q_stride_t, a->q_stride_h, a->dtype, "q"))) return rc;
-    if ((rc = check_rows(a->out, a->o_stride_t, a->o_stride_h, a->dtype, "out"))) return rc;
-    if (!a->req || !a->pos || !a->w || !a->lse || (a->k_lmk > 0 && !a->lmk_idx))
-        return fail(DSALT_ERR_INVALID, "req, pos, w, lse and lmk_idx are required");
     const dsalt::CacheAttnParams p = cache_attn_params(a);
-    const size_t need = dsalt::cache_attn_ws_bytes(p);
+    if ((rc = check_attn_buffers(a, dsalt::cache_attn_ws_bytes(p)))) return rc;
+    return hip_status(dsalt::cache_attn_launch(p, (hipStream_t)stream), "dsalt_cache_attn");
+}
+
+int dsalt_cache4_write(const dsalt_cache4_write_args* a, dsalt_stream_t stream) {
+    int rc = check_write(a);
+    if (rc || a->n_rows == 0 || a->n_pieces == 0) return rc;
+    return hip_status(dsalt::cache4_write_launch(write_params<dsalt::Cache4WriteParams>(a), (hipStream_t)stream), "dsalt_cache4_write");
+}
+
+int dsalt_cache4_read(const dsalt_cache4_read_args* a, dsalt_stream_t stream) {
+    int rc = check_read(a);
+    if (rc || a->n_rows == 0) return rc;
+    return hip_status(dsalt::cache4_read_launch(read_params<dsalt::Cache4ReadParams>(a), (hipStream_t)stream), "dsalt_cache4_read");
+}
+
+size_t dsalt_cache4_attn_workspace_bytes(const dsalt_cache4_attn_args* a) {
+    return check_attn_call(a) ? 0 : dsalt::cache4_attn_ws_bytes(cache_attn_params(a));
+}
+
+int dsalt_cache4_attn(const dsalt_cache4_attn_args* a, dsalt_stream_t stream) {
+    int rc = check_attn_call(a);
+    if (rc || a->n_rows == 0) return rc;
+    const dsalt::Cache4AttnParams p = cache_attn_params(a);
+    if ((rc = check_attn_buffers(a, dsalt::cache4_attn_ws_bytes(p)))) return rc;
+    return hip_status(dsalt::cache4_attn_launch(p, (hipStream_t)stream), "dsalt_cache4_attn");
+}
+
+size_t dsalt_verify_workspace_bytes(const dsalt_verify_args* a) {
+    return check_verify(a) ? 0 : dsalt::verify_ws_bytes(verify_params(a));
+}
+
+int dsalt_verify_rows(const dsalt_verify_args* a, dsalt_stream_t stream) {
+    int rc = check_verify(a);
+    if (rc || (a->n_reqs == 0 && a->n_rows == 0)) return rc;
+    const size_t es = esize(a->dtype);
+    if (!a->cu || (a->n_reqs > 0 && (!a->accepted || !a->v))) return fail(DSALT_ERR_INVALID, "cu, v and accepted are required");
+    if (a->n_rows > 0) {
+        if (!a->logits || (uintptr_t)a->logits % es || a->logits_stride < 0)
+            return fail(DSALT_ERR_INVALID, "logits need element alignment and a row stride >= 0");
+        if ((uintptr_t)a->draft_logits % es || (a->draft_logits && a->draft_stride < 0))
+            return fail(DSALT_ERR_INVALID, "draft_logits need element alignment and a row stride >= 0");
+        if (!a->tokens || !a->u || !a->out) return fail(DSALT_ERR_INVALID, "tokens, u and out are required");
+    }
+    const dsalt::VerifyParams p = verify_params(a);
+    const size_t need = dsalt::verify_ws_bytes(p);
     if (need && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need))
         return fail(DSALT_ERR_WORKSPACE, "workspace of %zu bytes required", need);
-    return hip_status(dsalt::cache_attn_launch(p, (hipStream_t)stream), "dsalt_cache_attn");
+    return hip_status(dsalt::verify_launch(p, (hipStream_t)stream), "dsalt_verify_rows");
 }
 
 int dsalt_sample_rows(const dsalt_sample_args* a, dsalt_stream_t stream) {

@@ -27,6 +27,7 @@
 #include "common.h"
 #include "sample.h"
 #include "timing.h"
+#include "weights.h"
 
 namespace dsalt {
 
@@ -34,7 +35,6 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 4096, kList = 2048;
 constexpr double kPerUnit = 94.0;
-constexpr unsigned long long kUnit = 1ull << 42;  // sums over 2^20 tokens stay below 2^62
 
 // keys: larger logits, larger keys; 0 where there is no element
 template <typename T> struct Key;
@@ -127,19 +127,6 @@ __device__ __forceinline__ unsigned long long wave_sum2(uint32_t low, uint32_t h
 // and for weights: sums of at most 64 x 8 of 2^42, in two parts of 25 and 20 bits a lane
 __device__ __forceinline__ unsigned long long wave_sum_weights(unsigned long long v) {
     return wave_sum2<25>((uint32_t)v & 0x1ffffffu, (uint32_t)(v >> 25));
-}
-
-// 2^42 (2^f - 1) = f P(f) for f in [-1/2, 1/2], P the degree 9 polynomial through the ten Chebyshev nodes (relative
-// error of 2^f below 2^-50)
-__device__ constexpr double kPow2[10] = {0x1.62e42fefa39f7p41, 0x1.ebfbdff82c590p39, 0x1.c6b08d7044119p37, 0x1.3b2ab6fba385fp35,
-                                         0x1.5d87fe908f88ap32, 0x1.4309130378460p29, 0x1.ffcb76789860fp25, 0x1.62bfe46117445p22,
-                                         0x1.b6571de2f2351p18, 0x1.e5e9f548e5725p14};
-
-// x f + c with c in scalar registers (from vector registers it would be copied before each sum)
-__device__ __forceinline__ double fma_s(double x, double f, double c) {
-    double y;
-    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(y) : "v"(x), "v"(f), "s"(c));
-    return y;
 }
 
 template <typename T>
@@ -286,19 +273,10 @@ struct Row {
     }
     __device__ __forceinline__ bool has(int i) const { return (unsigned)i < (unsigned)n; }
     // round(2^42 2^t), t = (v - m) log2(e) / temperature.  (v - m is exact, or rounded to 2^-53 of itself where the two lie
-    // far apart; t below -43 rounds to 0, NaN and absent elements among it.  Sums with 1.5 2^52 and 2^52 round to a whole number and leave it in the mantissa.)
+    // far apart; t below -43 rounds to 0, NaN and absent elements among it.)
     __device__ __forceinline__ unsigned long long weight(float v) const { return weight_of(exponent(v)); }
     __device__ __forceinline__ double exponent(float v) const { return fmin(fmax(((double)v - m) * rate, -60.0), 0.0); }
-    __device__ __forceinline__ static unsigned long long weight_of(double t) {
-        const double s = t + 6755399441055744.0;
-        const double f = t - (s - 6755399441055744.0);
-        double y = kPow2[9];
-#pragma unroll
-        for (int k = 8; k >= 0; --k) y = fma_s(y, f, kPow2[k]);
-        y = fma_s(y, f, 0x1p42);
-        y = __hiloint2double(__double2hiint(y) + (__double2loint(s) << 20), __double2loint(y)) + 4503599627370496.0;
-        return (unsigned long long)__double_as_longlong(y) & 0xfffffffffffffull;
-    }
+    __device__ __forceinline__ static unsigned long long weight_of(double t) { return whole_weight(t); }
     // The bin of an exponent: kBins even parts of (-43.6, 0], the highest at 0, bin 0 for all beyond (of weight 0).  Rounding
     // keeps the order, so larger logits are never in lower bins.
     __device__ __forceinline__ static int bin_of(double t) { return max(kBins - 1 - (int)(t * -kPerUnit), 0); }

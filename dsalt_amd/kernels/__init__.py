@@ -9,6 +9,7 @@ from .dsalt_attn import DSALTAttentionFunction, dsalt_attention, dsalt_triton_at
 from .dsalt_bwd import dsalt_backward, dsalt_triton_backward
 from .dsalt_train import DSALTTrainFunction, dsalt_train_attention, dsalt_triton_train_attention
 from .landmark_tokens_ker import hybrid_scores_per_head
+from .qk_norm_rope import QkNormRopeFunction, qk_norm_rope
 from .selectors import _build_landmark_kv, _build_seq_block_map, _compute_landmark_indices, _seq_meta
 from .sparse_attn import sparse_attention_forward, sparse_attention_forward_packed
 from .window_utils import (apply_rotary_emb, build_local_window_mask, build_local_window_mask_packed,
@@ -34,5 +35,5 @@ __all__ = [
     "hybrid_scores_per_head", "_compute_landmark_indices", "_build_landmark_kv", "_seq_meta",
     "_build_seq_block_map", "sparse_attention_forward", "sparse_attention_forward_packed",
     "build_local_window_mask", "build_local_window_mask_packed", "apply_rotary_emb", "build_rope_cache",
-    "autotune_blocks", "get_tuned_config",
+    "qk_norm_rope", "QkNormRopeFunction", "autotune_blocks", "get_tuned_config",
 ]

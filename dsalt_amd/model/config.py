@@ -2,7 +2,8 @@
 
 Mirrors ``DSALTConfig`` of ``dsalt/model/config.py:10-91`` (same fields, defaults, checks
 and JSON round trip), plus the attention layer's landmark variant: ``select_mode``
-("global" or "block"), ``block_size`` and ``stats_scope``.
+("global" or "block"), ``block_size`` and ``stats_scope``, and ``qk_norm`` (norms of its query and
+key heads).
 """
 from __future__ import annotations
 
@@ -35,6 +36,7 @@ class DSALTConfig:
     select_mode: str = "global"
     block_size: int = 512
     stats_scope: str = "packed"
+    qk_norm: bool = False
 
     def __post_init__(self) -> None:
         if self.d_model % self.n_heads != 0:

@@ -40,7 +40,8 @@ class DSALTLMHeadModel(nn.Module):
                  yarn_scale: float = 1.0, tie_weights: bool = True, padding_idx: int | None = None,
                  lm_head_chunk_size: int = 2048, loss_fn: str = "chunked", aux_loss_weight: float = 0.0,
                  n_kv_heads: int | None = None, qkv_bias: bool = False, rope_base: float = 10000.0,
-                 select_mode: str = "global", block_size: int = 512, stats_scope: str = "packed"):
+                 select_mode: str = "global", block_size: int = 512, stats_scope: str = "packed",
+                 qk_norm: bool = False):
         super().__init__()
         if loss_fn not in ("auto", "chunked", "liger"):
             raise ValueError(f"unknown loss_fn {loss_fn!r} (one of 'auto', 'chunked', 'liger')")
@@ -54,7 +55,7 @@ class DSALTLMHeadModel(nn.Module):
             DSALTTransformerBlock(d_model=d_model, n_heads=n_heads, n_min=n_min, n_max=n_max, k_lmk=k_lmk,
                                   max_seq_len=max_seq_len, d_ff=d_ff, dropout=dropout, yarn_scale=yarn_scale,
                                   layer_idx=i, n_kv_heads=n_kv_heads, qkv_bias=qkv_bias, rope_base=rope_base,
-                                  select_mode=select_mode, block_size=block_size, stats_scope=stats_scope)
+                                  select_mode=select_mode, block_size=block_size, stats_scope=stats_scope, qk_norm=qk_norm)
             for i in range(n_layers)])
         self.final_norm = RMSENorm(d_model)
         self.lm_head = nn.Linear(d_model, vocab_size, bias=False)

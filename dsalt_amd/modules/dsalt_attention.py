@@ -13,6 +13,9 @@ Inference branch of ``_packed`` (:610-634):
     in the reference) and the sparse operator with zero landmark bias (:622).
 ``select_mode="block"`` switches to block-causal landmarks (``block_size`` query rows per
 set, statistics of the prefix), the variant of ``results/causal_landmark_check.py:150-189``.
+``qk_norm=True`` (not in the reference) adds a root-mean-square norm of each query and key head
+with a learned weight (``q_norm``, ``k_norm``) before the rotation, in one kernel with it
+(``kernels.qk_norm_rope``), forward and backward.
 Batched ``[B, T, d]`` input is run as ``B`` packed sequences of length ``T``.
 
 Training branch (``self.training``, :597-603, :440-487): the differentiable selectors --
@@ -41,6 +44,8 @@ from .. import ops
 from ..kernels.dsalt_attn import dsalt_attention, pad_head_dim, padded_head_dim
 from ..kernels.dsalt_train import dsalt_train_attention
 from ..kernels.landmark_tokens_ker import hybrid_scores_per_head
+from ..kernels.qk_norm_rope import qk_norm_rope
+from ..kernels.RMSENorm import RMSENorm
 from ..kernels.selectors import _MODES, _SCOPES, _compute_landmark_indices
 from ..kernels.window_utils import apply_rotary_emb, build_rope_cache
 
@@ -49,7 +54,7 @@ class DSALTAttention(nn.Module):
     def __init__(self, d_model: int, n_heads: int, n_min: int, n_max: int, k_lmk: int, max_seq_len: int,
                  dropout: float = 0.0, yarn_scale: float = 1.0, layer_idx: int = 0, n_kv_heads: int | None = None,
                  qkv_bias: bool = False, rope_base: float = 10000.0, select_mode: str = "global",
-                 block_size: int = 512, stats_scope: str = "packed"):
+                 block_size: int = 512, stats_scope: str = "packed", qk_norm: bool = False):
         super().__init__()
         assert d_model % n_heads == 0
         self.d_model = d_model
@@ -71,6 +76,9 @@ class DSALTAttention(nn.Module):
         self.q_proj = nn.Linear(d_model, d_model, bias=qkv_bias)
         self.k_proj = nn.Linear(d_model, self.kv_dim, bias=qkv_bias)
         self.v_proj = nn.Linear(d_model, self.kv_dim, bias=qkv_bias)
+        self.qk_norm = qk_norm
+        if qk_norm:
+            self.q_norm, self.k_norm = RMSENorm(self.head_dim), RMSENorm(self.head_dim)
         self.out_proj = nn.Linear(d_model, d_model, bias=False)
         self.win_gate = nn.Linear(d_model, 1, bias=True)
         self.alpha_w = nn.Parameter(torch.full((n_heads,), math.log(0.6 / 0.4)))
@@ -175,6 +183,15 @@ class DSALTAttention(nn.Module):
             self._rope32 = (key, c.float(), s.float())
         return self._rope32[1], self._rope32[2]
 
+    def _norm_rope(self, q, k, cos, sin, cu_seqlens, max_seqlen):
+        """The heads normed and rotated; over the inputs without autograd, where the kernel can write there."""
+        w = (self.q_norm.weight, self.k_norm.weight)
+        if torch.is_grad_enabled():
+            return qk_norm_rope(q, k, *w, cos, sin, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, eps=self.q_norm.eps)
+        aligned = all(t.data_ptr() % 16 == 0 and t.stride(0) * t.element_size() % 16 == 0 for t in (q, k))
+        return ops.qk_norm_rope(q, k, *w, cos, sin, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, eps=self.q_norm.eps,
+                                inplace=aligned)
+
     def _selectors(self, x):
         """(integer windows [T] int32, alpha [H] float32) of the inference branch: one kernel after
         the gate's product, or the torch expressions where the methods are replaced (by a subclass,
@@ -196,12 +213,16 @@ class DSALTAttention(nn.Module):
         k = qkv[:, H * D:(H + G) * D].view(total_len, G, D)
         v = qkv[:, (H + G) * D:].view(total_len, G, D)
         maxlen = ops._max_seqlen(cu_seqlens, cu_list)
+        cu_rope, len_rope = cu_seqlens, maxlen
         if rope_cs is None:
             cos, sin = self._rope_tables32()
-            ops.rope_qk_(q, k, cu_seqlens, cos, sin, max_seqlen=maxlen)
         else:  # rows already gathered per token: token t reads row t
-            cu1 = torch.tensor([0, total_len], dtype=torch.int32, device=device)
-            ops.rope_qk_(q, k, cu1, rope_cs[0].float(), rope_cs[1].float(), max_seqlen=total_len)
+            cu_rope, len_rope = torch.tensor([0, total_len], dtype=torch.int32, device=device), total_len
+            cos, sin = rope_cs[0].float(), rope_cs[1].float()
+        if self.qk_norm:
+            q, k = self._norm_rope(q, k, cos, sin, cu_rope, len_rope)
+        else:
+            ops.rope_qk_(q, k, cu_rope, cos, sin, max_seqlen=len_rope)
         w32, alpha = self._selectors(x)
         mode = _MODES[self.select_mode]
         # landmarks on x W_V^T without the bias, whatever the projection's; the selection's first
@@ -243,16 +264,23 @@ class DSALTAttention(nn.Module):
         q = self.q_proj(x).view(total_len, self.n_heads, self.head_dim)
         k = self.k_proj(x).view(total_len, self.n_kv_heads, self.head_dim)
         v = self.v_proj(x).view(total_len, self.n_kv_heads, self.head_dim)
-        if rope_cs is None:
-            cu = cu_seqlens.long()
-            lens = cu[1:] - cu[:-1]
-            seq_ids = torch.repeat_interleave(torch.arange(lens.numel(), device=device), lens)
-            pos = torch.arange(total_len, device=device) - cu[:-1][seq_ids]
-            cos, sin = self.rope_cos[pos], self.rope_sin[pos]
+        if self.qk_norm:
+            if rope_cs is None:
+                q, k = self._norm_rope(q, k, *self._rope_tables32(), cu_seqlens, ops._max_seqlen(cu_seqlens, cu_list))
+            else:
+                cu1 = torch.tensor([0, total_len], dtype=torch.int32, device=device)
+                q, k = self._norm_rope(q, k, rope_cs[0].float(), rope_cs[1].float(), cu1, total_len)
         else:
-            cos, sin = rope_cs
-        cos, sin = cos.to(q.dtype), sin.to(q.dtype)
-        q, k = apply_rotary_emb(q, k, cos.unsqueeze(1), sin.unsqueeze(1))
+            if rope_cs is None:
+                cu = cu_seqlens.long()
+                lens = cu[1:] - cu[:-1]
+                seq_ids = torch.repeat_interleave(torch.arange(lens.numel(), device=device), lens)
+                pos = torch.arange(total_len, device=device) - cu[:-1][seq_ids]
+                cos, sin = self.rope_cos[pos], self.rope_sin[pos]
+            else:
+                cos, sin = rope_cs
+            cos, sin = cos.to(q.dtype), sin.to(q.dtype)
+            q, k = apply_rotary_emb(q, k, cos.unsqueeze(1), sin.unsqueeze(1))
         self._last_P = None
         if self.training:
             out = self._packed_train_triton(q.contiguous(), k.contiguous(), v.contiguous(), x, cu_seqlens,

@@ -3,7 +3,7 @@
 Mirrors ``SwiGLUFFN`` and ``DSALTTransformerBlock`` of
 ``dsalt/modules/dsalt_transformer.py:10-85`` (RMSNorm -> DSALTAttention -> residual, RMSNorm
 -> SwiGLU FFN -> residual; optional activation checkpointing), with the attention layer's
-landmark variant exposed (``select_mode``, ``block_size``, ``stats_scope``).  Without
+landmark variant exposed (``select_mode``, ``block_size``, ``stats_scope``), and its ``qk_norm``.  Without
 autograd the FFN runs its gate and up projections as one GEMM over the concatenated
 weights and the gated activation as one HIP kernel over that buffer (same per-element
 arithmetic as silu(g) * u).
@@ -62,7 +62,7 @@ class DSALTTransformerBlock(nn.Module):
     def __init__(self, d_model: int, n_heads: int, n_min: int, n_max: int, k_lmk: int, max_seq_len: int, d_ff: int,
                  dropout: float = 0.0, yarn_scale: float = 1.0, layer_idx: int = 0, n_kv_heads: int | None = None,
                  qkv_bias: bool = False, rope_base: float = 10000.0, select_mode: str = "global",
-                 block_size: int = 512, stats_scope: str = "packed"):
+                 block_size: int = 512, stats_scope: str = "packed", qk_norm: bool = False):
         super().__init__()
         self.layer_idx = layer_idx
         self.attn_norm = RMSENorm(d_model)
@@ -71,7 +71,7 @@ class DSALTTransformerBlock(nn.Module):
                                    max_seq_len=max_seq_len, dropout=dropout, yarn_scale=yarn_scale,
                                    layer_idx=layer_idx, n_kv_heads=n_kv_heads, qkv_bias=qkv_bias,
                                    rope_base=rope_base, select_mode=select_mode, block_size=block_size,
-                                   stats_scope=stats_scope)
+                                   stats_scope=stats_scope, qk_norm=qk_norm)
         self.ffn = SwiGLUFFN(d_model=d_model, d_ff=d_ff, dropout=dropout)
 
     def forward(self, x, cu_seqlens=None, max_seqlen=None, gradient_checkpointing: bool = False, rope_cs=None,

@@ -16,10 +16,10 @@ from torch.autograd import forward_ad
 from . import _lib
 from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, SELECT_BLOCK, SELECT_GLOBAL, STATS_PACKED,
                    STATS_SEQUENCE, VARIANT_DEFAULT, VARIANT_DQ_BN64, VARIANT_FWD_BN32, VARIANT_FWD_RG2,
-                   VARIANT_LMK_SHORT, BwdArgs, Cache, CacheAttnArgs, CacheReadArgs, CacheRowsArgs, CacheWriteArgs, CeArgs, FwdArgs,
-                   GatherArgs, Problem, ProbsArgs, RopeArgs, SampleArgs, SelectArgs, SelectorsArgs, SiluMulArgs, SortArgs,
-                   TrainBwdArgs,
-                   TrainFwdArgs)
+                   VARIANT_LMK_SHORT, BwdArgs, Cache, Cache4AttnArgs, Cache4ReadArgs, Cache4WriteArgs, CacheAttnArgs,
+                   CacheReadArgs, CacheRowsArgs, CacheWriteArgs, CeArgs, FwdArgs, GatherArgs, Problem, ProbsArgs, QkNormRopeArgs,
+                   QkNormRopeBwdArgs, RopeArgs, SampleArgs, SelectArgs, SelectorsArgs, SiluMulArgs, SortArgs, TrainBwdArgs,
+                   TrainFwdArgs, VerifyArgs)
 
 _DT = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
 MAX_LANDMARKS = 2048  # landmarks per set (the training variant: at most 512)
@@ -521,6 +521,113 @@ def rope_qk_(q, k, cu_seqlens, cos, sin, *, max_seqlen=None):
     return q, k
 
 
+def _vec16(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
+    """``t`` [n] contiguous and on a 16-byte boundary."""
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} must be [{n}], got shape {tuple(t.shape)}")
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _qk_args(q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, max_seqlen, eps, more=()):
+    """(device index, arguments without the outputs, tensors to keep alive, checked q and k) of qk_norm_rope."""
+    if q is None and k is None:
+        raise ValueError("q or k is required")
+    at = _on(*(t for t in (q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, *more) if t is not None))
+    ref = q if q is not None else k
+    rows = []
+    for t, w, n in ((q, q_weight, "q"), (k, k_weight, "k")):
+        if t is None:
+            rows.append((None, (None, 0, 0), None))
+            continue
+        t, where = _rows16(t, n)
+        if t.shape[0] != ref.shape[0] or t.shape[2] != ref.shape[2] or t.dtype != ref.dtype:
+            raise ValueError(f"q and k must share T, D and dtype, got {tuple(q.shape)} {q.dtype}, {tuple(k.shape)} {k.dtype}")
+        if w is None:
+            raise ValueError(f"{n}_weight is required")
+        rows.append((t, where, _vec16(w.detach(), ref.shape[2], n + "_weight")))
+    T, _, D = ref.shape
+    if q is not None and k is not None and q_weight.dtype != k_weight.dtype:
+        raise TypeError(f"q_weight and k_weight must share a dtype, got {q_weight.dtype}, {k_weight.dtype}")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != D:
+        raise ValueError(f"cos and sin must be float32 [max_pos, {D}], got {tuple(cos.shape)}, {tuple(sin.shape)}")
+    cos, sin = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (cos, sin))
+    if (cu_seqlens is None) == (pos is None):
+        raise ValueError("either cu_seqlens or pos is required")
+    S = 0
+    if cu_seqlens is not None:
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+            raise ValueError("cu_seqlens must be [S+1] with S >= 1")
+        S = cu_seqlens.shape[0] - 1
+        maxlen = max_seqlen if max_seqlen is not None else _max_seqlen(cu_seqlens)
+        if maxlen > cos.shape[0] and T:
+            raise ValueError(f"a sequence of {maxlen} rows passes the {cos.shape[0]} positions of cos and sin")
+        cu_seqlens = _i32(cu_seqlens)
+    else:
+        pos = _vec_i32(_positions(pos), T, "pos")
+    (q, q_at, qw), (k, k_at, kw) = rows
+    a = QkNormRopeArgs(T, S, q.shape[1] if q is not None else 0, k.shape[1] if k is not None else 0, D, dtype_code(ref.dtype),
+                       dtype_code((qw if q is not None else kw).dtype), cos.shape[0], float(eps), *q_at, *k_at, None, 0, 0, None, 0, 0, qw.data_ptr() if qw is not None else None,
+                       kw.data_ptr() if kw is not None else None, cu_seqlens.data_ptr() if cu_seqlens is not None else None,
+                       pos.data_ptr() if pos is not None else None, cos.data_ptr(), sin.data_ptr())
+    return at, a, q, k, (qw, kw, cu_seqlens, pos, cos, sin)
+
+
+def _positions(pos: torch.Tensor) -> torch.Tensor:
+    """``pos`` with 64-bit positions held to what int32 names (past every table, where they would turn into others)."""
+    return pos.clamp(-1, 0x7fffffff) if pos.dtype == torch.int64 else pos
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, cu_seqlens=None, pos=None, max_seqlen=None, eps=1e-6, inplace=False):
+    """(q, k) with a root-mean-square norm of each head, x / sqrt(mean(x^2) + eps) * weight, and the rotation of
+    rope_qk_ after it, in one pass and in float32, rounded once.  q [T, Hq, D], k [T, Hk, D] (either may be None, strided
+    views are read in place), weights [D], cos/sin [max_pos, D] fp32.  A row's position is its place in its sequence of
+    ``cu_seqlens``, or ``pos[t]`` (CacheRows.pos of a decoding step).  Rows in no sequence, or with a position
+    outside the tables (inert rows), become zeros; with ``inplace``, which writes over q and k, they stay as they are."""
+    at, a, q_in, k_in, keep = _qk_args(q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, max_seqlen, eps)  # noqa: F841 (kept alive)
+    out = []
+    for n, t, given in (("q", q_in, q), ("k", k_in, k)):
+        if t is None:
+            out.append(None)
+            continue
+        if inplace and t is not given:
+            raise ValueError(f"{n} must have unit stride along D and rows on 16-byte boundaries to be written in place")
+        y = given if inplace else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        setattr(a, n + "_out", y.data_ptr())
+        st = (getattr(a, n + "_stride_t"), getattr(a, n + "_stride_h")) if inplace else (t.shape[1] * t.shape[2], t.shape[2])
+        setattr(a, n + "o_stride_t", st[0])
+        setattr(a, n + "o_stride_h", st[1])
+        out.append(y)
+    _call("dsalt_qk_norm_rope", a, at)
+    return tuple(out)
+
+
+def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, *, cu_seqlens=None, pos=None, max_seqlen=None, eps=1e-6):
+    """Gradients (dq, dk, dq_weight, dk_weight) of qk_norm_rope from those of its outputs: the first two in the type of q and
+    k (zeros in rows without a position), the weights' in float32, summed over rows and heads in an order that does not
+    change from run to run."""
+    at, a, q, k, keep = _qk_args(q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, max_seqlen, eps, (dq, dk))  # noqa: F841 (kept alive)
+    b = QkNormRopeBwdArgs(a)
+    out, up = [], []
+    for n, t, d in (("q", q, dq), ("k", k, dk)):
+        if t is None:
+            out += [None, None]
+            continue
+        if d is None or d.shape != t.shape:
+            raise ValueError(f"d{n} must have the shape of {n}, {tuple(t.shape)}")
+        d, where = _rows16(d.to(t.dtype), "d" + n)
+        up.append(d)
+        for f, x in zip(("d" + n, f"d{n}_stride_t", f"d{n}_stride_h"), where):
+            setattr(b, f, x)
+        y, w = torch.empty(t.shape, dtype=t.dtype, device=t.device), torch.empty(t.shape[2], dtype=torch.float32, device=t.device)
+        for f, x in ((n + "_out", y.data_ptr()), (n + "o_stride_t", t.shape[1] * t.shape[2]), (n + "o_stride_h", t.shape[2])):
+            setattr(b.base, f, x)
+        setattr(b, f"d{n}_weight", w.data_ptr())
+        out += [y, w]
+    ws = _set_workspace(b, _lib.load().dsalt_qk_norm_rope_bwd_workspace_bytes(ctypes.byref(b)), at)  # noqa: F841 (kept alive)
+    _call("dsalt_qk_norm_rope_bwd", b, at)
+    return out[0], out[2], out[1], out[3]
+
+
 def export_probs(q, k, w, cu_seqlens, lmk_idx, lse, lmk_bias=None, *, seq=0, rows=None, w_cap=None, scale=None,
                  max_seqlen=None, select_mode=SELECT_GLOBAL, block_size=512, want_lmk=True, seq_len=None):
     """(p_win [H, rows, w_cap], p_lmk [H, rows, K] or None), fp32: the probabilities the
@@ -733,7 +840,7 @@ def sort_landmarks(idx: torch.Tensor, bias: torch.Tensor | None = None):
     return out, b, perm
 
 
-# ------------------------------------------------------------------ decoding over an 8-bit cache
+# ------------------------------------------------------------------ decoding over a paged cache
 BLOCK_TOKENS = (16, 32, 64, 128)  # tokens a page of the cache may hold
 MAX_VOCAB = 1 << 20               # columns of sample_rows
 
@@ -745,6 +852,14 @@ class Cache8(NamedTuple):
     v: torch.Tensor
     k_scale: torch.Tensor
     v_scale: torch.Tensor
+
+
+class Cache4(NamedTuple):
+    """Pages of a 4-bit key/value cache: kv [n_blocks, n_kv, block_tokens, 2, D/2] uint8 (two e2m1 codes a byte, the first
+    element in the lower half; a token's key, then its value) and scale [n_blocks, n_kv, block_tokens, 2, D/32] uint8, an
+    exponent for each 32 elements; an element is code * 2^(scale - 127), scale 255 stands for NaN."""
+    kv: torch.Tensor
+    scale: torch.Tensor
 
 
 class CacheRows(NamedTuple):
@@ -761,12 +876,18 @@ class CacheRows(NamedTuple):
     pieces: torch.Tensor
 
 
-def new_cache(n_blocks: int, n_kv_heads: int, head_dim: int, *, block_tokens: int = 64, device="cuda") -> Cache8:
-    """An empty cache of one layer (head_dim 64 or 128; other head_dims pad their heads with zeros, and give
-    cache_attention the ``scale`` of their own size)."""
+def new_cache(n_blocks: int, n_kv_heads: int, head_dim: int, *, block_tokens: int = 64, device="cuda", bits: int = 8):
+    """An empty cache of one layer, a Cache8 or (``bits=4``) a Cache4 (head_dim 64 or 128; other head_dims pad their heads
+    with zeros, and give cache_attention the ``scale`` of their own size).  Eight bits, e4m3 with a scale a page and head,
+    round to 2^-4 of an element; four, e2m1 with a scale for 32 elements of a token, to a quarter of it and up to 1/7 of
+    the largest of the 32, in 0.53 of the memory."""
     if block_tokens not in BLOCK_TOKENS or head_dim not in (64, 128):
         raise ValueError(f"block_tokens must be one of {BLOCK_TOKENS} and head_dim 64 or 128, got {block_tokens}, {head_dim}")
+    if bits not in (4, 8):
+        raise ValueError(f"bits must be 4 or 8, got {bits}")
     shape = (n_blocks, n_kv_heads, block_tokens, head_dim)
+    if bits == 4:
+        return Cache4(*(torch.zeros((*shape[:3], 2, head_dim // n), dtype=torch.uint8, device=device) for n in (2, 32)))
     codes = [torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
     return Cache8(*codes, *(torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)))
 
@@ -785,7 +906,15 @@ def _on(*ts) -> int:
     return at
 
 
-def _cache_args(c: Cache8) -> Cache:
+def _cache_args(c):
+    if isinstance(c, Cache4):
+        kv, sc = c
+        if kv.dim() != 5 or kv.shape[3] != 2 or kv.dtype != torch.uint8 or not kv.is_contiguous():
+            raise ValueError("the cache's kv must be contiguous uint8 [n_blocks, n_kv, block_tokens, 2, D/2]")
+        D = 2 * kv.shape[4]
+        if sc.shape != (*kv.shape[:4], D // 32) or sc.dtype != torch.uint8 or not sc.is_contiguous():
+            raise ValueError("the cache's scale must be contiguous uint8 [n_blocks, n_kv, block_tokens, 2, D/32]")
+        return _lib.Cache4(*kv.shape[:3], D, kv.data_ptr(), sc.data_ptr())
     k, v, ks, vs = c
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or k.dtype != _E4M3 or v.dtype != _E4M3 or not k.is_contiguous() \
@@ -835,19 +964,19 @@ def _windows(w: torch.Tensor) -> torch.Tensor:
     return w.clamp(-1, 0x7fffffff) if w.dtype == torch.int64 else w
 
 
-def _call(name: str, args, at: int):
+def _call(name: str, args, at: int, *more):
     """One library call on the current stream of device ``at`` (made current for it where it is not)."""
     fn = getattr(_lib.load(), name)
     if _device_now() != at:
         with torch.cuda.device(at):
-            rc = fn(ctypes.byref(args), _stream(torch.device("cuda", at)))
+            rc = fn(ctypes.byref(args), *more, _stream(torch.device("cuda", at)))
     else:
-        rc = fn(ctypes.byref(args), _raw_stream(at) if _raw_stream is not None else _stream(torch.device("cuda", at)))
+        rc = fn(ctypes.byref(args), *more, _raw_stream(at) if _raw_stream is not None else _stream(torch.device("cuda", at)))
     if rc:
         _lib.check(name, rc)
 
 
-def cache_rows_(seq_len, new_len, table, free_blocks, span, n_rows: int, *, block_tokens: int = 64) -> CacheRows:
+def cache_rows_(seq_len, new_len, table, free_blocks, span, n_rows: int, *, block_tokens: int = 64, held=None) -> CacheRows:
     """Row maps of one step over R requests, on the device alone (no synchronisation): request r holds
     ``seq_len[r]`` tokens and brings ``new_len[r]`` (negative: it ends).  ``table`` [R, pages] int32 receives
     the new pages, taken from the ring ``free_blocks`` (int32) at ``span`` [2] int64 (pages ever taken from
@@ -855,8 +984,10 @@ def cache_rows_(seq_len, new_len, table, free_blocks, span, n_rows: int, *, bloc
     batch (host value); rows past the requests' last are inert.  Requests are served in order, one whose pages
     are not there, or whose tokens fit neither the table nor the rows, is refused: it keeps its length and its
     rows are inert (position and slot -1).  ``seq_len`` and ``span`` stay as they are: the step's come back in
-    the CacheRows."""
-    at = _on(table, seq_len, new_len, free_blocks, span)
+    the CacheRows.  ``held`` [R] (optional): request r has pages for max(seq_len[r], held[r]) tokens, as one whose last
+    tokens were taken back has (refused drafts); it keeps them for its next tokens, and gives back all of them when it
+    ends.  After a step it is the larger of held and CacheRows.seq_len, 0 for a request that ended."""
+    at = _on(table, seq_len, new_len, free_blocks, span, held)
     R, M, st = _table_args(table)
     if free_blocks.dim() != 1 or free_blocks.dtype != torch.int32 or not free_blocks.is_contiguous():
         raise ValueError("free_blocks must be contiguous int32 [entries]")
@@ -865,6 +996,7 @@ def cache_rows_(seq_len, new_len, table, free_blocks, span, n_rows: int, *, bloc
     if not 0 <= n_rows <= 1 << 30 or block_tokens not in BLOCK_TOKENS:
         raise ValueError(f"n_rows must be in [0, 2^30] and block_tokens one of {BLOCK_TOKENS}, got {n_rows}, {block_tokens}")
     old, new = _vec_i32(seq_len, R, "seq_len"), _vec_i32(new_len, R, "new_len")
+    kept = _vec_i32(held, R, "held") if held is not None else None
     n_pieces = min(n_rows, n_rows // block_tokens + 2 * R)
     # the outputs lie side by side in two buffers
     pieces, seq, granted, cu, req, pos = torch.empty(4 * n_pieces + 3 * R + 1 + 2 * n_rows, dtype=torch.int32, device=at).split(
@@ -874,15 +1006,20 @@ def cache_rows_(seq_len, new_len, table, free_blocks, span, n_rows: int, *, bloc
                       table.data_ptr(), st, free_blocks.data_ptr(), span.data_ptr(), seq.data_ptr(), span_out.data_ptr(),
                       granted.data_ptr(), cu.data_ptr(), req.data_ptr(), pos.data_ptr(), slot.data_ptr(), pieces.data_ptr())
     ws = _set_workspace(a, _lib.load().dsalt_cache_rows_workspace_bytes(ctypes.byref(a)), at)  # noqa: F841 (kept alive)
-    _call("dsalt_cache_rows", a, at)
+    if kept is None:
+        _call("dsalt_cache_rows", a, at)
+    else:
+        _call("dsalt_cache_rows_held", a, at, kept.data_ptr())
     return CacheRows(seq, span_out, granted, cu, req, pos, slot, pieces.view(n_pieces, 4))
 
 
-def cache_write_(k, v, cache: Cache8, pieces) -> Cache8:
+def cache_write_(k, v, cache, pieces):
     """Writes the step's keys and values k, v [T, n_kv, D] into the cache, the rows of ``pieces`` [P, 4] int32
     (CacheRows.pieces: first row, rows, page, first token in the page; each page in one piece at most).  A page's
     scale is the least power of two that keeps its finite elements within 448 of it; codes it held follow a
-    larger one.  Values that are not finite are held as NaN."""
+    larger one.  Values that are not finite are held as NaN.  Of a Cache4 each 32 elements of a token's head have their
+    own scale, the least power of two that keeps them within 7 of it (those past 6 become 6), nothing held before
+    changes, and 32 elements of which one is not finite are held as NaN."""
     at = _on(k, v, *cache, pieces)
     (k, k_at), (v, v_at) = _rows16(k, "k"), _rows16(v, "v")
     c = _cache_args(cache)
@@ -890,12 +1027,13 @@ def cache_write_(k, v, cache: Cache8, pieces) -> Cache8:
         raise ValueError(f"k and v must be [T, {c.n_kv_heads}, {c.head_dim}] of one dtype, got {tuple(k.shape)}, {tuple(v.shape)}")
     if pieces.dim() != 2 or pieces.shape[1] != 4 or pieces.dtype != torch.int32 or not pieces.is_contiguous():
         raise ValueError("pieces must be contiguous int32 [P, 4]")
-    a = CacheWriteArgs(c, k.shape[0], pieces.shape[0], dtype_code(k.dtype), *k_at, *v_at, pieces.data_ptr())
-    _call("dsalt_cache_write", a, at)
+    kind, call = (Cache4WriteArgs, "dsalt_cache4_write") if isinstance(cache, Cache4) else (CacheWriteArgs, "dsalt_cache_write")
+    a = kind(c, k.shape[0], pieces.shape[0], dtype_code(k.dtype), *k_at, *v_at, pieces.data_ptr())
+    _call(call, a, at)
     return cache
 
 
-def cache_read(cache: Cache8, table, cu_seqlens, *, start=None, n_rows: int, dtype=torch.bfloat16):
+def cache_read(cache, table, cu_seqlens, *, start=None, n_rows: int, dtype=torch.bfloat16):
     """(k, v) [n_rows, n_kv, D]: tokens of the cache as a packed batch.  Row t is token ``start[r]`` (default 0)
     + t - cu_seqlens[r] of the request r whose rows hold it; zeros past the last row and where the table names
     no page."""
@@ -908,20 +1046,23 @@ def cache_read(cache: Cache8, table, cu_seqlens, *, start=None, n_rows: int, dty
         raise ValueError(f"n_rows must be in [0, 2^31), got {n_rows}")
     k = torch.empty(n_rows, c.n_kv_heads, c.head_dim, dtype=dtype, device=at)
     v = torch.empty_like(k)
-    a = CacheReadArgs(c, R, M, n_rows, dtype_code(dtype), table.data_ptr(), ts, cu.data_ptr(),
-                      st.data_ptr() if st is not None else None, k.data_ptr(), v.data_ptr())
-    _call("dsalt_cache_read", a, at)
+    kind, call = (Cache4ReadArgs, "dsalt_cache4_read") if isinstance(cache, Cache4) else (CacheReadArgs, "dsalt_cache_read")
+    a = kind(c, R, M, n_rows, dtype_code(dtype), table.data_ptr(), ts, cu.data_ptr(),
+             st.data_ptr() if st is not None else None, k.data_ptr(), v.data_ptr())
+    _call(call, a, at)
     return k, v
 
 
-def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None, *, scale=None, w_max=None):
+def cache_attention(q, cache, table, req, pos, w, lmk_idx, lmk_bias=None, *, scale=None, w_max=None, rows_per_req=1):
     """(out [T, H, D] in q.dtype, lse [T, H] fp32): the operator's attention of query tokens over the cache, the
     form for single tokens of many requests.  Row t is the token at position ``pos[t]`` of request ``req[t]``
     (CacheRows.req, .pos), its own key and value written; it attends its window [pos - w + 1, pos] and the
     landmarks before the window of its head's set in lmk_idx [H, R, 1, K] (any order, negative slots empty, a
     position may repeat; select_landmarks' sets; a bias of -inf masks its landmark).  Rows without a key (inert rows, pages that the table does not
     name) give zeros and -inf.  ``scale``: by default 1 / sqrt(D).  ``w_max``: no window is longer (host value;
-    splits the work, longer windows only cost time).  Not differentiable."""
+    splits the work, longer windows only cost time).  ``rows_per_req``: rows 0, n, 2 n ... begin runs of rows most of which
+    belong to one request, as drafted tokens do (host value; over a Cache4 such rows share what they read of it, any
+    rows give the same result).  Not differentiable."""
     at = _on(q, *cache, table, req, pos, w, lmk_idx, lmk_bias)
     q, q_at = _rows16(q, "q")
     c = _cache_args(cache)
@@ -929,6 +1070,8 @@ def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None
     R, M, ts = _table_args(table)
     if D != c.head_dim or c.n_kv_heads < 1 or H % c.n_kv_heads:
         raise ValueError(f"q must be [T, H, {c.head_dim}] with H a multiple of {c.n_kv_heads}, got {tuple(q.shape)}")
+    if rows_per_req < 1:
+        raise ValueError(f"rows_per_req must be positive, got {rows_per_req}")
     if lmk_idx.dim() != 4 or lmk_idx.shape[:3] != (H, R, 1):
         raise ValueError(f"lmk_idx must be [H, R, 1, K] = [{H}, {R}, 1, K], got {tuple(lmk_idx.shape)}")
     if lmk_bias is not None and lmk_bias.shape != lmk_idx.shape:
@@ -940,12 +1083,18 @@ def cache_attention(q, cache: Cache8, table, req, pos, w, lmk_idx, lmk_bias=None
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     out = torch.empty(T, H, D, dtype=q.dtype, device=at)
     lse = torch.empty(T, H, dtype=torch.float32, device=at)
-    a = CacheAttnArgs(c, T, H, R, M, K, dtype_code(q.dtype), 0 if w_max is None else max(-1, min(int(w_max), 1 << 30)), table.data_ptr(),
-                      ts, *q_at, rq.data_ptr(), ps.data_ptr(), wc.data_ptr(),
-                      li.data_ptr() if K else None, lb.data_ptr() if lb is not None and K else None,
-                      out.data_ptr(), H * D, D, lse.data_ptr(), scale)
-    ws = _set_workspace(a, _lib.load().dsalt_cache_attn_workspace_bytes(ctypes.byref(a)), at)  # noqa: F841 (kept alive)
-    _call("dsalt_cache_attn", a, at)
+    shape = (c, T, H, R, M, K, dtype_code(q.dtype), 0 if w_max is None else max(-1, min(int(w_max), 1 << 30)))
+    rest = (table.data_ptr(), ts, *q_at, rq.data_ptr(), ps.data_ptr(), wc.data_ptr(),
+            li.data_ptr() if K else None, lb.data_ptr() if lb is not None and K else None,
+            out.data_ptr(), H * D, D, lse.data_ptr(), scale)
+    if isinstance(cache, Cache4):
+        a = Cache4AttnArgs(*shape, min(int(rows_per_req), 0x7fffffff), *rest)
+        need, call = _lib.load().dsalt_cache4_attn_workspace_bytes(ctypes.byref(a)), "dsalt_cache4_attn"
+    else:
+        a = CacheAttnArgs(*shape, *rest)
+        need, call = _lib.load().dsalt_cache_attn_workspace_bytes(ctypes.byref(a)), "dsalt_cache_attn"
+    ws = _set_workspace(a, need, at)  # noqa: F841 (kept alive)
+    _call(call, a, at)
     return out, lse
 
 
@@ -990,3 +1139,58 @@ def sample_rows(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
                    0 if k is not None else max(-1, min(int(top_k), MAX_VOCAB)), token.data_ptr(), logp.data_ptr())
     _call("dsalt_sample_rows", a, at)
     return token, logp
+
+
+class Verified(NamedTuple):
+    """Drafts of a step verified (verify_rows): accepted [R] int32, the drafts taken of each request, and tokens [T] int64:
+    of a request's rows the taken drafts, the token that follows them, then -1."""
+    accepted: torch.Tensor
+    tokens: torch.Tensor
+
+
+def verify_rows(logits, tokens, cu, u, v, *, draft_logits=None, temperature=1.0, draft_temperature=None) -> Verified:
+    """Drafted tokens taken or refused against the target's probabilities, and the token that follows, from given random
+    numbers.  Request r has rows cu[r] .. cu[r + 1] (CacheRows.cu): ``tokens`` [T] int64 are what the step was run on, the
+    request's last token and its drafts, ``logits`` [T, V] the target's after each of them, so that row t's draft is tokens[t + 1]
+    and the last row has none.  ``draft_logits`` [T, V] are those it was drawn from (a request's last row is not
+    read; the type of ``logits``), None: drafts certain of themselves, as looked-up ones.  Probabilities are those of sample_rows
+    without filters, at ``temperature`` (number or [R]; <= 0: the largest logit) and, for the drafts, at
+    ``draft_temperature`` (None: the same); filters are applied by setting logits to -inf.  Draft x of row t is taken
+    while u[t] q(x) < p(x), with ``u`` [T] and ``v`` [R] in [0, 1) (float32 or float64); then comes a token drawn with v[r],
+    from max(p - q, 0) of the row that refused, or from p behind the last draft.  The tokens drawn are distributed as if
+    each came from the target."""
+    per_req = [t if isinstance(t, torch.Tensor) else None for t in (temperature, draft_temperature)]
+    at = _on(logits, tokens, cu, u, v, draft_logits, *per_req)
+    if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_VOCAB or logits.shape[0] > 1 << 22:
+        raise ValueError(f"logits must be [T, V] with T at most 2^22 and V in [1, {MAX_VOCAB}], got {tuple(logits.shape)}")
+    T, V = logits.shape
+    if draft_logits is not None and (draft_logits.shape != logits.shape or draft_logits.dtype != logits.dtype):
+        raise ValueError(f"draft_logits must have the shape and type of logits, {tuple(logits.shape)} {logits.dtype}")
+    if V > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    if draft_logits is not None and V > 1 and draft_logits.stride(1) != 1:
+        draft_logits = draft_logits.contiguous()
+    if cu.dim() != 1 or not 1 <= cu.shape[0] <= (1 << 22) + 1:
+        raise ValueError("cu must be [R+1] with R at most 2^22")
+    R = cu.shape[0] - 1
+    for t, n, name in ((tokens, T, "tokens"), (u, T, "u"), (v, R, "v"), (per_req[0], R, "temperature"), (per_req[1], R, "draft_temperature")):
+        if t is not None and (t.dim() != 1 or t.shape[0] != n):
+            raise ValueError(f"{name} must be [{n}], got shape {tuple(t.shape)}")
+    if tokens.is_floating_point():
+        raise TypeError(f"tokens must be integers, got {tokens.dtype}")
+    if u.dtype not in (torch.float32, torch.float64) or v.dtype != u.dtype:
+        raise TypeError(f"u and v must both be float32 or both float64, got {u.dtype}, {v.dtype}")
+    if draft_temperature is None:
+        draft_temperature, per_req[1] = temperature, per_req[0]
+    tokens, u, v, cu = tokens.to(torch.int64).contiguous(), u.contiguous(), v.contiguous(), _i32(cu)
+    t, dt = (x if x is None else _f32(x) for x in per_req)
+    accepted = torch.empty(R, dtype=torch.int32, device=at)
+    out = torch.empty(T, dtype=torch.int64, device=at)
+    a = VerifyArgs(R, T, V, dtype_code(logits.dtype), u.element_size(), logits.data_ptr(), logits.stride(0),
+                   draft_logits.data_ptr() if draft_logits is not None else None, draft_logits.stride(0) if draft_logits is not None else 0,
+                   tokens.data_ptr(), cu.data_ptr(), u.data_ptr(), v.data_ptr(), *(x.data_ptr() if x is not None else None for x in (t, dt)),
+                   *(0.0 if isinstance(x, torch.Tensor) else float(x) for x in (temperature, draft_temperature)),
+                   accepted.data_ptr(), out.data_ptr())
+    ws = _set_workspace(a, _lib.load().dsalt_verify_workspace_bytes(ctypes.byref(a)), at)  # noqa: F841 (kept alive)
+    _call("dsalt_verify_rows", a, at)
+    return Verified(accepted, out)

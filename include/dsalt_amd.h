@@ -235,6 +235,50 @@ typedef struct dsalt_rope_args {
 
 int    dsalt_rope_qk(const dsalt_rope_args* a, dsalt_stream_t stream);
 
+/* A root-mean-square norm of every query and key head and the rotation after it, in one pass (no counterpart in the
+ * reference): with r = 1 / sqrt(mean(x^2) + eps) and n = x r weight, halves n1 and n2,
+ *   n1[j] cos[p][j] - n2[j] sin[p][j],  n2[j] cos[p][D/2 + j] + n1[j] sin[p][D/2 + j]
+ * in float32, rounded once.  The position p of row t is pos[t], or its place in its sequence of cu_seqlens; rows whose
+ * position lies outside [0, max_pos), and those in no sequence, become zeros, or stay as they are where the outputs are the
+ * inputs (the same pointer and strides).  Needs no workspace. */
+typedef struct dsalt_qk_norm_rope_args {
+    int32_t total_len;         /* T                                                  */
+    int32_t num_seqs;          /* S (with cu_seqlens)                                */
+    int32_t n_q_heads;         /* heads of q (0: none)                               */
+    int32_t n_k_heads;         /* heads of k (0: none)                               */
+    int32_t head_dim;          /* multiple of 16, <= 256                             */
+    int32_t dtype;             /* DSALT_DTYPE_*                                      */
+    int32_t weight_dtype;      /* of the weights                                     */
+    int32_t max_pos;
+    float eps;
+    const void* q; int64_t q_stride_t; int64_t q_stride_h;
+    const void* k; int64_t k_stride_t; int64_t k_stride_h;
+    void* q_out; int64_t qo_stride_t; int64_t qo_stride_h;
+    void* k_out; int64_t ko_stride_t; int64_t ko_stride_h;
+    const void* q_weight;      /* [head_dim], 16-byte aligned                        */
+    const void* k_weight;      /* [head_dim], 16-byte aligned                        */
+    const int32_t* cu_seqlens; /* [S + 1], or NULL: pos                               */
+    const int32_t* pos;        /* [T], or NULL: cu_seqlens                            */
+    const float* cos;          /* [max_pos, head_dim], 16-byte aligned               */
+    const float* sin;          /* [max_pos, head_dim], 16-byte aligned               */
+} dsalt_qk_norm_rope_args;
+
+int    dsalt_qk_norm_rope(const dsalt_qk_norm_rope_args* a, dsalt_stream_t stream);
+
+/* Its gradients: base.q_out and base.k_out receive those of q and k (zeros in rows without a position; never the inputs'
+ * memory), dq_weight and dk_weight those of the weights, summed over rows and heads in a fixed order. */
+typedef struct dsalt_qk_norm_rope_bwd_args {
+    dsalt_qk_norm_rope_args base;
+    const void* dq; int64_t dq_stride_t; int64_t dq_stride_h;   /* gradient of the outputs */
+    const void* dk; int64_t dk_stride_t; int64_t dk_stride_h;
+    float* dq_weight;          /* [head_dim] (with n_q_heads)                        */
+    float* dk_weight;          /* [head_dim] (with n_k_heads)                        */
+    void* workspace; size_t workspace_bytes;
+} dsalt_qk_norm_rope_bwd_args;
+
+size_t dsalt_qk_norm_rope_bwd_workspace_bytes(const dsalt_qk_norm_rope_bwd_args* a);
+int    dsalt_qk_norm_rope_bwd(const dsalt_qk_norm_rope_bwd_args* a, dsalt_stream_t stream);
+
 /* Attention probabilities of one sequence over the keys each row attends, in banded
  * form (O(L (w + k)) memory).  Replaces the dense [H, L, L] rebuild of _last_P for the
  * analysis metrics, dsalt/modules/dsalt_attention.py:636-702 (consumer
@@ -412,6 +456,10 @@ typedef struct dsalt_cache_rows_args {
 
 size_t dsalt_cache_rows_workspace_bytes(const dsalt_cache_rows_args* a);
 int    dsalt_cache_rows(const dsalt_cache_rows_args* a, dsalt_stream_t stream);
+/* dsalt_cache_rows of requests that hold pages for max(seq_len[r], held[r]) tokens (held [n_reqs], or NULL): a
+ * request whose last tokens were taken back, as refused drafts are, keeps the pages it has for them, takes none
+ * twice and gives back all of them when it ends. */
+int    dsalt_cache_rows_held(const dsalt_cache_rows_args* a, const int32_t* held, dsalt_stream_t stream);
 
 /* Writes the rows of `pieces` (each within one page) into the cache: k and v [n_rows, n_kv_heads,
  * head_dim] in dtype.  A piece that does not lie within the rows and one page is skipped; no page
@@ -476,6 +524,110 @@ typedef struct dsalt_cache_attn_args {
 
 size_t dsalt_cache_attn_workspace_bytes(const dsalt_cache_attn_args* a);
 int    dsalt_cache_attn(const dsalt_cache_attn_args* a, dsalt_stream_t stream);
+
+/* The same cache in 4 bits.  A token of a head is its own: kv [n_blocks, n_kv_heads, block_tokens, 2, head_dim / 2]
+ * holds e2m1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6; bit 3 the sign), two a byte, the first in the lower half, the key's
+ * before the value's; scale [n_blocks, n_kv_heads, block_tokens, 2, head_dim / 32] the exponent above -127 of a power of
+ * two for each 32 elements.  An element is code * 2^(scale - 127); scale 255 stands for NaN.  The scale written is the
+ * least power of two s in [2^-126, 2^125] with all 32 magnitudes within 7 s; elements are rounded to the nearest code, ties
+ * to the even one, past 6 s to 6 s.  32 elements of which one is not finite are held as NaN. */
+typedef struct dsalt_cache4 {
+    int32_t n_blocks;
+    int32_t n_kv_heads;
+    int32_t block_tokens;      /* 16, 32, 64 or 128                                  */
+    int32_t head_dim;          /* 64 or 128                                          */
+    void* kv; void* scale;     /* bytes, 16-byte aligned                             */
+} dsalt_cache4;
+
+/* dsalt_cache_write into it (a page may appear in several pieces that share no token).  Needs no workspace. */
+typedef struct dsalt_cache4_write_args {
+    dsalt_cache4 c;
+    int32_t n_rows;
+    int32_t n_pieces;
+    int32_t dtype;             /* DSALT_DTYPE_*                                      */
+    const void* k; int64_t k_stride_t; int64_t k_stride_h;
+    const void* v; int64_t v_stride_t; int64_t v_stride_h;
+    const int32_t* pieces;     /* [n_pieces, 4], 16-byte aligned                     */
+} dsalt_cache4_write_args;
+
+int    dsalt_cache4_write(const dsalt_cache4_write_args* a, dsalt_stream_t stream);
+
+/* dsalt_cache_read of it.  Needs no workspace. */
+typedef struct dsalt_cache4_read_args {
+    dsalt_cache4 c;
+    int32_t n_reqs;
+    int32_t table_cols;
+    int32_t n_rows;
+    int32_t dtype;
+    const int32_t* table; int64_t table_stride;
+    const int32_t* cu_seqlens; /* [n_reqs + 1]                                       */
+    const int32_t* start;      /* [n_reqs] or NULL (0)                               */
+    void* k; void* v;
+} dsalt_cache4_read_args;
+
+int    dsalt_cache4_read(const dsalt_cache4_read_args* a, dsalt_stream_t stream);
+
+/* dsalt_cache_attn over it.  rows_per_req: rows t = 0, rows_per_req, 2 rows_per_req ... begin runs of rows most of which
+ * belong to one request (drafted tokens and the one before them); rows of a run and request share what they read.  It sets
+ * how the work is split: any rows give the same result. */
+typedef struct dsalt_cache4_attn_args {
+    dsalt_cache4 c;
+    int32_t n_rows;            /* T                                                  */
+    int32_t n_heads;           /* H, a multiple of c.n_kv_heads                      */
+    int32_t n_reqs;
+    int32_t table_cols;
+    int32_t k_lmk;             /* landmark slots per set, 0..2048                    */
+    int32_t dtype;             /* of q and out                                       */
+    int32_t w_max;             /* no window is longer (0: not known)                 */
+    int32_t rows_per_req;      /* >= 1                                               */
+    const int32_t* table; int64_t table_stride;
+    const void* q;  int64_t q_stride_t; int64_t q_stride_h;   /* [T, H, D]           */
+    const int32_t* req;        /* [T]                                                */
+    const int32_t* pos;        /* [T]                                                */
+    const int32_t* w;          /* [T] (values < 1 act as 1)                          */
+    const int32_t* lmk_idx;    /* [H, n_reqs, 1, k_lmk]                              */
+    const float* lmk_bias;     /* like lmk_idx, added to the landmark logits, or NULL */
+    void* out; int64_t o_stride_t; int64_t o_stride_h;
+    float* lse;                /* [T, H]                                             */
+    float scale;
+    void* workspace; size_t workspace_bytes;
+} dsalt_cache4_attn_args;
+
+size_t dsalt_cache4_attn_workspace_bytes(const dsalt_cache4_attn_args* a);
+int    dsalt_cache4_attn(const dsalt_cache4_attn_args* a, dsalt_stream_t stream);
+
+/* Drafted tokens of each request taken or refused against the target's probabilities, and the token that follows, from
+ * given random numbers in [0, 1).  Request r has rows cu[r] .. cu[r + 1]: row t holds the target's logits for the token after
+ * tokens[t], of which tokens[t + 1] is the draft; the last row has none.  In a row with largest logit m (NaN as -inf) a
+ * token weighs a = round(2^42 exp((x - m) / temperature)) (temperature <= 0: 2^42 for the first largest, 0 for the others)
+ * and has the probability p = a / sum a; the draft's logits give q in the same way (NULL: 1 for the draft).  The draft is taken
+ * while u[t] q < p; the token behind the taken ones is the first index whose running sum of round(2^52 max(p - q, 0)), or
+ * of a in the last row and where the former are all 0, passes v[r] times their total.  accepted[r]: drafts taken; out: of a
+ * request's rows, the taken drafts, that token, then -1; -1 in rows of no request and for a token of a row without a
+ * logit above -inf.  A draft outside the vocabulary is refused, with nothing (or the draft's whole q) taken from p.
+ * Comparisons and shares are formed in float64. */
+typedef struct dsalt_verify_args {
+    int32_t n_reqs;            /* at most 2^22                                       */
+    int32_t n_rows;            /* T, at most 2^22                                    */
+    int32_t n_cols;            /* vocabulary, 1 .. 2^20                              */
+    int32_t dtype;             /* DSALT_DTYPE_* of both logits                       */
+    int32_t u_bytes;           /* 4 (float32) or 8 (float64)                         */
+    const void* logits; int64_t logits_stride;
+    const void* draft_logits; int64_t draft_stride;  /* rows as logits (a request's last is not read), or NULL */
+    const int64_t* tokens;     /* [T]                                                */
+    const int32_t* cu;         /* [n_reqs + 1]                                       */
+    const void* u;             /* [T]                                                */
+    const void* v;             /* [n_reqs]                                           */
+    /* a value a request, or NULL: the one of the same name for all */
+    const float* temperature; const float* draft_temperature;
+    float temperature_all; float draft_temperature_all;
+    int32_t* accepted;         /* out [n_reqs]                                       */
+    int64_t* out;              /* out [T]                                            */
+    void* workspace; size_t workspace_bytes;
+} dsalt_verify_args;
+
+size_t dsalt_verify_workspace_bytes(const dsalt_verify_args* a);
+int    dsalt_verify_rows(const dsalt_verify_args* a, dsalt_stream_t stream);
 
 /* One token a row of logits from given random numbers u in [0, 1) (clamped into it).  In the order of
  * the logits, largest first, equal ones by index, NaN as -inf, a token weighs
