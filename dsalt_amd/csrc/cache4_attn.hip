@@ -12,6 +12,7 @@
 #include "common.h"
 #include "decode_attn.h"
 #include "fp4.h"
+#include "tiles.h"
 #include "timing.h"
 
 namespace dsalt {
@@ -25,24 +26,27 @@ struct AttnPlan {
     int nh, tiles;      // heads of a block, blocks of a key/value head's query heads
     int nr, run_tiles;  // rows of a block, blocks of a request's rows
     int ns, nl;         // splits of a row's window, and of its landmark slots
-    int waves, chunks;  // of a block; parts of a head's landmark slots within a block
-    int cols() const { return nr * nh; }
+    int waves;          // of a block
+    int chunk_log;      // a head's landmark slots are 2^chunk_log parts within a block (-1: there are none)
+    int kc, kr_log;     // slots of a part, and of a part with what fills it up to a power of two
+    int col_mul;        // c / nh = c col_mul >> 16 for columns c
+    __host__ __device__ int chunks() const { return chunk_log < 0 ? 0 : 1 << chunk_log; }
 };
 
 template <typename T, int D>
 struct Step {  // one wave's running maximum, sum and weighted values of 16 columns
     static constexpr int QP = Parts<T>::q, PP = Parts<T>::p, KS = D / 32, JN = D / 16, DL = D / 4, KW = DL / 8;
     typedef uint32_t kword __attribute__((ext_vector_type(KW)));
-    struct Keys {  // lane (row16, kg): elements kg DL ... of keys 16 half + row16
-        kword code[2];
-        uint32_t scale[2];
+    struct Tokens {  // lane (row16, kg): elements kg DL ... of tokens 16 half + row16, and their scales
+        kword key[2], value[2];
+        uint32_t key_scale[2], value_scale[2];
     };
-    struct Values {  // elements JN row16 ... of keys 16 (e / 4) + 4 kg + e % 4
-        uint32_t code[8], scale[8];
-    };
+    // a wave's values of a step in LDS: bfloat16 rows of a token each
+    static constexpr int VROW = D + 16, STAGE = kStep * VROW * 2;
     bf16x8 qf[KS][QP];
     floatx4 acc[JN];
     float m, l;
+    uint32_t poison;  // blocks of 32 elements of column row16 that a value which is not finite has reached
 
     // the lane's query: column row16, elements kg DL + 8 s + e of step s
     __device__ __forceinline__ void begin(const T* q, int kg) {
@@ -56,25 +60,37 @@ struct Step {  // one wave's running maximum, sum and weighted values of 16 colu
         for (int j = 0; j < JN; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
         m = -INFINITY;
         l = 0.f;
+        poison = 0;
     }
-    __device__ __forceinline__ static void load_key(const Cache4Pages& c, uint64_t token, int kg, kword& code, uint32_t& scale) {
-        code = *(const kword*)(c.kv + token * D + kg * (DL / 2));
-        scale = c.scale[token * (D / 16) + kg * DL / 32];
+    // a token's share of the lane, from the token's first bytes
+    __device__ __forceinline__ static void load(const uint8_t* kv, const uint8_t* sc, int kg, int half, Tokens& t) {
+        t.key[half] = *(const kword*)(kv + kg * (DL / 2));
+        t.value[half] = *(const kword*)(kv + D / 2 + kg * (DL / 2));
+        t.key_scale[half] = sc[kg * DL / 32];
+        t.value_scale[half] = sc[D / 32 + kg * DL / 32];
     }
-    __device__ __forceinline__ static void load_value(const Cache4Pages& c, uint64_t token, int row16, uint32_t& code, uint32_t& scale) {
-        const uint8_t* x = c.kv + token * D + D / 2 + row16 * (JN / 2);
-        code = JN == 8 ? *(const uint32_t*)x : *(const uint16_t*)x;
-        scale = c.scale[token * (D / 16) + D / 32 + row16 * JN / 32];
+    // Values are held apart from those that are NaN: nan[half] has a bit for each lane's, which are staged as zeros.
+    __device__ __forceinline__ static bool stage_values(bf16* lds, int row16, int kg, Tokens& t, unsigned long long* nan) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            nan[half] = __ballot(t.value_scale[half] == 255u);
+            if (nan[half] != 0 && t.value_scale[half] == 255u) t.value_scale[half] = 127u, t.value[half] = kword{};
+            const float scale = e8m0(t.value_scale[half]);
+#pragma unroll
+            for (int i = 0; i < KW; ++i)
+                *(bf16x8*)(lds + (half * 16 + row16) * VROW + kg * DL + 8 * i) = e2m1_op(t.value[half][i], scale);
+        }
+        return (nan[0] | nan[1]) != 0;
     }
     // scores of keys 16 half + 4 kg + r for column row16
-    __device__ __forceinline__ void scores(const Keys& k, float* x) const {
+    __device__ __forceinline__ void scores(const Tokens& t, float* x) const {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             floatx4 sc = {0.f, 0.f, 0.f, 0.f};
-            const float scale = e8m0(k.scale[half]);
+            const float scale = e8m0(t.key_scale[half]);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                const bf16x8 kf = e2m1_op(k.code[half][s], scale);
+                const bf16x8 kf = e2m1_op(t.key[half][s], scale);
 #pragma unroll
                 for (int i = 0; i < QP; ++i) sc = mma(kf, qf[s][i], sc);
             }
@@ -82,33 +98,19 @@ struct Step {  // one wave's running maximum, sum and weighted values of 16 colu
             for (int r = 0; r < 4; ++r) x[4 * half + r] = sc[r];
         }
     }
-    // weighted values of the step's keys added to `to`
-    __device__ __forceinline__ static void product(const Values& v, const bf16x8* pf, floatx4* to) {
-        float scale[8];
+    // The step's scores in base 2 (-inf: masked) and its staged values.  Columns share the matrix operand of the values but not
+    // the keys they attend: a value held as NaN (`any`, seldom) is noted for the columns that attend it.
+    __device__ __forceinline__ void take(const bf16* lds, int lane, bool any, const unsigned long long* nan, float* x) {
+        if (any) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) scale[e] = e8m0(v.scale[e]);
+            for (int e = 0; e < 8; ++e) {
+                uint32_t blocks = 0;
 #pragma unroll
-        for (int j = 0; j < JN; j += 2) {
-            uint32_t c[8];  // elements j and j + 1 of a key
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                c[e] = j == 0 ? e2m1_bf16<0>(v.code[e], scale[e])
-                     : j == 2 ? e2m1_bf16<1>(v.code[e], scale[e])
-                     : j == 4 ? e2m1_bf16<2>(v.code[e], scale[e])
-                              : e2m1_bf16<3>(v.code[e], scale[e]);
-#pragma unroll
-            for (int hi = 0; hi < 2; ++hi) {
-                const bf16x8 vf = __builtin_bit_cast(bf16x8, u32x4{half_pair(c[0], c[1], hi), half_pair(c[2], c[3], hi),
-                                                                   half_pair(c[4], c[5], hi), half_pair(c[6], c[7], hi)});
-#pragma unroll
-                for (int i = 0; i < PP; ++i) to[j + hi] = mma(vf, pf[i], to[j + hi]);
+                for (int c = 0; c < D / 32; ++c)
+                    blocks |= (uint32_t)(nan[e / 4] >> (c * (32 / DL) * 16 + 4 * (lane >> 4) + e % 4)) & 1u ? 1u << c : 0u;
+                if (!(x[e] == -INFINITY)) poison |= blocks;
             }
         }
-    }
-    // The step's scores in base 2 (-inf: masked) and values.  `mixed`: rows of the block's columns see different keys, so
-    // that values which are not finite are multiplied row by row: sees(e, r) tells whether row r sees the lane's key e.
-    template <typename F>
-    __device__ __forceinline__ void take(float* x, const Values& v, bool mixed, int rows, int my_row, F sees) {
         float mx = x[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
@@ -128,52 +130,36 @@ struct Step {  // one wave's running maximum, sum and weighted values of 16 colu
         }
         bf16x8 pf[PP];
         split8<PP>(x, pf);
-        if (mixed) {
-            bool nan = false;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) nan |= v.scale[e] == 255u;
-            if (__any(nan)) {
-#pragma unroll 1
-                for (int r = 0; r < rows; ++r) {
-                    Values u = v;
-                    floatx4 one[JN];
+        for (int j = 0; j < JN; ++j) {
+            const bf16x8 vf = tr_op16(lds, VROW, 16 * j, 0, lane);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (!sees(e, r)) u.code[e] = 0u, u.scale[e] = 127u;
-#pragma unroll
-                    for (int j = 0; j < JN; ++j) one[j] = floatx4{0.f, 0.f, 0.f, 0.f};
-                    product(u, pf, one);
-#pragma unroll
-                    for (int j = 0; j < JN; ++j)
-                        if (my_row == r) acc[j] += one[j];
-                }
-                return;
-            }
+            for (int i = 0; i < PP; ++i) acc[j] = mma(vf, pf[i], acc[j]);
         }
-        product(v, pf, acc);
     }
     // the wave's part of column row16: (maximum, sum) and, where it took any keys, the weighted values [D]
     __device__ __forceinline__ void end(float2* ml, float* out, int kg, bool column, bool any) {
         const float sum = sum_g4(l);
+        const uint32_t all = poison | __shfl_xor(poison, 16);
+        const uint32_t nan = all | __shfl_xor(all, 32);
         if (!column) return;
         if (kg == 0) *ml = make_float2(m, sum);
         if (any) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int j = 0; j < JN; ++j) out[kg * DL + r * JN + j] = acc[j][r];
+            for (int j = 0; j < JN; ++j) *(floatx4*)(out + 16 * j + 4 * kg) = nan >> (j / 2) & 1u ? floatx4{} + NAN : acc[j];
         }
     }
 };
 
-// The parts of a block's columns joined (ml and accs [part][stride columns]; column c is head c % nh of row c / nh):
-// written out, or to the workspace where the row is split.  A part with sum 0 attended nothing and left no values.
+// The parts of a block's columns joined (ml and accs [part][stride columns]; column c is head h0 + c % nh, below h1, of row
+// t0 + c / nh): written out, or to the workspace where the row is split.  A part with sum 0 attended nothing and left no values.
 template <typename T, int D, int THREADS>
-__device__ void join_columns(const Cache4AttnParams& p, float2* ml, const float* accs, int parts, int stride, int n, int nh, int t0, int h0,
-                             int split, int ns) {
+__device__ __forceinline__ void join_columns(const Cache4AttnParams& p, const AttnPlan& a, float2* ml, const float* accs, int parts, int stride,
+                                             int cols, int t0, int h0, int h1, int split) {
     float2* total = ml + parts * stride;  // maximum and sum of each column
+    const int ns = a.ns;
     __syncthreads();
-    for (int c = threadIdx.x; c < n; c += THREADS) {
+    for (int c = threadIdx.x; c < cols; c += THREADS) {
         float M = -INFINITY, L = 0.f;
         for (int k = 0; k < parts; ++k) M = fmaxf(M, ml[k * stride + c].x);
         const float mb = M == -INFINITY ? 0.f : M;
@@ -186,8 +172,9 @@ __device__ void join_columns(const Cache4AttnParams& p, float2* ml, const float*
         total[c] = make_float2(M, L);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < n * D; i += THREADS) {
-        const int c = i / D, d = i - c * D, row = c / nh, h = h0 + c - row * nh;
+    for (int i = threadIdx.x; i < cols * D; i += THREADS) {
+        const int c = i / D, d = i - c * D, row = c * a.col_mul >> 16, h = h0 + c - row * a.nh;
+        if (h >= h1) continue;
         float o = 0.f;
         for (int k = 0; k < parts; ++k) {
             const float2 v = ml[k * stride + c];
@@ -206,186 +193,259 @@ __device__ void join_columns(const Cache4AttnParams& p, float2* ml, const float*
     }
 }
 
-struct Slot {  // a landmark: page, head and token in one number (kNone: not attended), its position and bias in base 2
-    uint32_t key;
-    int pos;
-    float bias;
-};
+// waves a SIMD that the registers are held to
+#ifndef C4_MW
+#define C4_MW 3
+#endif
+template <typename T, int D> struct MinWaves { static constexpr int value = C4_MW; };
+template <> struct MinWaves<float, 64> { static constexpr int value = 2; };
+template <> struct MinWaves<float, 128> { static constexpr int value = 2; };
 
-constexpr int kSlots = 64;  // landmarks looked up at a time, a lane each
+// x as a number that the compiler knows nothing of: what is formed from it stays where it is used, where it would otherwise be
+// formed ahead of every loop and held in registers through all of them
+__device__ __forceinline__ int fresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+constexpr int kSlots = 128, kLook = kSlots / 64;  // landmarks that a wave looks up at a time
+
+// LDS of a block: (maximum, sum) and weighted values of each part and column, the columns' queries, and of each wave the
+// keys of its landmarks (page, head and token in one number; kNone: not attended), their positions and biases in base 2, and
+// the tokens of its step
+template <typename T, int D>
+struct Layout {
+    static constexpr int QS = D + 16 / (int)sizeof(T);  // a query's elements and what keeps rows apart in the banks
+    int parts, stride, waves;
+    __host__ __device__ Layout(const AttnPlan& a) : parts(a.waves + a.chunks()), stride(a.nr * a.nh), waves(a.waves) {}
+    __host__ __device__ int ml() const { return 0; }
+    __host__ __device__ int q() const { return (2 * (parts + 1) * stride + 3) / 4 * 16; }
+    __host__ __device__ int slots() const { return q() + stride * QS * (int)sizeof(T); }
+    __host__ __device__ int stage() const { return slots() + waves * kSlots * 12; }
+    __host__ __device__ int accs() const { return stage() + waves * Step<T, D>::STAGE; }
+    __host__ __device__ int bytes() const { return accs() + parts * stride * D * 4; }
+};
 
 // A block takes rows of one request, side by side, and query heads of one key/value head, 16 columns at most: their
 // window, then each head's landmarks.
 template <typename T, int D, int kWaves>
-__global__ __launch_bounds__(64 * kWaves) void cache4_attn_kernel(Cache4AttnParams p, AttnPlan a) {
+__global__ __launch_bounds__(64 * kWaves, (MinWaves<T, D>::value)) void cache4_attn_kernel(Cache4AttnParams p, AttnPlan a) {
     typedef Step<T, D> S;
-    extern __shared__ float lds[];
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, row16 = lane & 15, kg = lane >> 4;
+    constexpr int QS = Layout<T, D>::QS;
+    extern __shared__ char lds[];
+    const Layout<T, D> at(a);
+    const int wv = threadIdx.x >> 6;
     const int G = p.c.n_kv, group = p.n_heads / G, bt_log = p.c.bt_log, bt = 1 << bt_log;
-    const int hx = blockIdx.x % a.tiles, tg = blockIdx.x / a.tiles, g = tg % G, rt = tg / G, split = blockIdx.y;
-    const int h0 = g * group + hx * a.nh, nh = min(a.nh, group - hx * a.nh);
+    const int rt = xcd_swizzle(blockIdx.x, gridDim.x), split = blockIdx.z;
+    const int g = a.tiles == 1 ? blockIdx.y : blockIdx.y / a.tiles, hx = blockIdx.y - g * a.tiles;
+    const int h0 = g * group + hx * a.nh, h1 = min(h0 + a.nh, (g + 1) * group), nh = a.nh;
     const bool marks = split < a.nl;
-    const int parts = kWaves + (marks ? a.chunks : 0), stride = a.nr * a.nh;
-    float2* ml = (float2*)lds;
-    float* accs = lds + 2 * (kWaves + a.chunks + 1) * stride;
-    Slot* slots = (Slot*)(accs + (kWaves + a.chunks) * stride * D) + wv * kSlots;
+    const int parts = kWaves + (marks ? a.chunks() : 0), stride = at.stride;
+    float2* ml = (float2*)(lds + at.ml());
+    float* accs = (float*)(lds + at.accs());
+    T* qs = (T*)(lds + at.q());
+    uint32_t* keys = (uint32_t*)(lds + at.slots()) + wv * 3 * kSlots;
+    int* places = (int*)keys + kSlots;
+    float* biases = (float*)keys + 2 * kSlots;
+    bf16* stage = (bf16*)(lds + at.stage() + wv * S::STAGE);
     const float scale2 = p.scale * kLog2e;
-    const int run = rt / a.run_tiles;
+    const int run = a.run_tiles == 1 ? rt : rt / a.run_tiles;
     const int64_t t_first = (int64_t)run * p.per + (int64_t)(rt - run * a.run_tiles) * a.nr;
     const int64_t t_end = min(min(t_first + a.nr, ((int64_t)run + 1) * p.per), (int64_t)p.n_rows);
+    auto row_of = [&](int c) { return c * a.col_mul >> 16; };
+    // the tile's rows, a lane each
+    int rq = -1, ps = -1, wd = 1;
+    {
+        const int64_t t = t_first + (threadIdx.x & 15);
+        if (t < t_end) {
+            rq = p.req[t];
+            ps = p.pos[t];
+            wd = max(p.w[t], 1);
+        }
+    }
     S s;
 
     for (int64_t tt = t_first; tt < t_end;) {  // (once, unless the rows side by side belong to several requests)
-        const int t0 = (int)tt, req = p.req[t0];
-        int n = 1;
-        while (tt + n < t_end && p.req[t0 + n] == req) ++n;
+        const int tid = fresh(threadIdx.x), lane = tid & 63, row16 = lane & 15, kg = lane >> 4;
+        const int t0 = (int)tt, r0 = (int)(tt - t_first), req = __builtin_amdgcn_readlane(rq, r0);
+        const uint32_t others = (((uint32_t)__ballot(rq != req || t_first + row16 >= t_end) & 0xffffu) | 0x10000u) >> r0;
+        const int n = __builtin_ctz(others);
         tt += n;
+        const int cols = n * nh;
         const bool known = req >= 0 && req < p.n_reqs;
         const int32_t* table = p.table + (known ? (int64_t)req * p.table_st : 0);
         const int cap = (p.cols << bt_log) - 1;
         // rows: the lane's for columns of the window, and for those of landmarks
         struct Range { int low, end; };  // first and last key of the window; a row without keys sees nothing
         auto range = [&](int row) {
-            const int pos = p.pos[t0 + row];
+            const int pos = __shfl(ps, r0 + row), w = __shfl(wd, r0 + row);
             const bool live = known && pos >= 0;
-            return Range{live ? max(pos - max(p.w[t0 + row], 1) + 1, 0) : 0x7fffffff, live ? min(pos, cap) : -1};
+            return Range{live ? max(pos - w + 1, 0) : 0x7fffffff, live ? min(pos, cap) : -1};
         };
-        const int col = row16 < n * nh ? row16 : 0, wrow = col / nh, lrow = row16 < n ? row16 : 0;
-        const Range win = range(wrow), mark = range(lrow);
-        const int mark_low = mark.low == 0x7fffffff ? 0 : mark.low;
-        const int low_min = __builtin_amdgcn_readfirstlane(row_min16(win.low)), low_max = __builtin_amdgcn_readfirstlane(row_max16(win.low));
-        const int end_min = __builtin_amdgcn_readfirstlane(row_min16(win.end)), end_max = __builtin_amdgcn_readfirstlane(row_max16(win.end));
+        const int col = row16 < cols ? row16 : 0, lrow = row16 < n ? row16 : 0;
+        const Range win = range(row_of(col));
+        const int low_r = n == 1 ? win.low : range(lrow).low, mark_low = low_r == 0x7fffffff ? 0 : low_r;
+        auto lowest = [](int v) { return __builtin_amdgcn_readfirstlane(row_min16(v)); };
+        auto largest = [](int v) { return __builtin_amdgcn_readfirstlane(row_max16(v)); };
+        const int low_min = lowest(win.low), low_max = largest(win.low), end_min = lowest(win.end), end_max = largest(win.end);
+        const int mark_max = largest(mark_low);
+
+        // ---- the wave's landmarks: slot f of its items (head, part), one after the other
+        const int items = marks ? (h1 - h0) << a.chunk_log : 0, my_items = wv < items ? (items - 1 - wv) / kWaves + 1 : 0;
+        const int total = known ? my_items << a.kr_log : 0, k0 = split * (a.kc << max(a.chunk_log, 0));
+        int mj[kLook];
+        float mb[kLook];
+        auto look_marks = [&](int b) {
+#pragma unroll
+            for (int i = 0; i < kLook; ++i) {
+                mj[i] = -1;
+                mb[i] = 0.f;
+                if (b + i * 64 >= total) continue;
+                const int f = b + i * 64 + lane, it = wv + (f >> a.kr_log) * kWaves, hh = it >> a.chunk_log;
+                const int o = f & ((1 << a.kr_log) - 1), k = k0 + (it - (hh << a.chunk_log)) * a.kc + o;
+                if (f < total && o < a.kc && k < p.k_lmk) {
+                    const int64_t x = ((int64_t)(h0 + hh) * p.n_reqs + req) * p.k_lmk + k;
+                    mj[i] = p.lmk[x];
+                    if (p.lbias) mb[i] = p.lbias[x];
+                }
+            }
+        };
+        auto place_marks = [&](int b) {  // (after look_marks; a bias of minus infinity masks its key, which is then not read)
+            int page[kLook];
+#pragma unroll
+            for (int i = 0; i < kLook; ++i) {
+                const int pb = mj[i] >> bt_log;
+                page[i] = -1;
+                if (mj[i] >= 0 && mj[i] < mark_max && pb < p.cols && mb[i] != -INFINITY) page[i] = table[pb];
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < kLook; ++i) {
+                if (b + i * 64 >= total) continue;
+                const bool ok = page[i] >= 0 && page[i] < p.c.n_blocks;
+                keys[i * 64 + lane] = ok ? (((uint32_t)page[i] * (uint32_t)G + (uint32_t)g) << bt_log) + (uint32_t)(mj[i] & (bt - 1)) : kNone;
+                if (n > 1) places[i * 64 + lane] = mj[i];
+                // (the type's lowest values stay finite, as masks of them are apart from minus infinity)
+                if (p.lbias) biases[i * 64 + lane] = mb[i] > -INFINITY ? fmaxf(mb[i] * kLog2e, -3e38f) : mb[i];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        };
 
         // ---- window: keys base + 32 step ..., from the aligned position at or before the first
-        {
-            const int base = low_min & ~(kStep - 1);
-            const int steps = end_max >= low_min ? ((end_max - base) >> 5) + 1 : 0, per = ceil_div(steps, a.ns);
-            const int s0 = split * per, s1 = min(steps, s0 + per);
-            s.begin((const T*)p.q + (int64_t)(t0 + wrow) * p.q_st + (int64_t)(h0 + col - wrow * nh) * p.q_sh, kg);
-            const int first = s0 + wv, mine = first < s1 ? (s1 - 1 - first) / kWaves + 1 : 0;
-            // lane 2 i + half: page (-1: none) of the 16 keys `half` of step i of the batch of 32 steps from b0
-            auto look = [&](int b0) {
-                const int b = (base + (first + (b0 + (lane >> 1)) * kWaves) * kStep + (lane & 1) * 16) >> bt_log;
-                const bool in = b0 + (lane >> 1) < mine && b < p.cols;
-                const int page = table[in ? b : 0];
-                return in && page >= 0 && page < p.c.n_blocks ? page : -1;
-            };
-            for (int b0 = 0; b0 < mine; b0 += 32) {
-                const int page = look(b0), m = min(32, mine - b0);
-                auto token_at = [&](int i, int half) -> uint64_t {  // of the first of 16 keys (page 0 where there is none)
-                    const int pg = max(__builtin_amdgcn_readlane(page, 2 * i + half), 0);
-                    const int at = base + (first + (b0 + i) * kWaves) * kStep + half * 16;
-                    return (((uint64_t)pg * G + g) << bt_log) + (at & (bt - 1));
-                };
-                typename S::Keys k;
-                typename S::Values v;
-                auto load_k = [&](int i) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) S::load_key(p.c, token_at(i, half) + row16, kg, k.code[half], k.scale[half]);
-                };
-                auto load_v = [&](int i) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint64_t token = token_at(i, half) + 4 * kg;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) S::load_value(p.c, token + e, row16, v.code[4 * half + e], v.scale[4 * half + e]);
-                    }
-                };
-                load_k(0);
-                load_v(0);
-                for (int i = 0; i < m; ++i) {
-                    const int at = base + (first + (b0 + i) * kWaves) * kStep;
-                    const int pg0 = __builtin_amdgcn_readlane(page, 2 * i), pg1 = __builtin_amdgcn_readlane(page, 2 * i + 1);
-                    float x[8];
-                    s.scores(k, x);
-                    if (i + 1 < m) load_k(i + 1);
-                    const bool whole = at >= low_max && at + kStep - 1 <= end_min && pg0 >= 0 && pg1 >= 0;
-                    auto key = [&](int e) { return at + (e & 4) * 4 + 4 * kg + (e & 3); };
-                    auto held = [&](int e) { return (e < 4 ? pg0 : pg1) >= 0; };
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] *= scale2;
-                    if (!whole) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int j = key(e);
-                            if (j < win.low || j > win.end || !held(e)) x[e] = -INFINITY;
-                            if (j < low_min || j > end_max || !held(e)) v.code[e] = 0u, v.scale[e] = 127u;  // no column's
-                        }
-                    }
-                    s.take(x, v, !whole && n > 1, n, wrow, [&](int e, int r) {
-                        const int j = key(e);
-                        // (lanes differ in what they have compared so far, so that none of them may be asked by a shuffle)
-                        return j >= __builtin_amdgcn_readlane(win.low, r * nh) && j <= __builtin_amdgcn_readlane(win.end, r * nh) && held(e);
-                    });
-                    if (i + 1 < m) load_v(i + 1);
-                }
+        const int base = low_min & ~(kStep - 1);
+        const int steps = end_max >= low_min ? ((end_max - base) >> 5) + 1 : 0, per = a.ns == 1 ? steps : ceil_div(steps, a.ns);
+        const int s0 = split * per, s1 = min(steps, s0 + per);
+        const int first = s0 + wv, mine = first < s1 ? (s1 - 1 - first) / kWaves + 1 : 0;
+        // lane 2 i + half: page (-1: none) of the 16 keys `half` of step i of the batch of 32 steps from b0
+        auto look = [&](int b0) {
+            const int b = (base + (first + (b0 + (lane >> 1)) * kWaves) * kStep + (lane & 1) * 16) >> bt_log;
+            const bool in = b0 + (lane >> 1) < mine && b < p.cols;
+            const int page = table[in ? b : 0];
+            return in && page >= 0 && page < p.c.n_blocks ? page : -1;
+        };
+        int page = mine > 0 ? look(0) : -1;
+        look_marks(0);
+        {  // the columns' queries; parts of landmarks that no item writes hold nothing
+            constexpr int VEC = 16 / (int)sizeof(T);
+            for (int i = tid; i < cols * (D / VEC); i += 64 * kWaves) {
+                const int c = i / (D / VEC), e = i - c * (D / VEC), row = row_of(c), h = min(h0 + c - row * nh, h1 - 1);
+                *(u32x4*)(qs + c * QS + e * VEC) =
+                    *(const u32x4*)((const T*)p.q + (int64_t)(t0 + row) * p.q_st + (int64_t)h * p.q_sh + e * VEC);
             }
-            s.end(ml + wv * stride + row16, accs + (wv * stride + row16) * D, kg, row16 < n * nh, mine > 0);
+            for (int i = tid; i < (parts - kWaves) * stride; i += 64 * kWaves) ml[kWaves * stride + i] = make_float2(-INFINITY, 0.f);
+        }
+        typename S::Tokens tk;
+        {
+            auto token_at = [&](int i, int half) -> uint64_t {  // of the first of 16 keys (page 0 where there is none)
+                const int pg = max(__builtin_amdgcn_readlane(page, 2 * (i & 31) + half), 0);
+                const int j = base + (first + i * kWaves) * kStep + half * 16;
+                return (((uint64_t)pg * G + g) << bt_log) + (j & (bt - 1));
+            };
+            auto load = [&](int i) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint64_t token = token_at(i, half);
+                    S::load(p.c.kv + token * D + row16 * D, p.c.scale + token * (D / 16) + row16 * (D / 16), kg, half, tk);
+                }
+            };
+            if (mine > 0) load(0);
+            if (total > 0) place_marks(0);
+            __syncthreads();
+            s.begin(qs + col * QS, kg);
+#pragma unroll 1
+            for (int i = 0; i < mine; ++i) {
+                const int j0 = base + (first + i * kWaves) * kStep;
+                const bool held0 = __builtin_amdgcn_readlane(page, 2 * (i & 31)) >= 0, held1 = __builtin_amdgcn_readlane(page, 2 * (i & 31) + 1) >= 0;
+                float x[8];
+                unsigned long long nan[2];
+                s.scores(tk, x);
+                const bool any = S::stage_values(stage, row16, kg, tk, nan);
+                if (((i + 1) & 31) == 0 && i + 1 < mine) page = look(i + 1);
+                if (i + 1 < mine) load(i + 1);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] *= scale2;
+                if (!(j0 >= low_max && j0 + kStep - 1 <= end_min && held0 && held1)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int j = j0 + (e & 4) * 4 + 4 * kg + (e & 3);
+                        if (j < win.low || j > win.end || !(e < 4 ? held0 : held1)) x[e] = -INFINITY;
+                    }
+                }
+                s.take(stage, lane, any, nan, x);
+            }
+            s.end(ml + wv * stride + row16, accs + (wv * stride + row16) * D, kg, row16 < cols, mine > 0);
         }
 
-        // ---- landmarks: item (head hh, chunk c) of slots c0 .. c1
-        const int kl = marks ? ceil_div(p.k_lmk, a.nl) : 0, k0 = min(split * kl, p.k_lmk), k1 = min(k0 + kl, p.k_lmk);
-        const int kc = marks ? ceil_div(k1 - k0, a.chunks) : 0, items = marks ? nh * a.chunks : 0;
-        for (int it = wv; it < items; it += kWaves) {
-            const int hh = it / a.chunks, c = it - hh * a.chunks;
-            const int c0 = min(k0 + c * kc, k1), c1 = known ? min(c0 + kc, k1) : c0;
-            s.begin((const T*)p.q + (int64_t)(t0 + lrow) * p.q_st + (int64_t)(h0 + hh) * p.q_sh, kg);
-            for (int b = c0; b < c1; b += kSlots) {
-                {  // the lane's slot
-                    Slot sl = {kNone, 0, 0.f};
-                    if (b + lane < c1) {
-                        const int64_t at = ((int64_t)(h0 + hh) * p.n_reqs + req) * p.k_lmk + b + lane;
-                        sl.pos = p.lmk[at];
-                        const int pb = sl.pos >> bt_log;
-                        if (sl.pos >= 0 && pb < p.cols) {
-                            const int page = table[pb];
-                            if (p.lbias) sl.bias = p.lbias[at];
-                            if (page >= 0 && page < p.c.n_blocks && sl.bias != -INFINITY) {
-                                sl.key = (((uint32_t)page * (uint32_t)G + (uint32_t)g) << bt_log) + (uint32_t)(sl.pos & (bt - 1));
-                                // (the type's lowest values stay finite, as masks of them are apart from minus infinity)
-                                if (sl.bias > -INFINITY) sl.bias = fmaxf(sl.bias * kLog2e, -3e38f);
-                            }
-                        }
-                    }
-                    __builtin_amdgcn_wave_barrier();
-                    slots[lane] = sl;
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    __builtin_amdgcn_wave_barrier();
+        // ---- landmarks, whole steps of one item each
+        for (int b = 0; b < total; b += kSlots) {
+            if (b > 0) {
+                look_marks(b);
+                place_marks(b);
+            }
+            const int lane = fresh(threadIdx.x) & 63, row16 = lane & 15, kg = lane >> 4;
+            auto load = [&](int i) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t key = keys[i * kStep + half * 16 + row16];
+                    tk.key[half] = tk.value[half] = typename S::kword{};
+                    tk.key_scale[half] = tk.value_scale[half] = 127u;
+                    if (key != kNone) S::load(p.c.kv + (uint64_t)key * D, p.c.scale + (uint64_t)key * (D / 16), kg, half, tk);
                 }
-                const int steps = ceil_div(min(kSlots, c1 - b), kStep);
-                for (int i = 0; i < steps; ++i) {
-                    typename S::Keys k;
-                    typename S::Values v;
-                    Slot sl[8];
+            };
+            const int n_steps = min(kSlots, total - b) / kStep;
+            load(0);
+#pragma unroll 1
+            for (int i = 0; i < n_steps; ++i) {
+                const int f = b + i * kStep, o = f & ((1 << a.kr_log) - 1), it = wv + (f >> a.kr_log) * kWaves, hh = it >> a.chunk_log;
+                if (o == 0) s.begin(qs + (lrow * nh + hh) * QS, kg);
+                float x[8];
+                unsigned long long nan[2];
+                s.scores(tk, x);
+                const bool any = S::stage_values(stage, row16, kg, tk, nan);
+                if (i + 1 < n_steps) load(i + 1);
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint32_t key = slots[i * kStep + half * 16 + row16].key;
-                        k.code[half] = typename S::kword{};
-                        k.scale[half] = 127u;
-                        if (key != kNone) S::load_key(p.c, key, kg, k.code[half], k.scale[half]);
-                    }
+                for (int half = 0; half < 2; ++half) {
+                    const int q0 = i * kStep + half * 16 + 4 * kg;
+                    const u32x4 key = *(const u32x4*)(keys + q0);
+                    u32x4 place = {};
+                    if (n > 1) place = *(const u32x4*)(places + q0);
+                    floatx4 bias = {};
+                    if (p.lbias) bias = *(const floatx4*)(biases + q0);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        sl[e] = slots[i * kStep + (e & 4) * 4 + 4 * kg + (e & 3)];
-                        v.code[e] = 0u;
-                        v.scale[e] = 127u;
-                        if (sl[e].key != kNone) S::load_value(p.c, sl[e].key, row16, v.code[e], v.scale[e]);
+                    for (int e = 0; e < 4; ++e) {
+                        const bool on = key[e] != kNone && (n == 1 || (int)place[e] < mark_low);
+                        x[4 * half + e] = on ? x[4 * half + e] * scale2 + bias[e] : -INFINITY;
                     }
-                    float x[8];
-                    s.scores(k, x);
-                    auto seen = [&](int e, int low) { return sl[e].key != kNone && sl[e].pos < low; };
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[e] = seen(e, mark_low) ? x[e] * scale2 + sl[e].bias : -INFINITY;
-                        if (n == 1 && !seen(e, mark_low)) v.code[e] = 0u, v.scale[e] = 127u;
-                    }
-                    s.take(x, v, n > 1, n, lrow, [&](int e, int r) { return seen(e, __builtin_amdgcn_readlane(mark_low, r)); });
+                }
+                s.take(stage, lane, any, nan, x);
+                if (o + kStep == 1 << a.kr_log) {
+                    const int part = kWaves + it - (hh << a.chunk_log), slot = part * stride + row16 * nh + hh;
+                    s.end(ml + slot, accs + (int64_t)slot * D, kg, row16 < n, true);
                 }
             }
-            const int at = (kWaves + c) * stride + row16 * nh + hh;
-            s.end(ml + at, accs + (int64_t)at * D, kg, row16 < n, c0 < c1);
         }
-        join_columns<T, D, 64 * kWaves>(p, ml, accs, parts, stride, n * nh, nh, t0, h0, split, a.ns);
+        join_columns<T, D, 64 * kWaves>(p, a, ml, accs, parts, stride, cols, t0, h0, h1, split);
         __syncthreads();
     }
 }
@@ -400,21 +460,31 @@ AttnPlan attn_plan(const Cache4AttnParams& p) {
     a.nr = std::min(p.per, 16 / a.nh);
     a.run_tiles = ceil_div(p.per, a.nr);
     const int64_t groups = (rows + p.per - 1) / p.per * a.run_tiles * p.c.n_kv;
+    if (w <= 1024)
     while (a.nh > 1 && groups * ceil_div(group, a.nh) < 256) a.nh = ceil_div(a.nh, 2);
+    if (const char* e = getenv("C4_NH")) a.nh = std::min(group, atoi(e));
     a.tiles = ceil_div(group, a.nh);
     const int64_t blocks = groups * a.tiles;
-    a.waves = blocks <= 256 ? 8 : 4;
+    a.waves = 4;
     a.ns = (int)std::max(std::min(512 / blocks, w / 1024), (int64_t)1);
-    a.nl = std::min(ceil_div(p.k_lmk, 64), a.ns);
-    a.chunks = p.k_lmk == 0 ? 0 : std::max(a.waves / a.nh, 1);
+    if (const char* e = getenv("C4_WAVES")) a.waves = atoi(e);
+    if (const char* e = getenv("C4_NS")) a.ns = atoi(e);
+    a.nl = p.k_lmk == 0 ? 0 : std::min(ceil_div(p.k_lmk, 64), a.ns);
+    a.chunk_log = p.k_lmk == 0 ? -1 : 0;
+    if (p.k_lmk > 0)  // (no more parts than leave room for two blocks in a compute unit's LDS)
+        while ((2 << a.chunk_log) * a.nh <= a.waves && (a.waves + (2 << a.chunk_log)) * a.nr * a.nh * p.c.head_dim * 4 <= 1 << 16) ++a.chunk_log;
+    a.kc = p.k_lmk == 0 ? 0 : ceil_div(ceil_div(p.k_lmk, a.nl), a.chunks());
+    a.kr_log = 5;
+    while (1 << a.kr_log < a.kc) ++a.kr_log;
+    a.col_mul = ceil_div(1 << 16, a.nh);
     return a;
 }
 
 template <typename T, int D>
 hipError_t run_rows(const Cache4AttnParams& p, const AttnPlan& a, hipStream_t stream) {
     const int64_t runs = ((int64_t)p.n_rows + p.per - 1) / p.per;
-    const dim3 grid((unsigned)(runs * a.run_tiles * p.c.n_kv * a.tiles), (unsigned)a.ns);
-    const unsigned lds = (unsigned)((((a.waves + a.chunks) * (D + 2) + 2) * a.cols()) * sizeof(float) + a.waves * kSlots * sizeof(Slot));
+    const dim3 grid((unsigned)(runs * a.run_tiles), (unsigned)(p.c.n_kv * a.tiles), (unsigned)a.ns);
+    const unsigned lds = (unsigned)Layout<T, D>(a).bytes();
     auto kernel = a.waves == 8 ? cache4_attn_kernel<T, D, 8> : cache4_attn_kernel<T, D, 4>;
     if (lds > 65536)
         if (hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)) return e;
@@ -430,7 +500,7 @@ template <typename T, int D>
 hipError_t run(const Cache4AttnParams& p, hipStream_t stream) {
     const AttnPlan a = attn_plan(p);
     // runs of rows of a launch (more than one launch: blocks of four waves, no splits)
-    const int64_t most = std::max(kLaunchThreads / 256 / ((int64_t)p.c.n_kv * a.tiles * a.run_tiles), (int64_t)1) * p.per;
+    const int64_t most = std::max(kLaunchThreads / 256 / a.run_tiles, (int64_t)1) * p.per;
     Cache4AttnParams s = p;
     for (int64_t t = 0; t < p.n_rows; t += s.n_rows) {
         s.n_rows = (int)std::min(most, p.n_rows - t);
