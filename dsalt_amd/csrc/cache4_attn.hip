@@ -20,15 +20,16 @@ namespace dsalt {
 namespace {
 
 constexpr int kStep = 32;  // keys of a step
+constexpr int kWaves = 4;  // of a block
 constexpr uint32_t kNone = 0xffffffffu;
 
 struct AttnPlan {
     int nh, tiles;      // heads of a block, blocks of a key/value head's query heads
     int nr, run_tiles;  // rows of a block, blocks of a request's rows
     int ns, nl;         // splits of a row's window, and of its landmark slots
-    int waves;          // of a block
     int chunk_log;      // a head's landmark slots are 2^chunk_log parts within a block (-1: there are none)
     int kc, kr_log;     // slots of a part, and of a part with what fills it up to a power of two
+    int slots, fields;  // slots that a wave looks up at a time, and numbers it keeps of each
     int col_mul;        // c / nh = c col_mul >> 16 for columns c
     __host__ __device__ int chunks() const { return chunk_log < 0 ? 0 : 1 << chunk_log; }
 };
@@ -72,15 +73,21 @@ struct Step {  // one wave's running maximum, sum and weighted values of 16 colu
     // Values are held apart from those that are NaN: nan[half] has a bit for each lane's, which are staged as zeros.
     __device__ __forceinline__ static bool stage_values(bf16* lds, int row16, int kg, Tokens& t, unsigned long long* nan) {
 #pragma unroll
+        for (int half = 0; half < 2; ++half) nan[half] = __ballot(t.value_scale[half] == 255u);
+        const bool any = __builtin_expect((nan[0] | nan[1]) != 0, 0);
+        if (any) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                if (t.value_scale[half] == 255u) t.value_scale[half] = 127u, t.value[half] = kword{};
+        }
+#pragma unroll
         for (int half = 0; half < 2; ++half) {
-            nan[half] = __ballot(t.value_scale[half] == 255u);
-            if (nan[half] != 0 && t.value_scale[half] == 255u) t.value_scale[half] = 127u, t.value[half] = kword{};
             const float scale = e8m0(t.value_scale[half]);
 #pragma unroll
             for (int i = 0; i < KW; ++i)
                 *(bf16x8*)(lds + (half * 16 + row16) * VROW + kg * DL + 8 * i) = e2m1_op(t.value[half][i], scale);
         }
-        return (nan[0] | nan[1]) != 0;
+        return any;
     }
     // scores of keys 16 half + 4 kg + r for column row16
     __device__ __forceinline__ void scores(const Tokens& t, float* x) const {
@@ -153,13 +160,13 @@ struct Step {  // one wave's running maximum, sum and weighted values of 16 colu
 
 // The parts of a block's columns joined (ml and accs [part][stride columns]; column c is head h0 + c % nh, below h1, of row
 // t0 + c / nh): written out, or to the workspace where the row is split.  A part with sum 0 attended nothing and left no values.
-template <typename T, int D, int THREADS>
+template <typename T, int D>
 __device__ __forceinline__ void join_columns(const Cache4AttnParams& p, const AttnPlan& a, float2* ml, const float* accs, int parts, int stride,
                                              int cols, int t0, int h0, int h1, int split) {
     float2* total = ml + parts * stride;  // maximum and sum of each column
     const int ns = a.ns;
     __syncthreads();
-    for (int c = threadIdx.x; c < cols; c += THREADS) {
+    for (int c = threadIdx.x; c < cols; c += 64 * kWaves) {
         float M = -INFINITY, L = 0.f;
         for (int k = 0; k < parts; ++k) M = fmaxf(M, ml[k * stride + c].x);
         const float mb = M == -INFINITY ? 0.f : M;
@@ -172,7 +179,7 @@ __device__ __forceinline__ void join_columns(const Cache4AttnParams& p, const At
         total[c] = make_float2(M, L);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < cols * D; i += THREADS) {
+    for (int i = threadIdx.x; i < cols * D; i += 64 * kWaves) {
         const int c = i / D, d = i - c * D, row = c * a.col_mul >> 16, h = h0 + c - row * a.nh;
         if (h >= h1) continue;
         float o = 0.f;
@@ -193,14 +200,6 @@ __device__ __forceinline__ void join_columns(const Cache4AttnParams& p, const At
     }
 }
 
-// waves a SIMD that the registers are held to
-#ifndef C4_MW
-#define C4_MW 3
-#endif
-template <typename T, int D> struct MinWaves { static constexpr int value = C4_MW; };
-template <> struct MinWaves<float, 64> { static constexpr int value = 2; };
-template <> struct MinWaves<float, 128> { static constexpr int value = 2; };
-
 // x as a number that the compiler knows nothing of: what is formed from it stays where it is used, where it would otherwise be
 // formed ahead of every loop and held in registers through all of them
 __device__ __forceinline__ int fresh(int x) {
@@ -208,7 +207,7 @@ __device__ __forceinline__ int fresh(int x) {
     return x;
 }
 
-constexpr int kSlots = 128, kLook = kSlots / 64;  // landmarks that a wave looks up at a time
+constexpr int kLook = 4;  // slots that a lane looks up at a time, at most
 
 // LDS of a block: (maximum, sum) and weighted values of each part and column, the columns' queries, and of each wave the
 // keys of its landmarks (page, head and token in one number; kNone: not attended), their positions and biases in base 2, and
@@ -216,25 +215,25 @@ constexpr int kSlots = 128, kLook = kSlots / 64;  // landmarks that a wave looks
 template <typename T, int D>
 struct Layout {
     static constexpr int QS = D + 16 / (int)sizeof(T);  // a query's elements and what keeps rows apart in the banks
-    int parts, stride, waves;
-    __host__ __device__ Layout(const AttnPlan& a) : parts(a.waves + a.chunks()), stride(a.nr * a.nh), waves(a.waves) {}
+    int parts, stride, wave_slots;
+    __host__ __device__ Layout(const AttnPlan& a) : parts(kWaves + a.chunks()), stride(a.nr * a.nh), wave_slots(a.slots * a.fields) {}
     __host__ __device__ int ml() const { return 0; }
     __host__ __device__ int q() const { return (2 * (parts + 1) * stride + 3) / 4 * 16; }
     __host__ __device__ int slots() const { return q() + stride * QS * (int)sizeof(T); }
-    __host__ __device__ int stage() const { return slots() + waves * kSlots * 12; }
-    __host__ __device__ int accs() const { return stage() + waves * Step<T, D>::STAGE; }
+    __host__ __device__ int stage() const { return slots() + kWaves * wave_slots * 4; }
+    __host__ __device__ int accs() const { return stage() + kWaves * Step<T, D>::STAGE; }
     __host__ __device__ int bytes() const { return accs() + parts * stride * D * 4; }
 };
 
 // A block takes rows of one request, side by side, and query heads of one key/value head, 16 columns at most: their
 // window, then each head's landmarks.
-template <typename T, int D, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, (MinWaves<T, D>::value)) void cache4_attn_kernel(Cache4AttnParams p, AttnPlan a) {
+template <typename T, int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void cache4_attn_kernel(Cache4AttnParams p, AttnPlan a) {
     typedef Step<T, D> S;
     constexpr int QS = Layout<T, D>::QS;
     extern __shared__ char lds[];
     const Layout<T, D> at(a);
-    const int wv = threadIdx.x >> 6;
+    const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int G = p.c.n_kv, group = p.n_heads / G, bt_log = p.c.bt_log, bt = 1 << bt_log;
     const int rt = xcd_swizzle(blockIdx.x, gridDim.x), split = blockIdx.z;
     const int g = a.tiles == 1 ? blockIdx.y : blockIdx.y / a.tiles, hx = blockIdx.y - g * a.tiles;
@@ -244,9 +243,9 @@ __global__ __launch_bounds__(64 * kWaves, (MinWaves<T, D>::value)) void cache4_a
     float2* ml = (float2*)(lds + at.ml());
     float* accs = (float*)(lds + at.accs());
     T* qs = (T*)(lds + at.q());
-    uint32_t* keys = (uint32_t*)(lds + at.slots()) + wv * 3 * kSlots;
-    int* places = (int*)keys + kSlots;
-    float* biases = (float*)keys + 2 * kSlots;
+    uint32_t* keys = (uint32_t*)(lds + at.slots()) + wv * at.wave_slots;
+    int* places = (int*)keys + (a.nr > 1 ? a.slots : 0);  // (where there are several rows)
+    float* biases = (float*)places + a.slots;             // (where there are any)
     bf16* stage = (bf16*)(lds + at.stage() + wv * S::STAGE);
     const float scale2 = p.scale * kLog2e;
     const int run = a.run_tiles == 1 ? rt : rt / a.run_tiles;
@@ -300,7 +299,7 @@ __global__ __launch_bounds__(64 * kWaves, (MinWaves<T, D>::value)) void cache4_a
             for (int i = 0; i < kLook; ++i) {
                 mj[i] = -1;
                 mb[i] = 0.f;
-                if (b + i * 64 >= total) continue;
+                if (i * 64 >= a.slots || b + i * 64 >= total) continue;
                 const int f = b + i * 64 + lane, it = wv + (f >> a.kr_log) * kWaves, hh = it >> a.chunk_log;
                 const int o = f & ((1 << a.kr_log) - 1), k = k0 + (it - (hh << a.chunk_log)) * a.kc + o;
                 if (f < total && o < a.kc && k < p.k_lmk) {
@@ -321,7 +320,7 @@ __global__ __launch_bounds__(64 * kWaves, (MinWaves<T, D>::value)) void cache4_a
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int i = 0; i < kLook; ++i) {
-                if (b + i * 64 >= total) continue;
+                if (i * 64 >= a.slots || b + i * 64 >= total) continue;
                 const bool ok = page[i] >= 0 && page[i] < p.c.n_blocks;
                 keys[i * 64 + lane] = ok ? (((uint32_t)page[i] * (uint32_t)G + (uint32_t)g) << bt_log) + (uint32_t)(mj[i] & (bt - 1)) : kNone;
                 if (n > 1) places[i * 64 + lane] = mj[i];
@@ -355,75 +354,79 @@ __global__ __launch_bounds__(64 * kWaves, (MinWaves<T, D>::value)) void cache4_a
             }
             for (int i = tid; i < (parts - kWaves) * stride; i += 64 * kWaves) ml[kWaves * stride + i] = make_float2(-INFINITY, 0.f);
         }
-        typename S::Tokens tk;
+        // Tokens of a step, requested two steps ahead: memory answers later than one step takes.
+        typename S::Tokens tk[2];
         {
-            auto token_at = [&](int i, int half) -> uint64_t {  // of the first of 16 keys (page 0 where there is none)
-                const int pg = max(__builtin_amdgcn_readlane(page, 2 * (i & 31) + half), 0);
-                const int j = base + (first + i * kWaves) * kStep + half * 16;
-                return (((uint64_t)pg * G + g) << bt_log) + (j & (bt - 1));
-            };
-            auto load = [&](int i) {
+            int held[2] = {0, 0};  // whether the table names the pages of a step's halves
+            auto load = [&](int i, typename S::Tokens& t, int& on) {
+                if ((i & 31) == 0 && i > 0) page = look(i);
+                on = 0;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const uint64_t token = token_at(i, half);
-                    S::load(p.c.kv + token * D + row16 * D, p.c.scale + token * (D / 16) + row16 * (D / 16), kg, half, tk);
+                    const int pg = __builtin_amdgcn_readlane(page, 2 * (i & 31) + half);
+                    on |= pg >= 0 ? 1 << half : 0;
+                    const int j = base + (first + i * kWaves) * kStep + half * 16;  // (page 0 where there is none)
+                    const uint64_t token = (((uint64_t)max(pg, 0) * G + g) << bt_log) + (j & (bt - 1));
+                    S::load(p.c.kv + token * D + row16 * D, p.c.scale + token * (D / 16) + row16 * (D / 16), kg, half, t);
                 }
             };
-            if (mine > 0) load(0);
+            if (mine > 0) load(0, tk[0], held[0]);
+            if (mine > 1) load(1, tk[1], held[1]);
             if (total > 0) place_marks(0);
             __syncthreads();
             s.begin(qs + col * QS, kg);
-#pragma unroll 1
-            for (int i = 0; i < mine; ++i) {
-                const int j0 = base + (first + i * kWaves) * kStep;
-                const bool held0 = __builtin_amdgcn_readlane(page, 2 * (i & 31)) >= 0, held1 = __builtin_amdgcn_readlane(page, 2 * (i & 31) + 1) >= 0;
+            auto step = [&](int i, typename S::Tokens& t, int& on) {
+                const int j0 = base + (first + i * kWaves) * kStep, both = on;
                 float x[8];
                 unsigned long long nan[2];
-                s.scores(tk, x);
-                const bool any = S::stage_values(stage, row16, kg, tk, nan);
-                if (((i + 1) & 31) == 0 && i + 1 < mine) page = look(i + 1);
-                if (i + 1 < mine) load(i + 1);
+                s.scores(t, x);
+                const bool any = S::stage_values(stage, row16, kg, t, nan);
+                if (i + 2 < mine) load(i + 2, t, on);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] *= scale2;
-                if (!(j0 >= low_max && j0 + kStep - 1 <= end_min && held0 && held1)) {
+                if (!(j0 >= low_max && j0 + kStep - 1 <= end_min && both == 3)) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const int j = j0 + (e & 4) * 4 + 4 * kg + (e & 3);
-                        if (j < win.low || j > win.end || !(e < 4 ? held0 : held1)) x[e] = -INFINITY;
+                        const bool out = (j < win.low) | (j > win.end) | !(both >> e / 4 & 1);
+                        x[e] = out ? -INFINITY : x[e];
                     }
                 }
                 s.take(stage, lane, any, nan, x);
+            };
+#pragma unroll 1
+            for (int i = 0; i < mine; i += 2) {
+                step(i, tk[0], held[0]);
+                if (i + 1 < mine) step(i + 1, tk[1], held[1]);
             }
             s.end(ml + wv * stride + row16, accs + (wv * stride + row16) * D, kg, row16 < cols, mine > 0);
         }
 
         // ---- landmarks, whole steps of one item each
-        for (int b = 0; b < total; b += kSlots) {
+        for (int b = 0; b < total; b += a.slots) {
             if (b > 0) {
                 look_marks(b);
                 place_marks(b);
             }
             const int lane = fresh(threadIdx.x) & 63, row16 = lane & 15, kg = lane >> 4;
-            auto load = [&](int i) {
+            auto load = [&](int i, typename S::Tokens& t) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t key = keys[i * kStep + half * 16 + row16];
-                    tk.key[half] = tk.value[half] = typename S::kword{};
-                    tk.key_scale[half] = tk.value_scale[half] = 127u;
-                    if (key != kNone) S::load(p.c.kv + (uint64_t)key * D, p.c.scale + (uint64_t)key * (D / 16), kg, half, tk);
+                    t.key[half] = t.value[half] = typename S::kword{};
+                    t.key_scale[half] = t.value_scale[half] = 127u;
+                    if (key != kNone) S::load(p.c.kv + (uint64_t)key * D, p.c.scale + (uint64_t)key * (D / 16), kg, half, t);
                 }
             };
-            const int n_steps = min(kSlots, total - b) / kStep;
-            load(0);
-#pragma unroll 1
-            for (int i = 0; i < n_steps; ++i) {
+            const int n_steps = min(a.slots, total - b) / kStep;
+            auto step = [&](int i, typename S::Tokens& t) {
                 const int f = b + i * kStep, o = f & ((1 << a.kr_log) - 1), it = wv + (f >> a.kr_log) * kWaves, hh = it >> a.chunk_log;
                 if (o == 0) s.begin(qs + (lrow * nh + hh) * QS, kg);
                 float x[8];
                 unsigned long long nan[2];
-                s.scores(tk, x);
-                const bool any = S::stage_values(stage, row16, kg, tk, nan);
-                if (i + 1 < n_steps) load(i + 1);
+                s.scores(t, x);
+                const bool any = S::stage_values(stage, row16, kg, t, nan);
+                if (i + 2 < n_steps) load(i + 2, t);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int q0 = i * kStep + half * 16 + 4 * kg;
@@ -434,7 +437,7 @@ __global__ __launch_bounds__(64 * kWaves, (MinWaves<T, D>::value)) void cache4_a
                     if (p.lbias) bias = *(const floatx4*)(biases + q0);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const bool on = key[e] != kNone && (n == 1 || (int)place[e] < mark_low);
+                        const bool on = (key[e] != kNone) & ((n == 1) | ((int)place[e] < mark_low));
                         x[4 * half + e] = on ? x[4 * half + e] * scale2 + bias[e] : -INFINITY;
                     }
                 }
@@ -443,9 +446,16 @@ __global__ __launch_bounds__(64 * kWaves, (MinWaves<T, D>::value)) void cache4_a
                     const int part = kWaves + it - (hh << a.chunk_log), slot = part * stride + row16 * nh + hh;
                     s.end(ml + slot, accs + (int64_t)slot * D, kg, row16 < n, true);
                 }
+            };
+            load(0, tk[0]);
+            if (n_steps > 1) load(1, tk[1]);
+#pragma unroll 1
+            for (int i = 0; i < n_steps; i += 2) {
+                step(i, tk[0]);
+                if (i + 1 < n_steps) step(i + 1, tk[1]);
             }
         }
-        join_columns<T, D, 64 * kWaves>(p, a, ml, accs, parts, stride, cols, t0, h0, h1, split);
+        join_columns<T, D>(p, a, ml, accs, parts, stride, cols, t0, h0, h1, split);
         __syncthreads();
     }
 }
@@ -456,26 +466,29 @@ AttnPlan attn_plan(const Cache4AttnParams& p) {
     const int64_t cap = (int64_t)p.cols << p.c.bt_log;
     const int64_t w = p.w_max > 0 && p.w_max < cap ? p.w_max : cap;
     const int64_t rows = std::max(p.n_rows, 1);  // (the workspace of a call without rows is asked for too)
-    a.nh = std::min(group, 16);
-    a.nr = std::min(p.per, 16 / a.nh);
-    a.run_tiles = ceil_div(p.per, a.nr);
+    a.run_tiles = ceil_div(p.per, 16);
+    a.nr = ceil_div(p.per, a.run_tiles);
+    a.nh = ceil_div(group, ceil_div(group, 16 / a.nr));
     const int64_t groups = (rows + p.per - 1) / p.per * a.run_tiles * p.c.n_kv;
-    if (w <= 1024)
-    while (a.nh > 1 && groups * ceil_div(group, a.nh) < 256) a.nh = ceil_div(a.nh, 2);
-    if (const char* e = getenv("C4_NH")) a.nh = std::min(group, atoi(e));
+    auto blocks = [&] { return groups * ceil_div(group, a.nh); };
+    auto splits = [&](int64_t most) { return std::max(std::min(most / blocks(), w / 256), (int64_t)1); };
+    if (w <= 1024) {
+        while (a.nh > 1 && blocks() <= 256 && (a.nh > 2 || blocks() < 256)) a.nh = ceil_div(a.nh, 2);
+        a.ns = w > 512 ? (int)splits(256) : 1;
+    } else {
+        while (a.nh > 4 && blocks() * splits(512) <= 128) a.nh = ceil_div(a.nh, 2);
+        a.ns = (int)splits(512);
+    }
     a.tiles = ceil_div(group, a.nh);
-    const int64_t blocks = groups * a.tiles;
-    a.waves = 4;
-    a.ns = (int)std::max(std::min(512 / blocks, w / 1024), (int64_t)1);
-    if (const char* e = getenv("C4_WAVES")) a.waves = atoi(e);
-    if (const char* e = getenv("C4_NS")) a.ns = atoi(e);
-    a.nl = p.k_lmk == 0 ? 0 : std::min(ceil_div(p.k_lmk, 64), a.ns);
+    a.nl = p.k_lmk == 0 ? 0 : std::min(ceil_div(p.k_lmk, 32), a.ns);
     a.chunk_log = p.k_lmk == 0 ? -1 : 0;
     if (p.k_lmk > 0)  // (no more parts than leave room for two blocks in a compute unit's LDS)
-        while ((2 << a.chunk_log) * a.nh <= a.waves && (a.waves + (2 << a.chunk_log)) * a.nr * a.nh * p.c.head_dim * 4 <= 1 << 16) ++a.chunk_log;
+        while ((2 << a.chunk_log) * a.nh <= kWaves && (kWaves + (2 << a.chunk_log)) * a.nr * a.nh * p.c.head_dim * 4 <= 1 << 15) ++a.chunk_log;
     a.kc = p.k_lmk == 0 ? 0 : ceil_div(ceil_div(p.k_lmk, a.nl), a.chunks());
     a.kr_log = 5;
     while (1 << a.kr_log < a.kc) ++a.kr_log;
+    a.slots = p.k_lmk == 0 ? 0 : std::min((ceil_div(a.nh << a.chunk_log, kWaves) << a.kr_log) + 63 & ~63, 64 * kLook);
+    a.fields = 1 + (a.nr > 1) + (p.lbias != nullptr);
     a.col_mul = ceil_div(1 << 16, a.nh);
     return a;
 }
@@ -485,10 +498,10 @@ hipError_t run_rows(const Cache4AttnParams& p, const AttnPlan& a, hipStream_t st
     const int64_t runs = ((int64_t)p.n_rows + p.per - 1) / p.per;
     const dim3 grid((unsigned)(runs * a.run_tiles), (unsigned)(p.c.n_kv * a.tiles), (unsigned)a.ns);
     const unsigned lds = (unsigned)Layout<T, D>(a).bytes();
-    auto kernel = a.waves == 8 ? cache4_attn_kernel<T, D, 8> : cache4_attn_kernel<T, D, 4>;
+    auto kernel = cache4_attn_kernel<T, D>;
     if (lds > 65536)
         if (hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)) return e;
-    DSALT_LAUNCH("cache4_attn", kernel, grid, dim3(64 * a.waves), lds, stream, p, a);
+    DSALT_LAUNCH("cache4_attn", kernel, grid, dim3(64 * kWaves), lds, stream, p, a);
     if (a.ns > 1) {
         const dim3 join((unsigned)((int64_t)p.n_rows * p.n_heads));
         DSALT_LAUNCH("cache4_attn_join", (cache_attn_join_kernel<T, D, Cache4AttnParams>), join, dim3(64 * kJoinWaves), 0, stream, p, a.ns);
