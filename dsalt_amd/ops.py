@@ -14,6 +14,7 @@ import torch
 from torch.autograd import forward_ad
 
 from . import _lib
+from ._lib import Cache4 as Cache4Struct
 from ._lib import (DTYPE_BF16, DTYPE_F16, DTYPE_F32, SELECT_BLOCK, SELECT_GLOBAL, STATS_PACKED,
                    STATS_SEQUENCE, VARIANT_DEFAULT, VARIANT_DQ_BN64, VARIANT_FWD_BN32, VARIANT_FWD_RG2,
                    VARIANT_LMK_SHORT, BwdArgs, Cache, Cache4AttnArgs, Cache4ReadArgs, Cache4WriteArgs, CacheAttnArgs,
@@ -521,55 +522,61 @@ def rope_qk_(q, k, cu_seqlens, cos, sin, *, max_seqlen=None):
     return q, k
 
 
-def _vec16(t: torch.Tensor, n: int, name: str) -> torch.Tensor:
-    """``t`` [n] contiguous and on a 16-byte boundary."""
-    if t.dim() != 1 or t.shape[0] != n:
-        raise ValueError(f"{name} must be [{n}], got shape {tuple(t.shape)}")
-    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+def _qk_side(t, w, name: str, shape, dtype):
+    """(tensor or a copy, its (address, strides), weight, its address) of one side of qk_norm_rope."""
+    if t is None:
+        return None, (None, 0, 0), None, None
+    t, where = _rows16(t, name)
+    if t.shape[0] != shape[0] or t.shape[2] != shape[2] or t.dtype is not dtype:
+        raise ValueError(f"q and k must share T, D and dtype, got {name} {tuple(t.shape)} {t.dtype} beside {tuple(shape)} {dtype}")
+    if w is None or w.shape != shape[2:]:
+        raise ValueError(f"{name}_weight must be [{shape[2]}], got {w if w is None else tuple(w.shape)}")
+    at = w.data_ptr()
+    if at % 16 or not w.is_contiguous():
+        w = w.detach().clone(memory_format=torch.contiguous_format)
+        at = w.data_ptr()
+    return t, where, w, at
 
 
-def _qk_args(q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, max_seqlen, eps, more=()):
-    """(device index, arguments without the outputs, tensors to keep alive, checked q and k) of qk_norm_rope."""
-    if q is None and k is None:
-        raise ValueError("q or k is required")
-    at = _on(*(t for t in (q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, *more) if t is not None))
+def _qk_args(q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, max_seqlen, eps, *more):
+    """(device index, the sides (see _qk_side), first and last arguments of QkNormRopeArgs, tensors to keep alive)."""
     ref = q if q is not None else k
-    rows = []
-    for t, w, n in ((q, q_weight, "q"), (k, k_weight, "k")):
-        if t is None:
-            rows.append((None, (None, 0, 0), None))
-            continue
-        t, where = _rows16(t, n)
-        if t.shape[0] != ref.shape[0] or t.shape[2] != ref.shape[2] or t.dtype != ref.dtype:
-            raise ValueError(f"q and k must share T, D and dtype, got {tuple(q.shape)} {q.dtype}, {tuple(k.shape)} {k.dtype}")
-        if w is None:
-            raise ValueError(f"{n}_weight is required")
-        rows.append((t, where, _vec16(w.detach(), ref.shape[2], n + "_weight")))
-    T, _, D = ref.shape
-    if q is not None and k is not None and q_weight.dtype != k_weight.dtype:
-        raise TypeError(f"q_weight and k_weight must share a dtype, got {q_weight.dtype}, {k_weight.dtype}")
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != D:
+    if ref is None:
+        raise ValueError("q or k is required")
+    at = _on(ref, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, *more)
+    shape = ref.shape
+    if len(shape) != 3:
+        raise ValueError(f"q and k must be [T, H, D], got shape {tuple(shape)}")
+    T, _, D = shape
+    sides = _qk_side(q, q_weight, "q", shape, ref.dtype), _qk_side(k, k_weight, "k", shape, ref.dtype)
+    wd = (q_weight if q is not None else k_weight).dtype
+    if q is not None and k is not None and k_weight.dtype is not wd:
+        raise TypeError(f"q_weight and k_weight must share a dtype, got {wd}, {k_weight.dtype}")
+    n_pos = cos.shape[0]
+    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.shape != sin.shape or cos.shape != (n_pos, D):
         raise ValueError(f"cos and sin must be float32 [max_pos, {D}], got {tuple(cos.shape)}, {tuple(sin.shape)}")
-    cos, sin = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (cos, sin))
+    ca, sa = cos.data_ptr(), sin.data_ptr()
+    if ca % 16 or sa % 16 or not cos.is_contiguous() or not sin.is_contiguous():
+        cos, sin = (t.clone(memory_format=torch.contiguous_format) for t in (cos, sin))
+        ca, sa = cos.data_ptr(), sin.data_ptr()
     if (cu_seqlens is None) == (pos is None):
         raise ValueError("either cu_seqlens or pos is required")
     S = 0
-    if cu_seqlens is not None:
-        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
-            raise ValueError("cu_seqlens must be [S+1] with S >= 1")
+    if pos is None:
         S = cu_seqlens.shape[0] - 1
+        if cu_seqlens.dim() != 1 or S < 1:
+            raise ValueError("cu_seqlens must be [S+1] with S >= 1")
         maxlen = max_seqlen if max_seqlen is not None else _max_seqlen(cu_seqlens)
-        if maxlen > cos.shape[0] and T:
-            raise ValueError(f"a sequence of {maxlen} rows passes the {cos.shape[0]} positions of cos and sin")
+        if maxlen > n_pos and T:
+            raise ValueError(f"a sequence of {maxlen} rows passes the {n_pos} positions of cos and sin")
         cu_seqlens = _i32(cu_seqlens)
+        where = (cu_seqlens.data_ptr(), None)
     else:
         pos = _vec_i32(_positions(pos), T, "pos")
-    (q, q_at, qw), (k, k_at, kw) = rows
-    a = QkNormRopeArgs(T, S, q.shape[1] if q is not None else 0, k.shape[1] if k is not None else 0, D, dtype_code(ref.dtype),
-                       dtype_code((qw if q is not None else kw).dtype), cos.shape[0], float(eps), *q_at, *k_at, None, 0, 0, None, 0, 0, qw.data_ptr() if qw is not None else None,
-                       kw.data_ptr() if kw is not None else None, cu_seqlens.data_ptr() if cu_seqlens is not None else None,
-                       pos.data_ptr() if pos is not None else None, cos.data_ptr(), sin.data_ptr())
-    return at, a, q, k, (qw, kw, cu_seqlens, pos, cos, sin)
+        where = (None, pos.data_ptr())
+    head = (T, S, q.shape[1] if q is not None else 0, k.shape[1] if k is not None else 0, D, dtype_code(ref.dtype), dtype_code(wd), n_pos,
+            float(eps))
+    return at, sides, head, (sides[0][3], sides[1][3], *where, ca, sa), (cu_seqlens, pos, cos, sin)
 
 
 def _positions(pos: torch.Tensor) -> torch.Tensor:
@@ -583,21 +590,22 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, cu_seqlens=None, pos=Non
     views are read in place), weights [D], cos/sin [max_pos, D] fp32.  A row's position is its place in its sequence of
     ``cu_seqlens``, or ``pos[t]`` (CacheRows.pos of a decoding step).  Rows in no sequence, or with a position
     outside the tables (inert rows), become zeros; with ``inplace``, which writes over q and k, they stay as they are."""
-    at, a, q_in, k_in, keep = _qk_args(q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, max_seqlen, eps)  # noqa: F841 (kept alive)
-    out = []
-    for n, t, given in (("q", q_in, q), ("k", k_in, k)):
+    at, sides, head, tail, keep = _qk_args(q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, max_seqlen, eps)  # noqa: F841 (kept alive)
+    out, at_out = [], []
+    for t, where, _, _ in sides:
         if t is None:
             out.append(None)
-            continue
-        if inplace and t is not given:
-            raise ValueError(f"{n} must have unit stride along D and rows on 16-byte boundaries to be written in place")
-        y = given if inplace else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        setattr(a, n + "_out", y.data_ptr())
-        st = (getattr(a, n + "_stride_t"), getattr(a, n + "_stride_h")) if inplace else (t.shape[1] * t.shape[2], t.shape[2])
-        setattr(a, n + "o_stride_t", st[0])
-        setattr(a, n + "o_stride_h", st[1])
-        out.append(y)
-    _call("dsalt_qk_norm_rope", a, at)
+            at_out.append(where)
+        elif inplace:
+            if t is not q and t is not k:
+                raise ValueError("q and k must have unit stride along D and rows on 16-byte boundaries to be written in place")
+            out.append(t)
+            at_out.append(where)
+        else:
+            y = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            out.append(y)
+            at_out.append((y.data_ptr(), t.shape[1] * t.shape[2], t.shape[2]))
+    _call("dsalt_qk_norm_rope", QkNormRopeArgs(*head, *sides[0][1], *sides[1][1], *at_out[0], *at_out[1], *tail), at)
     return tuple(out)
 
 
@@ -605,27 +613,29 @@ def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, *, cu_seql
     """Gradients (dq, dk, dq_weight, dk_weight) of qk_norm_rope from those of its outputs: the first two in the type of q and
     k (zeros in rows without a position), the weights' in float32, summed over rows and heads in an order that does not
     change from run to run."""
-    at, a, q, k, keep = _qk_args(q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, max_seqlen, eps, (dq, dk))  # noqa: F841 (kept alive)
-    b = QkNormRopeBwdArgs(a)
-    out, up = [], []
-    for n, t, d in (("q", q, dq), ("k", k, dk)):
+    at, sides, head, tail, keep = _qk_args(q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, max_seqlen, eps, dq, dk)  # noqa: F841 (kept alive)
+    out, grads, ups, at_out, at_up = [], [], [], [], []
+    for (t, where, _, _), d, n in zip(sides, (dq, dk), "qk"):
         if t is None:
-            out += [None, None]
+            out.append(None)
+            grads.append(None)
+            at_out.append(where)
+            at_up.append(where)
             continue
         if d is None or d.shape != t.shape:
             raise ValueError(f"d{n} must have the shape of {n}, {tuple(t.shape)}")
-        d, where = _rows16(d.to(t.dtype), "d" + n)
-        up.append(d)
-        for f, x in zip(("d" + n, f"d{n}_stride_t", f"d{n}_stride_h"), where):
-            setattr(b, f, x)
-        y, w = torch.empty(t.shape, dtype=t.dtype, device=t.device), torch.empty(t.shape[2], dtype=torch.float32, device=t.device)
-        for f, x in ((n + "_out", y.data_ptr()), (n + "o_stride_t", t.shape[1] * t.shape[2]), (n + "o_stride_h", t.shape[2])):
-            setattr(b.base, f, x)
-        setattr(b, f"d{n}_weight", w.data_ptr())
-        out += [y, w]
+        d, d_at = _rows16(d.to(t.dtype), "d" + n)
+        y = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        out.append(y)
+        grads.append(torch.empty(t.shape[2], dtype=torch.float32, device=t.device))
+        ups.append(d)
+        at_out.append((y.data_ptr(), t.shape[1] * t.shape[2], t.shape[2]))
+        at_up.append(d_at)
+    b = QkNormRopeBwdArgs(QkNormRopeArgs(*head, *sides[0][1], *sides[1][1], *at_out[0], *at_out[1], *tail), *at_up[0], *at_up[1],
+                          *(g.data_ptr() if g is not None else None for g in grads))
     ws = _set_workspace(b, _lib.load().dsalt_qk_norm_rope_bwd_workspace_bytes(ctypes.byref(b)), at)  # noqa: F841 (kept alive)
     _call("dsalt_qk_norm_rope_bwd", b, at)
-    return out[0], out[2], out[1], out[3]
+    return (*out, *grads)
 
 
 def export_probs(q, k, w, cu_seqlens, lmk_idx, lse, lmk_bias=None, *, seq=0, rows=None, w_cap=None, scale=None,
@@ -909,12 +919,13 @@ def _on(*ts) -> int:
 def _cache_args(c):
     if isinstance(c, Cache4):
         kv, sc = c
-        if kv.dim() != 5 or kv.shape[3] != 2 or kv.dtype != torch.uint8 or not kv.is_contiguous():
+        shape = kv.shape
+        if len(shape) != 5 or shape[3] != 2 or kv.dtype is not torch.uint8 or not kv.is_contiguous():
             raise ValueError("the cache's kv must be contiguous uint8 [n_blocks, n_kv, block_tokens, 2, D/2]")
-        D = 2 * kv.shape[4]
-        if sc.shape != (*kv.shape[:4], D // 32) or sc.dtype != torch.uint8 or not sc.is_contiguous():
+        n, g, bt, _, half = shape
+        if sc.shape != (n, g, bt, 2, half // 16) or sc.dtype is not torch.uint8 or not sc.is_contiguous():
             raise ValueError("the cache's scale must be contiguous uint8 [n_blocks, n_kv, block_tokens, 2, D/32]")
-        return _lib.Cache4(*kv.shape[:3], D, kv.data_ptr(), sc.data_ptr())
+        return Cache4Struct(n, g, bt, 2 * half, kv.data_ptr(), sc.data_ptr())
     k, v, ks, vs = c
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or k.dtype != _E4M3 or v.dtype != _E4M3 or not k.is_contiguous() \
