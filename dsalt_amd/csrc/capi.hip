@@ -887,7 +887,7 @@ int dsalt_qk_norm_rope(const dsalt_qk_norm_rope_args* a, dsalt_stream_t stream) 
 
 size_t dsalt_qk_norm_rope_bwd_workspace_bytes(const dsalt_qk_norm_rope_bwd_args* a) {
     return check_qk(a ? &a->base : nullptr)
-               ? 0 : dsalt::qk_norm_rope_bwd_ws_bytes(a->base.total_len, a->base.n_q_heads + a->base.n_k_heads, a->base.head_dim);
+               ? 0 : dsalt::qk_norm_rope_bwd_ws_bytes(a->base.total_len, a->base.n_q_heads, a->base.n_k_heads, a->base.head_dim, a->base.dtype);
 }
 
 int dsalt_qk_norm_rope_bwd(const dsalt_qk_norm_rope_bwd_args* a, dsalt_stream_t stream) {
@@ -901,7 +901,7 @@ int dsalt_qk_norm_rope_bwd(const dsalt_qk_norm_rope_bwd_args* a, dsalt_stream_t 
     }
     if ((b->n_q_heads && !a->dq_weight) || (b->n_k_heads && !a->dk_weight))
         return fail(DSALT_ERR_INVALID, "dq_weight and dk_weight are required");
-    const size_t need = dsalt::qk_norm_rope_bwd_ws_bytes(b->total_len, b->n_q_heads + b->n_k_heads, b->head_dim);
+    const size_t need = dsalt::qk_norm_rope_bwd_ws_bytes(b->total_len, b->n_q_heads, b->n_k_heads, b->head_dim, b->dtype);
     if (need && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need))
         return fail(DSALT_ERR_WORKSPACE, "workspace of %zu bytes required", need);
     dsalt::QkNormParams p = qk_params(b);

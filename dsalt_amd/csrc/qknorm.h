@@ -30,7 +30,7 @@ struct QkNormParams {
 };
 
 hipError_t qk_norm_rope_launch(const QkNormParams& p, hipStream_t stream);
-size_t qk_norm_rope_bwd_ws_bytes(int total_len, int heads, int head_dim);
+size_t qk_norm_rope_bwd_ws_bytes(int total_len, int q_heads, int k_heads, int head_dim, int dtype);
 hipError_t qk_norm_rope_bwd_launch(const QkNormParams& p, hipStream_t stream);
 
 }  // namespace dsalt
