@@ -5,7 +5,17 @@
 // step takes 32 keys: their codes become bfloat16 operands with the scales taken in (exact), and both products run on the
 // matrix cores, with up to 16 columns of queries.  Columns of a window are the query heads that share a key/value head, of
 // one row or of rows of one request side by side (drafted tokens); columns of a head's landmarks, which are its own, are those rows.
-// Scores, weights and sums are kept in 32 bits.
+// Scores, weights and sums are kept in 32 bits.  A key's share of a query is read once for the columns that share it: at 256
+// requests (16 query heads on 2, windows of 512, 128 landmarks a head) 93 MB, most of them landmarks, each head its own.
+//
+// A block has four waves, each with every fourth step of the window and then parts of the landmarks; their maxima, sums and
+// values meet in LDS (the windows' pairwise, which leaves room for a second block where there are sixteen columns of 128).  What
+// bounds it are dependent reads, not their volume: position, table, tokens and, for landmarks, position, table, token.  So the
+// tokens of a step are in registers two steps ahead, a wave's landmarks are looked up while its window is read, and numbers of
+// the whole wave (step, page, head) stay in scalar registers.  Values pass through LDS as bfloat16 rows, from where the matrix
+// operand is read transposed.  Two blocks a compute unit (256 registers a lane): three would spill, 45 us for the 33 us of the
+// 256 requests; eight waves a block 42 us.  One request (windows of 512): 11.8 us; 64 requests of five rows in float16, 16 heads of
+// 64 on 4: 18.5 us; four requests with windows of 131072: 40 us, 143 MB at 3.6 TB/s, 4 us of it the join of the splits.
 #include <algorithm>
 
 #include "cache4.h"
@@ -21,6 +31,7 @@ namespace {
 
 constexpr int kStep = 32;  // keys of a step
 constexpr int kWaves = 4;  // of a block
+constexpr int kParts = 2;  // that their windows are left in: waves kParts and up first, the others join theirs
 constexpr uint32_t kNone = 0xffffffffu;
 
 struct AttnPlan {
@@ -144,6 +155,17 @@ struct Step {  // one wave's running maximum, sum and weighted values of 16 colu
             for (int i = 0; i < PP; ++i) acc[j] = mma(vf, pf[i], acc[j]);
         }
     }
+    // a part that `end` left, taken in
+    __device__ __forceinline__ void join(const float2* ml, const float* out, int kg) {
+        const float2 o = *ml;
+        if (o.y == 0.f) return;  // (it attended nothing and left no values)
+        const float m1 = fmaxf(m, o.x), mb = m1 == -INFINITY ? 0.f : m1;
+        const float f = m == -INFINITY ? 1.f : exp2_(m - mb), fo = o.x == -INFINITY ? 1.f : exp2_(o.x - mb);
+        m = m1;
+        l = l * f + (kg == 0 ? o.y * fo : 0.f);
+#pragma unroll
+        for (int j = 0; j < JN; ++j) acc[j] = acc[j] * f + *(const floatx4*)(out + 16 * j + 4 * kg) * fo;
+    }
     // the wave's part of column row16: (maximum, sum) and, where it took any keys, the weighted values [D]
     __device__ __forceinline__ void end(float2* ml, float* out, int kg, bool column, bool any) {
         const float sum = sum_g4(l);
@@ -216,7 +238,7 @@ template <typename T, int D>
 struct Layout {
     static constexpr int QS = D + 16 / (int)sizeof(T);  // a query's elements and what keeps rows apart in the banks
     int parts, stride, wave_slots;
-    __host__ __device__ Layout(const AttnPlan& a) : parts(kWaves + a.chunks()), stride(a.nr * a.nh), wave_slots(a.slots * a.fields) {}
+    __host__ __device__ Layout(const AttnPlan& a) : parts(kParts + a.chunks()), stride(a.nr * a.nh), wave_slots(a.slots * a.fields) {}
     __host__ __device__ int ml() const { return 0; }
     __host__ __device__ int q() const { return (2 * (parts + 1) * stride + 3) / 4 * 16; }
     __host__ __device__ int slots() const { return q() + stride * QS * (int)sizeof(T); }
@@ -239,7 +261,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache4_attn_kernel(Cache4AttnP
     const int g = a.tiles == 1 ? blockIdx.y : blockIdx.y / a.tiles, hx = blockIdx.y - g * a.tiles;
     const int h0 = g * group + hx * a.nh, h1 = min(h0 + a.nh, (g + 1) * group), nh = a.nh;
     const bool marks = split < a.nl;
-    const int parts = kWaves + (marks ? a.chunks() : 0), stride = at.stride;
+    const int parts = kParts + (marks ? a.chunks() : 0), stride = at.stride;
     float2* ml = (float2*)(lds + at.ml());
     float* accs = (float*)(lds + at.accs());
     T* qs = (T*)(lds + at.q());
@@ -352,7 +374,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache4_attn_kernel(Cache4AttnP
                 *(u32x4*)(qs + c * QS + e * VEC) =
                     *(const u32x4*)((const T*)p.q + (int64_t)(t0 + row) * p.q_st + (int64_t)h * p.q_sh + e * VEC);
             }
-            for (int i = tid; i < (parts - kWaves) * stride; i += 64 * kWaves) ml[kWaves * stride + i] = make_float2(-INFINITY, 0.f);
+            for (int i = tid; i < (parts - kParts) * stride; i += 64 * kWaves) ml[kParts * stride + i] = make_float2(-INFINITY, 0.f);
         }
         // Tokens of a step, requested two steps ahead: memory answers later than one step takes.
         typename S::Tokens tk[2];
@@ -399,7 +421,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache4_attn_kernel(Cache4AttnP
                 step(i, tk[0], held[0]);
                 if (i + 1 < mine) step(i + 1, tk[1], held[1]);
             }
-            s.end(ml + wv * stride + row16, accs + (wv * stride + row16) * D, kg, row16 < cols, mine > 0);
+            // (a wave has steps wherever a later one has)
+            const int slot = (wv & (kParts - 1)) * stride + row16;
+            if (wv >= kParts) s.end(ml + slot, accs + slot * D, kg, row16 < cols, mine > 0);
+            __syncthreads();
+            if (wv < kParts) {
+                if (row16 < cols) s.join(ml + slot, accs + slot * D, kg);
+                s.end(ml + slot, accs + slot * D, kg, row16 < cols, mine > 0);
+            }
         }
 
         // ---- landmarks, whole steps of one item each
@@ -443,7 +472,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache4_attn_kernel(Cache4AttnP
                 }
                 s.take(stage, lane, any, nan, x);
                 if (o + kStep == 1 << a.kr_log) {
-                    const int part = kWaves + it - (hh << a.chunk_log), slot = part * stride + row16 * nh + hh;
+                    const int part = kParts + it - (hh << a.chunk_log), slot = part * stride + row16 * nh + hh;
                     s.end(ml + slot, accs + (int64_t)slot * D, kg, row16 < n, true);
                 }
             };
@@ -460,6 +489,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache4_attn_kernel(Cache4AttnP
     }
 }
 
+// How a launch is cut.  The most columns that fit share each key; where that leaves compute units without work, heads go to blocks
+// of their own (their landmarks are their own anyhow, and the window's keys are then read from the caches) and long windows to splits.
+// Measured, bfloat16, 16 query heads of 128 on 2 with 128 landmarks, us by heads of a block:
+//   windows of 512, one row a request: 256 requests 8 heads 33, 4 43; 128: 8 27, 4 24; 64: 8 26, 4 19.5, 2 19.3; 32: 4 18.3, 2 15.4,
+//     1 17.6; 8: 2 14.3, 1 13.6; 1: 8 22, 1 11; five rows a request: 256 requests 3 heads 76, 2 82; 64: 3 28, 2 24; 16: 3 22, 2 18,
+//     1 16.4.  So heads are halved while that leaves no more than 512 blocks, two a compute unit, which the card holds at once, and to
+//     single heads from fewer than 256.
+//   sixteen rows of 64 requests, 16 heads of 128: all in a block 51, eight 76, four 128.
+//   one request, windows of 4096: 4 heads in 16 splits 16.4, single heads without splits 39.8; 16 requests, 16384: 8 heads in
+//     16 splits 32.4; 4 requests, 131072: 48 splits 47, 64 42 (40 since), 96 54, 128 52.  So long windows are split until
+//     there are 512 blocks, 256 keys to a split at least, and heads halved only where that is not enough.
 AttnPlan attn_plan(const Cache4AttnParams& p) {
     AttnPlan a;
     const int group = p.n_heads / p.c.n_kv;
@@ -470,10 +510,11 @@ AttnPlan attn_plan(const Cache4AttnParams& p) {
     a.nr = ceil_div(p.per, a.run_tiles);
     a.nh = ceil_div(group, ceil_div(group, 16 / a.nr));
     const int64_t groups = (rows + p.per - 1) / p.per * a.run_tiles * p.c.n_kv;
-    auto blocks = [&] { return groups * ceil_div(group, a.nh); };
+    auto blocks_of = [&](int nh) { return groups * ceil_div(group, nh); };
+    auto blocks = [&] { return blocks_of(a.nh); };
     auto splits = [&](int64_t most) { return std::max(std::min(most / blocks(), w / 256), (int64_t)1); };
     if (w <= 1024) {
-        while (a.nh > 1 && blocks() <= 256 && (a.nh > 2 || blocks() < 256)) a.nh = ceil_div(a.nh, 2);
+        while (a.nh > 1 && blocks_of(ceil_div(a.nh, 2)) <= 512 && (a.nh > 2 || blocks() < 256)) a.nh = ceil_div(a.nh, 2);
         a.ns = w > 512 ? (int)splits(256) : 1;
     } else {
         while (a.nh > 4 && blocks() * splits(512) <= 128) a.nh = ceil_div(a.nh, 2);
@@ -482,8 +523,9 @@ AttnPlan attn_plan(const Cache4AttnParams& p) {
     a.tiles = ceil_div(group, a.nh);
     a.nl = p.k_lmk == 0 ? 0 : std::min(ceil_div(p.k_lmk, 32), a.ns);
     a.chunk_log = p.k_lmk == 0 ? -1 : 0;
-    if (p.k_lmk > 0)  // (no more parts than leave room for two blocks in a compute unit's LDS)
-        while ((2 << a.chunk_log) * a.nh <= kWaves && (kWaves + (2 << a.chunk_log)) * a.nr * a.nh * p.c.head_dim * 4 <= 1 << 15) ++a.chunk_log;
+    if (p.k_lmk > 0)  // (no more parts than leave room for two blocks in a compute unit's LDS: sixteen columns of 128 with four 51 us,
+                      // three 53, a block alone 88)
+        while ((2 << a.chunk_log) * a.nh <= kWaves && (kParts + (2 << a.chunk_log)) * a.nr * a.nh * p.c.head_dim * 4 <= 1 << 15) ++a.chunk_log;
     a.kc = p.k_lmk == 0 ? 0 : ceil_div(ceil_div(p.k_lmk, a.nl), a.chunks());
     a.kr_log = 5;
     while (1 << a.kr_log < a.kc) ++a.kr_log;
@@ -512,7 +554,7 @@ hipError_t run_rows(const Cache4AttnParams& p, const AttnPlan& a, hipStream_t st
 template <typename T, int D>
 hipError_t run(const Cache4AttnParams& p, hipStream_t stream) {
     const AttnPlan a = attn_plan(p);
-    // runs of rows of a launch (more than one launch: blocks of four waves, no splits)
+    // runs of rows of a launch (where there is more than one launch, rows are not split)
     const int64_t most = std::max(kLaunchThreads / 256 / a.run_tiles, (int64_t)1) * p.per;
     Cache4AttnParams s = p;
     for (int64_t t = 0; t < p.n_rows; t += s.n_rows) {

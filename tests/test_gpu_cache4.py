@@ -264,9 +264,11 @@ RULES = {
     "split, heads of a group": (1, 8, 2, 64, 16, 9, [4500], 4500, 4500, 1),
     "split, most splits empty": (3, 8, 2, 64, 16, 130, [300, 33, 1], 290, 1 << 15, 1),
     "split, rows of a request": (2, 8, 2, 128, 64, 200, [2500, 40], 2400, 1 << 13, 3),
-    "eight waves, groups": (110, 8, 2, 64, 64, 17, 90, 60, 300, 1),
-    "four waves": (280, 8, 2, 128, 32, 33, 90, 60, 300, 1),
-    "four waves, rows of a request": (150, 4, 2, 64, 32, 33, 90, 60, 300, 4),
+    "many requests, heads of a group apart": (110, 8, 2, 64, 64, 17, 90, 60, 300, 1),
+    "many requests": (280, 8, 2, 128, 32, 33, 90, 60, 300, 1),
+    "many requests, rows of a request": (150, 4, 2, 64, 32, 33, 90, 60, 300, 4),
+    "five rows, heads in threes": (130, 8, 1, 64, 16, 9, 60, 40, 150, 5),
+    "five rows, heads in pairs": (70, 8, 1, 128, 16, 9, 60, 40, 150, 5),
     "groups of 17 heads": (140, 34, 2, 64, 16, 5, 70, 40, 150, 1),
     "groups of 16 heads of 128": (80, 32, 2, 128, 64, 6, 150, 100, 256, 2),
 }
