@@ -26,12 +26,9 @@ __device__ __forceinline__ uint32_t max_of4(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, false));  // 2, 3, 0, 1
 }
 
-constexpr int kParts = 4;  // blocks to a piece
-
 // ---------------------------------------------------------------------- write
-// Four blocks take a piece (rows of one request within one page: one, or up to a page of them; both kernels at the 16001 rows with one
-// block to a piece 37.9 us, four 34.9, sixteen 33.7; a block of one wave 66.7; at pieces of single rows all the same); a thread eight
-// elements of a row and head, four threads the 32 of a scale.  Magnitudes are compared as the integers of their bits, in
+// gridDim.y blocks take a piece (rows of one request within one page); a thread eight elements of a row and head, four threads the
+// 32 of a scale.  Magnitudes are compared as the integers of their bits, in
 // which everything not finite lies at the infinity or above.
 template <typename T>
 __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4WriteParams p) {
@@ -42,7 +39,7 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(Cache4WriteParams p) 
     if (rows <= 0 || row0 < 0 || rows > p.n_rows - row0 || page < 0 || page >= p.c.n_blocks || off < 0 || rows > bt - off) return;
     const int heads = 2 * G;  // keys, then values
     const int n = (rows * heads) << per_log;
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < n; i += kParts * 256) {
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < n; i += gridDim.y * 256) {
         const int c = i & ((1 << per_log) - 1), rh = i >> per_log, r = rh / heads, h = rh - r * heads;
         const int val = h >= G, g = h - val * G;
         const T* x = val ? (const T*)p.v + (int64_t)(row0 + r) * p.v_st + (int64_t)g * p.v_sh
@@ -102,13 +99,18 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(Cache4ReadParams p) {
     }
 }
 
+// As many blocks to a piece as give each thread eight elements of an average piece, up to sixteen.  (Write and read of the 16001
+// rows with one block to a piece 37.9 us, four 34.9, sixteen 33.7; pieces of single rows, which have work for one, take 6.1 with
+// any number.)
 template <typename T>
 void write_pieces(const Cache4WriteParams& p, hipStream_t stream) {
+    const int64_t threads = (int64_t)p.n_rows * 2 * p.c.n_kv * (p.c.head_dim / 8) / p.n_pieces;
+    const unsigned parts = (unsigned)std::max(std::min((threads + 255) / 256, (int64_t)16), (int64_t)1);
     Cache4WriteParams s = p;
     for (int64_t k = 0; k < p.n_pieces; k += s.n_pieces) {
         s.n_pieces = (int)std::min(p.n_pieces - k, kLaunchThreads / 256);
         s.pieces = p.pieces + 4 * k;
-        DSALT_LAUNCH("cache4_write", cache4_write_kernel<T>, dim3((unsigned)s.n_pieces, kParts), dim3(256), 0, stream, s);
+        DSALT_LAUNCH("cache4_write", cache4_write_kernel<T>, dim3((unsigned)s.n_pieces, parts), dim3(256), 0, stream, s);
     }
 }
 
