@@ -295,6 +295,8 @@ __global__ __launch_bounds__(kThreads) void verify_top_kernel(VerifyParams p, Ve
     }
 }
 
+constexpr int64_t kMostParts = 64;
+
 // largest logit and sum of a row from its parts, a lane each (all lanes of a wave take part and get them)
 __device__ __forceinline__ u64 row_top(const Work& w, const VerifyPlan& a, int t, int side) {
     const int lane = threadIdx.x & 63;
@@ -659,8 +661,8 @@ VerifyPlan verify_plan(const VerifyParams& p) {
     const int reqs = std::max(p.n_reqs, 1);
     VerifyPlan a;
     a.chunks = (int)((vecs + 63) / 64);
-    const int64_t parts = std::min({1024 / rows, vecs / 512, (int64_t)64}), spread = std::min((int64_t)(512 / reqs), (int64_t)(a.chunks + kWaves - 1) / kWaves);
-    const int64_t by_value = std::max(1280 / rows, (int64_t)1), pick_by_value = std::max(256 / reqs, 1);
+    const int64_t parts = std::min({1024 / rows, vecs / 512, kMostParts}), spread = std::min((int64_t)(512 / reqs), (int64_t)(a.chunks + kWaves - 1) / kWaves);
+    const int64_t by_value = std::clamp(1280 / rows, (int64_t)1, kMostParts), pick_by_value = std::max(256 / reqs, 1);
     a.sum_table = p.dtype == 1 && vecs / by_value >= 1500 && vecs / by_value < (1 << 17);
     a.pick_table = p.dtype == 1 && vecs / pick_by_value >= 1500;
     a.parts = (int)std::max(a.sum_table ? by_value : parts, (int64_t)1);

@@ -78,6 +78,17 @@ def test_one_row_split_over_many_blocks():
         _check(x, tok, cu, u, v, None, 0.9)
 
 
+@pytest.mark.parametrize("rows", [8, 15, 16, 20])
+def test_largest_vocabulary_in_few_rows(rows):
+    """Rows in as many parts as they are ever cut into, with most of the weight behind the first parts."""
+    V = 1 << 20
+    x, tok, cu, u, v, _ = _case([rows // 2, rows - rows // 2 - 1, 1], V, torch.bfloat16, rows)
+    x[:, V - V // 8:] += 4
+    tok[1] = V - 3
+    _check(x, tok, cu, u * 1e-7, v, None)
+    _check(x, tok, cu, u, torch.full_like(v, 0.03), None)
+
+
 def test_infinities_nan_and_empty_rows():
     V = 40
     x, tok, cu, u, v, y = _case([2] * 10, V, torch.float32, 3)
