@@ -663,8 +663,9 @@ VerifyPlan verify_plan(const VerifyParams& p) {
     a.chunks = (int)((vecs + 63) / 64);
     const int64_t parts = std::min({1024 / rows, vecs / 512, kMostParts}), spread = std::min((int64_t)(512 / reqs), (int64_t)(a.chunks + kWaves - 1) / kWaves);
     const int64_t by_value = std::clamp(1280 / rows, (int64_t)1, kMostParts), pick_by_value = std::max(256 / reqs, 1);
-    a.sum_table = p.dtype == 1 && vecs / by_value >= 1500 && vecs / by_value < (1 << 17);
-    a.pick_table = p.dtype == 1 && vecs / pick_by_value >= 1500;
+    // (launches of at most 2^32 - 1 threads)
+    a.sum_table = p.dtype == 1 && vecs / by_value >= 1500 && vecs / by_value < (1 << 17) && rows < (1ll << 32) / kTableThreads;
+    a.pick_table = p.dtype == 1 && vecs / pick_by_value >= 1500 && reqs < (1ll << 32) / kPickThreads;
     a.parts = (int)std::max(a.sum_table ? by_value : parts, (int64_t)1);
     a.spread = (int)std::max(a.pick_table ? pick_by_value : spread, (int64_t)1);
     return a;

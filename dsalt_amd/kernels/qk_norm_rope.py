@@ -26,7 +26,8 @@ class QkNormRopeFunction(torch.autograd.Function):
     def backward(ctx, dq, dk):
         q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos = ctx.saved_tensors
         dq, dk, dqw, dkw = ops.qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, cu_seqlens=cu_seqlens, pos=pos, **ctx.at)
-        return dq, dk, dqw.to(q_weight.dtype), dkw.to(k_weight.dtype), None, None, None, None, None, None
+        dqw, dkw = (d if d is None else d.to(w.dtype) for d, w in ((dqw, q_weight), (dkw, k_weight)))
+        return dq, dk, dqw, dkw, None, None, None, None, None, None
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, cu_seqlens=None, pos=None, max_seqlen=None, eps=1e-6):

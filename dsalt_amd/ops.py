@@ -599,6 +599,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, cu_seqlens=None, pos=Non
         elif inplace:
             if t is not q and t is not k:
                 raise ValueError("q and k must have unit stride along D and rows on 16-byte boundaries to be written in place")
+            if where[2] < t.shape[2] or (t.shape[0] > 1 and where[1] < t.shape[2]):
+                raise ValueError("heads of q and k must not share elements to be written in place")
             out.append(t)
             at_out.append(where)
         else:

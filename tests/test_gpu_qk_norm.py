@@ -228,6 +228,40 @@ def test_autograd():
         torch.autograd.grad(g.sum(), y)
 
 
+def test_autograd_of_one_side():
+    """Queries or keys alone, forward and backward: the results that they have beside the others."""
+    T, H, G, D = 20, 4, 2, 64
+    x, w, tab, d = _case(T, H, G, D, torch.bfloat16, 12)
+    cu, t = torch.tensor([0, T], device=DEV), [a.to(DEV) for a in tab]
+
+    def run(q_on, k_on):
+        y = x.to(DEV).requires_grad_()
+        ws = [a.to(DEV).requires_grad_() for a in w]
+        q, k = qk_norm_rope(y[:, :H] if q_on else None, y[:, H:H + G] if k_on else None, ws[0] if q_on else None, ws[1] if k_on else None,
+                            *t, cu_seqlens=cu)
+        sum((o * g.to(DEV)).sum() for o, g in ((q, d[0]), (k, d[1])) if o is not None).backward()
+        return q, k, y.grad[:, :H], y.grad[:, H:H + G], *(a.grad for a in ws)
+
+    both = run(True, True)
+    q, none, gq, _, gw, nw = run(True, False)
+    assert none is None and nw is None and torch.equal(q, both[0]) and torch.equal(gq, both[2])
+    # (the weights' sums are cut by the heads that are there: up to T H products in another order, float32)
+    assert (gw - both[4]).abs().max() <= 2 * (T * H + D) * E * T * H * 8
+    none, k, _, gk, nw, gw = run(False, True)
+    assert none is None and nw is None and torch.equal(k, both[1]) and torch.equal(gk, both[3])
+
+
+def test_heads_that_share_elements_are_not_written():
+    x = torch.randn(6, 1, 64, device=DEV)
+    w, tab = torch.ones(64, device=DEV), [torch.ones(6, 64, device=DEV)] * 2
+    cu = torch.tensor([0, 6], device=DEV)
+    for q in (x.expand(6, 3, 64), x[:1].expand(6, 1, 64)):
+        with pytest.raises(ValueError):
+            ops.qk_norm_rope(q, None, w, None, *tab, cu_seqlens=cu, inplace=True)
+        assert torch.equal(ops.qk_norm_rope(q, None, w, None, *tab, cu_seqlens=cu)[0],
+                           ops.qk_norm_rope(q.contiguous(), None, w, None, *tab, cu_seqlens=cu)[0])
+
+
 @pytest.mark.parametrize("D", [64, 96])
 @pytest.mark.parametrize("mode", ["train", "eval with autograd", "inference"])
 def test_layer(monkeypatch, mode, D):
