@@ -13,9 +13,10 @@
 // bounds it are dependent reads, not their volume: position, table, tokens and, for landmarks, position, table, token.  So the
 // tokens of a step are in registers two steps ahead, a wave's landmarks are looked up while its window is read, and numbers of
 // the whole wave (step, page, head) stay in scalar registers.  Values pass through LDS as bfloat16 rows, from where the matrix
-// operand is read transposed.  Two blocks a compute unit (256 registers a lane): three would spill, 45 us for the 33 us of the
-// 256 requests; eight waves a block 42 us.  One request (windows of 512): 11.8 us; 64 requests of five rows in float16, 16 heads of
-// 64 on 4: 18.5 us; four requests with windows of 131072: 40 us, 143 MB at 3.6 TB/s, 4 us of it the join of the splits.
+// operand is read transposed.  Two blocks a compute unit (256 registers a lane): three would spill, 45 us for the 32 us of the
+// 256 requests; eight waves a block 42 us.  (The same landmarks for all heads, read from the caches, save 3 of 37 us there.)  One request
+// (windows of 512): 11.8 us; 64 requests of five rows in float16, 16 heads of 64 on 4: 18.3 us; four requests with windows of 131072: 39.6 us,
+// 143 MB at 3.6 TB/s, 4 us of it the join of the splits.
 #include <algorithm>
 
 #include "cache4.h"
@@ -45,6 +46,33 @@ struct AttnPlan {
     __host__ __device__ int chunks() const { return chunk_log < 0 ? 0 : 1 << chunk_log; }
 };
 
+// Eight floats as PARTS bfloat16 operands that sum to them: two parts leave up to 2^-16 of a float, three nothing.  All but the last
+// part are cut off rather than rounded, moves of bytes in place of conversions (a call 1 to 3 % shorter).
+template <int PARTS>
+__device__ __forceinline__ void cut8(const float* x, bf16x8* o) {
+    typedef bf16 pair __attribute__((ext_vector_type(2)));
+    typedef float floats __attribute__((ext_vector_type(2)));
+    float r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = x[e];
+#pragma unroll
+    for (int k = 0; k < PARTS; ++k) {
+        u32x4 u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (k + 1 < PARTS) {
+                const uint32_t a = __float_as_uint(r[2 * e]), b = __float_as_uint(r[2 * e + 1]);
+                u[e] = __builtin_amdgcn_perm(b, a, 0x07060302u);  // the upper halves
+                r[2 * e] -= __uint_as_float(a & 0xffff0000u);
+                r[2 * e + 1] -= __uint_as_float(b & 0xffff0000u);
+            } else {
+                u[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector((floats{r[2 * e], r[2 * e + 1]}), pair));
+            }
+        }
+        o[k] = __builtin_bit_cast(bf16x8, u);
+    }
+}
+
 template <typename T, int D>
 struct Step {  // one wave's running maximum, sum and weighted values of 16 columns
     static constexpr int QP = Parts<T>::q, PP = Parts<T>::p, KS = D / 32, JN = D / 16, DL = D / 4, KW = DL / 8;
@@ -66,7 +94,7 @@ struct Step {  // one wave's running maximum, sum and weighted values of 16 colu
         for (int s = 0; s < KS; ++s) {
             float x[8];
             load8(q + kg * DL + 8 * s, x);
-            split8<QP>(x, qf[s]);
+            cut8<QP>(x, qf[s]);
         }
 #pragma unroll
         for (int j = 0; j < JN; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -147,7 +175,7 @@ struct Step {  // one wave's running maximum, sum and weighted values of 16 colu
             l += x[e];
         }
         bf16x8 pf[PP];
-        split8<PP>(x, pf);
+        cut8<PP>(x, pf);
 #pragma unroll
         for (int j = 0; j < JN; ++j) {
             const bf16x8 vf = tr_op16(lds, VROW, 16 * j, 0, lane);
