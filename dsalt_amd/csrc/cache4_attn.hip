@@ -10,13 +10,14 @@
 //
 // A block has four waves, each with every fourth step of the window and then parts of the landmarks; their maxima, sums and
 // values meet in LDS (the windows' pairwise, which leaves room for a second block where there are sixteen columns of 128).  What
-// bounds it are dependent reads, not their volume: position, table, tokens and, for landmarks, position, table, token.  So the
-// tokens of a step are in registers two steps ahead, a wave's landmarks are looked up while its window is read, and numbers of
-// the whole wave (step, page, head) stay in scalar registers.  Values pass through LDS as bfloat16 rows, from where the matrix
-// operand is read transposed.  Two blocks a compute unit (256 registers a lane): three would spill, 45 us for the 32 us of the
-// 256 requests; eight waves a block 42 us.  (The same landmarks for all heads, read from the caches, save 3 of 37 us there.)  One request
-// (windows of 512): 11.8 us; 64 requests of five rows in float16, 16 heads of 64 on 4: 18.3 us; four requests with windows of 131072: 39.6 us,
-// 143 MB at 3.6 TB/s, 4 us of it the join of the splits.
+// bounds it is the chain of a step, codes to operands, product, maximum, exponents, product, half of whose cycles are vector
+// instructions, with two waves a SIMD to fill the rest (256 registers a lane; three would spill, 45 us for the 32 us of the 256
+// requests; eight waves a block 42 us).  The memory is not: landmarks read from the caches save 3 of 37 us there.  With few rows it is
+// dependent reads: position, table, tokens, and for landmarks position, table, token.  So the tokens of a step are in registers two
+// steps ahead, a wave's landmarks are looked up while its window is read, and numbers of the whole wave (step, page, head) stay in
+// scalar registers.  Values pass through LDS as bfloat16 rows, from where the matrix operand is read transposed.
+// One request (windows of 512): 11.8 us; 64 requests of five rows in float16, 16 heads of 64 on 4: 18.3 us; four requests with windows
+// of 131072: 39.6 us, 143 MB at 3.6 TB/s, 4 us of it the join of the splits.
 #include <algorithm>
 
 #include "cache4.h"
