@@ -307,7 +307,7 @@ QkPlan qk_plan(int total_len, int q_heads, int k_heads, int head_dim, int most) 
     return a;
 }
 
-int bwd_waves(int dtype) { return dtype == 0 ? 2048 : 3072; }
+int bwd_waves(int dtype) { return 256 * (dtype == 0 ? 8 : 12); }
 
 template <typename T, int LP>
 hipError_t run(const QkNormParams& p, const QkPlan& a, bool backward, hipStream_t stream) {
@@ -339,7 +339,7 @@ hipError_t run_type(const QkNormParams& p, const QkPlan& a, bool backward, hipSt
 
 hipError_t qk_norm_rope_launch(const QkNormParams& p, hipStream_t stream) {
     if (p.total_len == 0 || p.q.heads + p.k.heads == 0) return hipSuccess;
-    return run_type(p, qk_plan(p.total_len, p.q.heads, p.k.heads, p.head_dim, 4096), false, stream);
+    return run_type(p, qk_plan(p.total_len, p.q.heads, p.k.heads, p.head_dim, 256 * 16), false, stream);
 }
 
 size_t qk_norm_rope_bwd_ws_bytes(int total_len, int q_heads, int k_heads, int head_dim, int dtype) {
