@@ -8,7 +8,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// number of bfloat16 parts of a query element (exact: 8, 11 and 24 bits) and of a weight: 16 bits of it for
+// number of bfloat16 parts of a query element (exact: 8, 11 and 24 bits) and of a weight over the 8-bit cache: 16 bits of it for
 // 16-bit outputs, whose own rounding, half a step of 2^-8 or 2^-11 of a value, is far coarser, 24 for float32 (lists keep
 // weights in float32)
 template <typename T> struct Parts;

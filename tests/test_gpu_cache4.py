@@ -4,8 +4,8 @@ back, and a run of speculative steps.
 Tolerances, from the arithmetic.  Codes and scales are exact.  Attention: keys and values are exact in bfloat16, so that the
 errors are those of the sums and weights.  A weight's relative error is at most twice its logit's absolute error; a logit is a
 float32 dot product of D terms in any order and tree, (D + 8) 2^-24 of the largest sum |scale q k| of its row (``reach``); sums
-over n keys add n 2^-24, weights handed to the matrix products of 16-bit types in two bfloat16 parts 2^-16; the output is
-rounded once to its type, half a step being 2^-8 (bfloat16), 2^-11 (float16) or 2^-24.  Errors of weights act on sum p |v|
+over n keys add n 2^-24, weights of 16-bit types are granted 2^-16 (they are handed to the matrix products whole: see the test of
+weights in 32 bits, which grants none); the output is rounded once to its type, half a step being 2^-8 (bfloat16), 2^-11 (float16) or 2^-24.  Errors of weights act on sum p |v|
 (``mass``)."""
 from __future__ import annotations
 
@@ -719,3 +719,40 @@ def test_two_graphs_of_split_windows_replayed_in_turn():
         torch.cuda.synchronize()
         for x, y in zip(outs, ref):
             assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1]), rep
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("place", ["window", "landmarks"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_keeps_weights_in_32_bits(dt, place, D):
+    """Two keys of nearly equal weight whose values cancel, so that an output is a hundredth of its ``mass`` and shows what the
+    weights lose.  A logit is at most ``reach`` = 2^-4 here and off by (D + 8) 2^-24 of it; a weight by twice that and 3 2^-24 for its
+    exponent and power; the sum of two values in three parts each by 6 2^-24, that of the weights by 2 2^-24, joins and quotient by
+    3 2^-24: 16 2^-24 of the mass in all beside the logits'.  (Weights of 16 bits are off by up to 2^-16, 256 2^-24.)"""
+    R, H, G, bt = 64, 4, 2, 16
+    g = torch.Generator().manual_seed(D)
+    k = torch.randint(-4, 5, (2 * R, G, D), generator=g) / 2.0
+    v = torch.tensor([0.5, 1.0, 1.5, 2.0, 3.0])[torch.randint(0, 5, (R, 1, G, D), generator=g)]
+    k[..., ::32], v[..., ::32] = 2.0, 3.0  # every 32 elements have the scale 1/2: all of these are codes of it
+    v = (v * torch.tensor([1.0, -1.0])[None, :, None, None]).reshape(2 * R, G, D)
+    cache = ops.new_cache(R, G, D, block_tokens=bt, device=DEV, bits=4)
+    ops.cache_write_(k.to(DEV), v.to(DEV), cache, _i32([[2 * i, 2, i, 0] for i in range(R)]))
+    got = ops.cache_read(cache, torch.arange(R, device=DEV, dtype=torch.int32)[:, None], _i32(range(0, 2 * R + 1, 2)), n_rows=2 * R,
+                         dtype=torch.float32)
+    assert torch.equal(got[0].cpu(), k) and torch.equal(got[1].cpu(), v)
+    q = torch.randn(R, H, D, generator=g)
+    q = (q / (q[:, :, None].abs() * k.view(R, 2, G, D).abs().repeat_interleave(H // G, 2).transpose(1, 2)).sum(-1).amax(-1, keepdim=True)).to(dt)
+    table = np.arange(R)[:, None]
+    if place == "window":
+        pos, w, lmk = [1] * R, [2] * R, np.full((H, R, 1, 0), -1)
+    else:  # both lie before a window without a page, side by side in a set (a part of it that holds one key weighs it 1)
+        table = np.concatenate([table, np.full((R, 1), -1)], 1)
+        pos, w, lmk = [bt] * R, [1] * R, np.full((H, R, 1, 128), -1)
+        lmk[..., :2] = [1, 0]
+    scale = 2.0 ** -4
+    out, _ = ops.cache_attention(q.to(DEV), cache, *(_i32(x) for x in (table, range(R), pos, w)), _i32(lmk).view(*lmk.shape), scale=scale,
+                                 w_max=16)
+    ref, _, mass, reach, keys = OD.attention(f64(q), _host_pages(cache), table, list(range(R)), pos, w, lmk, None, scale)
+    assert (keys == 2).all() and (reach <= 2.0 ** -4 * 1.01).all() and (np.abs(ref) < mass / 30).mean() > 0.9
+    tol = (2 * (D + 8) * reach + 16)[..., None] * 2.0 ** -24 * mass + U[dt] * np.abs(ref) + (2.0 ** -25 if dt == torch.float16 else 0)
+    assert (np.abs(f64(out) - ref) <= tol).all(), float((np.abs(f64(out) - ref) / tol).max())
