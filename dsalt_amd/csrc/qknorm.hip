@@ -302,7 +302,7 @@ QkPlan qk_plan(int total_len, int q_heads, int k_heads, int head_dim, int most) 
     a.chunks = a.q_chunks + chunks(k_heads);
     a.q_heads = a.q_chunks ? (q_heads - 1) / a.q_chunks + 1 : 0;
     a.k_heads = a.chunks > a.q_chunks ? (k_heads - 1) / (a.chunks - a.q_chunks) + 1 : 0;
-    a.lines = (int)std::min(groups, (int64_t)std::max(1, most / a.chunks));
+    a.lines = a.chunks ? (int)std::min(groups, (int64_t)std::max(1, most / a.chunks)) : 0;  // (no heads: no blocks)
     a.blocks = (int)(((int64_t)a.lines * a.chunks + kWaves - 1) / kWaves);
     return a;
 }

@@ -629,7 +629,7 @@ def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, *, cu_seql
         d, d_at = _rows16(d.to(t.dtype), "d" + n)
         y = torch.empty(t.shape, dtype=t.dtype, device=t.device)
         out.append(y)
-        grads.append(torch.empty(t.shape[2], dtype=torch.float32, device=t.device))
+        grads.append((torch.empty if t.shape[1] else torch.zeros)(t.shape[2], dtype=torch.float32, device=t.device))
         ups.append(d)
         at_out.append((y.data_ptr(), t.shape[1] * t.shape[2], t.shape[2]))
         at_up.append(d_at)

@@ -266,7 +266,8 @@ typedef struct dsalt_qk_norm_rope_args {
 int    dsalt_qk_norm_rope(const dsalt_qk_norm_rope_args* a, dsalt_stream_t stream);
 
 /* Its gradients: base.q_out and base.k_out receive those of q and k (zeros in rows without a position; never the inputs'
- * memory), dq_weight and dk_weight those of the weights, summed over rows and heads in a fixed order. */
+ * memory), dq_weight and dk_weight those of the weights, summed over rows and heads in a fixed order (left as they are
+ * where there are no heads). */
 typedef struct dsalt_qk_norm_rope_bwd_args {
     dsalt_qk_norm_rope_args base;
     const void* dq; int64_t dq_stride_t; int64_t dq_stride_h;   /* gradient of the outputs */

@@ -357,3 +357,16 @@ def test_two_streams_and_captured():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, ref)), rep
+
+
+def test_sides_without_heads():
+    x, w, tab, d = _case(10, 2, 2, 64, torch.bfloat16, 6)
+    a = [t.to(DEV) for t in w + tab]
+    cu = torch.tensor([0, 10], device=DEV)
+    q, k, dk = x.to(DEV)[:, :0], x.to(DEV)[:, 2:4], d[1].to(DEV)
+    ref = ops.qk_norm_rope_backward(None, dk, None, k, None, *a[1:], cu_seqlens=cu)
+    dq, dkey, dqw, dkw = ops.qk_norm_rope_backward(q, dk, q, k, *a, cu_seqlens=cu)
+    assert dq.shape == q.shape and not dqw.any() and torch.equal(dkey, ref[1]) and torch.equal(dkw, ref[3])
+    dq, dkey, dqw, dkw = ops.qk_norm_rope_backward(q, q, q, q, *a, cu_seqlens=cu)
+    assert dq.shape == dkey.shape == q.shape and not dqw.any() and not dkw.any()
+    assert ops.qk_norm_rope(q, q, *a, cu_seqlens=cu)[0].shape == q.shape

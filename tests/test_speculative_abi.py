@@ -145,6 +145,33 @@ def test_qk_backward_refusals(field, value, code):
     _refused("dsalt_qk_norm_rope_bwd", b, code)
 
 
+def test_qk_without_heads(monkeypatch):
+    """No heads on either side: nothing to do, no workspace, and gradients of the weights that are zeros (as beside a side that
+    has heads)."""
+    lib = _lib.load()
+    for n_rows in (0, 1, 10):
+        b = _lib.QkNormRopeBwdArgs(_qk_args())
+        b.base.total_len, b.base.n_q_heads, b.base.n_k_heads = n_rows, 0, 0
+        assert lib.dsalt_qk_norm_rope_bwd_workspace_bytes(ctypes.byref(b)) == 0
+        assert lib.dsalt_qk_norm_rope_bwd(ctypes.byref(b), None) == 0 and lib.dsalt_qk_norm_rope(ctypes.byref(b.base), None) == 0
+    for q_heads, k_heads in ((0, 3), (3, 0)):
+        b = _qk_bwd_args()
+        b.base.n_q_heads, b.base.n_k_heads = q_heads, k_heads
+        assert lib.dsalt_qk_norm_rope_bwd_workspace_bytes(ctypes.byref(b)) > 0
+    monkeypatch.setattr(ops, "_on", lambda *ts: 0)
+    monkeypatch.setattr(ops, "_set_workspace", lambda a, need, at: None)
+    monkeypatch.setattr(ops, "_call", lambda name, a, at, *more: None)
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *s, **kw: empty(*s, **kw).fill_(9))  # (as memory that is not written)
+    q, w, tab = torch.zeros(10, 0, 64), torch.ones(64), torch.zeros(8, 64)
+    where = dict(pos=torch.zeros(10, dtype=torch.int32))
+    dq, dk, dqw, dkw = ops.qk_norm_rope_backward(q, None, q, None, w, None, tab, tab, **where)
+    assert dq.shape == q.shape and dk is None and dkw is None and not dqw.any()
+    k = torch.zeros(10, 2, 64)
+    assert not ops.qk_norm_rope_backward(q, k, q, k, w, w, tab, tab, **where)[2].any()
+    assert not ops.qk_norm_rope_backward(k, q, k, q, w, w, tab, tab, **where)[3].any()
+
+
 def test_null_structs_and_empty_calls():
     lib = _lib.load()
     for name in ("dsalt_cache4_write", "dsalt_cache4_read", "dsalt_cache4_attn", "dsalt_verify_rows", "dsalt_qk_norm_rope",
