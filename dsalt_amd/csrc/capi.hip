@@ -3,6 +3,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <algorithm>
 #include <map>
 #include <mutex>
 #include <string>
@@ -351,6 +352,55 @@ int check_qk_rows(const dsalt_qk_norm_rope_args* a) {
                          (rc = check_rows(a->k_out, a->ko_stride_t, a->ko_stride_h, a->dtype, "k_out"))))
         return rc;
     return DSALT_OK;
+}
+
+// heads of T rows, as an operand of the norm and rotation has them; strides in elements
+struct Heads {
+    const void* at;
+    int64_t st, sh;
+    int n;
+};
+
+// Whether heads of a and b share elements; of one side with itself (same), whether two of its heads do.  Two sides that
+// cross and differ in token stride count as sharing.
+bool share(const Heads& a, const Heads& b, bool same, int64_t T, int64_t D, size_t es) {
+    if (T == 0 || a.n == 0 || b.n == 0) return false;
+    const int64_t a_row = (a.n - 1) * a.sh + D, b_row = (b.n - 1) * b.sh + D, st = a.st;
+    const int64_t off = ((int64_t)(uintptr_t)b.at - (int64_t)(uintptr_t)a.at) / (int64_t)es;
+    auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+    auto meet = [&](int64_t x) {  // heads x apart in some two rows
+        const int64_t i = T > 1 ? -floor_div(x, st) : 0;
+        for (int64_t n : {i, i - 1}) {
+            const int64_t y = x + std::clamp(n, 1 - T, T - 1) * st;
+            if (-D < y && y < D) return true;
+        }
+        return false;
+    };
+    if (same) {
+        if (a.sh >= D && (T == 1 || st >= a_row)) return false;
+        bool any = T > 1 && st < D;
+        for (int h = 1; h < a.n && !any; ++h) any = meet(h * a.sh);
+        return any;
+    }
+    if (off >= (T - 1) * st + a_row || off + (T - 1) * b.st + b_row <= 0) return false;
+    if (T > 1 && st != b.st) return true;
+    const int64_t r = off - floor_div(off, st) * st;
+    if (T > 1 && r >= a_row && r + b_row <= st) return false;  // columns of one row beside each other
+    for (int h = 0; h < b.n; ++h)
+        for (int n = 0; n < a.n; ++n)
+            if (meet(off + h * b.sh - n * a.sh)) return true;
+    return false;
+}
+
+// Waves read and write heads in any order: those written must share elements neither with each other nor with those read, `in`
+// (none of them where each head is written over itself).
+int check_qk_written(const dsalt_qk_norm_rope_args* a, const Heads* in, int n_in) {
+    const int64_t T = a->total_len, D = a->head_dim;
+    const size_t es = esize(a->dtype);
+    const Heads q = {a->q_out, a->qo_stride_t, a->qo_stride_h, a->n_q_heads}, k = {a->k_out, a->ko_stride_t, a->ko_stride_h, a->n_k_heads};
+    bool any = share(q, q, true, T, D, es) || share(k, k, true, T, D, es) || share(q, k, false, T, D, es);
+    for (int i = 0; i < n_in && !any; ++i) any = share(q, in[i], false, T, D, es) || share(k, in[i], false, T, D, es);
+    return any ? fail(DSALT_ERR_INVALID, "heads that are written must not share elements with others") : DSALT_OK;
 }
 
 dsalt::QkNormParams qk_params(const dsalt_qk_norm_rope_args* a) {
@@ -882,6 +932,8 @@ int dsalt_qk_norm_rope(const dsalt_qk_norm_rope_args* a, dsalt_stream_t stream) 
         (p.q.heads && p.k.heads && same(p.q) != same(p.k)))
         return fail(DSALT_ERR_INVALID, "the outputs are both the inputs, with their strides, or neither is");
     p.inplace = same(p.q) && same(p.k);
+    const Heads in[2] = {{a->q, a->q_stride_t, a->q_stride_h, a->n_q_heads}, {a->k, a->k_stride_t, a->k_stride_h, a->n_k_heads}};
+    if ((rc = check_qk_written(a, in, p.inplace ? 0 : 2))) return rc;
     return hip_status(dsalt::qk_norm_rope_launch(p, (hipStream_t)stream), "dsalt_qk_norm_rope");
 }
 
@@ -904,6 +956,9 @@ int dsalt_qk_norm_rope_bwd(const dsalt_qk_norm_rope_bwd_args* a, dsalt_stream_t 
     const size_t need = dsalt::qk_norm_rope_bwd_ws_bytes(b->total_len, b->n_q_heads, b->n_k_heads, b->head_dim, b->dtype);
     if (need && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need))
         return fail(DSALT_ERR_WORKSPACE, "workspace of %zu bytes required", need);
+    const Heads in[4] = {{b->q, b->q_stride_t, b->q_stride_h, b->n_q_heads}, {b->k, b->k_stride_t, b->k_stride_h, b->n_k_heads},
+                         {a->dq, a->dq_stride_t, a->dq_stride_h, b->n_q_heads}, {a->dk, a->dk_stride_t, a->dk_stride_h, b->n_k_heads}};
+    if ((rc = check_qk_written(b, in, 4))) return rc;
     dsalt::QkNormParams p = qk_params(b);
     p.q.d = a->dq;
     p.q.d_st = a->dq_stride_t;

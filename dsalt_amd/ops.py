@@ -584,12 +584,39 @@ def _positions(pos: torch.Tensor) -> torch.Tensor:
     return pos.clamp(-1, 0x7fffffff) if pos.dtype == torch.int64 else pos
 
 
+def _share(a, b, a_heads: int, b_heads: int, t) -> bool:
+    """Whether two sides' heads, of (address, token stride, head stride) in rows like ``t``'s, share elements; of one side with
+    itself, whether two of its heads do.  Two sides that cross and differ in token stride count as sharing."""
+    T, D = t.shape[0], t.shape[2]
+    if T == 0 or a_heads == 0 or b_heads == 0:
+        return False
+    (a_at, st, a_sh), (b_at, b_st, b_sh) = a, b
+    a_row, b_row = (a_heads - 1) * a_sh + D, (b_heads - 1) * b_sh + D
+    off = (b_at - a_at) // t.element_size()
+
+    def meet(x):  # heads x apart in some two rows
+        i = -(x // st) if T > 1 else 0
+        return any(abs(x + max(min(n, T - 1), 1 - T) * st) < D for n in (i, i - 1))
+    if a is b:
+        if a_sh >= D and (T == 1 or st >= a_row):
+            return False
+        return (T > 1 and st < D) or any(meet(h * a_sh) for h in range(1, a_heads))
+    if off >= (T - 1) * st + a_row or off + (T - 1) * b_st + b_row <= 0:
+        return False
+    if T > 1 and st != b_st:
+        return True
+    if T > 1 and off % st >= a_row and off % st + b_row <= st:  # columns of one row beside each other
+        return False
+    return any(meet(off + h * b_sh - n * a_sh) for h in range(b_heads) for n in range(a_heads))
+
+
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, cu_seqlens=None, pos=None, max_seqlen=None, eps=1e-6, inplace=False):
     """(q, k) with a root-mean-square norm of each head, x / sqrt(mean(x^2) + eps) * weight, and the rotation of
     rope_qk_ after it, in one pass and in float32, rounded once.  q [T, Hq, D], k [T, Hk, D] (either may be None, strided
     views are read in place), weights [D], cos/sin [max_pos, D] fp32.  A row's position is its place in its sequence of
     ``cu_seqlens``, or ``pos[t]`` (CacheRows.pos of a decoding step).  Rows in no sequence, or with a position
-    outside the tables (inert rows), become zeros; with ``inplace``, which writes over q and k, they stay as they are."""
+    outside the tables (inert rows), become zeros; with ``inplace``, which writes over q and k (views that cannot be written
+    where they lie, and heads that share elements, are refused), they stay as they are."""
     at, sides, head, tail, keep = _qk_args(q, k, q_weight, k_weight, cos, sin, cu_seqlens, pos, max_seqlen, eps)  # noqa: F841 (kept alive)
     out, at_out = [], []
     for t, where, _, _ in sides:
@@ -599,7 +626,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, cu_seqlens=None, pos=Non
         elif inplace:
             if t is not q and t is not k:
                 raise ValueError("q and k must have unit stride along D and rows on 16-byte boundaries to be written in place")
-            if where[2] < t.shape[2] or (t.shape[0] > 1 and where[1] < t.shape[2]):
+            if _share(where, where, t.shape[1], t.shape[1], t):
                 raise ValueError("heads of q and k must not share elements to be written in place")
             out.append(t)
             at_out.append(where)
@@ -607,6 +634,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, *, cu_seqlens=None, pos=Non
             y = torch.empty(t.shape, dtype=t.dtype, device=t.device)
             out.append(y)
             at_out.append((y.data_ptr(), t.shape[1] * t.shape[2], t.shape[2]))
+    if inplace and q is not None and k is not None and _share(*at_out, q.shape[1], k.shape[1], q):
+        raise ValueError("q and k must not share elements to be written in place")
     _call("dsalt_qk_norm_rope", QkNormRopeArgs(*head, *sides[0][1], *sides[1][1], *at_out[0], *at_out[1], *tail), at)
     return tuple(out)
 

@@ -240,7 +240,8 @@ int    dsalt_rope_qk(const dsalt_rope_args* a, dsalt_stream_t stream);
  *   n1[j] cos[p][j] - n2[j] sin[p][j],  n2[j] cos[p][D/2 + j] + n1[j] sin[p][D/2 + j]
  * in float32, rounded once.  The position p of row t is pos[t], or its place in its sequence of cu_seqlens; rows whose
  * position lies outside [0, max_pos), and those in no sequence, become zeros, or stay as they are where the outputs are the
- * inputs (the same pointer and strides).  Needs no workspace. */
+ * inputs (the same pointer and strides).  Heads that are written must share elements neither with each other nor, beside
+ * themselves, with those read: such calls are refused.  Needs no workspace. */
 typedef struct dsalt_qk_norm_rope_args {
     int32_t total_len;         /* T                                                  */
     int32_t num_seqs;          /* S (with cu_seqlens)                                */

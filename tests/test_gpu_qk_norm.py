@@ -370,3 +370,22 @@ def test_sides_without_heads():
     dq, dkey, dqw, dkw = ops.qk_norm_rope_backward(q, q, q, q, *a, cu_seqlens=cu)
     assert dq.shape == dkey.shape == q.shape and not dqw.any() and not dkw.any()
     assert ops.qk_norm_rope(q, q, *a, cu_seqlens=cu)[0].shape == q.shape
+
+
+def test_written_in_place_beside_each_other():
+    """Heads that lie apart in one buffer, in the layouts that are taken: the results of new outputs."""
+    T, D = 300, 64
+    x, w, tab, _ = _case(T, 4, 0, D, torch.bfloat16, 9, max_pos=T)
+    a, cu = [t.to(DEV) for t in w + tab], torch.tensor([0, 100, T], device=DEV)
+    heads_first = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    for split in (lambda t: (t[:, :3], t[:, 3:]), lambda t: (t[:, ::2], t[:, 1::2]), lambda t: (t[:, 2:], t[:, :1]),
+                  lambda t: (heads_first(t)[:, :2], heads_first(t)[:, 2:])):
+        q, k = split(x.to(DEV))
+        ref = ops.qk_norm_rope(q, k, *a, cu_seqlens=cu)
+        got = ops.qk_norm_rope(q, k, *a, cu_seqlens=cu, inplace=True)
+        assert got[0] is q and got[1] is k and torch.equal(q, ref[0]) and torch.equal(k, ref[1])
+    y = torch.zeros((T + 1) * D, device=DEV, dtype=torch.bfloat16)
+    for q, k in ((y.as_strided((T, 2, D), (D, D, 1)), None), (y[:T * D].view(T, 1, D),) * 2):
+        with pytest.raises(ValueError):
+            ops.qk_norm_rope(q, k, a[0], a[1] if k is not None else None, *a[2:], cu_seqlens=cu, inplace=True)
+    assert not y.any()

@@ -145,6 +145,97 @@ def test_qk_backward_refusals(field, value, code):
     _refused("dsalt_qk_norm_rope_bwd", b, code)
 
 
+def _elements(at, st, sh, heads, T, D):
+    return [at + t * st + h * sh + d for t in range(T) for h in range(heads) for d in range(D)]
+
+
+def _layouts():
+    """Random sides of few rows and heads, and those that a user meets: (T, (place, strides, heads) of two sides, exact)."""
+    r, D = np.random.RandomState(0), 16
+    for _ in range(2000):
+        T, H, G = (int(x) for x in r.randint(1, 5, 3))
+        a, b = ((int(r.randint(0, 12) * 8), int(r.randint(1, 14) * 8), int(r.randint(0, 8) * 8), n) for n in (H, G))
+        if r.rand() < 0.6:
+            b = (b[0], a[1], *b[2:])
+        yield T, a, b
+    for T in (1, 2, 5):
+        for H, G in ((4, 2), (1, 1), (2, 4), (3, 1)):
+            row = (H + 2 * G) * D
+            yield T, (0, row, D, H), (H * D, row, D, G)                         # columns of one projection
+            yield T, (0, row, D, H), (H * D - 8, row, D, G)                     # and half a head too near
+            yield T, (0, D, T * D, H), (H * T * D, D, T * D, G)                 # heads first
+            yield T, (0, 2 * H * D, 2 * D, H), (D, 2 * H * D, 2 * D, min(H, G))  # query and key heads in turn
+            yield T, (0, D, D, H), (T * H * D + D, D, D, G)                     # a row's second head is the next row's first
+            yield T, (0, row, D, H), (0, row, D, H)                             # the same memory
+
+
+def test_heads_that_share_elements_are_found():
+    """Against the sets of elements themselves, through Python and the C entry points (which then launch nothing); only two sides that
+    cross at different token strides may be taken to share what they do not."""
+    D, lib = 16, _lib.load()
+    ref = lambda at, st, sh, n: _elements(at, st, sh, n, T, D)  # noqa: E731
+    found = [0, 0, 0]
+    for T, a, b in _layouts():
+        x = torch.empty(T, 1, D, dtype=torch.bfloat16)
+        where = [(FAKE + 2 * at, st, sh) for at, st, sh, _ in (a, b)]
+        own = [len(set(ref(*s))) < len(ref(*s)) for s in (a, b)]
+        for w, s, want in zip(where, (a, b), own):
+            assert ops._share(w, w, s[3], s[3], x) == want
+        cross, got = bool(set(ref(*a)) & set(ref(*b))), ops._share(*where, a[3], b[3], x)
+        apart = min(ref(*a)) > max(ref(*b)) or min(ref(*b)) > max(ref(*a))
+        assert got == cross or (got and T > 1 and a[1] != b[1] and not apart)
+        found[0 if any(own) else 1 if got else 2] += 1
+        if any(own) or got:
+            c = _qk_args()
+            c.total_len, c.head_dim, c.n_q_heads, c.n_k_heads = T, D, a[3], b[3]
+            for n, w in zip("qk", where):
+                setattr(c, n, w[0])
+                setattr(c, n + "_out", w[0])
+                for f in (n, n + "o"):
+                    setattr(c, f + "_stride_t", w[1])
+                    setattr(c, f + "_stride_h", w[2])
+            _refused("dsalt_qk_norm_rope", c, 1)
+            g = _lib.QkNormRopeBwdArgs(c, FAKE << 8, 4096, 64, FAKE << 8, 4096, 64, FAKE, FAKE)
+            g.base.q = g.base.k = FAKE << 9
+            g.workspace, g.workspace_bytes = FAKE, 1 << 30
+            _refused("dsalt_qk_norm_rope_bwd", g, 1)
+    assert min(found) > 100, found
+
+
+def test_qk_outputs_over_what_is_read_are_refused():
+    for field, at, stride in (("q_out", FAKE + 128, 256), ("k_out", FAKE + 10 * 4 * 64 * 2 - 16, 128), ("q_out", FAKE - 16, 512)):
+        a = _qk_args()
+        a.k, a.q_out, a.k_out = 2 * FAKE, 4 * FAKE, 8 * FAKE
+        setattr(a, field, at)
+        setattr(a, field[0] + "o_stride_t", stride)
+        _refused("dsalt_qk_norm_rope", a, 1)
+        b = _qk_bwd_args()
+        b.base = a
+        b.base.q = b.base.k = 16 * FAKE
+        b.workspace_bytes = 1 << 30
+        _refused("dsalt_qk_norm_rope_bwd", b, 1)  # over dq, dk
+
+
+def test_heads_that_share_elements_are_not_written_in_place(monkeypatch):
+    """Refused before anything is launched, whichever way they share; what lies apart in one buffer is taken."""
+    launched = []
+    monkeypatch.setattr(ops, "_on", lambda *ts: 0)
+    monkeypatch.setattr(ops, "_call", lambda name, a, at, *more: launched.append(name))
+    w, tab = torch.ones(64), torch.zeros(8, 64)
+    x = torch.zeros(8192)
+    where = dict(pos=torch.zeros(6, dtype=torch.int32), inplace=True)
+    chain, rows = x.as_strided((6, 2, 64), (64, 64, 1)), x[:6 * 256].view(6, 4, 64)
+    for q, k in ((chain, None), (None, chain), (rows, rows), (rows[:, :3], rows[:, 2:]), (rows[:, :2], x[64:64 + 6 * 256].view(6, 4, 64)[:, :2]),
+                 (rows, x[6 * 256 - 64:6 * 512 - 64].view(6, 4, 64)), (rows[:, :1].expand(6, 2, 64), None)):
+        with pytest.raises(ValueError, match="share"):
+            ops.qk_norm_rope(q, k, w if q is not None else None, w if k is not None else None, tab, tab, **where)
+    assert not launched
+    for q, k in ((rows[:, :2], rows[:, 2:]), (rows[:, ::2], rows[:, 1::2]), (rows[:, 3:], rows[:, :3]), (rows, x[6 * 256:6 * 512].view(6, 4, 64)),
+                 (x[:6 * 256].view(4, 6, 64).transpose(0, 1), x[6 * 256:6 * 512].view(4, 6, 64).transpose(0, 1))):
+        assert ops.qk_norm_rope(q, k, w, w, tab, tab, **where) == (q, k)
+    assert len(launched) == 5
+
+
 def test_qk_without_heads(monkeypatch):
     """No heads on either side: nothing to do, no workspace, and gradients of the weights that are zeros (as beside a side that
     has heads)."""
