@@ -184,9 +184,11 @@ class DSALTAttention(nn.Module):
         return self._rope32[1], self._rope32[2]
 
     def _norm_rope(self, q, k, cos, sin, cu_seqlens, max_seqlen):
-        """The heads normed and rotated; over the inputs without autograd, where the kernel can write there."""
+        """The heads normed and rotated.  Inference writes over them where the kernel can, columns of its own projection; the
+        other branches, without autograd too, leave what the projections returned (which a hook may keep, and which may be
+        the layer's input)."""
         w = (self.q_norm.weight, self.k_norm.weight)
-        if torch.is_grad_enabled():
+        if self.training or torch.is_grad_enabled():
             return qk_norm_rope(q, k, *w, cos, sin, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, eps=self.q_norm.eps)
         aligned = all(t.data_ptr() % 16 == 0 and t.stride(0) * t.element_size() % 16 == 0 for t in (q, k))
         return ops.qk_norm_rope(q, k, *w, cos, sin, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, eps=self.q_norm.eps,

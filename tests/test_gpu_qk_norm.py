@@ -389,3 +389,20 @@ def test_written_in_place_beside_each_other():
         with pytest.raises(ValueError):
             ops.qk_norm_rope(q, k, a[0], a[1] if k is not None else None, *a[2:], cu_seqlens=cu, inplace=True)
     assert not y.any()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_layer_in_training_leaves_what_projections_return(grad):
+    """With and without autograd: an output that a hook keeps, and the layer's input where a projection returns it."""
+    torch.manual_seed(2)
+    layer = DSALTAttention(128, 2, 4, 16, 4, 64, qk_norm=True).to(DEV).train()
+    x, cu = torch.randn(40, 128, device=DEV), torch.tensor([0, 15, 40], dtype=torch.int32, device=DEV)
+    kept = []
+    layer.k_proj.register_forward_hook(lambda m, i, o: kept.append((o, o.detach().clone())))
+    layer.q_proj = torch.nn.Identity()
+    before = x.clone()
+    with torch.set_grad_enabled(grad):
+        out, _ = layer(x, cu)
+    assert torch.equal(x, before) and all(torch.equal(o, c) for o, c in kept) and len(kept) == 1
+    with torch.set_grad_enabled(not grad):
+        assert torch.equal(layer(x, cu)[0], out)

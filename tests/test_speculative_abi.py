@@ -13,6 +13,7 @@ import torch
 from dsalt_amd import _lib, ops
 from dsalt_amd.kernels import qk_norm_rope
 from dsalt_amd.model import DSALTConfig
+from dsalt_amd.modules import DSALTAttention
 from oracle import decode4 as O4
 from oracle import qk_norm as OQ
 
@@ -350,6 +351,30 @@ def test_argument_checks(monkeypatch):
     for bad in (dict(tokens=tok.float()), dict(u=u.half()), dict(v=v.double())):
         with pytest.raises(TypeError):
             ops.verify_rows(**{**ver, **bad})
+
+
+@pytest.fixture
+def norm_calls(monkeypatch):
+    """A layer of two heads of 64 whose norm-and-rotation calls are noted in place of running."""
+    calls = []
+    monkeypatch.setattr(ops, "_on", lambda *ts: 0)
+    monkeypatch.setattr(ops, "_call", lambda name, a, at, *more: calls.append(a))
+    layer = DSALTAttention(128, 2, 2, 8, 4, 32, n_kv_heads=1, qk_norm=True)
+    layer.run = lambda q, k: layer._norm_rope(q, k, *layer._rope_tables32(), torch.tensor([0, len(q)], dtype=torch.int32), len(q))
+    return layer, calls
+
+
+@pytest.mark.parametrize("training,grad", [(True, True), (True, False), (False, True), (False, False)])
+def test_layer_writes_over_its_own_projection_alone(norm_calls, training, grad):
+    layer, calls = norm_calls
+    layer.train(training)
+    x = torch.randn(5, 3, 64)
+    with torch.set_grad_enabled(grad):
+        q, k = layer.run(x[:, :2], x[:, 2:])
+    a, = calls
+    over = not training and not grad  # the branch whose queries and keys are columns of a buffer that it made
+    assert (a.q_out == a.q == x.data_ptr()) == over and (a.k_out == a.k) == over
+    assert (q.data_ptr() == x.data_ptr()) == over
 
 
 def test_config_carries_qk_norm(tmp_path):
