@@ -184,15 +184,20 @@ class DSALTAttention(nn.Module):
         return self._rope32[1], self._rope32[2]
 
     def _norm_rope(self, q, k, cos, sin, cu_seqlens, max_seqlen):
-        """The heads normed and rotated.  Inference writes over them where the kernel can, columns of its own projection; the
-        other branches, without autograd too, leave what the projections returned (which a hook may keep, and which may be
-        the layer's input)."""
-        w = (self.q_norm.weight, self.k_norm.weight)
-        if self.training or torch.is_grad_enabled():
-            return qk_norm_rope(q, k, *w, cos, sin, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, eps=self.q_norm.eps)
-        aligned = all(t.data_ptr() % 16 == 0 and t.stride(0) * t.element_size() % 16 == 0 for t in (q, k))
-        return ops.qk_norm_rope(q, k, *w, cos, sin, cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, eps=self.q_norm.eps,
-                                inplace=aligned)
+        """The heads normed and rotated, each side with its own norm's weight and ``eps``.  Inference writes over them where the
+        kernel can, columns of its own projection; the other branches, without autograd too, leave what the projections
+        returned (which a hook may keep, and which may be the layer's input)."""
+        def run(q, k, wq, wk, eps):
+            where = dict(cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, eps=eps)
+            if self.training or torch.is_grad_enabled():
+                return qk_norm_rope(q, k, wq, wk, cos, sin, **where)
+            aligned = all(t is None or (t.data_ptr() % 16 == 0 and t.stride(0) * t.element_size() % 16 == 0) for t in (q, k))
+            return ops.qk_norm_rope(q, k, wq, wk, cos, sin, **where, inplace=aligned)
+
+        nq, nk = self.q_norm, self.k_norm
+        if nq.eps == nk.eps and nq.weight.dtype == nk.weight.dtype:  # what a launch has one of
+            return run(q, k, nq.weight, nk.weight, nq.eps)
+        return run(q, None, nq.weight, None, nq.eps)[0], run(None, k, None, nk.weight, nk.eps)[1]
 
     def _selectors(self, x):
         """(integer windows [T] int32, alpha [H] float32) of the inference branch: one kernel after

@@ -406,3 +406,33 @@ def test_layer_in_training_leaves_what_projections_return(grad):
     assert torch.equal(x, before) and all(torch.equal(o, c) for o, c in kept) and len(kept) == 1
     with torch.set_grad_enabled(not grad):
         assert torch.equal(layer(x, cu)[0], out)
+
+
+@pytest.mark.parametrize("mode", ["train", "eval with autograd", "inference"])
+def test_layer_with_two_eps(mode):
+    """Each side by its own norm: the results of torch operations, to the layer's float32 tolerance (as test_layer)."""
+    torch.manual_seed(3)
+    H, G, D, T = 4, 2, 64, 90
+    layer = DSALTAttention(H * D, H, 8, 40, 6, 256, n_kv_heads=G, qk_norm=True).to(DEV).train(mode == "train")
+    layer.q_norm.eps, layer.k_norm.eps = 1e-6, 0.3
+    x = torch.randn(T, H * D, device=DEV)
+    cu, pos = torch.tensor([0, T], dtype=torch.int32, device=DEV), torch.arange(T, device=DEV)
+
+    def run():
+        layer.zero_grad()
+        y = x.clone().requires_grad_(mode != "inference")
+        with torch.set_grad_enabled(mode != "inference"):
+            out, _ = layer(y, cu)
+        if mode == "inference":
+            return [out]
+        (out * torch.linspace(-1, 1, out.numel(), device=DEV).view_as(out)).sum().backward()
+        return [out.detach(), y.grad, layer.q_norm.weight.grad.clone(), layer.k_norm.weight.grad.clone()]
+
+    own = run()
+
+    def plain(q, k, cos, sin, c, m):
+        a = (layer.q_norm.weight, layer.k_norm.weight, layer.rope_cos, layer.rope_sin, pos)
+        return _torch_norm_rope(q, k, *a, 1e-6)[0], _torch_norm_rope(q, k, *a, 0.3)[1]
+    layer._norm_rope = plain
+    for a, b in zip(own, run()):
+        assert (a - b).abs().max() <= 1e-4 * b.abs().max().clamp(min=1e-3)

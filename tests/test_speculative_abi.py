@@ -377,6 +377,25 @@ def test_layer_writes_over_its_own_projection_alone(norm_calls, training, grad):
     assert (q.data_ptr() == x.data_ptr()) == over
 
 
+@pytest.mark.parametrize("grad", [True, False])
+def test_layer_takes_each_norms_own_eps(norm_calls, grad):
+    layer, calls = norm_calls
+    layer.eval()
+    layer.k_norm.eps = 0.5
+    x = torch.randn(5, 3, 64)
+    with torch.set_grad_enabled(grad):
+        layer.run(x[:, :2], x[:, 2:])
+        assert [(a.n_q_heads, a.n_k_heads, a.eps) for a in calls] == [(2, 0, pytest.approx(1e-6)), (0, 1, 0.5)]
+        del calls[:]
+        layer.q_norm.eps = 0.5
+        layer.run(x[:, :2], x[:, 2:])
+        assert [(a.n_q_heads, a.n_k_heads, a.eps) for a in calls] == [(2, 1, 0.5)]
+        del calls[:]
+        layer.k_norm.to(torch.bfloat16)  # weights of two types are two calls as well
+        layer.run(x[:, :2], x[:, 2:])
+        assert [(a.n_q_heads, a.n_k_heads, a.weight_dtype) for a in calls] == [(2, 0, 0), (0, 1, 1)]
+
+
 def test_config_carries_qk_norm(tmp_path):
     c = DSALTConfig(vocab_size=64, d_model=64, n_layers=1, n_heads=2, n_min=2, n_max=8, k_lmk=4, max_seq_len=32, qk_norm=True)
     c.save(tmp_path / "c.json")
