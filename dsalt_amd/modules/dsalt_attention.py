@@ -186,7 +186,8 @@ class DSALTAttention(nn.Module):
     def _norm_rope(self, q, k, cos, sin, cu_seqlens, max_seqlen):
         """The heads normed and rotated, each side with its own norm's weight and ``eps``.  Inference writes over them where the
         kernel can, columns of its own projection; the other branches, without autograd too, leave what the projections
-        returned (which a hook may keep, and which may be the layer's input)."""
+        returned (which a hook may keep, and which may be the layer's input).  A norm that is not RMSENorm as it comes (another
+        module in its place, a replaced ``forward``, hooks) is called, and its side rotated by torch operations."""
         def run(q, k, wq, wk, eps):
             where = dict(cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, eps=eps)
             if self.training or torch.is_grad_enabled():
@@ -194,10 +195,20 @@ class DSALTAttention(nn.Module):
             aligned = all(t is None or (t.data_ptr() % 16 == 0 and t.stride(0) * t.element_size() % 16 == 0) for t in (q, k))
             return ops.qk_norm_rope(q, k, wq, wk, cos, sin, **where, inplace=aligned)
 
+        def called(n, x):
+            if max_seqlen > cos.shape[0]:
+                raise ValueError(f"a sequence of {max_seqlen} rows passes the {cos.shape[0]} positions of cos and sin")
+            t = torch.arange(x.shape[0], device=x.device)
+            cu = cu_seqlens.to(t)
+            seq = torch.searchsorted(cu[1:], t, right=True).clamp(max=cu.shape[0] - 2)
+            pos = (t - cu[seq]).clamp(0, cos.shape[0] - 1)  # (rows of no sequence: any)
+            return apply_rotary_emb(n(x).to(x.dtype), x[:, :0], *(c[pos].to(x.dtype).unsqueeze(1) for c in (cos, sin)))[0]
+
         nq, nk = self.q_norm, self.k_norm
-        if nq.eps == nk.eps and nq.weight.dtype == nk.weight.dtype:  # what a launch has one of
+        if _own_norm(nq) and _own_norm(nk) and nq.eps == nk.eps and nq.weight.dtype == nk.weight.dtype:
             return run(q, k, nq.weight, nk.weight, nq.eps)
-        return run(q, None, nq.weight, None, nq.eps)[0], run(None, k, None, nk.weight, nk.eps)[1]
+        return (run(q, None, nq.weight, None, nq.eps)[0] if _own_norm(nq) else called(nq, q),
+                run(None, k, None, nk.weight, nk.eps)[1] if _own_norm(nk) else called(nk, k))
 
     def _selectors(self, x):
         """(integer windows [T] int32, alpha [H] float32) of the inference branch: one kernel after
@@ -307,3 +318,9 @@ class DSALTAttention(nn.Module):
 
 # what the selector kernel computes; anything else in their place is called instead
 _OWN_SELECTORS = {n: DSALTAttention.__dict__[n] for n in ("_alpha", "_window_continuous", "_window_sizes")}
+_OWN_NORM = RMSENorm.forward
+
+
+def _own_norm(n) -> bool:
+    return type(n) is RMSENorm and getattr(n.forward, "__func__", None) is _OWN_NORM and n.eps is not None \
+        and not (n._forward_pre_hooks or n._forward_hooks or n._backward_pre_hooks or n._backward_hooks)

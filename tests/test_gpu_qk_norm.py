@@ -436,3 +436,32 @@ def test_layer_with_two_eps(mode):
     layer._norm_rope = plain
     for a, b in zip(own, run()):
         assert (a - b).abs().max() <= 1e-4 * b.abs().max().clamp(min=1e-3)
+
+
+@pytest.mark.parametrize("mode", ["train", "eval with autograd", "inference"])
+def test_layer_with_a_hooked_norm(mode):
+    """A hook on a norm is called and does not move the results past the layer's float32 tolerance (as test_layer); a norm that is
+    replaced is used."""
+    torch.manual_seed(4)
+    layer = DSALTAttention(256, 4, 8, 40, 6, 256, n_kv_heads=2, qk_norm=True).to(DEV).train(mode == "train")
+    x, cu = torch.randn(90, 256, device=DEV), torch.tensor([0, 33, 90], dtype=torch.int32, device=DEV)
+
+    def run():
+        layer.zero_grad()
+        y = x.clone().requires_grad_(mode != "inference")
+        with torch.set_grad_enabled(mode != "inference"):
+            out, _ = layer(y, cu)
+        if mode == "inference":
+            return [out]
+        (out * torch.linspace(-1, 1, out.numel(), device=DEV).view_as(out)).sum().backward()
+        return [out.detach(), y.grad, *(n.weight.grad.clone() for n in (layer.q_norm, layer.k_norm) if hasattr(n, "weight"))]
+
+    own, seen = run(), []
+    for n in (layer.q_norm, layer.k_norm):
+        n.register_forward_hook(lambda m, i, o: seen.append((o, o.detach().clone())))
+    for a, b in zip(own, run()):
+        assert (a - b).abs().max() <= 1e-4 * b.abs().max().clamp(min=1e-3)
+    assert len(seen) == 2 and all(torch.equal(o, c) for o, c in seen)
+    layer.q_norm = torch.nn.Identity()
+    other = run()
+    assert not torch.allclose(other[0], own[0], rtol=1e-2)

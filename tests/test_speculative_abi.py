@@ -396,6 +396,60 @@ def test_layer_takes_each_norms_own_eps(norm_calls, grad):
         assert [(a.n_q_heads, a.n_k_heads, a.weight_dtype) for a in calls] == [(2, 0, 0), (0, 1, 1)]
 
 
+class _Double(torch.nn.Module):
+    def forward(self, x):
+        return (2 * x).double()
+
+
+def _rotated(x, tab, pos):
+    half = x.shape[-1] // 2
+    return x * tab[0][pos][:, None] + torch.cat([-x[..., half:], x[..., :half]], -1) * tab[1][pos][:, None]
+
+
+@pytest.mark.parametrize("training,grad", [(True, True), (True, False), (False, True), (False, False)])
+def test_layer_calls_a_norm_in_the_place_of_its_own(norm_calls, training, grad):
+    """Another module, a replaced ``forward``, hooks of each kind: the norm is called and its side rotated; the other stays with the
+    kernel."""
+    layer, calls = norm_calls
+    layer.train(training)
+    x = torch.randn(5, 3, 64)
+    tab, pos, seen = layer._rope_tables32(), torch.tensor([0, 1, 2, 0, 1]), []
+    before = x.clone()
+
+    def run():
+        del calls[:]
+        with torch.set_grad_enabled(grad):
+            return layer._norm_rope(x[:, :2], x[:, 2:], *tab, torch.tensor([0, 3, 5], dtype=torch.int32), 3)
+
+    own = layer.q_norm
+    layer.q_norm = _Double()
+    q, _ = run()
+    assert q.dtype == x.dtype and torch.equal(q, _rotated(2 * x[:, :2], tab, pos)) and [(a.n_q_heads, a.n_k_heads) for a in calls] == [(0, 1)]
+    layer.q_norm, layer.k_norm = layer.k_norm, _Double()
+    _, k = run()
+    assert torch.equal(k, _rotated(2 * x[:, 2:], tab, pos)) and [(a.n_q_heads, a.n_k_heads) for a in calls] == [(2, 0)]
+    layer.q_norm, layer.k_norm = own, type(own)(64)
+    want = _rotated(own.forward(x[:, :2]).detach(), tab, pos)
+    for add in (lambda: own.register_forward_hook(lambda m, i, o: seen.append(1)), lambda: own.register_forward_pre_hook(lambda m, i: seen.append(1)),
+                lambda: own.register_full_backward_hook(lambda m, i, o: None), lambda: own.register_full_backward_pre_hook(lambda m, o: None)):
+        handle = add()
+        q, _ = run()
+        assert torch.allclose(q, want, atol=1e-6) and [(a.n_q_heads, a.n_k_heads) for a in calls] == [(0, 1)]
+        handle.remove()
+        run()
+        assert [(a.n_q_heads, a.n_k_heads) for a in calls] == [(2, 1)]
+        x.copy_(before)
+    assert len(seen) == 2
+    own.forward = lambda t: 0 * t
+    assert not run()[0].any() and len(calls) == 1
+    with pytest.raises(ValueError, match="positions"):
+        layer._norm_rope(x[:, :2], x[:, 2:], *(t[:4] for t in tab), torch.tensor([0, 5], dtype=torch.int32), 5)
+    del own.forward
+    own.eps = None  # the type's own, which the module knows
+    run()
+    assert [(a.n_q_heads, a.n_k_heads) for a in calls] == [(0, 1)]
+
+
 def test_config_carries_qk_norm(tmp_path):
     c = DSALTConfig(vocab_size=64, d_model=64, n_layers=1, n_heads=2, n_min=2, n_max=8, k_lmk=4, max_seq_len=32, qk_norm=True)
     c.save(tmp_path / "c.json")
