@@ -78,6 +78,8 @@ class DSALTAttention(nn.Module):
         self.v_proj = nn.Linear(d_model, self.kv_dim, bias=qkv_bias)
         self.qk_norm = qk_norm
         if qk_norm:
+            if self.head_dim % 16 or self.head_dim > 256:
+                raise ValueError(f"qk_norm takes heads of a multiple of 16 up to 256, got head_dim {self.head_dim}")
             self.q_norm, self.k_norm = RMSENorm(self.head_dim), RMSENorm(self.head_dim)
         self.out_proj = nn.Linear(d_model, d_model, bias=False)
         self.win_gate = nn.Linear(d_model, 1, bias=True)

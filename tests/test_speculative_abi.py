@@ -12,7 +12,7 @@ import torch
 
 from dsalt_amd import _lib, ops
 from dsalt_amd.kernels import qk_norm_rope
-from dsalt_amd.model import DSALTConfig
+from dsalt_amd.model import DSALTConfig, DSALTLMHeadModel
 from dsalt_amd.modules import DSALTAttention
 from oracle import decode4 as O4
 from oracle import qk_norm as OQ
@@ -448,6 +448,18 @@ def test_layer_calls_a_norm_in_the_place_of_its_own(norm_calls, training, grad):
     own.eps = None  # the type's own, which the module knows
     run()
     assert [(a.n_q_heads, a.n_k_heads) for a in calls] == [(0, 1)]
+
+
+def test_head_sizes_that_the_norm_does_not_take_are_refused_when_built():
+    size = dict(n_heads=2, n_min=2, n_max=8, k_lmk=4, max_seq_len=32)
+    for d in (72, 8, 24, 272):
+        with pytest.raises(ValueError, match="head_dim"):
+            DSALTAttention(2 * d, **size, qk_norm=True)
+        with pytest.raises(ValueError, match="head_dim"):
+            DSALTLMHeadModel.from_config(DSALTConfig(vocab_size=16, d_model=2 * d, n_layers=1, **size, qk_norm=True))
+        assert DSALTAttention(2 * d, **size).head_dim == d  # (as without the norm)
+    for d in (16, 48, 128, 256):
+        assert DSALTAttention(2 * d, **size, qk_norm=True).k_norm.weight.shape == (d,)
 
 
 def test_config_carries_qk_norm(tmp_path):
