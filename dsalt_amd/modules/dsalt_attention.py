@@ -192,7 +192,8 @@ class DSALTAttention(nn.Module):
         module in its place, a replaced ``forward``, hooks) is called, and its side rotated by torch operations."""
         def run(q, k, wq, wk, eps):
             where = dict(cu_seqlens=cu_seqlens, max_seqlen=max_seqlen, eps=eps)
-            if self.training or torch.is_grad_enabled():
+            # (forward-mode tangents, transforms and the like go through the differentiable call, which refuses what it cannot carry)
+            if self.training or torch.is_grad_enabled() or not ops._plain(q, k, wq, wk):
                 return qk_norm_rope(q, k, wq, wk, cos, sin, **where)
             aligned = all(t is None or (t.data_ptr() % 16 == 0 and t.stride(0) * t.element_size() % 16 == 0) for t in (q, k))
             return ops.qk_norm_rope(q, k, wq, wk, cos, sin, **where, inplace=aligned)

@@ -9,6 +9,7 @@ import subprocess
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad as fwAD
 
 from dsalt_amd import _lib, ops
 from dsalt_amd.kernels import qk_norm_rope
@@ -448,6 +449,25 @@ def test_layer_calls_a_norm_in_the_place_of_its_own(norm_calls, training, grad):
     own.eps = None  # the type's own, which the module knows
     run()
     assert [(a.n_q_heads, a.n_k_heads) for a in calls] == [(0, 1)]
+
+
+@pytest.mark.parametrize("training", [True, False])
+@pytest.mark.parametrize("which", ["heads", "weight"])
+def test_layer_drops_no_forward_mode_tangents(norm_calls, training, which):
+    """Without autograd as with it: the norm and rotation has no forward-mode derivative, and says so."""
+    layer, calls = norm_calls
+    layer.train(training)
+    x = torch.randn(5, 3, 64)
+    with fwAD.dual_level():
+        if which == "heads":
+            x = fwAD.make_dual(x, torch.ones_like(x))
+        else:
+            w = layer.k_norm.weight
+            del layer.k_norm.weight
+            layer.k_norm.weight = fwAD.make_dual(w.detach(), torch.ones_like(w))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                layer.run(x[:, :2], x[:, 2:])
 
 
 def test_head_sizes_that_the_norm_does_not_take_are_refused_when_built():
