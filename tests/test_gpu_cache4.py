@@ -756,3 +756,31 @@ def test_attention_keeps_weights_in_32_bits(dt, place, D):
     assert (keys == 2).all() and (reach <= 2.0 ** -4 * 1.01).all() and (np.abs(ref) < mass / 30).mean() > 0.9
     tol = (2 * (D + 8) * reach + 16)[..., None] * 2.0 ** -24 * mass + U[dt] * np.abs(ref) + (2.0 ** -25 if dt == torch.float16 else 0)
     assert (np.abs(f64(out) - ref) <= tol).all(), float((np.abs(f64(out) - ref) / tol).max())
+
+
+def test_speculative_step_of_refused_requests():
+    """Requests without pages are answered from inert rows; what a caller keeps, masked by ``granted`` and ``pos``, is that of the
+    others alone, as where all found their pages, and the refused ones' tokens come again in the next step."""
+    a = Run(6, 4, 2, 64, 16, 97, 3, torch.bfloat16, 4)
+    R, n, T = a.R, a.n, a.R * 4
+    g = torch.Generator(device=DEV).manual_seed(3)
+    tokens, new = torch.randint(0, a.V, (T,), generator=g, device=DEV), torch.full((R,), n + 1, dtype=torch.int32, device=DEV)
+    u, v = 0.3 * torch.rand(T, generator=g, device=DEV), torch.rand(R, generator=g, device=DEV)
+    draft = 0.1 * torch.randn(T, a.V, generator=g, device=DEV).to(a.dt)
+    s, full = a.copy(a.state), a.copy(a.state)
+    s["span"][1] = 4  # a page each for four of six
+    accepted_all, tokens_all = a.step(full, tokens, new, u, v, draft)[0][-2:]
+    granted, pos, *_, accepted, toks = a.step(s, tokens, new, u, v, draft)[0]
+    assert granted.tolist() == [1, 1, 1, 1, 0, 0] and (pos.view(R, -1)[4:] == -1).all()
+    ran = (granted > 0) & (new > 0)
+    accepted, answer = torch.where(ran, accepted, 0), torch.where(pos >= 0, toks, -1)
+    assert torch.equal(accepted[:4], accepted_all[:4]) and torch.equal(answer.view(R, -1)[:4], tokens_all.view(R, -1)[:4])
+    assert not accepted[4:].any() and (answer.view(R, -1)[4:] == -1).all()
+    s["seq"].copy_(torch.where(ran, s["seq"], 0))  # (nothing of theirs is held)
+    s["held"].copy_(torch.where(ran, s["held"], 0))
+    s["span"][1] = 3 * R
+    only = torch.where(ran, 0, new)
+    t = torch.cat([tokens[16:], tokens[:16]])  # their rows come first
+    uu, dd = torch.cat([u[16:], u[:16]]), torch.cat([draft[16:], draft[:16]])
+    granted, pos, *_, accepted, toks = a.step(s, t, only, uu, v, dd)[0]
+    assert granted.all() and torch.equal(accepted[4:], accepted_all[4:]) and torch.equal(toks[:8], tokens_all[16:])
