@@ -784,3 +784,47 @@ def test_speculative_step_of_refused_requests():
     uu, dd = torch.cat([u[16:], u[:16]]), torch.cat([draft[16:], draft[:16]])
     granted, pos, *_, accepted, toks = a.step(s, t, only, uu, v, dd)[0]
     assert granted.all() and torch.equal(accepted[4:], accepted_all[4:]) and torch.equal(toks[:8], tokens_all[16:])
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("G,per,split", [(2, 1, False), (8, 1, False), (2, 3, False), (2, 1, True), (1, 2, True)])
+def test_attention_of_keys_that_are_nan(dt, G, per, split):
+    """Keys held as NaN where they are attended: through scores, maximum, sums and joins they make the outputs and logarithms of the rows
+    and heads that attend them NaN, and leave the others' as they were.  One in the newest token (the last row's alone), in each
+    wave's part of the windows, in a landmark of one head, and in every key, where no maximum is found."""
+    H, D, bt = 8, 64, 16
+    lens, wide = ([3000, 45, 3], 2900) if split else ([400, 45, 3], 200)
+    q, cache, table, req, pos, w, lmk = _attend_case(3, H, G, D, bt, 40, dt, 31, max(lens), 30, lens=lens, per=per)
+    w = [x for x in (wide, 7, 3) for _ in range(per)]
+    lmk[..., 0] = 1  # of every head; before the windows of requests 0 and 1
+    kw = dict(w_max=1 << 15 if split else wide, per=per)
+    if split:
+        table = _widened(table, bt, 1 << 15)
+    a, al = _check_attend(q, cache, table, req, pos, w, lmk, **kw)
+    assert np.isfinite(a).all() and np.isfinite(al).all()
+    clean = cache.scale.clone()
+
+    def put(spots):
+        cache.scale.copy_(clean)
+        for i, p, g in spots:
+            cache.scale[int(table[i, p // bt]), g, p % bt, 0, -1] = 255
+        out, lse = _check_attend(q, cache, table, req, pos, w, lmk, **kw)
+        hit = np.zeros(out.shape[:2], dtype=bool)
+        for t in range(len(req)):
+            low = max(pos[t] - w[t] + 1, 0)
+            for h in range(H):
+                mine = {x for x in lmk[h, req[t], 0] if 0 <= x < low}
+                hit[t, h] = any(i == req[t] and g == h // (H // G) and (low <= p <= pos[t] or p in mine) for i, p, g in spots)
+        assert np.isnan(out[hit]).all() and np.isnan(lse[hit]).all() and np.array_equal(out[~hit], a[~hit]) and np.array_equal(lse[~hit], al[~hit])
+        return hit
+    newest = put([(0, pos[per - 1], 0)])
+    assert newest.any() and newest[:per - 1].sum() == 0
+    for back in (40, 70, 100, 130):  # of each wave of the block
+        assert put([(0, pos[0] - back, G - 1)])[0, -1]
+    assert put([(0, 1, 0), (1, 1, G - 1)]).any()
+    only = max(int(p) for p in lmk[3, 0, 0] if p < pos[0] - wide + 1)  # (1, or one that few heads have)
+    assert put([(0, only, 3 // (H // G))])[0, 3]
+    assert put([(2, p, g) for p in range(3) for g in range(G)])[2 * per:].all()
+    cache.scale[:] = 255
+    out, lse = ops.cache_attention(q.to(DEV), cache, *(_i32(x) for x in (table, req, pos, w, lmk)), w_max=kw["w_max"], rows_per_req=per)
+    assert out.isnan().all() and lse.isnan().all()
