@@ -10,14 +10,16 @@
 //
 // A block has four waves, each with every fourth step of the window and then parts of the landmarks; their maxima, sums and
 // values meet in LDS (the windows' pairwise, which leaves room for a second block where there are sixteen columns of 128).  What
-// bounds it is the chain of a step, codes to operands, product, maximum, exponents, product, half of whose cycles are vector
-// instructions, with two waves a SIMD to fill the rest (256 registers a lane; three would spill, 45 us for the 32 us of the 256
-// requests; eight waves a block 42 us).  The memory is not: landmarks read from the caches save 3 of 37 us there.  With few rows it is
+// bounds it is the chain of a step, codes to operands, product, maximum, exponents, product, with two waves a SIMD to hide it
+// behind (142 to 226 registers a lane, 57 to 63 scalar ones held in vector registers; three waves would spill vector ones, 45 us for
+// the 32 us of the 256 requests; eight waves a block 42 us): vector instructions take 0.39 to 0.41 of the cycles, matrix ones 0.07 to 0.18.
+// Four fifths of the steps of the 256 requests are landmarks', with one live column of sixteen.  The memory does not bound it: landmarks
+// read from the caches save 3 of 37 us there.  With few rows it is
 // dependent reads: position, table, tokens, and for landmarks position, table, token.  So the tokens of a step are in registers two
 // steps ahead, a wave's landmarks are looked up while its window is read, and numbers of the whole wave (step, page, head) stay in
 // scalar registers.  Values pass through LDS as bfloat16 rows, from where the matrix operand is read transposed.
-// One request (windows of 512): 11.8 us; 64 requests of five rows in float16, 16 heads of 64 on 4: 18.3 us; four requests with windows
-// of 131072: 39.6 us, 143 MB at 3.6 TB/s, 4 us of it the join of the splits.
+// One request (windows of 512): 12.1 us; 256: 33.8; 64 requests of five rows in float16, 16 heads of 64 on 4: 19.0 us; four requests
+// with windows of 131072: 42 us, 143 MB at 3.4 TB/s, 4 us of it the join of the splits.
 #include <algorithm>
 
 #include "cache4.h"
@@ -522,7 +524,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void cache4_attn_kernel(Cache4AttnP
 
 // How a launch is cut.  The most columns that fit share each key; where that leaves compute units without work, heads go to blocks
 // of their own (their landmarks are their own anyhow, and the window's keys are then read from the caches) and long windows to splits.
-// Measured, bfloat16, 16 query heads of 128 on 2 with 128 landmarks, us by heads of a block:
+// Measured, bfloat16, 16 query heads of 128 on 2 with 128 landmarks, us by heads of a block (weights in two parts; three add 2 to 6 %):
 //   windows of 512, one row a request: 256 requests 8 heads 33, 4 43; 128: 8 27, 4 24; 64: 8 26, 4 19.5, 2 19.3; 32: 4 18.3, 2 15.4,
 //     1 17.6; 8: 2 14.3, 1 13.6; 1: 8 22, 1 11; five rows a request: 256 requests 3 heads 76, 2 82; 64: 3 28, 2 24; 16: 3 22, 2 18,
 //     1 16.4.  So heads are halved while that leaves no more than 512 blocks, two a compute unit, which the card holds at once, and to
@@ -555,7 +557,7 @@ AttnPlan attn_plan(const Cache4AttnParams& p) {
     a.nl = p.k_lmk == 0 ? 0 : std::min(ceil_div(p.k_lmk, 32), a.ns);
     a.chunk_log = p.k_lmk == 0 ? -1 : 0;
     if (p.k_lmk > 0)  // (no more parts than leave room for two blocks in a compute unit's LDS: sixteen columns of 128 with four 51 us,
-                      // three 53, a block alone 88)
+                      // three 53, a block alone 88; float32 rows in pairs with biases, eight heads a block, pass it by 768 bytes)
         while ((2 << a.chunk_log) * a.nh <= kWaves && (kParts + (2 << a.chunk_log)) * a.nr * a.nh * p.c.head_dim * 4 <= 1 << 15) ++a.chunk_log;
     a.kc = p.k_lmk == 0 ? 0 : ceil_div(ceil_div(p.k_lmk, a.nl), a.chunks());
     a.kr_log = 5;

@@ -14,7 +14,8 @@
 // first head's elements are asked for before its position is looked up.  The weights' gradients stay in registers over all that
 // a wave takes, are joined over the block and then, in the order of the blocks, by a second kernel: no atomics, the same bits
 // in every run.  At 32768 tokens of 16 and 2 heads of 128 in bfloat16 the forward moves its 302 MB (and 34 MB of cosines and
-// sines) in 70 us, the backward its 453 MB in 100 us.
+// sines) in 70 us, the backward its 453 MB in 100 us.  At 16001 tokens of 16 and 16 heads of 64 the backward takes 50 us: 38 in its
+// kernel, 4 in the second and the rest between the two.
 #include <algorithm>
 
 #include "common.h"
@@ -289,8 +290,9 @@ int lanes_of(int head_dim) {
 // sixteen), each with every so many-th group of tokens, and up to four heads to a wave where that leaves enough waves: a token's
 // cosines are read once for them.  32768 tokens, 16 and 2 heads of 128, bfloat16, us: forward 70.5 (two heads 71.8, eight 73.3;
 // 2048 waves 86, 8192 waves 69.8, and then 9.1 instead of 7.4 at 2049 tokens), backward 100.3 (eight heads 99.6, sixteen 106.7;
-// 1536 waves 120, 6144 waves 103); 16001 tokens, 16 and 16 heads of 64, backward 46.7 (sixteen heads 46.9, 6144 waves 48.3;
-// with queries and keys in every wave's turn, which needs 224 registers, 61).
+// 1536 waves 120, 6144 waves 103); 16001 tokens, 16 and 16 heads of 64, backward, a call
+// among others, 47 (sixteen heads 47, 6144 waves 48; with queries and keys in every wave's turn, which needs 224 registers, 61).
+// The float16 backward keeps two registers of a lane in memory for heads of 32 to 64 and past 128.
 QkPlan qk_plan(int total_len, int q_heads, int k_heads, int head_dim, int most) {
     const int tok = 64 / lanes_of(head_dim);
     const int64_t groups = ((int64_t)total_len + tok - 1) / tok;

@@ -9,7 +9,7 @@
 //
 // Four launches: the largest logit of each part of a row; each part's sum of weights; each request's first refused row (its
 // probabilities follow from the sums) and the sums over its chunks of what the token is drawn from; the draw, in the one chunk
-// that holds it.  The first reads the rows from memory and is bound by that (97 MB 20.7 us), the others find them in the caches
+// that holds it.  The first reads the rows from memory and is bound by that (91 MB 18 us), the others find them in the caches
 // and are bound by the arithmetic of the weights, in float64 (a float32 one is off by 2^-24 of itself, which over a vocabulary
 // moves a border of the running sums past v once in some thousand draws), or where those of bfloat16 logits are looked up by
 // value, by LDS.  One request of five rows: 4, 6, 7 and 6 us, what a launch and its dependent loads take.
@@ -649,8 +649,8 @@ __global__ __launch_bounds__(kThreads) void verify_draw_kernel(VerifyParams p, V
     }
 }
 
-// How rows are cut.  us on the device, 364 rows (targets and drafts of 64 requests) of 151936 bfloat16 logits:
-//  * By value, 28 for the sums and 22 for what 64 tokens are drawn from, with every weight formed 53 and 35.  A block forms up to
+// How rows are cut.  us on the device, 300 rows (182 of 64 requests and 118 of their drafts, 91 MB) of 151936 bfloat16 logits:
+//  * By value, 31 for the sums and 22 for what 64 tokens are drawn from, with every weight formed 53 and 35.  A block forms up to
 //    4096 entries, so that it takes 12000 logits or more.  1280 blocks for the sums (640 rows: all four launches 128 with 640
 //    blocks, 112 with 1920), 256 of 1024 threads for the draw (128: 90, 512: 86, against 78).
 //  * With every weight formed: blocks begin with a row's parts and a draft's shares, some hundred instructions, so that there are
